@@ -274,6 +274,40 @@ int mmae_masked_ce(const void* logits, int logits_is_bf16, const int64_t* target
                    int W, int patch, float label_smoothing, float* loss, void* d_logits, void* workspace,
                    size_t workspace_bytes, mmae_stream_t stream);
 
+/* ---- class distributions (no counterpart in the reference; beside the masked cross entropy) -----------------------
+ * logits: `outer` samples of `classes` x `inner` values, class j of position (b, i) at b * ld + j * inner + i (rows [N, C]:
+ * inner = 1; class maps [B, C, H, W]: inner = H * W); f32, bf16 or f16 (MMAE_DT_*), any alignment of the element type.
+ * Per-position arrays are [outer, inner], per-alternative arrays [outer, k, inner].  x = z / temperature throughout.
+ *
+ * mmae_class_log_probs: log_prob = log softmax(x)[target] (0 where target is outside [0, classes), e.g. -100), entropy of
+ * softmax(x), and the top_k (<= 64, <= classes) classes by z with their log probabilities: descending, equal values by the
+ * lower class, NaN first.  row_max / row_log_sum: what the backward pass needs.  A position whose logits are all -inf
+ * has log_prob = -inf (at a valid target), entropy 0 and no gradient.  NaN and +inf logits give NaN, as in torch.
+ * mmae_class_log_probs_bwd: d_logits (contiguous, the logits' dtype) for the gradients that arrive at log_prob and entropy
+ * (either may be NULL). */
+enum { MMAE_DT_F32 = 0, MMAE_DT_BF16 = 1, MMAE_DT_F16 = 2 };
+size_t mmae_class_log_probs_workspace_bytes(int outer, int classes, int inner, int top_k);
+int mmae_class_log_probs(const void* logits, int dtype, int outer, int classes, int inner, long ld, const int64_t* target,
+                         int top_k, float temperature, float* log_prob, float* entropy, float* row_max, float* row_log_sum,
+                         float* top_log_prob, int64_t* top_class, void* workspace, size_t workspace_bytes, mmae_stream_t stream);
+int mmae_class_log_probs_bwd(const void* logits, int dtype, int outer, int classes, int inner, long ld, const int64_t* target,
+                             float temperature, const float* entropy, const float* row_max, const float* row_log_sum,
+                             const float* d_log_prob, const float* d_entropy, void* d_logits, mmae_stream_t stream);
+/* Distillation from a teacher's k (<= 64) top classes per position: top_class (int32 or int64: class_bytes 4 / 8) and
+ * top_value (f32, bf16 or f16: value_dtype), [outer, k, inner].  kind 0: the values are the teacher's logits, q = softmax(value /
+ * temperature) over the k; kind 1: its log probabilities at this temperature, q = exp(value), and what they leave, 1 - sum q,
+ * stands for all other classes as one outcome.  A class outside [0, classes) is padding; one listed twice counts twice.
+ *   loss = temperature^2 * mean of KL(q || p): over the positions in the mask of each sample, then over the samples with any
+ * mask i64 [outer, (rows / patch) * (width / patch)] over inner = rows x width positions (nonzero = in the loss), or NULL: the
+ * mean over all positions.  loss (f32 scalar) or d_logits (contiguous, the logits' dtype: the loss's gradient times
+ * *upstream, a device scalar, or times 1 if NULL) may be NULL, not both.  skip_unit: leave everything as it is where
+ * *upstream is 1. */
+size_t mmae_distill_workspace_bytes(int outer, int classes, int inner, int k);
+int mmae_distill(const void* logits, int dtype, int outer, int classes, int inner, long ld, const void* top_class,
+                 int class_bytes, const void* top_value, int value_dtype, int k, int kind, float temperature,
+                 const int64_t* mask, int width, int patch, const float* upstream, int skip_unit, float* loss, void* d_logits,
+                 void* workspace, size_t workspace_bytes, mmae_stream_t stream);
+
 /* Truncated depth standardisation (run_pretraining_multimae.py:448-459): per sample (B rows of n values),
  * out = (x - mean) / sqrt(var + eps) with mean / unbiased var over the sorted values of ranks
  * [int(lo_frac * n), int(hi_frac * n)) (0.1, 0.9, eps 1e-6 in the reference).  Order statistics by radix select; no sort.

@@ -896,14 +896,72 @@ class MaskedCEFn(torch.autograd.Function):
         return d_logits * g.to(d_logits.dtype), None, None, None, None
 
 
+def _class_scores(x: torch.Tensor) -> torch.Tensor:
+    return x if x.dim() < 2 or ops.class_geometry(x) is not None else x.contiguous()
+
+
+class ClassLogProbsFn(torch.autograd.Function):
+    """(log probability of the given class, entropy, top log probabilities, top classes) of each position's distribution;
+    the first two carry gradients."""
+
+    @staticmethod
+    def forward(ctx, logits, target, top_k, temperature):
+        logits = _class_scores(logits)
+        log_prob, entropy, top_log_prob, top_class, stats = ops.class_log_probs(logits, target.contiguous(), top_k, temperature)
+        ctx.temperature = temperature
+        ctx.set_materialize_grads(False)
+        ctx.mark_non_differentiable(*(t for t in (top_log_prob, top_class) if t is not None))
+        ctx.save_for_backward(logits, target.contiguous(), entropy, stats)
+        return log_prob, entropy, top_log_prob, top_class
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, g_log_prob, g_entropy, _top_log_prob, _top_class):
+        if g_log_prob is None and g_entropy is None:
+            return None, None, None, None
+        logits, target, entropy, stats = ctx.saved_tensors
+        g = [None if t is None else t.float().contiguous() for t in (g_log_prob, g_entropy)]
+        return ops.class_log_probs_bwd(logits, target, entropy, stats, *g, ctx.temperature), None, None, None
+
+
+class DistillFn(torch.autograd.Function):
+    """Distillation loss with its gradient from one pass over the logits, for an upstream gradient of 1.  The backward pass
+    looks at the upstream gradient on the device: 1 leaves that gradient as it is, another value computes it anew with the
+    factor inside the one rounding to the logits' type.  The buffer goes to the caller of the first backward pass; a
+    further one (retain_graph) fills a buffer of its own."""
+
+    @staticmethod
+    def forward(ctx, logits, top_class, top_value, mask, patch, temperature, log_probs):
+        logits, top_class, top_value = _class_scores(logits), top_class.contiguous(), top_value.contiguous()
+        ctx.d_logits = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device) if ctx.needs_input_grad[0] else None
+        loss = ops.distill(logits, top_class, top_value, mask, patch, temperature, log_probs, d_logits=ctx.d_logits)
+        if ctx.d_logits is not None:
+            ctx.save_for_backward(logits, top_class, top_value, mask)
+            ctx.options = (patch, temperature, log_probs)
+        return loss
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, g):
+        d_logits, ctx.d_logits = ctx.d_logits, None
+        if d_logits is None or not getattr(ctx, "unit_upstream", False):
+            logits, top_class, top_value, mask = ctx.saved_tensors
+            first = d_logits is not None
+            if not first:
+                d_logits = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
+            ops.distill(logits, top_class, top_value, mask, *ctx.options, want_loss=False, d_logits=d_logits, upstream=g.float().contiguous(),
+                        skip_unit=first)
+        return d_logits, None, None, None, None, None, None
+
+
 def mark_unit_upstream(losses) -> None:
-    """Tell the graph nodes of these loss tensors (outputs of MaskedLossFn / MaskedCEFn) that the gradient arriving at them
+    """Tell the graph nodes of these loss tensors (outputs of MaskedLossFn / MaskedCEFn / DistillFn) that the gradient arriving at them
     will be exactly 1, as for the terms of a plain sum that backward() is called on: their backward then hands out the
     gradient the forward kernel wrote instead of a scaled copy (an image-sized multiply per loss).  The mark sits on the
     node of one forward call, so it ends with that graph; other tensors and other graphs are unaffected."""
     for t in losses:
         node = getattr(t, "grad_fn", None)
-        if isinstance(node, (MaskedLossFn._backward_cls, MaskedCEFn._backward_cls)):
+        if isinstance(node, (MaskedLossFn._backward_cls, MaskedCEFn._backward_cls, DistillFn._backward_cls)):
             node.unit_upstream = True
 
 

@@ -625,6 +625,8 @@ class PretrainStep:
         """clip_grad / skip_grad: max_norm / max_skip_norm of the reference's train_one_epoch
         (run_pretraining_multimae.py:512-519).  lr_schedule_values / wd_schedule_values: per-iteration arrays
         (cosine_scheduler) applied before each step as at :424-436; iteration = start_step + calls so far.
+        losses: task -> (loss module, key of its target in the batch), or (loss module, key, domain whose mask it takes) where
+        the target is not an input domain itself (a teacher's (classes, values) for MaskedDistillationLoss).
         loss_on_unmasked: the losses average over every token instead of the masked ones (:491-496).
         keep_grads: leave the step's gradients in `p.grad` after the call (for inspection).  By default the bucket-wise
         update clears each gradient range behind its read, which is the next iteration's `optimizer.zero_grad()` (:507)
@@ -712,8 +714,8 @@ class PretrainStep:
         inputs = {d: t for d, t in batch.items() if d in self.model.input_adapters}
         preds, masks = self.model(inputs, num_encoded_tokens=self.k, alphas=self.alphas, mask_randomness=mask_randomness,
                                   sample_tasks_uniformly=self.uniform, fp32_output_adapters=self.fp32_out)
-        task_losses = {t: fn(preds[t], batch[tgt], mask=None if self.loss_on_unmasked else masks.get(tgt))
-                       for t, (fn, tgt) in self.losses.items()}
+        task_losses = {t: fn(preds[t], batch[tgt], mask=None if self.loss_on_unmasked else masks.get(dom[0] if dom else tgt))
+                       for t, (fn, tgt, *dom) in self.losses.items()}
         loss = sum(task_losses.values())
         Fn.mark_unit_upstream(task_losses.values())  # loss is their plain sum: d(loss) / d(task loss) = 1 for every task
         self.buckets.reset()        # completion signals left by a backward pass outside this step
