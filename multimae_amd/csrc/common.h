@@ -72,13 +72,12 @@ __device__ __forceinline__ float add_bf16x8(float acc, const bf16x8& v) {
     return acc;
 }
 
-// GELU and its derivative on the packed fp32 ALU, without transcendentals.  Both Phi(x) - 1/2 and gelu'(x) - 1/2 are odd
+// GELU and its derivative on the fp32 ALU, without transcendentals.  Both Phi(x) - 1/2 and gelu'(x) - 1/2 are odd
 // functions: x * P(u) with u = x^2 scaled to [-1, 1] (least squares on Chebyshev nodes, scripts/fit_gelu_poly.py), fitted
 // under the condition that the value at the end of the range is exactly 1/2: the argument is clamped to the range and the
 // saturated branches (+-1/2 beyond |x| = 4, 4.5) need no select.  Absolute error <= 3.8e-5 (6.9e-5), below the bf16
 // rounding of the stored result for every value that matters; a GEMM epilogue with the rcp/exp2 form spent a quarter of the
-// tile time here.  NP pairs are evaluated side by side, coefficient by coefficient: a dependent chain of packed FMAs costs
-// a wait state per link, independent chains fill them.
+// tile time here.  NP pairs are evaluated side by side, coefficient by coefficient.
 typedef __attribute__((ext_vector_type(2))) float f32x2;
 // r = xc * P(w) + 1/2 with xc = clamp(x, -xmax, xmax) and w = xc^2 * scale + shift (scale = 1, shift = 0: P is given in x^2
 // itself, one instruction fewer; accurate enough in fp32 for the degree-7 polynomial of GELU, not for the degree-9 one of
