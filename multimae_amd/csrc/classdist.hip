@@ -18,21 +18,65 @@ constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
 
 typedef _Float16 f16;
 
+// 16 bytes of a row: VEC elements.  Loads and stores take any alignment of the element type.
+struct Piece { uint32_t w[4]; };
+// KEY_BITS: leading bits of ordered(v) that tell all values of the type apart
 struct F32 {
     typedef float E;
+    static constexpr int VEC = 4, KEY_BITS = 32;
+    static constexpr uint32_t NEG_INF = 0xff800000u;  // as a word of a piece
     static __device__ __forceinline__ float up(float v) { return v; }
     static __device__ __forceinline__ float down(float v) { return v; }
+    static __device__ __forceinline__ float get(const Piece& q, int e) { return __uint_as_float(q.w[e]); }
+    static __device__ __forceinline__ void put(Piece& q, int e, float v) { q.w[e] = __float_as_uint(v); }
+    static __device__ __forceinline__ Piece pack(const float (&v)[4]) { return {__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3])}; }
 };
 struct B16 {
     typedef bf16 E;
+    static constexpr int VEC = 8, KEY_BITS = 16;
+    static constexpr uint32_t NEG_INF = 0xff80ff80u;
     static __device__ __forceinline__ float up(bf16 v) { return (float)v; }
     static __device__ __forceinline__ bf16 down(float v) { return (bf16)v; }
+    static __device__ __forceinline__ float get(const Piece& q, int e) { return __uint_as_float(e & 1 ? q.w[e >> 1] & 0xffff0000u : q.w[e >> 1] << 16); }
+    static __device__ __forceinline__ void put(Piece& q, int e, float v) {
+        const uint32_t b = __builtin_bit_cast(uint16_t, (bf16)v);
+        q.w[e >> 1] = e & 1 ? (q.w[e >> 1] & 0xffffu) | b << 16 : (q.w[e >> 1] & 0xffff0000u) | b;
+    }
+    static __device__ __forceinline__ Piece pack(const float (&v)[8]) {
+        typedef __attribute__((ext_vector_type(8))) bf16 V;
+        V r;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) r[e] = (bf16)v[e];
+        return __builtin_bit_cast(Piece, r);
+    }
 };
 struct H16 {
     typedef f16 E;
+    static constexpr int VEC = 8, KEY_BITS = 20;  // sign, 8 exponent bits of fp32, 10 mantissa bits (and one spare)
+    static constexpr uint32_t NEG_INF = 0xfc00fc00u;
     static __device__ __forceinline__ float up(f16 v) { return (float)v; }
     static __device__ __forceinline__ f16 down(float v) { return (f16)v; }
+    static __device__ __forceinline__ float get(const Piece& q, int e) {
+        return (float)__builtin_bit_cast(f16, (uint16_t)(e & 1 ? q.w[e >> 1] >> 16 : q.w[e >> 1]));
+    }
+    static __device__ __forceinline__ void put(Piece& q, int e, float v) {
+        const uint32_t b = __builtin_bit_cast(uint16_t, (f16)v);
+        q.w[e >> 1] = e & 1 ? (q.w[e >> 1] & 0xffffu) | b << 16 : (q.w[e >> 1] & 0xffff0000u) | b;
+    }
+    static __device__ __forceinline__ Piece pack(const float (&v)[8]) {
+        typedef __attribute__((ext_vector_type(8))) f16 V;
+        V r;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) r[e] = (f16)v[e];
+        return __builtin_bit_cast(Piece, r);
+    }
 };
+template <class T> __device__ __forceinline__ Piece load_piece(const typename T::E* p) {
+    Piece q;
+    __builtin_memcpy(&q, p, 16);
+    return q;
+}
+template <class T> __device__ __forceinline__ void store_piece(typename T::E* p, const Piece& q) { __builtin_memcpy(p, &q, 16); }
 
 __device__ __forceinline__ float exp2_(float v) { return __builtin_amdgcn_exp2f(v); }
 __device__ __forceinline__ float log2_(float v) { return __builtin_amdgcn_logf(v); }
@@ -44,6 +88,11 @@ __device__ __forceinline__ uint32_t ordered(float v) {
     return b ^ ((uint32_t)((int32_t)b >> 31) | 0x80000000u);
 }
 __device__ __forceinline__ uint64_t rank_key(float v, uint32_t cls) { return (uint64_t)ordered(v) << 32 | (0xffffffffu - cls); }
+__device__ __forceinline__ float key_value(uint64_t key) {  // (NaN stays NaN)
+    const uint32_t u = (uint32_t)(key >> 32);
+    return __uint_as_float(u & 0x80000000u ? u ^ 0x80000000u : ~u);
+}
+__device__ __forceinline__ uint32_t key_class(uint64_t key) { return 0xffffffffu - (uint32_t)key; }
 
 __device__ __forceinline__ float load_any(const void* p, int dtype, long i) {
     if (dtype == MMAE_DT_F32) return ((const float*)p)[i];
@@ -151,6 +200,362 @@ __global__ __launch_bounds__(256) void log_probs_kernel(LogProbArgs a) {
     }
 }
 
+// ---- rows: one pass over a row, or a slice of it --------------------------------------------------------------------
+// Sums in the base-2 domain against a reference exponent R: s = sum 2^(z c - R), t = sum (z c - R) 2^(z c - R), m = max z.
+// z c - R is one fused multiply-add without intermediate overflow; R = m c, held to +-FAR, is the same rounded number wherever
+// it is used, so its rounding cancels.  Beyond FAR (every class left at the type's lowest value, say) the row's sums are
+// formed anew from (z - m) c.
+constexpr float FAR = 1e38f;
+struct Sums { float m, R, s, t; };
+__device__ __forceinline__ float reference_exponent(float m, float c) { return __builtin_amdgcn_fmed3f(m * c, -FAR, FAR); }
+__device__ __forceinline__ Sums join(const Sums& a, const Sums& b) {
+    const float R = fmaxf(a.R, b.R), da = a.R - R, db = b.R - R, fa = exp2_(da), fb = exp2_(db);
+    return {fmaxf(a.m, b.m), R, a.s * fa + b.s * fb, fa * (a.t + bounded(da) * a.s) + fb * (b.t + bounded(db) * b.s)};
+}
+__device__ __forceinline__ Sums wave_sums(Sums v) {
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) v = join(v, {__shfl_xor(v.m, o, 64), __shfl_xor(v.R, o, 64), __shfl_xor(v.s, o, 64), __shfl_xor(v.t, o, 64)});
+    return v;
+}
+template <int NT>
+__device__ Sums block_sums(Sums v, Sums* red) {
+    v = wave_sums(v);
+    if (NT == 64) return v;
+    __syncthreads();
+    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
+    __syncthreads();
+    Sums r = red[0];
+    for (int i = 1; i < NT / 64; ++i) r = join(r, red[i]);
+    return r;
+}
+__device__ __forceinline__ bool is_far(float m, float c) { return fabsf(m) < INFINITY && fabsf(m * c) > FAR; }
+
+// The sums of a whole row by (z - m) c, for the rows beyond FAR.
+template <class T, int NT>
+__device__ __noinline__ Sums far_sums(const typename T::E* z, int C, float m, float c, Sums* red) {
+    Sums v = {m, 0.f, 0.f, 0.f};
+    for (int j = threadIdx.x; j < C; j += NT) {
+        const float d = (T::up(z[j]) - m) * c, e = exp2_(d);
+        v.s += e;
+        v.t += e * bounded(d);
+    }
+    return block_sums<NT>(v, red);
+}
+
+// log p of one logit, in natural units.  l2 = log2 of the sum (+inf: nothing left).
+__device__ __forceinline__ float row_log_p(const Geometry& g, float z, float m, float l2) {
+    const float d = __builtin_fmaf(z, g.c, -reference_exponent(m, g.c)) - l2;
+    // the lowest finite values leave the base-2 range before they leave the natural one
+    return is_far(m, g.c) || (d == -INFINITY && z != -INFINITY) ? g.log_p(z, m, l2) : d * LN2;
+}
+
+template <class T, int NT, int NV>
+__device__ __forceinline__ void load_tile(Piece (&q)[NV], const typename T::E* z, int base, int end) {
+    constexpr int VEC = T::VEC;
+    if (base + NT * NV * VEC <= end) {
+#pragma unroll
+        for (int i = 0; i < NV; ++i) q[i] = load_piece<T>(z + base + (i * NT + threadIdx.x) * VEC);
+    } else {
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const int j = base + (i * NT + threadIdx.x) * VEC;
+            if (j + VEC <= end) {
+                q[i] = load_piece<T>(z + j);
+            } else {
+                q[i] = {T::NEG_INF, T::NEG_INF, T::NEG_INF, T::NEG_INF};
+#pragma unroll
+                for (int e = 0; e < VEC; ++e)
+                    if (j + e < end) T::put(q[i], e, T::up(z[j + e]));
+            }
+        }
+    }
+}
+
+// Most keys a tile can append: the list's own, and those above the k-th largest of the threads' maxima, which belong to
+// fewer than k threads.
+template <int EPT> constexpr int list_room() { return MAX_TOP + (MAX_TOP - 1) * EPT; }
+
+template <int ROOM, int NT>
+struct TopList {
+    uint64_t keys[ROOM];    // sorted up to `have` between tiles, appended behind it
+    uint64_t sorted[MAX_TOP];
+    float maxima[NT];
+    int count, wave_count[NT / 64];
+};
+
+// ordered() of the k-th largest of the NT maxima, searched bit by bit: each wave looks at all maxima and counts by ballots, so
+// no wave waits for another.
+template <class T, int NT>
+__device__ __forceinline__ uint32_t kth_maximum(const float* maxima, int k) {
+    const int lane = threadIdx.x & 63;
+    uint32_t key[NT / 64];
+#pragma unroll
+    for (int i = 0; i < NT / 64; ++i) key[i] = ordered(maxima[i * 64 + lane]);
+    uint32_t at = 0;
+    for (int b = 31; b >= 32 - T::KEY_BITS; --b) {
+        const uint32_t next = at | 1u << b;
+        int n = 0;
+#pragma unroll
+        for (int i = 0; i < NT / 64; ++i) n += __popcll(__ballot(key[i] >= next));
+        if (n >= k) at = next;
+    }
+    return at & 0x80000000u ? at : at | ((1ull << (32 - T::KEY_BITS)) - 1);  // (negative values are inverted, their later bits are set)
+}
+
+// Ranks the `n` keys of the list and keeps the first k, sorted.  Returns the value a further key has to exceed.
+template <int NT, class L>
+__device__ float keep_best(L& list, int n, int k) {
+    for (int i = threadIdx.x; i < n; i += NT) {
+        const uint64_t key = list.keys[i];
+        int rank = 0;
+        for (int j = 0; j < n; ++j) rank += list.keys[j] > key;
+        if (rank < k) list.sorted[rank] = key;
+    }
+    __syncthreads();
+    const int have = n < k ? n : k;
+    for (int i = threadIdx.x; i < have; i += NT) list.keys[i] = list.sorted[i];
+    if (threadIdx.x == 0) list.count = have;
+    __syncthreads();
+    return have < k ? -INFINITY : key_value(list.keys[k - 1]);
+}
+
+// Takes a tile's elements into the list.  floor: the value a key has to exceed (the k-th best so far: an equal one has a
+// higher class), -inf with `open` while the list holds fewer than k.
+template <class T, int NT, int NV, class L>
+__device__ __forceinline__ void take_tile(L& list, const Piece (&q)[NV], float tile_max, int base, int end, int k, float& floor, bool& open) {
+    constexpr int VEC = T::VEC, ROOM = sizeof(list.keys) / 8;
+    const int above = NT == 64 ? __popcll(__ballot(open || tile_max > floor)) : __syncthreads_count(open || tile_max > floor);
+    if (above == 0) return;
+    const int have = list.count;
+    float least = floor;     // take values above this one ...
+    bool equals = open;      // ... and equal to it
+    if (above >= k) {        // else fewer than k threads hold values above the floor: they all fit
+        list.maxima[threadIdx.x] = tile_max;
+        __syncthreads();
+        const uint32_t kth = kth_maximum<T, NT>(list.maxima, k);
+        const float v = key_value((uint64_t)kth << 32);
+        if (open || v > floor) { least = v; equals = true; }
+    }
+    if (NT != 64) __syncthreads();  // (list.count is read)
+    if (tile_max > least || (equals && tile_max == least)) {
+#pragma unroll
+        for (int i = 0; i < NV; ++i)
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) {
+                const float v = T::get(q[i], e);
+                const int j = base + (i * NT + threadIdx.x) * VEC + e;
+                if ((v > least || (equals && v == least)) && j < end) {
+                    const int n = atomicAdd(&list.count, 1);
+                    if (n < ROOM) list.keys[n] = rank_key(v, j);
+                }
+            }
+    }
+    __syncthreads();
+    int n = list.count;
+    if (n > ROOM) {
+        // More equal values than the list holds: the greater ones (fewer than k threads have any), then the equal ones of
+        // the lowest classes, piece by piece in the order of classes.
+        __syncthreads();
+        if (threadIdx.x == 0) list.count = have;
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < NV; ++i)
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) {
+                const float v = T::get(q[i], e);
+                if (v > least) {
+                    const int n = atomicAdd(&list.count, 1);
+                    if (n < ROOM) list.keys[n] = rank_key(v, base + (i * NT + threadIdx.x) * VEC + e);
+                }
+            }
+        __syncthreads();
+        n = list.count < ROOM ? list.count : ROOM;
+        int left = k < ROOM - n ? k : ROOM - n;  // equal values taken: k cover every need, keep_best cuts
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const int j = base + (i * NT + threadIdx.x) * VEC;
+            int mine = 0;
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) mine += T::get(q[i], e) == least && j + e < end;
+            int before = mine;  // inclusive prefix over the wave, then over the waves
+#pragma unroll
+            for (int o = 1; o < 64; o <<= 1) {
+                const int w = __shfl_up(before, o, 64);
+                if ((int)(threadIdx.x & 63) >= o) before += w;
+            }
+            __syncthreads();
+            if ((threadIdx.x & 63) == 63) list.wave_count[threadIdx.x >> 6] = before;
+            __syncthreads();
+            int all = 0;
+            before -= mine;
+            for (int w = 0; w < NT / 64; ++w) {
+                if (w < (int)(threadIdx.x >> 6)) before += list.wave_count[w];
+                all += list.wave_count[w];
+            }
+#pragma unroll
+            for (int e = 0; e < VEC; ++e)
+                if (T::get(q[i], e) == least && j + e < end) {
+                    if (before < left) list.keys[n + before] = rank_key(least, j + e);
+                    ++before;
+                }
+            n += all < left ? all : left;
+            left -= all < left ? all : left;
+        }
+        __syncthreads();
+    }
+    floor = keep_best<NT>(list, n, k);
+    open = list.count < k;
+}
+
+// The k best of z[first, end) by k scans, for slices that hold NaN (which compare with nothing).
+template <class T, int NT, class L>
+__device__ __noinline__ void scan_top(L& list, const typename T::E* z, int first, int end, int k) {
+    uint64_t last = ~0ull;
+    const int n = end - first < k ? end - first : k;
+    for (int i = 0; i < n; ++i) {
+        uint64_t top = 0;
+        for (int j = first + threadIdx.x; j < end; j += NT) {
+            const uint64_t key = rank_key(T::up(z[j]), j);
+            if (key < last && key > top) top = key;
+        }
+#pragma unroll
+        for (int o = 32; o > 0; o >>= 1) {
+            const uint64_t w = __shfl_xor((unsigned long long)top, o, 64);
+            top = w > top ? w : top;
+        }
+        __syncthreads();
+        if ((threadIdx.x & 63) == 0) list.sorted[threadIdx.x >> 6] = top;
+        __syncthreads();
+        for (int w = 0; w < NT / 64; ++w) top = list.sorted[w] > top ? list.sorted[w] : top;
+        last = top;
+        if (threadIdx.x == 0) list.keys[i] = top;
+    }
+    __syncthreads();
+    if (threadIdx.x == 0) list.count = n;
+    __syncthreads();
+}
+
+// A row's results from its sums and its sorted best keys (keys[i], i < k); the threads of one wave.
+template <class T, int NT>
+__device__ __forceinline__ void finish_row(const LogProbArgs& a, long p, const typename T::E* z, Sums v, const uint64_t* keys, Sums* red) {
+    const float c = a.g.c;
+    if (is_far(v.m, c)) v = far_sums<T, NT>(z, a.g.classes, v.m, c, red);
+    if (v.m == INFINITY) v.s = __builtin_nanf("");
+    const bool empty = v.m == -INFINITY && v.s == 0.f;
+    const float l2 = empty ? INFINITY : log2_(v.s);
+    if (threadIdx.x == 0) {
+        const long y = a.target[p];
+        a.log_prob[p] = y >= 0 && y < a.g.classes ? row_log_p(a.g, T::up(z[y]), v.m, l2) : 0.f;
+        a.entropy[p] = empty ? 0.f : (l2 - v.t / v.s) * LN2;
+        a.row_max[p] = v.m;
+        a.row_log_sum[p] = l2;
+    }
+    if ((int)threadIdx.x < a.k) {
+        const uint64_t key = keys[threadIdx.x];
+        a.top_class[p * a.k + threadIdx.x] = key_class(key);
+        a.top_log_prob[p * a.k + threadIdx.x] = row_log_p(a.g, key_value(key), v.m, l2);
+    }
+}
+
+// What a slice leaves for the join: its sums, then its k keys (0 where it holds fewer classes).
+__host__ __device__ inline size_t slice_bytes(int k) { return sizeof(Sums) + sizeof(uint64_t) * (size_t)k; }
+
+template <class T, int NT, int NV, bool TOP>
+__global__ __launch_bounds__(NT) void log_probs_rows_kernel(LogProbArgs a, int slices, int slice_tiles, char* parts) {
+    constexpr int VEC = T::VEC, TILE = NT * NV * VEC, ROOM = TOP ? list_room<NV * VEC>() : 1;
+    __shared__ Sums red[NT / 64];
+    __shared__ TopList<ROOM, NT> list;
+    const long p = blockIdx.x / slices;
+    const int slice = blockIdx.x % slices;
+    const typename T::E* z = (const typename T::E*)a.g.logits + p * a.g.ld;
+    const int C = a.g.classes, first = slice * slice_tiles * TILE;
+    const int end = first + slice_tiles * TILE < C ? first + slice_tiles * TILE : C;
+    const float c = a.g.c;
+    Sums v = {-INFINITY, -FAR, 0.f, 0.f};
+    float floor = -INFINITY;
+    bool open = true;
+    if (TOP) {
+        if (threadIdx.x == 0) list.count = 0;
+        __syncthreads();
+    }
+    Piece q[NV], next[NV];
+    load_tile<T, NT, NV>(q, z, first, end);
+    for (int base = first;;) {
+        const bool more = base + TILE < end;
+        if (more) load_tile<T, NT, NV>(next, z, base + TILE, end);
+        float m = T::get(q[0], 0);
+#pragma unroll
+        for (int i = 0; i < NV; ++i)
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) m = fmaxf(m, T::get(q[i], e));
+        if (m > v.m) {
+            v.m = m;
+            const float R = reference_exponent(m, c), d = v.R - R, f = exp2_(d);
+            v.t = f * (v.t + bounded(d) * v.s);
+            v.s *= f;
+            v.R = R;
+        }
+        float s = 0.f, t = 0.f;
+#pragma unroll
+        for (int i = 0; i < NV; ++i)
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) {
+                const float d = __builtin_fmaf(T::get(q[i], e), c, -v.R), x = exp2_(d);
+                s += x;
+                t = __builtin_fmaf(x, bounded(d), t);
+            }
+        v.s += s;
+        v.t += t;
+        if (TOP) take_tile<T, NT, NV>(list, q, m, base, end, a.k, floor, open);
+        if (!more) break;
+        base += TILE;
+#pragma unroll
+        for (int i = 0; i < NV; ++i) q[i] = next[i];
+    }
+    v = block_sums<NT>(v, red);
+    if (TOP && v.s != v.s) scan_top<T, NT>(list, z, first, end, a.k);
+    if (slices == 1) {
+        finish_row<T, NT>(a, p, z, v, list.keys, red);
+        return;
+    }
+    char* out = parts + (size_t)blockIdx.x * slice_bytes(a.k);
+    if (threadIdx.x == 0) *(Sums*)out = v;
+    if (TOP && (int)threadIdx.x < a.k) ((uint64_t*)(out + sizeof(Sums)))[threadIdx.x] = (int)threadIdx.x < list.count ? list.keys[threadIdx.x] : 0;
+}
+
+// Joins the slices of a row: one wave per row, lane i walks slice i's sorted keys.
+constexpr int MAX_SLICES = 64;
+template <class T>
+__global__ __launch_bounds__(64) void log_probs_join_kernel(LogProbArgs a, int slices, const char* parts) {
+    extern __shared__ uint64_t s_keys[];  // [slices][k], then the k best
+    __shared__ Sums red[1];
+    const long p = blockIdx.x;
+    const int lane = threadIdx.x, k = a.k;
+    const char* part = parts + (size_t)p * slices * slice_bytes(k);
+    Sums v = {-INFINITY, -FAR, 0.f, 0.f};
+    if (lane < slices) v = *(const Sums*)(part + lane * slice_bytes(k));
+    for (int i = lane; i < slices * k; i += 64) s_keys[i] = ((const uint64_t*)(part + (i / k) * slice_bytes(k) + sizeof(Sums)))[i % k];
+    v = wave_sums(v);
+    __syncthreads();
+    int at = 0;
+    uint64_t head = lane < slices && k ? s_keys[lane * k] : 0;
+    for (int i = 0; i < k; ++i) {
+        uint64_t top = head;
+#pragma unroll
+        for (int o = 32; o > 0; o >>= 1) {
+            const uint64_t w = __shfl_xor((unsigned long long)top, o, 64);
+            top = w > top ? w : top;
+        }
+        if (head == top && top) {  // keys are unique: one lane
+            ++at;
+            head = at < k ? s_keys[lane * k + at] : 0;
+        }
+        if (lane == 0) s_keys[slices * k + i] = top;
+    }
+    __syncthreads();
+    finish_row<T, 64>(a, p, (const typename T::E*)a.g.logits + p * a.g.ld, v, s_keys + slices * k, red);
+}
+
 struct LogProbBwdArgs {
     Geometry g;
     const int64_t* target;
@@ -173,6 +578,47 @@ __global__ __launch_bounds__(256) void log_probs_bwd_kernel(LogProbBwdArgs a) {
         const float lp2 = (T::up(z[base + j * cs]) - m) * c - l2;
         const float q = exp2_(lp2);
         dz[out + j * cs] = T::down((j == y ? gl : 0.f) - q * (gl + gh * (bounded(lp2) * LN2 + h)));
+    }
+}
+
+// Rows, forward: a tile per workgroup.  -(gl + gh (log p + H)) p is p (A + B log2 p).
+template <class T, int NT, int NV>
+__global__ __launch_bounds__(NT) void log_probs_bwd_rows_kernel(LogProbBwdArgs a, int tiles) {
+    constexpr int VEC = T::VEC, TILE = NT * NV * VEC;
+    const long p = blockIdx.x / tiles;
+    const int base = (blockIdx.x % tiles) * TILE, C = a.g.classes;
+    const typename T::E* z = (const typename T::E*)a.g.logits + p * a.g.ld;
+    typename T::E* dz = (typename T::E*)a.d_logits + p * C;
+    Piece q[NV];
+    load_tile<T, NT, NV>(q, z, base, C);
+    const float m = a.row_max[p], l2 = a.row_log_sum[p], c = a.g.c;
+    const long y = a.target[p];
+    const float gl = a.d_log_prob && y >= 0 && y < C && l2 != INFINITY ? a.d_log_prob[p] * a.g.inv_t : 0.f;
+    const float gh = a.d_entropy ? a.d_entropy[p] * a.g.inv_t : 0.f;
+    const float A = -(gl + gh * a.entropy[p]), B = -gh * LN2;
+    const int at = y >= 0 && y < C ? (int)y : -VEC;
+    const bool far = is_far(m, c);
+    const float R = far ? 0.f : reference_exponent(m, c);
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+        const int j = base + (i * NT + threadIdx.x) * VEC;
+        if (j >= C) break;
+        float o[VEC];
+        const bool named = (unsigned)(at - j) < (unsigned)VEC;
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) {
+            const float x = T::get(q[i], e);
+            const float d = (far ? (x - m) * c : __builtin_fmaf(x, c, -R)) - l2, w = exp2_(d);
+            float g = w * __builtin_fmaf(B, bounded(d), A);
+            o[e] = named && at - j == e ? g + gl : g;
+        }
+        if (j + VEC <= C) {
+            store_piece<T>(dz + j, T::pack(o));
+        } else {
+#pragma unroll
+            for (int e = 0; e < VEC; ++e)
+                if (j + e < C) dz[j + e] = T::down(o[e]);
+        }
     }
 }
 
@@ -333,6 +779,7 @@ int check_logits(const char* name, const void* logits, int dtype, int outer, int
     MMAE_REQUIRE(logits, MMAE_EINVAL, "%s: null pointer", name);
     MMAE_REQUIRE(dtype >= MMAE_DT_F32 && dtype <= MMAE_DT_F16, MMAE_EINVAL, "%s: dtype code %d", name, dtype);
     MMAE_REQUIRE(outer > 0 && classes > 0 && inner > 0, MMAE_ESHAPE, "%s: empty input (%d x %d x %d)", name, outer, classes, inner);
+    MMAE_REQUIRE(classes <= 1 << 30, MMAE_ESHAPE, "%s: %d classes", name, classes);
     MMAE_REQUIRE((long)outer * inner <= 0x7fffffffL, MMAE_ESHAPE, "%s: %d x %d positions are more than 2^31 - 1", name, outer, inner);
     MMAE_REQUIRE(ld >= (long)classes * inner, MMAE_ESHAPE, "%s: samples %ld elements apart hold %d x %d values", name, ld, classes, inner);
     MMAE_REQUIRE(temperature > 0.f && temperature < INFINITY, MMAE_EINVAL, "%s: temperature %g is not positive and finite", name, temperature);
@@ -348,7 +795,38 @@ int check_logits(const char* name, const void* logits, int dtype, int outer, int
 
 }  // namespace
 
-extern "C" size_t mmae_class_log_probs_workspace_bytes(int outer, int classes, int inner, int top_k) { return 0; }
+// Tiles of the row kernels: 32 elements a thread; one wave up to 2048 classes, four beyond.
+constexpr int SHORT_ROW = 2048, ROW_TILE = 8192;
+// Workgroups a row is split into: enough for every CU to hold eight, at least a tile each.
+static int row_slices(int rows, int classes) {
+    if (classes <= SHORT_ROW) return 1;
+    const int tiles = (classes + ROW_TILE - 1) / ROW_TILE, want = (2048 + rows - 1) / rows;
+    int n = want < tiles ? want : tiles;
+    if (n > MAX_SLICES) n = MAX_SLICES;
+    const int per = (tiles + n - 1) / n;
+    return (tiles + per - 1) / per;  // (no slice is empty)
+}
+
+extern "C" size_t mmae_class_log_probs_workspace_bytes(int outer, int classes, int inner, int top_k) {
+    if (inner != 1 || outer < 1 || top_k < 0) return 0;
+    const int n = row_slices(outer, classes);
+    return n == 1 ? 0 : (size_t)outer * n * slice_bytes(top_k);
+}
+
+template <class T>
+static void launch_log_probs_rows(const LogProbArgs& a, void* workspace, hipStream_t stream) {
+    constexpr int NV = 32 / T::VEC;
+    const int rows = a.g.outer, n = row_slices(rows, a.g.classes);
+#define ROWS(NT, TOP, tiles) hipLaunchKernelGGL((log_probs_rows_kernel<T, NT, NV, TOP>), dim3((unsigned)rows * n), dim3(NT), 0, stream, a, n, tiles, (char*)workspace)
+    if (a.g.classes <= SHORT_ROW) {
+        if (a.k) ROWS(64, true, 1); else ROWS(64, false, 1);
+        return;
+    }
+    const int tiles = (a.g.classes + ROW_TILE - 1) / ROW_TILE, per = (tiles + n - 1) / n;
+    if (a.k) ROWS(256, true, per); else ROWS(256, false, per);
+#undef ROWS
+    if (n > 1) hipLaunchKernelGGL(log_probs_join_kernel<T>, dim3(rows), dim3(64), sizeof(uint64_t) * (size_t)(n + 1) * a.k, stream, a, n, (const char*)workspace);
+}
 
 extern "C" int mmae_class_log_probs(const void* logits, int dtype, int outer, int classes, int inner, long ld, const int64_t* target,
                                     int top_k, float temperature, float* log_prob, float* entropy, float* row_max,
@@ -362,9 +840,17 @@ extern "C" int mmae_class_log_probs(const void* logits, int dtype, int outer, in
                  "class_log_probs: %d top classes of %d (at most %d)", top_k, classes, MAX_TOP);
     LogProbArgs a = {{logits, ld, outer, classes, inner, LOG2E / temperature, 1.f / temperature}, target, top_k, log_prob, entropy, row_max,
                      row_log_sum, top_log_prob, top_class};
-#define CALL(T) hipLaunchKernelGGL(log_probs_kernel<T>, dim3(outer * inner), dim3(256), 0, stream, a)
-    BY_DTYPE(dtype, CALL);
+    MMAE_REQUIRE(workspace_bytes >= mmae_class_log_probs_workspace_bytes(outer, classes, inner, top_k) && (workspace || !workspace_bytes),
+                 MMAE_EWORKSPACE, "class_log_probs: workspace too small");
+    if (inner == 1) {
+#define CALL(T) launch_log_probs_rows<T>(a, workspace, stream)
+        BY_DTYPE(dtype, CALL);
 #undef CALL
+    } else {
+#define CALL(T) hipLaunchKernelGGL(log_probs_kernel<T>, dim3(outer * inner), dim3(256), 0, stream, a)
+        BY_DTYPE(dtype, CALL);
+#undef CALL
+    }
     MMAE_CHECK_LAUNCH("class_log_probs");
     return MMAE_OK;
 }
@@ -378,9 +864,19 @@ extern "C" int mmae_class_log_probs_bwd(const void* logits, int dtype, int outer
     MMAE_REQUIRE(target && entropy && row_max && row_log_sum && d_logits, MMAE_EINVAL, "class_log_probs_bwd: null pointer");
     LogProbBwdArgs a = {{logits, ld, outer, classes, inner, LOG2E / temperature, 1.f / temperature}, target, entropy, row_max, row_log_sum,
                         d_log_prob, d_entropy, d_logits};
-#define CALL(T) hipLaunchKernelGGL(log_probs_bwd_kernel<T>, dim3(outer * inner), dim3(256), 0, stream, a)
-    BY_DTYPE(dtype, CALL);
+    if (inner == 1) {
+        const int tile = classes <= SHORT_ROW ? SHORT_ROW : ROW_TILE, tiles = (classes + tile - 1) / tile;
+        MMAE_REQUIRE((long)outer * tiles <= 0x7fffffffL, MMAE_ESHAPE, "class_log_probs_bwd: %d rows of %d classes", outer, classes);
+#define CALL(T)                                                                                                                   \
+    if (classes <= SHORT_ROW) hipLaunchKernelGGL((log_probs_bwd_rows_kernel<T, 64, 32 / T::VEC>), dim3((unsigned)outer * tiles), dim3(64), 0, stream, a, tiles); \
+    else hipLaunchKernelGGL((log_probs_bwd_rows_kernel<T, 256, 32 / T::VEC>), dim3((unsigned)outer * tiles), dim3(256), 0, stream, a, tiles)
+        BY_DTYPE(dtype, CALL);
 #undef CALL
+    } else {
+#define CALL(T) hipLaunchKernelGGL(log_probs_bwd_kernel<T>, dim3(outer * inner), dim3(256), 0, stream, a)
+        BY_DTYPE(dtype, CALL);
+#undef CALL
+    }
     MMAE_CHECK_LAUNCH("class_log_probs_bwd");
     return MMAE_OK;
 }
