@@ -651,7 +651,7 @@ __device__ __forceinline__ float position_weight(const DistillArgs& a, long p) {
     const int b = (int)(p / a.g.inner), i = (int)(p % a.g.inner);
     const int tok = a.tokens == 1 ? 0 : (i / a.W / a.patch) * a.tok_w + (i % a.W) / a.patch;
     if (a.mask[(long)b * a.tokens + tok] == 0) return 0.f;
-    return a.temperature * a.temperature / (a.count[b] * (float)(a.patch * a.patch) * a.valid[0]);
+    return a.temperature * a.temperature / ((a.tokens == 1 ? 1.f : a.count[b]) * (float)(a.patch * a.patch) * a.valid[0]);
 }
 
 // One wave: lane i < k holds kept class i; returns class (-1 for padding), q, log q and the totals over the wave.
@@ -685,24 +685,17 @@ __device__ __forceinline__ Kept load_kept(const DistillArgs& a, long p, int lane
     return e;
 }
 
-template <class T>
-__global__ __launch_bounds__(256) void distill_kernel(DistillArgs a) {
-    __shared__ Stats red[4];
-    __shared__ int s_cls[MAX_TOP];
-    __shared__ float s_q[MAX_TOP], s_l[1], s_tot[2];
-    if (a.upstream && a.skip_unit && a.upstream[0] == 1.f) return;
+// One position, any layout, by a whole workgroup: class after class from memory, differences (z - m) c.
+template <class T, int NT>
+__device__ void distill_position(const DistillArgs& a, long p, float w, Stats* red, int* s_cls, float* s_q, float* s_tot) {
     const typename T::E* z = (const typename T::E*)a.g.logits;
-    const long p = blockIdx.x, base = a.g.base(p), cs = a.g.inner;
+    const long base = a.g.base(p), cs = a.g.inner;
     const int C = a.g.classes, lane = threadIdx.x & 63;
-    const float c = a.g.c, w = position_weight(a, p);
+    const float c = a.g.c;
     typename T::E* dz = (typename T::E*)a.d_logits;
     const long out = a.g.inner == 1 ? p * C : (p / a.g.inner) * C * cs + p % a.g.inner;
-    if (w == 0.f) {
-        if (dz) for (int j = threadIdx.x; j < C; j += 256) dz[out + j * cs] = T::down(0.f);
-        if (threadIdx.x == 0 && a.part) a.part[p] = 0.f;
-        return;
-    }
     Kept e = {};
+    __syncthreads();
     if (threadIdx.x < 64) {
         e = load_kept(a, p, lane);
         s_cls[lane] = e.cls;
@@ -711,7 +704,7 @@ __global__ __launch_bounds__(256) void distill_kernel(DistillArgs a) {
     }
     __syncthreads();
     Stats v = {-INFINITY, 0.f, 0.f}, u = {-INFINITY, 0.f, 0.f};  // all classes; the ones not kept
-    for (int j = threadIdx.x; j < C; j += 256) {
+    for (int j = threadIdx.x; j < C; j += NT) {
         const float x = T::up(z[base + j * cs]);
         bool kept = !a.log_probs;
         for (int i = 0; i < a.k && !kept; ++i) kept = s_cls[i] == j;
@@ -733,7 +726,7 @@ __global__ __launch_bounds__(256) void distill_kernel(DistillArgs a) {
     }
     if (!dz) return;
     const float gs = empty ? 0.f : w * a.g.inv_t * (a.upstream ? a.upstream[0] : 1.f);
-    for (int j = threadIdx.x; j < C; j += 256) {
+    for (int j = threadIdx.x; j < C; j += NT) {
         const float x = T::up(z[base + j * cs]);
         float q = 0.f;
         bool kept = false;
@@ -745,7 +738,299 @@ __global__ __launch_bounds__(256) void distill_kernel(DistillArgs a) {
     }
 }
 
-// Masked tokens per sample; then the number of samples that have any.
+template <class T>
+__global__ __launch_bounds__(256) void distill_kernel(DistillArgs a) {
+    __shared__ Stats red[4];
+    __shared__ int s_cls[MAX_TOP];
+    __shared__ float s_q[MAX_TOP], s_tot[2];
+    if (a.upstream && a.skip_unit && a.upstream[0] == 1.f) return;
+    const long p = blockIdx.x, cs = a.g.inner;
+    const float w = position_weight(a, p);
+    if (w == 0.f) {
+        typename T::E* dz = (typename T::E*)a.d_logits + (p / cs) * a.g.classes * cs + p % cs;
+        if (a.d_logits) for (int j = threadIdx.x; j < a.g.classes; j += 256) dz[j * cs] = T::down(0.f);
+        if (threadIdx.x == 0 && a.part) a.part[p] = 0.f;
+        return;
+    }
+    distill_position<T, 256>(a, p, w, red, s_cls, s_q, s_tot);
+}
+
+// ---- distillation of rows -------------------------------------------------------------------------------------------
+// The sums over a row leave the kept classes out (their logits become -inf in the registers); what they add comes from their
+// k logits.  So P, the mass outside, is a sum of its own and not a difference, and the gradient of every other class is one
+// factor F times its exponential:  gs (Q 2^(R' - R) / s - r / s'),  s' and R' the sums outside, s and R those of the whole row.
+struct KeptLane {  // what one wave knows of its lane's kept class
+    Kept e;
+    float z;         // the student's logit
+    float q_class;   // the class's whole share of q (it may be listed twice)
+    bool first;      // no earlier lane lists the class
+};
+template <class T>
+__device__ __forceinline__ KeptLane load_kept_lane(const DistillArgs& a, long p, const typename T::E* z, int lane) {
+    KeptLane l;
+    l.e = load_kept(a, p, lane);
+    l.z = l.e.cls >= 0 ? T::up(z[l.e.cls]) : -INFINITY;
+    l.q_class = 0.f;
+    l.first = l.e.cls >= 0;
+    for (int i = 0; i < a.k; ++i) {
+        const int cls = __shfl(l.e.cls, i, 64);
+        const float q = __shfl(l.e.q, i, 64);
+        if (cls == l.e.cls) {
+            l.q_class += q;
+            if (i < lane) l.first = false;
+        }
+    }
+    return l;
+}
+
+struct RowResult { Sums all; float factor, ref; };  // factor F, R'
+// One wave: the row from the sums outside the kept classes.  Writes the row's loss, returns the lane's class gradient in d.
+template <class T>
+__device__ __forceinline__ RowResult join_row(const DistillArgs& a, long p, float w, const KeptLane& l, const Sums& rest, float& d, int lane, bool write) {
+    const float c = a.g.c;
+    Sums v = {-INFINITY, -FAR, 0.f, 0.f};
+    if (l.first) {
+        v.m = l.z == l.z ? l.z : -INFINITY;
+        v.R = reference_exponent(v.m, c);
+        v.s = exp2_(__builtin_fmaf(l.z, c, -v.R));
+    }
+    v = join(wave_sums(v), rest);
+    if (v.m == INFINITY) v.s = __builtin_nanf("");
+    const bool empty = v.m == -INFINITY && v.s == 0.f;
+    const float l2 = empty ? INFINITY : log2_(v.s);
+    const float r = rest.s != 0.f ? l.e.rest : 0.f, Q = l.e.total + r;
+    const float gs = empty ? 0.f : w * a.g.inv_t * (a.upstream ? a.upstream[0] : 1.f);
+    if (write && a.part) {
+        float x = l.e.q != 0.f ? l.e.q * (l.e.lq - row_log_p(a.g, l.z, v.m, l2)) : 0.f;
+        x = wave_sum(x);
+        if (r != 0.f) x += r * (log2_(r) - ((rest.R - v.R) + log2_(rest.s) - l2)) * LN2;
+        if (lane == 0) a.part[p] = w * x;
+    }
+    d = gs * (exp2_(__builtin_fmaf(l.z, c, -v.R) - l2) * Q - l.q_class);
+    return {v, gs * (Q * exp2_(rest.R - v.R - l2) - (r != 0.f ? r / rest.s : 0.f)), rest.R};
+}
+
+template <class T, int NT>
+__device__ __forceinline__ void zero_row(typename T::E* dz, int first, int end) {
+    for (int j = first + (int)threadIdx.x * T::VEC; j < end; j += NT * T::VEC) {
+        if (j + T::VEC <= end) store_piece<T>(dz + j, Piece{});
+        else for (int e = j; e < end; ++e) dz[e] = T::down(0.f);
+    }
+}
+
+template <class T, int NT, int NV>
+__device__ __forceinline__ Sums tile_sums(const Piece (&q)[NV], float c) {  // one thread's
+    Sums v = {T::get(q[0], 0), 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+#pragma unroll
+        for (int e = 0; e < T::VEC; ++e) v.m = fmaxf(v.m, T::get(q[i], e));
+    if (v.m != v.m) v.m = -INFINITY;
+    v.R = reference_exponent(v.m, c);
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+        float s = 0.f;
+#pragma unroll
+        for (int e = 0; e < T::VEC; ++e) s += exp2_(__builtin_fmaf(T::get(q[i], e), c, -v.R));
+        v.s += s;
+    }
+    return v;
+}
+
+// A row held in the registers of one workgroup: read once, its gradient written once.
+template <class T, int NT, int NV>
+__global__ __launch_bounds__(NT) void distill_rows_kernel(DistillArgs a) {
+    constexpr int VEC = T::VEC;
+    __shared__ __align__(16) uint32_t flags[NT * NV / 4];  // a byte per piece: which of its elements are kept classes
+    __shared__ Sums red[NT / 64];
+    __shared__ Stats red_far[NT / 64];
+    __shared__ int s_cls[MAX_TOP];
+    __shared__ float s_d[MAX_TOP], s_row[4];
+    if (a.upstream && a.skip_unit && a.upstream[0] == 1.f) return;
+    const long p = blockIdx.x;
+    const int C = a.g.classes, lane = threadIdx.x & 63;
+    const typename T::E* z = (const typename T::E*)a.g.logits + p * a.g.ld;
+    typename T::E* dz = (typename T::E*)a.d_logits + p * C;
+    const float w = position_weight(a, p), c = a.g.c;
+    if (w == 0.f) {
+        if (a.d_logits) zero_row<T, NT>(dz, 0, C);
+        if (threadIdx.x == 0 && a.part) a.part[p] = 0.f;
+        return;
+    }
+    Piece q[NV];
+    load_tile<T, NT, NV>(q, z, 0, C);
+    for (int i = threadIdx.x; i < NT * NV / 4; i += NT) flags[i] = 0;
+    __syncthreads();
+    KeptLane l;
+    if (threadIdx.x < 64) {
+        l = load_kept_lane<T>(a, p, z, lane);
+        s_cls[lane] = l.e.cls;
+        if (l.e.cls >= 0) atomicOr(&flags[l.e.cls / VEC / 4], 1u << (l.e.cls / VEC % 4 * 8 + l.e.cls % VEC));
+    }
+    __syncthreads();
+    const uint8_t* flag = (const uint8_t*)flags;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+        const uint32_t f = flag[i * NT + threadIdx.x];
+        if (f) {
+#pragma unroll
+            for (int e = 0; e < VEC; ++e)
+                if (f >> e & 1) T::put(q[i], e, -INFINITY);
+        }
+    }
+    const Sums rest = block_sums<NT>(tile_sums<T, NT, NV>(q, c), red);
+    if (threadIdx.x < 64) {
+        float d;
+        const RowResult row = join_row<T>(a, p, w, l, rest, d, lane, true);
+        s_d[lane] = d;
+        if (lane == 0) { s_row[0] = row.factor; s_row[1] = row.ref; s_row[2] = row.all.m; }
+    }
+    __syncthreads();
+    if (is_far(s_row[2], c)) {
+        distill_position<T, NT>(a, p, w, red_far, s_cls, s_d, s_row);
+        return;
+    }
+    if (!a.d_logits) return;
+    const float F = s_row[0], R = s_row[1];
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+        const int j = (i * NT + threadIdx.x) * VEC;
+        if (j >= C) break;
+        float o[VEC];
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) o[e] = F * exp2_(__builtin_fmaf(T::get(q[i], e), c, -R));
+        const uint32_t f = flag[i * NT + threadIdx.x];
+        if (f)
+            for (int k = 0; k < a.k; ++k) {
+                const int at = s_cls[k] - j;
+#pragma unroll
+                for (int e = 0; e < VEC; ++e) o[e] = at == e ? s_d[k] : o[e];
+            }
+        if (j + VEC <= C) {
+            store_piece<T>(dz + j, T::pack(o));
+        } else {
+#pragma unroll
+            for (int e = 0; e < VEC; ++e)
+                if (j + e < C) dz[j + e] = T::down(o[e]);
+        }
+    }
+}
+
+// Calls put(i, e, lane) for every kept class inside a tile: lane holds the class, i and e name the piece and element of the
+// thread that is asked about.  Uniform over the wave but for `mine`.
+template <class T, int NT, int NV, class F>
+__device__ __forceinline__ void each_kept(int cls, int base, int end, F put) {
+    uint64_t in = __ballot(cls >= base && cls < end && cls < base + NT * NV * T::VEC);
+    while (in) {
+        const int k = __builtin_ctzll(in);
+        in &= in - 1;
+        const int off = __shfl(cls, k, 64) - base, piece = off / T::VEC;
+        if (piece % NT == (int)threadIdx.x) put(piece / NT, off % T::VEC, k);
+    }
+}
+
+// Few or long rows, first pass: the sums outside the kept classes, a slice per workgroup.
+template <class T, int NT, int NV>
+__global__ __launch_bounds__(NT) void distill_slices_kernel(DistillArgs a, int slices, int slice_tiles, Sums* parts) {
+    constexpr int VEC = T::VEC, TILE = NT * NV * VEC;
+    __shared__ Sums red[NT / 64];
+    if (a.upstream && a.skip_unit && a.upstream[0] == 1.f) return;
+    const long p = blockIdx.x / slices;
+    if (position_weight(a, p) == 0.f) return;
+    const int C = a.g.classes, lane = threadIdx.x & 63, first = blockIdx.x % slices * slice_tiles * TILE;
+    const int end = first + slice_tiles * TILE < C ? first + slice_tiles * TILE : C;
+    const typename T::E* z = (const typename T::E*)a.g.logits + p * a.g.ld;
+    const long cls64 = lane < a.k ? load_class(a.top_class, a.class_bytes, p * a.k + lane) : -1;
+    const int cls = cls64 >= 0 && cls64 < C ? (int)cls64 : -1;
+    Sums v = {-INFINITY, -FAR, 0.f, 0.f};
+    Piece q[NV], next[NV];
+    load_tile<T, NT, NV>(q, z, first, end);
+    for (int base = first;;) {
+        const bool more = base + TILE < end;
+        if (more) load_tile<T, NT, NV>(next, z, base + TILE, end);
+        each_kept<T, NT, NV>(cls, base, end, [&](int pi, int pe, int) {
+#pragma unroll
+            for (int i = 0; i < NV; ++i)
+#pragma unroll
+                for (int e = 0; e < VEC; ++e)
+                    if (i == pi && e == pe) T::put(q[i], e, -INFINITY);
+        });
+        v = join(v, tile_sums<T, NT, NV>(q, a.g.c));
+        if (!more) break;
+        base += TILE;
+#pragma unroll
+        for (int i = 0; i < NV; ++i) q[i] = next[i];
+    }
+    v = block_sums<NT>(v, red);
+    if (threadIdx.x == 0) parts[blockIdx.x] = v;
+}
+
+// Second pass: the gradient, a tile per workgroup; the first tile's workgroup writes the row's loss.
+template <class T, int NT, int NV>
+__global__ __launch_bounds__(NT) void distill_tiles_kernel(DistillArgs a, int tiles, int slices, const Sums* parts) {
+    constexpr int VEC = T::VEC, TILE = NT * NV * VEC;
+    __shared__ Stats red_far[NT / 64];
+    __shared__ int s_cls[MAX_TOP];
+    __shared__ float s_d[MAX_TOP], s_row[4];
+    if (a.upstream && a.skip_unit && a.upstream[0] == 1.f) return;
+    const long p = blockIdx.x / tiles;
+    const int tile = blockIdx.x % tiles, base = tile * TILE, C = a.g.classes, lane = threadIdx.x & 63;
+    const typename T::E* z = (const typename T::E*)a.g.logits + p * a.g.ld;
+    typename T::E* dz = (typename T::E*)a.d_logits + p * C;
+    const float w = position_weight(a, p), c = a.g.c;
+    if (w == 0.f) {
+        if (a.d_logits) zero_row<T, NT>(dz, base, base + TILE < C ? base + TILE : C);
+        if (tile == 0 && threadIdx.x == 0 && a.part) a.part[p] = 0.f;
+        return;
+    }
+    Piece q[NV];
+    if (a.d_logits) load_tile<T, NT, NV>(q, z, base, C);
+    if (threadIdx.x < 64) {
+        Sums rest = {-INFINITY, -FAR, 0.f, 0.f};
+        if (lane < slices) rest = parts[p * slices + lane];
+        rest = wave_sums(rest);
+        const KeptLane l = load_kept_lane<T>(a, p, z, lane);
+        float d;
+        const RowResult row = join_row<T>(a, p, w, l, rest, d, lane, tile == 0);
+        s_cls[lane] = l.e.cls;
+        s_d[lane] = d;
+        if (lane == 0) { s_row[0] = row.factor; s_row[1] = row.ref; s_row[2] = row.all.m; }
+    }
+    __syncthreads();
+    if (is_far(s_row[2], c)) {
+        if (tile == 0) distill_position<T, NT>(a, p, w, red_far, s_cls, s_d, s_row);
+        return;
+    }
+    if (!a.d_logits) return;
+    const float F = s_row[0], R = s_row[1];
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+        float o[VEC];
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) o[e] = F * exp2_(__builtin_fmaf(T::get(q[i], e), c, -R));
+        q[i] = T::pack(o);
+    }
+    each_kept<T, NT, NV>(s_cls[lane], base, C, [&](int pi, int pe, int k) {
+#pragma unroll
+        for (int i = 0; i < NV; ++i)
+#pragma unroll
+            for (int e = 0; e < VEC; ++e)
+                if (i == pi && e == pe) T::put(q[i], e, s_d[k]);
+    });
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+        const int j = base + (i * NT + threadIdx.x) * VEC;
+        if (j + VEC <= C) {
+            store_piece<T>(dz + j, q[i]);
+        } else {
+#pragma unroll
+            for (int e = 0; e < VEC; ++e)
+                if (j + e < C) dz[j + e] = T::down(T::get(q[i], e));
+        }
+    }
+}
+
+// Masked tokens per sample; then the number of samples that have any (of rows, and of samples of one token: from the mask).
 __global__ __launch_bounds__(64) void distill_count_kernel(const int64_t* mask, int outer, int tokens, float* count) {
     const int b = blockIdx.x;
     int n = 0;
@@ -753,10 +1038,10 @@ __global__ __launch_bounds__(64) void distill_count_kernel(const int64_t* mask, 
     const float s = wave_sum((float)n);
     if (threadIdx.x == 0) count[b] = s;
 }
-__global__ __launch_bounds__(1024) void distill_valid_kernel(const float* count, int outer, float* valid) {
+__global__ __launch_bounds__(1024) void distill_valid_kernel(const float* count, const int64_t* mask, int outer, float* valid) {
     __shared__ float red[16];
-    float n = 0.f;
-    for (int b = threadIdx.x; b < outer; b += 1024) n += count[b] > 0.f ? 1.f : 0.f;
+    float n = 0.f;  // (whole numbers: exact in any order up to 2^24 per thread)
+    for (int b = threadIdx.x; b < outer; b += 1024) n += (mask ? mask[b] != 0 : count[b] > 0.f) ? 1.f : 0.f;
     n = block_sum(n, red);
     if (threadIdx.x == 0) valid[0] = n;
 }
@@ -881,8 +1166,40 @@ extern "C" int mmae_class_log_probs_bwd(const void* logits, int dtype, int outer
     return MMAE_OK;
 }
 
+// Rows held in registers where a workgroup takes them; in two passes over slices where there are too few rows for the card or
+// they are longer.
+template <class T> constexpr int longest_held_row() { return T::VEC == 8 ? 131072 : 65536; }
+static bool held_rows(int rows, int classes, int dtype) {
+    if (classes <= ROW_TILE) return true;
+    return rows >= 256 && classes <= (dtype == MMAE_DT_F32 ? longest_held_row<F32>() : longest_held_row<B16>());
+}
+static size_t distill_floats(int outer, int inner) { return (4 + (size_t)outer + (size_t)outer * inner + 3) / 4 * 4; }
+
 extern "C" size_t mmae_distill_workspace_bytes(int outer, int classes, int inner, int k) {
-    return sizeof(float) * (4 + (size_t)outer + (size_t)outer * inner);
+    if (outer < 1 || inner < 1) return 0;
+    const size_t parts = inner == 1 ? sizeof(Sums) * (size_t)outer * row_slices(outer, classes) : 0;
+    return sizeof(float) * distill_floats(outer, inner) + parts;
+}
+
+template <class T>
+static void launch_distill_rows(const DistillArgs& a, int dtype, Sums* parts, hipStream_t stream) {
+    const int rows = a.g.outer, C = a.g.classes;
+    constexpr int V = T::VEC;
+#define HELD(NT, EPT) hipLaunchKernelGGL((distill_rows_kernel<T, NT, EPT / V>), dim3(rows), dim3(NT), 0, stream, a)
+    if (held_rows(rows, C, dtype)) {
+        if (C <= 2048) HELD(64, 32);
+        else if (C <= 8192) HELD(256, 32);
+        else if (C <= 16384) HELD(512, 32);
+        else if (C <= 32768) HELD(1024, 32);
+        else if (C <= 65536) HELD(1024, 64);
+        else if constexpr (V == 8) HELD(1024, 128);
+        return;
+    }
+#undef HELD
+    const int tiles = (C + ROW_TILE - 1) / ROW_TILE, n = row_slices(rows, C), per = (tiles + n - 1) / n;
+    hipLaunchKernelGGL((distill_slices_kernel<T, 256, 32 / V>), dim3((unsigned)rows * n), dim3(256), 0, stream, a, n, per, parts);
+    hipLaunchKernelGGL((distill_tiles_kernel<T, 256, 32 / V>), dim3((unsigned)rows * (a.d_logits ? tiles : 1)), dim3(256), 0, stream, a,
+                       a.d_logits ? tiles : 1, n, (const Sums*)parts);
 }
 
 extern "C" int mmae_distill(const void* logits, int dtype, int outer, int classes, int inner, long ld, const void* top_class,
@@ -909,14 +1226,24 @@ extern "C" int mmae_distill(const void* logits, int dtype, int outer, int classe
     a.valid = ws; a.count = ws + 4; a.part = loss ? ws + 4 + outer : nullptr;
     a.upstream = upstream; a.skip_unit = skip_unit; a.d_logits = d_logits;
     if (mask) {
-        hipLaunchKernelGGL(distill_count_kernel, dim3(outer), dim3(64), 0, stream, mask, outer, a.tokens, ws + 4);
-        MMAE_CHECK_LAUNCH("distill_count");
-        hipLaunchKernelGGL(distill_valid_kernel, dim3(1), dim3(1024), 0, stream, ws + 4, outer, ws);
+        if (a.tokens > 1) {
+            hipLaunchKernelGGL(distill_count_kernel, dim3(outer), dim3(64), 0, stream, mask, outer, a.tokens, ws + 4);
+            MMAE_CHECK_LAUNCH("distill_count");
+        }
+        hipLaunchKernelGGL(distill_valid_kernel, dim3(1), dim3(1024), 0, stream, ws + 4, a.tokens > 1 ? nullptr : mask, outer, ws);
         MMAE_CHECK_LAUNCH("distill_valid");
     }
-#define CALL(T) hipLaunchKernelGGL(distill_kernel<T>, dim3(outer * inner), dim3(256), 0, stream, a)
-    BY_DTYPE(dtype, CALL);
+    if (inner == 1) {
+        MMAE_REQUIRE((long)outer * ((classes + ROW_TILE - 1) / ROW_TILE) <= 0x7fffffffL, MMAE_ESHAPE, "distill: %d rows of %d classes", outer, classes);
+        Sums* parts = (Sums*)(ws + distill_floats(outer, inner));
+#define CALL(T) launch_distill_rows<T>(a, dtype, parts, stream)
+        BY_DTYPE(dtype, CALL);
 #undef CALL
+    } else {
+#define CALL(T) hipLaunchKernelGGL(distill_kernel<T>, dim3(outer * inner), dim3(256), 0, stream, a)
+        BY_DTYPE(dtype, CALL);
+#undef CALL
+    }
     MMAE_CHECK_LAUNCH("distill");
     if (loss) {
         hipLaunchKernelGGL(distill_sum_kernel, dim3(1), dim3(1024), 0, stream, a.part, (long)outer * inner, loss);
