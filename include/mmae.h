@@ -281,7 +281,7 @@ int mmae_masked_ce(const void* logits, int logits_is_bf16, const int64_t* target
  *
  * mmae_class_log_probs: log_prob = log softmax(x)[target] (0 where target is outside [0, classes), e.g. -100), entropy of
  * softmax(x), and the top_k (<= 64, <= classes) classes by z with their log probabilities: descending, equal values by the
- * lower class, NaN first.  row_max / row_log_sum: what the backward pass needs.  A position whose logits are all -inf
+ * lower class, NaN as +inf.  row_max / row_log_sum: what the backward pass needs.  A position whose logits are all -inf
  * has log_prob = -inf (at a valid target), entropy 0 and no gradient.  NaN and +inf logits give NaN, as in torch.
  * mmae_class_log_probs_bwd: d_logits (contiguous, the logits' dtype) for the gradients that arrive at log_prob and entropy
  * (either may be NULL). */
@@ -302,7 +302,7 @@ int mmae_class_log_probs_bwd(const void* logits, int dtype, int outer, int class
  * mean over all positions.  loss (f32 scalar) or d_logits (contiguous, the logits' dtype: the loss's gradient times
  * *upstream, a device scalar, or times 1 if NULL) may be NULL, not both.  skip_unit: leave everything as it is where
  * *upstream is 1. */
-size_t mmae_distill_workspace_bytes(int outer, int classes, int inner, int k);
+size_t mmae_distill_workspace_bytes(int dtype, int outer, int classes, int inner, int k);
 int mmae_distill(const void* logits, int dtype, int outer, int classes, int inner, long ld, const void* top_class,
                  int class_bytes, const void* top_value, int value_dtype, int k, int kind, float temperature,
                  const int64_t* mask, int width, int patch, const float* upstream, int skip_unit, float* loss, void* d_logits,

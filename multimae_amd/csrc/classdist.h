@@ -1,0 +1,322 @@
+// Class distributions: log probabilities of given classes with entropy and top alternatives (forward and backward), and
+// distillation from a teacher's top classes (loss and gradient).
+//
+// logits hold `outer` samples of `classes` x `inner` values: class j of position (b, i) is at b * ld + j * inner + i, so
+// rows [N, C] are inner = 1 and class maps [B, C, H, W] are inner = H * W.  With x = z / T, m = max x, s = sum exp(x - m):
+//   log p_j = x_j - m - log s,   H = -sum p_j log p_j (terms of p = 0 are 0)
+//   d/dz_j (gl log p_y + gh H) = (gl ([j = y] - p_j) - gh p_j (log p_j + H)) / T
+// Everything between the loads and the stores is fp32; exponentials are taken of differences (z - m) * log2(e) / T, formed
+// before scaling, so that logits of the type's lowest value (a mask) stay finite differences where a whole row has them.
+#pragma once
+#include "common.h"
+
+#include <math.h>
+
+namespace classdist {
+
+constexpr int MAX_TOP = 64;  // classes a call ranks or takes: one lane of a wave each
+constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
+
+typedef _Float16 f16;
+
+// 16 bytes of a row: VEC elements.  Loads and stores take any alignment of the element type.
+struct __attribute__((may_alias)) Piece { uint32_t w[4]; };
+// KEY_BITS: leading bits of ordered(v) that tell all values of the type apart
+struct F32 {
+    typedef float E;
+    static constexpr int VEC = 4, KEY_BITS = 32;
+    static constexpr uint32_t NEG_INF = 0xff800000u;  // as a word of a piece
+    static __device__ __forceinline__ float up(float v) { return v; }
+    static __device__ __forceinline__ float down(float v) { return v; }
+    static __device__ __forceinline__ float get(const Piece& q, int e) { return __uint_as_float(q.w[e]); }
+    static __device__ __forceinline__ void put(Piece& q, int e, float v) { q.w[e] = __float_as_uint(v); }
+    static __device__ __forceinline__ Piece pack(const float (&v)[4]) { return {__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3])}; }
+};
+struct B16 {
+    typedef bf16 E;
+    static constexpr int VEC = 8, KEY_BITS = 16;
+    static constexpr uint32_t NEG_INF = 0xff80ff80u;
+    static __device__ __forceinline__ float up(bf16 v) { return (float)v; }
+    static __device__ __forceinline__ bf16 down(float v) { return (bf16)v; }
+    static __device__ __forceinline__ float get(const Piece& q, int e) { return __uint_as_float(e & 1 ? q.w[e >> 1] & 0xffff0000u : q.w[e >> 1] << 16); }
+    static __device__ __forceinline__ void put(Piece& q, int e, float v) {
+        const uint32_t b = __builtin_bit_cast(uint16_t, (bf16)v);
+        q.w[e >> 1] = e & 1 ? (q.w[e >> 1] & 0xffffu) | b << 16 : (q.w[e >> 1] & 0xffff0000u) | b;
+    }
+    static __device__ __forceinline__ Piece pack(const float (&v)[8]) {
+        typedef __attribute__((ext_vector_type(8))) bf16 V;
+        V r;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) r[e] = (bf16)v[e];
+        return __builtin_bit_cast(Piece, r);
+    }
+};
+struct H16 {
+    typedef f16 E;
+    static constexpr int VEC = 8, KEY_BITS = 20;  // sign, 8 exponent bits of fp32, 10 mantissa bits (and one spare)
+    static constexpr uint32_t NEG_INF = 0xfc00fc00u;
+    static __device__ __forceinline__ float up(f16 v) { return (float)v; }
+    static __device__ __forceinline__ f16 down(float v) { return (f16)v; }
+    static __device__ __forceinline__ float get(const Piece& q, int e) {
+        return (float)__builtin_bit_cast(f16, (uint16_t)(e & 1 ? q.w[e >> 1] >> 16 : q.w[e >> 1]));
+    }
+    static __device__ __forceinline__ void put(Piece& q, int e, float v) {
+        const uint32_t b = __builtin_bit_cast(uint16_t, (f16)v);
+        q.w[e >> 1] = e & 1 ? (q.w[e >> 1] & 0xffffu) | b << 16 : (q.w[e >> 1] & 0xffff0000u) | b;
+    }
+    static __device__ __forceinline__ Piece pack(const float (&v)[8]) {
+        typedef __attribute__((ext_vector_type(8))) f16 V;
+        V r;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) r[e] = (f16)v[e];
+        return __builtin_bit_cast(Piece, r);
+    }
+};
+template <class T> __device__ __forceinline__ Piece load_piece(const typename T::E* p) {
+    Piece q;
+    __builtin_memcpy(&q, p, 16);
+    return q;
+}
+template <class T> __device__ __forceinline__ void store_piece(typename T::E* p, const Piece& q) { __builtin_memcpy(p, &q, 16); }
+
+__device__ __forceinline__ float exp2_(float v) { return __builtin_amdgcn_exp2f(v); }
+__device__ __forceinline__ float log2_(float v) { return __builtin_amdgcn_logf(v); }
+
+// Rank of (value, class) as one integer: larger first, NaN as +inf, -0 = +0, equal values by the lower class.
+__device__ __forceinline__ uint32_t ordered(float v) {
+    const uint32_t b = __float_as_uint(v + 0.0f);
+    if (v != v) return 0xff800000u;
+    return b ^ ((uint32_t)((int32_t)b >> 31) | 0x80000000u);
+}
+__device__ __forceinline__ uint64_t rank_key(float v, uint32_t cls) { return (uint64_t)ordered(v) << 32 | (0xffffffffu - cls); }
+__device__ __forceinline__ float key_value(uint64_t key) {
+    const uint32_t u = (uint32_t)(key >> 32);
+    return __uint_as_float(u & 0x80000000u ? u ^ 0x80000000u : ~u);
+}
+__device__ __forceinline__ uint32_t key_class(uint64_t key) { return 0xffffffffu - (uint32_t)key; }
+
+__device__ __forceinline__ float load_any(const void* p, int dtype, long i) {
+    if (dtype == MMAE_DT_F32) return ((const float*)p)[i];
+    if (dtype == MMAE_DT_BF16) return (float)((const bf16*)p)[i];
+    return (float)((const f16*)p)[i];
+}
+__device__ __forceinline__ long load_class(const void* p, int bytes, long i) {
+    return bytes == 8 ? (long)((const int64_t*)p)[i] : (long)((const int32_t*)p)[i];
+}
+
+// (m, s, t): maximum, sum of 2^d and sum of d 2^d with d = (z - m) * c.  d is bounded below in t, where 0 * -inf would be NaN.
+struct Stats { float m, s, t; };
+__device__ __forceinline__ float finite_ref(float m) { return m == -INFINITY ? 0.f : m; }
+__device__ __forceinline__ float bounded(float d) { return fmaxf(d, -10000.f); }
+__device__ __forceinline__ Stats join(const Stats& a, const Stats& b, float c) {
+    const float m = fmaxf(a.m, b.m), r = finite_ref(m);
+    const float da = (a.m - r) * c, db = (b.m - r) * c;
+    const float fa = exp2_(da), fb = exp2_(db);
+    return {m, a.s * fa + b.s * fb, fa * (a.t + bounded(da) * a.s) + fb * (b.t + bounded(db) * b.s)};
+}
+
+struct Geometry {
+    const void* logits;
+    long ld;
+    int outer, classes, inner;
+    float c, inv_t;  // log2(e) / T, 1 / T
+    // log p of logit z, formed in natural units: a finite lowest logit times log2(e) would leave the range of fp32
+    __device__ __forceinline__ float log_p(float z, float m, float l2) const { return (z - m) * inv_t - l2 * LN2; }
+    __device__ __forceinline__ long base(long p) const { return inner == 1 ? p * ld : (p / inner) * ld + p % inner; }
+};
+
+__device__ Stats block_stats(Stats v, float c, Stats* red) {
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) {
+        const Stats w = {__shfl_xor(v.m, o, 64), __shfl_xor(v.s, o, 64), __shfl_xor(v.t, o, 64)};
+        v = join(v, w, c);
+    }
+    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, nw = (blockDim.x + 63) >> 6;
+    __syncthreads();
+    if (lane == 0) red[w] = v;
+    __syncthreads();
+    Stats r = red[0];
+    for (int i = 1; i < nw; ++i) r = join(r, red[i], c);
+    return r;
+}
+
+// Sums in the base-2 domain against a reference exponent R: s = sum 2^(z c - R), t = sum (z c - R) 2^(z c - R), m = max z.
+// z c - R is one fused multiply-add without intermediate overflow; R = m c, held to +-FAR, is the same rounded number wherever
+// it is used, so its rounding cancels.  Beyond FAR (every class left at the type's lowest value, say) the row's sums are
+// formed anew from (z - m) c.
+constexpr float FAR = 1e38f;
+struct Sums { float m, R, s, t; };
+__device__ __forceinline__ float reference_exponent(float m, float c) { return __builtin_amdgcn_fmed3f(m * c, -FAR, FAR); }
+__device__ __forceinline__ Sums join(const Sums& a, const Sums& b) {
+    const float R = fmaxf(a.R, b.R), da = a.R - R, db = b.R - R, fa = exp2_(da), fb = exp2_(db);
+    return {fmaxf(a.m, b.m), R, a.s * fa + b.s * fb, fa * (a.t + bounded(da) * a.s) + fb * (b.t + bounded(db) * b.s)};
+}
+__device__ __forceinline__ Sums wave_sums(Sums v) {
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) v = join(v, {__shfl_xor(v.m, o, 64), __shfl_xor(v.R, o, 64), __shfl_xor(v.s, o, 64), __shfl_xor(v.t, o, 64)});
+    return v;
+}
+__device__ __forceinline__ bool is_far(float m, float c) { return fabsf(m) < INFINITY && fabsf(m * c) > FAR; }
+
+// log p of one logit, in natural units.  l2 = log2 of the sum (+inf: nothing left).
+__device__ __forceinline__ float row_log_p(const Geometry& g, float z, float m, float l2) {
+    const float d = __builtin_fmaf(z, g.c, -reference_exponent(m, g.c)) - l2;
+    // the lowest finite values leave the base-2 range before they leave the natural one
+    return is_far(m, g.c) || (d == -INFINITY && z != -INFINITY) ? g.log_p(z, m, l2) : d * LN2;
+}
+
+struct LogProbArgs {
+    Geometry g;
+    const int64_t* target;
+    int k;
+    float *log_prob, *entropy, *row_max, *row_log_sum, *top_log_prob;
+    int64_t* top_class;
+};
+
+struct LogProbBwdArgs {
+    Geometry g;
+    const int64_t* target;
+    const float *entropy, *row_max, *row_log_sum, *d_log_prob, *d_entropy;
+    void* d_logits;  // contiguous
+};
+
+// ---- distillation ----------------------------------------------------------------------------------------------------
+// q_i: the teacher's probabilities of the kept classes c_i, from its logits (softmax over the kept ones of value / T) or from
+// its log probabilities (exp value; the rest r = 1 - sum q is one more outcome).  Per position
+//   l = sum_i q_i (log q_i - log p_{c_i})  [+ r (log r - log P), P = the student's probability of all classes not kept]
+//   dl/dx_j = p_j Q - sum_{i: c_i = j} q_i  [- r p_j / P where j is not kept],   Q = sum q [+ r]
+// loss = T^2 * sum_p w_p l_p.  Padding (a class outside [0, C)) is left out; a class listed twice counts twice.  Where no
+// mass is left outside the kept classes (P = 0) the rest's term is left out; a position whose logits are all -inf has no
+// gradient.
+struct DistillArgs {
+    Geometry g;
+    const void *top_class, *top_value;
+    int class_bytes, value_dtype, k, log_probs;
+    const int64_t* mask;
+    int W, patch, tok_w, tokens;  // map geometry of the mask
+    float weight;                 // without a mask: T^2 / positions
+    float temperature;
+    const float *count, *valid;   // with a mask: masked tokens per sample, samples that have any
+    const float* upstream;        // gradient arriving at the loss (device scalar) or NULL
+    int skip_unit;                // do nothing where it is 1
+    float* part;                  // weighted loss per position
+    void* d_logits;
+};
+
+// What one position's loss counts (T^2 included).
+__device__ __forceinline__ float position_weight(const DistillArgs& a, long p) {
+    if (!a.mask) return a.weight;
+    const int b = (int)(p / a.g.inner), i = (int)(p % a.g.inner);
+    const int tok = a.tokens == 1 ? 0 : (i / a.W / a.patch) * a.tok_w + (i % a.W) / a.patch;
+    if (a.mask[(long)b * a.tokens + tok] == 0) return 0.f;
+    return a.temperature * a.temperature / ((a.tokens == 1 ? 1.f : a.count[b]) * (float)(a.patch * a.patch) * a.valid[0]);
+}
+
+// One wave: lane i < k holds kept class i; returns class (-1 for padding), q, log q and the totals over the wave.
+struct Kept { int cls; float q, lq; float total, rest; };
+__device__ __forceinline__ Kept load_kept(const DistillArgs& a, long p, int lane) {
+    const long at = (p / a.g.inner) * a.k * (long)a.g.inner + p % a.g.inner + (long)lane * a.g.inner;
+    Kept e = {-1, 0.f, 0.f, 0.f, 0.f};
+    float v = -INFINITY;
+    if (lane < a.k) {
+        const long cls = load_class(a.top_class, a.class_bytes, at);
+        if (cls >= 0 && cls < a.g.classes) {
+            e.cls = (int)cls;
+            v = load_any(a.top_value, a.value_dtype, at);
+        }
+    }
+    if (a.log_probs) {
+        e.lq = v;
+        e.q = e.cls >= 0 ? expf(v) : 0.f;
+        double t = e.cls >= 0 ? exp((double)v) : 0.0;  // 64 bits: the rest is what a sum near 1 leaves
+#pragma unroll
+        for (int o = 32; o > 0; o >>= 1) t += __shfl_xor(t, o, 64);
+        e.rest = t != t ? (float)t : fmaxf((float)(1.0 - t), 0.f);
+        e.total = (float)t;
+    } else {
+        const float m = finite_ref(wave_max(v)), c = LOG2E * a.g.inv_t;
+        const float d = (v - m) * c, x = e.cls >= 0 ? exp2_(d) : 0.f, s = wave_sum(x);
+        e.q = s > 0.f || s != s ? x / s : 0.f;
+        e.lq = (v - m) * a.g.inv_t - log2_(s) * LN2;
+        e.total = s > 0.f ? 1.f : (s != s ? s : 0.f);
+    }
+    return e;
+}
+
+// One position, any layout, by a whole workgroup: class after class from memory, differences (z - m) c.  Returns its weighted loss
+// (in the first wave).
+template <class T>
+__device__ float distill_position(const DistillArgs& a, long p, float w, Stats* red, int* s_cls, float* s_q, float* s_tot) {
+    const typename T::E* z = (const typename T::E*)a.g.logits;
+    const long base = a.g.base(p), cs = a.g.inner;
+    const int C = a.g.classes, lane = threadIdx.x & 63;
+    const float c = a.g.c;
+    typename T::E* dz = (typename T::E*)a.d_logits;
+    const long out = a.g.inner == 1 ? p * C : (p / a.g.inner) * C * cs + p % a.g.inner;
+    Kept e = {};
+    __syncthreads();
+    if (threadIdx.x < 64) {
+        e = load_kept(a, p, lane);
+        s_cls[lane] = e.cls;
+        s_q[lane] = e.q;
+        if (lane == 0) { s_tot[0] = e.total; s_tot[1] = e.rest; }
+    }
+    __syncthreads();
+    Stats v = {-INFINITY, 0.f, 0.f}, u = {-INFINITY, 0.f, 0.f};  // all classes; the ones not kept
+    for (int j = threadIdx.x; j < C; j += blockDim.x) {
+        const float x = T::up(z[base + j * cs]);
+        bool kept = !a.log_probs;
+        for (int i = 0; i < a.k && !kept; ++i) kept = s_cls[i] == j;
+        v = join(v, Stats{x, x == -INFINITY ? 0.f : 1.f, 0.f}, c);
+        if (!kept) u = join(u, Stats{x, x == -INFINITY ? 0.f : 1.f, 0.f}, c);
+    }
+    v = block_stats(v, c, red);
+    u = block_stats(u, c, red);
+    const bool empty = v.m == -INFINITY && v.s == 0.f;
+    const float m = finite_ref(v.m), l2 = empty ? 0.f : log2_(v.s);
+    const float um = finite_ref(u.m), ul2 = log2_(u.s);
+    const float rest = u.s != 0.f ? s_tot[1] : 0.f, Q = s_tot[0] + rest;
+    float l = 0.f;
+    if (threadIdx.x < 64) {
+        if (e.q != 0.f) l = e.q * (e.lq - a.g.log_p(T::up(z[base + e.cls * cs]), m, l2));
+        l = wave_sum(l);
+        if (rest != 0.f) l += rest * ((log2_(rest) - (ul2 - l2)) * LN2 - (um - m) * a.g.inv_t);
+        l *= w;
+    }
+    if (!dz) return l;
+    const float gs = empty ? 0.f : w * a.g.inv_t * (a.upstream ? a.upstream[0] : 1.f);
+    for (int j = threadIdx.x; j < C; j += blockDim.x) {
+        const float x = T::up(z[base + j * cs]);
+        float q = 0.f;
+        bool kept = false;
+        for (int i = 0; i < a.k; ++i)
+            if (s_cls[i] == j) { q += s_q[i]; kept = true; }
+        float d = exp2_((x - m) * c - l2) * Q - q;
+        if (!kept && rest != 0.f) d -= rest * exp2_((x - um) * c - ul2);
+        dz[out + j * cs] = T::down(gs * d);
+    }
+    return l;
+}
+
+#define BY_DTYPE(dtype, CALL)            \
+    do {                                 \
+        if ((dtype) == MMAE_DT_F32) { CALL(F32); } \
+        else if ((dtype) == MMAE_DT_BF16) { CALL(B16); } \
+        else { CALL(H16); }              \
+    } while (0)
+
+// classdist_rows.hip: rows, inner = 1
+size_t log_probs_rows_workspace(int rows, int classes, int top_k);
+void log_probs_rows(int dtype, const LogProbArgs& a, void* workspace, hipStream_t stream);
+int log_probs_bwd_rows(int dtype, const LogProbBwdArgs& a, hipStream_t stream);
+size_t distill_rows_workspace(int rows, int classes);
+int distill_rows(int dtype, const DistillArgs& a, void* workspace, hipStream_t stream);
+// classdist_maps.hip: maps, inner > 1; *_fits: the classes of 64 positions fit the LDS
+bool log_probs_map_fits(int dtype, int classes, int top_k);
+int log_probs_map(int dtype, const LogProbArgs& a, hipStream_t stream);
+int log_probs_bwd_map(int dtype, const LogProbBwdArgs& a, hipStream_t stream);
+bool distill_map_fits(int dtype, int classes, int k);
+long distill_map_parts(int outer, int inner);
+int distill_map(int dtype, const DistillArgs& a, hipStream_t stream);
+
+}  // namespace classdist

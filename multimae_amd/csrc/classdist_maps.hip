@@ -1,0 +1,582 @@
+// Class distributions over maps [B, C, inner]: the classes of 64 positions in the LDS of a workgroup, a lane per position.
+//
+// A class's 64 positions are 128 or 256 contiguous bytes, read and written in 16-byte pieces; in the LDS class c of position i is
+// tile[c * 64 + i], which every lane reads without a conflict and at any class.  The waves of a workgroup share the classes.
+#include "classdist.h"
+
+namespace classdist {
+namespace {
+
+constexpr int POS = 64;            // positions of a tile: one wave
+constexpr int LDS_BYTES = 160 * 1024;
+constexpr uint32_t NONE = 0xffffffffu;
+
+template <class T>
+__device__ __forceinline__ Piece load_positions(const typename T::E* z, int px, int n) {  // px .. px + VEC of n
+    if (px + T::VEC <= n) return load_piece<T>(z + px);
+    Piece q = {};
+#pragma unroll
+    for (int e = 0; e < T::VEC; ++e)
+        if (px + e < n) T::put(q, e, T::up(z[px + e]));
+    return q;
+}
+template <class T>
+__device__ __forceinline__ void store_positions(typename T::E* z, int px, int n, const Piece& q) {
+    if (px + T::VEC <= n) {
+        store_piece<T>(z + px, q);
+    } else {
+#pragma unroll
+        for (int e = 0; e < T::VEC; ++e)
+            if (px + e < n) z[px + e] = T::down(T::get(q, e));
+    }
+}
+
+// z: the tile's first position in class 0; n positions of it exist.
+template <class T>
+__device__ __forceinline__ void load_map_tile(typename T::E* tile, const typename T::E* z, int C, int inner, int n) {
+    constexpr int PPR = POS / T::VEC, U = 8;
+    const int pieces = C * PPR, step = blockDim.x;
+    for (int at = threadIdx.x; at < pieces; at += step * U) {
+        Piece q[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int id = at + u * step;
+            if (id < pieces) q[u] = load_positions<T>(z + (long)(id / PPR) * inner, id % PPR * T::VEC, n);
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int id = at + u * step;
+            if (id < pieces) *(Piece*)(tile + (size_t)id * T::VEC) = q[u];
+        }
+    }
+}
+
+// Adds the exponentials of N logits to a lane's running sums.
+template <int N, bool ENTROPY>
+__device__ __forceinline__ void add_logits(Sums& v, const float (&x)[N], float c) {
+    float m = x[0];
+#pragma unroll
+    for (int i = 1; i < N; ++i) m = fmaxf(m, x[i]);
+    if (m > v.m) {
+        v.m = m;
+        const float R = reference_exponent(m, c), d = v.R - R, f = exp2_(d);
+        if (ENTROPY) v.t = f * (v.t + bounded(d) * v.s);
+        v.s *= f;
+        v.R = R;
+    }
+    float s = 0.f, t = 0.f;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        const float d = __builtin_fmaf(x[i], c, -v.R), e = exp2_(d);
+        s += e;
+        if (ENTROPY) t = __builtin_fmaf(e, bounded(d), t);
+    }
+    v.s += s;
+    if (ENTROPY) v.t += t;
+}
+
+// ---- log probabilities ----------------------------------------------------------------------------------------------
+// One pass makes the sums and each lane's K best values: a sorted list takes a value with one median of three per slot.
+// The waves' lists are joined (the larger ends of two sorted lists, sorted again by halving strides).  A second pass finds
+// the classes: those that reach the k-th best value wait in a short queue per lane and go to the slot their rank names;
+// equal values share a run of slots, which atomic minima keep in the order of classes whatever wave comes first.
+constexpr int QUEUE = 16;
+
+template <int K>
+__device__ __forceinline__ void list_add(float (&a)[K], float x) {
+#pragma unroll
+    for (int i = K - 1; i > 0; --i) a[i] = __builtin_amdgcn_fmed3f(a[i - 1], a[i], x);
+    a[0] = fmaxf(a[0], x);
+}
+
+// (a list of 64 takes more registers than 16 waves leave a lane)
+__host__ __device__ constexpr int most_waves(int slots) { return slots == 64 ? 8 : 16; }
+__host__ __device__ inline int list_slots(int k) { return k == 0 ? 0 : k <= 8 ? 8 : k <= 16 ? 16 : k <= 32 ? 32 : 64; }
+// Bytes behind the tile: the waves' sums; their lists, later their queues; the slots.
+inline int log_probs_map_bytes(int element, int classes, int k, int waves) {
+    const int lists = waves * POS * list_slots(k) * 4, queues = k ? waves * POS * QUEUE * 4 : 0;
+    return (classes * POS * element + 15) / 16 * 16 + waves * POS * (int)sizeof(Sums) + (lists > queues ? lists : queues) + k * POS * 4;
+}
+
+template <class T, int K>
+__global__ __launch_bounds__(64 * most_waves(K)) void log_probs_map_kernel(LogProbArgs a, int tiles) {
+    extern __shared__ __align__(16) char smem[];
+    const int C = a.g.classes, inner = a.g.inner, k = a.k, waves = blockDim.x / 64, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    typename T::E* tile = (typename T::E*)smem;
+    Sums* s_sums = (Sums*)(smem + (C * POS * sizeof(typename T::E) + 15) / 16 * 16);
+    float* s_list = (float*)(s_sums + waves * POS);
+    uint32_t* s_queue = (uint32_t*)s_list;
+    constexpr int REGION = K * 4 > QUEUE * 4 ? K * 4 : QUEUE * 4;
+    uint32_t* s_slot = (uint32_t*)((char*)s_list + (K ? waves * POS * REGION : 0));
+    const int b = blockIdx.x / tiles, i0 = blockIdx.x % tiles * POS, n = inner - i0 < POS ? inner - i0 : POS;
+    const typename T::E* z = (const typename T::E*)a.g.logits + b * a.g.ld + i0;
+    const float c = a.g.c;
+    load_map_tile<T>(tile, z, C, inner, n);
+    for (int i = threadIdx.x; i < k * POS; i += blockDim.x) s_slot[i] = NONE;
+    __syncthreads();
+
+    const int c0 = (int)((long)C * wave / waves), c1 = (int)((long)C * (wave + 1) / waves);
+    Sums v = {-INFINITY, -FAR, 0.f, 0.f};
+    float best[K ? K : 1];
+#pragma unroll
+    for (int i = 0; i < K; ++i) best[i] = -INFINITY;
+    for (int j = c0; j < c1; j += 8) {
+        float x[8];
+#pragma unroll
+        for (int u = 0; u < 8; ++u) x[u] = j + u < c1 ? T::up(tile[(j + u) * POS + lane]) : -INFINITY;
+        add_logits<8, true>(v, x, c);
+        if constexpr (K > 0) {
+#pragma unroll
+            for (int u = 0; u < 8; ++u) list_add(best, x[u]);
+        }
+    }
+    if constexpr (K > 0) {
+        if (__any(v.s != v.s)) {  // NaN ranks as +inf: written so into the tile, the wave's lists anew
+#pragma unroll
+            for (int i = 0; i < K; ++i) best[i] = -INFINITY;
+            for (int j = c0; j < c1; ++j) {
+                float x = T::up(tile[j * POS + lane]);
+                if (x != x) {
+                    x = INFINITY;
+                    tile[j * POS + lane] = T::down(x);
+                }
+                list_add(best, x);
+            }
+        }
+    }
+    s_sums[wave * POS + lane] = v;
+    if constexpr (K > 0) {
+#pragma unroll
+        for (int i = 0; i < K; ++i) s_list[(wave * K + i) * POS + lane] = best[i];
+    }
+    __syncthreads();
+    v = s_sums[lane];
+    for (int w = 1; w < waves; ++w) v = join(v, s_sums[w * POS + lane]);
+    const bool far = is_far(v.m, c) && v.s == v.s;
+    if (__any(far)) {
+        float s = 0.f, t = 0.f;
+        for (int j = 0; j < C; ++j) {
+            const float d = (T::up(tile[j * POS + lane]) - v.m) * c, e = exp2_(d);
+            s += e;
+            t += e * bounded(d);
+        }
+        if (far) { v.s = s; v.t = t; }
+    }
+    if (v.m == INFINITY) v.s = __builtin_nanf("");
+    const bool empty = v.m == -INFINITY && v.s == 0.f;
+    const float l2 = empty ? INFINITY : log2_(v.s);
+    const long p = (long)b * inner + i0 + lane;
+    if (wave == 0 && lane < n) {
+        const long y = a.target[p];
+        a.log_prob[p] = y >= 0 && y < C ? row_log_p(a.g, T::up(tile[y * POS + lane]), v.m, l2) : 0.f;
+        a.entropy[p] = empty ? 0.f : (l2 - v.t / v.s) * LN2;
+        a.row_max[p] = v.m;
+        a.row_log_sum[p] = l2;
+    }
+    if constexpr (K > 0) {
+#pragma unroll
+        for (int i = 0; i < K; ++i) best[i] = s_list[i * POS + lane];
+        for (int w = 1; w < waves; ++w) {
+#pragma unroll
+            for (int i = 0; i < K; ++i) best[i] = fmaxf(best[i], s_list[(w * K + K - 1 - i) * POS + lane]);
+#pragma unroll
+            for (int o = K / 2; o > 0; o >>= 1)
+#pragma unroll
+                for (int i = 0; i < K; ++i)
+                    if (!(i & o)) {
+                        const float hi = fmaxf(best[i], best[i + o]), lo = fminf(best[i], best[i + o]);
+                        best[i] = hi;
+                        best[i + o] = lo;
+                    }
+        }
+        float least = best[0];  // the k-th best
+#pragma unroll
+        for (int i = 1; i < K; ++i) least = i == k - 1 ? best[i] : least;
+        __syncthreads();  // the lists are read: their room is the queues' now
+        uint32_t* queue = s_queue + wave * QUEUE * POS + lane;
+        int queued = 0;
+        auto drain = [&]() {
+            for (int i = 0; __any(i < queued); ++i)
+                if (i < queued) {
+                    uint32_t cls = queue[i * POS];
+                    const float x = T::up(tile[cls * POS + lane]);
+                    int rank = 0, end = 0;
+#pragma unroll
+                    for (int r = 0; r < K; ++r) {
+                        rank += best[r] > x;
+                        end += best[r] >= x;
+                    }
+                    if (end > k) end = k;
+                    for (int s = rank; s < end && cls != NONE; ++s) {
+                        const uint32_t old = atomicMin(&s_slot[s * POS + lane], cls);
+                        cls = old > cls ? old : cls;
+                    }
+                }
+            queued = 0;
+        };
+        for (int j = c0; j < c1; ++j) {
+            if (lane < n && T::up(tile[j * POS + lane]) >= least) queue[queued++ * POS] = j;
+            if (__any(queued == QUEUE)) drain();
+        }
+        drain();
+        __syncthreads();
+        if (lane < n)
+            for (int i = wave; i < k; i += waves) {
+                const uint32_t cls = s_slot[i * POS + lane];
+                const long at = ((long)b * k + i) * inner + i0 + lane;
+                a.top_class[at] = cls;
+                a.top_log_prob[at] = row_log_p(a.g, T::up(tile[cls * POS + lane]), v.m, l2);
+            }
+    }
+}
+
+// ---- log probabilities, backward: a thread's piece of positions stays the same from class to class ---------------------
+template <class T>
+__global__ __launch_bounds__(256) void log_probs_bwd_map_kernel(LogProbBwdArgs a, int tiles, int splits) {
+    constexpr int VEC = T::VEC, PPR = POS / VEC, ROWS = 256 / PPR, U = 4;
+    __shared__ float s_ref[POS], s_l2[POS], s_A[POS], s_B[POS], s_gl[POS];
+    __shared__ int s_at[POS], s_is_far[POS], s_far;
+    const int C = a.g.classes, inner = a.g.inner, tid = threadIdx.x;
+    const int t = blockIdx.x / splits, split = blockIdx.x % splits;
+    const int b = t / tiles, i0 = t % tiles * POS, n = inner - i0 < POS ? inner - i0 : POS;
+    const typename T::E* z = (const typename T::E*)a.g.logits + b * a.g.ld + i0;
+    typename T::E* dz = (typename T::E*)a.d_logits + (long)b * C * inner + i0;
+    const float c = a.g.c;
+    if (tid < POS) {
+        const long p = (long)b * inner + i0 + (tid < n ? tid : 0);
+        const float m = a.row_max[p], l2 = a.row_log_sum[p];
+        const long y = a.target[p];
+        const bool named = y >= 0 && y < C;
+        const float gl = a.d_log_prob && named && l2 != INFINITY ? a.d_log_prob[p] * a.g.inv_t : 0.f;
+        const float gh = a.d_entropy ? a.d_entropy[p] * a.g.inv_t : 0.f;
+        const bool far = is_far(m, c);
+        s_ref[tid] = far ? m : reference_exponent(m, c);
+        s_l2[tid] = l2;
+        s_A[tid] = -(gl + gh * a.entropy[p]);
+        s_B[tid] = -gh * LN2;
+        s_gl[tid] = gl;
+        s_at[tid] = named ? (int)y : -1;
+        s_is_far[tid] = far;
+        const bool any = __any(far);
+        if (tid == 0) s_far = any;
+    }
+    __syncthreads();
+    const int px = tid % PPR * VEC;
+    if (px >= n) return;
+    float ref[VEC], l2[VEC], A[VEC], B[VEC], gl[VEC];
+    int at[VEC];
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) {
+        ref[e] = s_ref[px + e]; l2[e] = s_l2[px + e]; A[e] = s_A[px + e]; B[e] = s_B[px + e]; gl[e] = s_gl[px + e]; at[e] = s_at[px + e];
+    }
+    const bool any_far = s_far;
+    const int c0 = (int)((long)C * split / splits), c1 = (int)((long)C * (split + 1) / splits);
+    for (int j = c0 + tid / PPR; j < c1; j += ROWS * U) {
+        Piece q[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+            if (j + u * ROWS < c1) q[u] = load_positions<T>(z + (long)(j + u * ROWS) * inner, px, n);
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int cls = j + u * ROWS;
+            if (cls >= c1) break;
+            float o[VEC];
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) {
+                const float x = T::get(q[u], e);
+                float d = __builtin_fmaf(x, c, -ref[e]);
+                if (any_far && s_is_far[px + e]) d = (x - ref[e]) * c;
+                d -= l2[e];
+                const float g = exp2_(d) * __builtin_fmaf(B[e], bounded(d), A[e]);
+                o[e] = cls == at[e] ? g + gl[e] : g;
+            }
+            store_positions<T>(dz + (long)cls * inner, px, n, T::pack(o));
+        }
+    }
+}
+
+// ---- distillation ---------------------------------------------------------------------------------------------------
+// Wave 0 prepares the kept classes, a lane per position: each class once (an entry listed again adds its q to the entry whose
+// number the tile's element holds last), the student's logits beside them, and -inf in the tile where the sums leave them out.
+// After the sums the tile's logits become the gradient in place, the kept classes get theirs, and the tile is stored.
+inline int distill_map_bytes(int element, int classes, int k, int waves) {
+    return (classes * POS * element + 15) / 16 * 16 + waves * POS * (int)sizeof(Sums) + 3 * k * POS * 4 + 2 * POS * 4;
+}
+
+template <class T> struct Bits { typedef uint16_t U; };  // an element as a whole number
+template <> struct Bits<F32> { typedef uint32_t U; };
+
+template <class T, bool REST>
+__global__ __launch_bounds__(1024) void distill_map_kernel(DistillArgs a, int tiles) {
+    extern __shared__ __align__(16) char smem[];
+    __shared__ Stats red_far[16];
+    __shared__ int far_cls[MAX_TOP];
+    __shared__ float far_q[MAX_TOP], far_tot[2];
+    __shared__ uint64_t s_far;
+    if (a.upstream && a.skip_unit && a.upstream[0] == 1.f) return;
+    typedef typename T::E E;
+    typedef typename Bits<T>::U U;
+    constexpr int VEC = T::VEC, PPR = POS / VEC;
+    const int C = a.g.classes, inner = a.g.inner, k = a.k, waves = blockDim.x / 64, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    E* tile = (E*)smem;
+    Sums* s_sums = (Sums*)(smem + (C * POS * sizeof(E) + 15) / 16 * 16);
+    int* s_cls = (int*)(s_sums + waves * POS);   // [k][POS]: the class, -1 for padding and for entries listed before
+    float* s_q = (float*)(s_cls + k * POS);      // its share of q, later its gradient
+    float* s_z = s_q + k * POS;                  // the student's logit
+    float *s_F = s_z + k * POS, *s_R = s_F + POS;
+    const int b = blockIdx.x / tiles, i0 = blockIdx.x % tiles * POS, n = inner - i0 < POS ? inner - i0 : POS;
+    const E* z = (const E*)a.g.logits + b * a.g.ld + i0;
+    E* dz = (E*)a.d_logits + (long)b * C * inner + i0;
+    const long p = (long)b * inner + i0 + lane;
+    const float c = a.g.c, w = lane < n ? position_weight(a, p) : 0.f;
+    if (!__any(w != 0.f)) {  // (the same in every wave)
+        if (a.d_logits)
+            for (int id = threadIdx.x; id < C * PPR; id += blockDim.x) store_positions<T>(dz + (long)(id / PPR) * inner, id % PPR * VEC, n, Piece{});
+        if (threadIdx.x == 0 && a.part) a.part[blockIdx.x] = 0.f;
+        return;
+    }
+    load_map_tile<T>(tile, z, C, inner, n);
+    float total = 0.f, left = 0.f, loss = 0.f;  // sum of q, what it leaves, the position's loss
+    if (wave == 0) {
+        const long at = (long)b * k * inner + i0 + lane;
+        float m = -INFINITY;
+        for (int i = 0; i < k; ++i) {
+            long cls = -1;
+            float x = -INFINITY;
+            if (lane < n) {
+                cls = load_class(a.top_class, a.class_bytes, at + (long)i * inner);
+                if (cls < 0 || cls >= C) cls = -1;
+                else x = load_any(a.top_value, a.value_dtype, at + (long)i * inner);
+            }
+            s_cls[i * POS + lane] = (int)cls;
+            s_q[i * POS + lane] = x;
+            m = fmaxf(m, x);
+        }
+        if (REST) {
+            double sum = 0.0;  // 64 bits: the rest is what a sum near 1 leaves
+            for (int i = 0; i < k; ++i) {
+                const float x = s_q[i * POS + lane], q = expf(x);
+                sum += exp((double)x);
+                if (q != 0.f) loss += q * x;
+                s_q[i * POS + lane] = q;
+            }
+            total = (float)sum;
+            left = sum != sum ? total : fmaxf((float)(1.0 - sum), 0.f);
+        } else {
+            m = finite_ref(m);
+            float sum = 0.f;
+            for (int i = 0; i < k; ++i) {
+                const float d = s_q[i * POS + lane] - m, q = exp2_(d * c);
+                sum += q;
+                if (q != 0.f) loss += q * d;
+                s_q[i * POS + lane] = q;
+            }
+            const float inv = sum != 0.f ? 1.f / sum : 0.f;
+            for (int i = 0; i < k; ++i) s_q[i * POS + lane] *= inv;
+            total = sum > 0.f ? 1.f : (sum != sum ? sum : 0.f);
+            loss = sum != 0.f ? loss * inv * a.g.inv_t - log2_(sum) * LN2 : 0.f;
+        }
+    }
+    __syncthreads();
+    if (wave == 0) {
+        for (int i = 0; i < k; ++i) {
+            const int cls = s_cls[i * POS + lane];
+            s_z[i * POS + lane] = cls >= 0 ? T::up(tile[cls * POS + lane]) : -INFINITY;
+        }
+        for (int i = 0; i < k; ++i) {
+            const int cls = s_cls[i * POS + lane];
+            if (cls >= 0) tile[cls * POS + lane] = __builtin_bit_cast(E, (U)i);
+        }
+        for (int i = 0; i < k; ++i) {
+            const int cls = s_cls[i * POS + lane];
+            if (cls < 0) continue;
+            const int last = __builtin_bit_cast(U, tile[cls * POS + lane]);
+            if (last != i) {
+                s_q[last * POS + lane] += s_q[i * POS + lane];
+                s_cls[i * POS + lane] = -1;
+            }
+        }
+        for (int i = 0; i < k; ++i) {
+            const int cls = s_cls[i * POS + lane];
+            if (cls >= 0) tile[cls * POS + lane] = T::down(REST ? -INFINITY : s_z[i * POS + lane]);
+        }
+    }
+    __syncthreads();
+    const int c0 = (int)((long)C * wave / waves), c1 = (int)((long)C * (wave + 1) / waves);
+    Sums v = {-INFINITY, -FAR, 0.f, 0.f};
+    for (int j = c0; j < c1; j += 8) {
+        float x[8];
+#pragma unroll
+        for (int u = 0; u < 8; ++u) x[u] = j + u < c1 ? T::up(tile[(j + u) * POS + lane]) : -INFINITY;
+        add_logits<8, false>(v, x, c);
+    }
+    s_sums[wave * POS + lane] = v;
+    __syncthreads();
+    if (wave == 0) {
+        Sums rest = s_sums[lane];
+        for (int i = 1; i < waves; ++i) rest = join(rest, s_sums[i * POS + lane]);
+        v = rest;  // the whole position
+        if (REST)
+            for (int i = 0; i < k; ++i)
+                if (s_cls[i * POS + lane] >= 0) {
+                    const float x[1] = {s_z[i * POS + lane]};
+                    add_logits<1, false>(v, x, c);
+                }
+        if (v.m == INFINITY) v.s = __builtin_nanf("");
+        const bool empty = v.m == -INFINITY && v.s == 0.f;
+        const float l2 = empty ? INFINITY : log2_(v.s);
+        const float r = REST && rest.s != 0.f ? left : 0.f, Q = total + r;
+        const float gs = empty ? 0.f : w * a.g.inv_t * (a.upstream ? a.upstream[0] : 1.f);
+        const bool far = w != 0.f && is_far(v.m, c);
+        const uint64_t fars = __ballot(far);
+        for (int i = 0; i < k; ++i) {
+            const int cls = s_cls[i * POS + lane];
+            if (cls < 0) continue;
+            const float q = s_q[i * POS + lane], x = s_z[i * POS + lane];
+            if (q != 0.f) loss -= q * row_log_p(a.g, x, v.m, l2);
+            s_q[i * POS + lane] = w != 0.f ? gs * (exp2_(__builtin_fmaf(x, c, -v.R) - l2) * Q - q) : 0.f;
+        }
+        if (r != 0.f) loss += r * (log2_(r) - ((rest.R - v.R) + log2_(rest.s) - l2)) * LN2;
+        loss = w != 0.f && !far ? w * loss : 0.f;
+        loss = wave_sum(loss);
+        if (lane == 0) {
+            s_far = fars;
+            if (a.part) a.part[blockIdx.x] = loss;
+        }
+        s_F[lane] = w != 0.f ? gs * (Q * exp2_(rest.R - v.R - l2) - (r != 0.f ? r / rest.s : 0.f)) : 0.f;
+        s_R[lane] = rest.R;
+    }
+    __syncthreads();
+    const uint64_t fars = s_far;
+    if (a.d_logits) {
+        const int px = threadIdx.x % PPR * VEC;  // (the workgroup's size is a multiple of PPR)
+        float F[VEC], R[VEC];
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) { F[e] = s_F[px + e]; R[e] = s_R[px + e]; }
+        for (int id = threadIdx.x; id < C * PPR; id += blockDim.x) {
+            const Piece q = *(const Piece*)(tile + (size_t)id * VEC);
+            float o[VEC];
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) {  // (outside the loss a logit may be anything)
+                const float d = F[e] * exp2_(__builtin_fmaf(T::get(q, e), c, -R[e]));
+                o[e] = F[e] != 0.f ? d : 0.f;
+            }
+            *(Piece*)(tile + (size_t)id * VEC) = T::pack(o);
+        }
+        __syncthreads();
+        for (int i = wave; i < k; i += waves) {
+            const int cls = s_cls[i * POS + lane];
+            if (cls >= 0) tile[cls * POS + lane] = T::down(s_q[i * POS + lane]);
+        }
+        __syncthreads();
+        for (int id = threadIdx.x; id < C * PPR; id += blockDim.x)
+            store_positions<T>(dz + (long)(id / PPR) * inner, id % PPR * VEC, n, *(const Piece*)(tile + (size_t)id * VEC));
+    }
+    for (uint64_t f = fars; f; f &= f - 1) {
+        const long at = (long)b * inner + i0 + __builtin_ctzll(f);
+        __syncthreads();
+        const float x = distill_position<T>(a, at, position_weight(a, at), red_far, far_cls, far_q, far_tot);
+        if (threadIdx.x == 0 && a.part) a.part[blockIdx.x] += x;
+    }
+}
+
+// Waves of a workgroup: enough that the workgroups whose tiles fit a CU bring 16, more where the map has few tiles.
+int map_waves(long tiles, int bytes, int classes) {
+    const int on_cu = LDS_BYTES / bytes < 1 ? 1 : LDS_BYTES / bytes;
+    int waves = 1;
+    while (waves < 16 && waves * 16 <= classes && (waves * on_cu < 16 || tiles * waves < 2048)) waves *= 2;
+    return waves;
+}
+
+int allow_lds(const void* kernel, int bytes, const char* name) {
+    const hipError_t e = hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    MMAE_REQUIRE(e == hipSuccess, MMAE_ELAUNCH, "%s: %d bytes of LDS refused: %s", name, bytes, hipGetErrorString(e));
+    return MMAE_OK;
+}
+
+int element_bytes(int dtype) { return dtype == MMAE_DT_F32 ? 4 : 2; }
+int map_tiles(int inner) { return (inner + POS - 1) / POS; }
+constexpr int DISTILL_STATIC = 1024;  // the distillation kernel's fixed arrays (an upper bound)
+
+// The largest number of waves that map_waves may ask for and that fits.
+template <class F>
+int fitting_waves(long tiles, int classes, F bytes, int room, int most) {
+    int waves = map_waves(tiles, bytes(4), classes);
+    if (waves > most) waves = most;
+    while (waves > 1 && bytes(waves) > room) waves /= 2;
+    return waves;
+}
+
+template <class T, int K>
+int launch_log_probs_map(const LogProbArgs& a, hipStream_t stream) {
+    const int tiles = map_tiles(a.g.inner), C = a.g.classes, k = a.k;
+    const int waves = fitting_waves((long)a.g.outer * tiles, C, [&](int w) { return log_probs_map_bytes(sizeof(typename T::E), C, k, w); }, LDS_BYTES, most_waves(K));
+    const int bytes = log_probs_map_bytes(sizeof(typename T::E), C, k, waves);
+    if (bytes > 65536) {
+        const int rc = allow_lds((const void*)log_probs_map_kernel<T, K>, bytes, "class_log_probs");
+        if (rc != MMAE_OK) return rc;
+    }
+    hipLaunchKernelGGL((log_probs_map_kernel<T, K>), dim3((unsigned)((long)a.g.outer * tiles)), dim3(64 * waves), bytes, stream, a, tiles);
+    return MMAE_OK;
+}
+template <class T>
+int launch_log_probs_map(const LogProbArgs& a, hipStream_t stream) {
+    switch (list_slots(a.k)) {
+        case 0: return launch_log_probs_map<T, 0>(a, stream);
+        case 8: return launch_log_probs_map<T, 8>(a, stream);
+        case 16: return launch_log_probs_map<T, 16>(a, stream);
+        case 32: return launch_log_probs_map<T, 32>(a, stream);
+        default: return launch_log_probs_map<T, 64>(a, stream);
+    }
+}
+
+template <class T, bool REST>
+int launch_distill_map(const DistillArgs& a, hipStream_t stream) {
+    const int tiles = map_tiles(a.g.inner), C = a.g.classes, k = a.k;
+    const int waves = fitting_waves((long)a.g.outer * tiles, C, [&](int w) { return distill_map_bytes(sizeof(typename T::E), C, k, w); },
+                                    LDS_BYTES - DISTILL_STATIC, 16);
+    const int bytes = distill_map_bytes(sizeof(typename T::E), C, k, waves);
+    if (bytes > 65536 - DISTILL_STATIC) {
+        const int rc = allow_lds((const void*)distill_map_kernel<T, REST>, bytes, "distill");
+        if (rc != MMAE_OK) return rc;
+    }
+    hipLaunchKernelGGL((distill_map_kernel<T, REST>), dim3((unsigned)((long)a.g.outer * tiles)), dim3(64 * waves), bytes, stream, a, tiles);
+    return MMAE_OK;
+}
+
+}  // namespace
+
+bool log_probs_map_fits(int dtype, int classes, int top_k) {
+    return classes <= 4096 && log_probs_map_bytes(element_bytes(dtype), classes, top_k, 1) <= LDS_BYTES;
+}
+bool distill_map_fits(int dtype, int classes, int k) {
+    return classes <= 4096 && distill_map_bytes(element_bytes(dtype), classes, k, 1) <= LDS_BYTES - DISTILL_STATIC;
+}
+long distill_map_parts(int outer, int inner) { return (long)outer * map_tiles(inner); }
+
+int log_probs_map(int dtype, const LogProbArgs& a, hipStream_t stream) {
+    return dtype == MMAE_DT_F32 ? launch_log_probs_map<F32>(a, stream)
+                                : dtype == MMAE_DT_BF16 ? launch_log_probs_map<B16>(a, stream) : launch_log_probs_map<H16>(a, stream);
+}
+
+int log_probs_bwd_map(int dtype, const LogProbBwdArgs& a, hipStream_t stream) {
+    const int tiles = map_tiles(a.g.inner);
+    const long all = (long)a.g.outer * tiles;
+    int splits = 1;  // workgroups that share a tile's classes, where there are few tiles
+    while (splits < 16 && all * splits < 2048 && splits * 64 < a.g.classes) splits *= 2;
+    MMAE_REQUIRE(all * splits <= 0x7fffffffL, MMAE_ESHAPE, "class_log_probs_bwd: %d x %d positions", a.g.outer, a.g.inner);
+#define CALL(T) hipLaunchKernelGGL(log_probs_bwd_map_kernel<T>, dim3((unsigned)(all * splits)), dim3(256), 0, stream, a, tiles, splits)
+    BY_DTYPE(dtype, CALL);
+#undef CALL
+    return MMAE_OK;
+}
+
+int distill_map(int dtype, const DistillArgs& a, hipStream_t stream) {
+    int rc = MMAE_OK;
+#define CALL(T) rc = a.log_probs ? launch_distill_map<T, true>(a, stream) : launch_distill_map<T, false>(a, stream)
+    BY_DTYPE(dtype, CALL);
+#undef CALL
+    return rc;
+}
+
+}  // namespace classdist

@@ -1,0 +1,749 @@
+// Class distributions over rows [N, C]: a row, or a slice of it, per workgroup.
+#include "classdist.h"
+
+namespace classdist {
+namespace {
+
+// ---- log probabilities: one pass over a row, or a slice of it -------------------------------------------------------
+template <int NT>
+__device__ Sums block_sums(Sums v, Sums* red) {
+    v = wave_sums(v);
+    if (NT == 64) return v;
+    __syncthreads();
+    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
+    __syncthreads();
+    Sums r = red[0];
+    for (int i = 1; i < NT / 64; ++i) r = join(r, red[i]);
+    return r;
+}
+// The sums of a whole row by (z - m) c, for the rows beyond FAR.
+template <class T, int NT>
+__device__ __noinline__ Sums far_sums(const typename T::E* z, int C, float m, float c, Sums* red) {
+    Sums v = {m, 0.f, 0.f, 0.f};
+    for (int j = threadIdx.x; j < C; j += NT) {
+        const float d = (T::up(z[j]) - m) * c, e = exp2_(d);
+        v.s += e;
+        v.t += e * bounded(d);
+    }
+    return block_sums<NT>(v, red);
+}
+
+template <class T, int NT, int NV>
+__device__ __forceinline__ void load_tile(Piece (&q)[NV], const typename T::E* z, int base, int end) {
+    constexpr int VEC = T::VEC;
+    if (base + NT * NV * VEC <= end) {
+#pragma unroll
+        for (int i = 0; i < NV; ++i) q[i] = load_piece<T>(z + base + (i * NT + threadIdx.x) * VEC);
+    } else {
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const int j = base + (i * NT + threadIdx.x) * VEC;
+            if (j + VEC <= end) {
+                q[i] = load_piece<T>(z + j);
+            } else {
+                q[i] = {T::NEG_INF, T::NEG_INF, T::NEG_INF, T::NEG_INF};
+#pragma unroll
+                for (int e = 0; e < VEC; ++e)
+                    if (j + e < end) T::put(q[i], e, T::up(z[j + e]));
+            }
+        }
+    }
+}
+
+// Most keys a tile can append: the list's own, and those above the k-th largest of the threads' maxima, which belong to
+// fewer than k threads.
+template <int EPT> constexpr int list_room() { return MAX_TOP + (MAX_TOP - 1) * EPT; }
+
+template <int ROOM, int NT>
+struct TopList {
+    uint64_t keys[ROOM];    // sorted up to `have` between tiles, appended behind it
+    uint64_t sorted[MAX_TOP];
+    float maxima[NT];
+    int count, wave_count[NT / 64];
+};
+
+// ordered() of the k-th largest of the NT maxima, searched bit by bit: each wave looks at all maxima and counts by ballots, so
+// no wave waits for another.
+template <class T, int NT>
+__device__ __forceinline__ uint32_t kth_maximum(const float* maxima, int k) {
+    const int lane = threadIdx.x & 63;
+    uint32_t key[NT / 64];
+#pragma unroll
+    for (int i = 0; i < NT / 64; ++i) key[i] = ordered(maxima[i * 64 + lane]);
+    uint32_t at = 0;
+    for (int b = 31; b >= 32 - T::KEY_BITS; --b) {
+        const uint32_t next = at | 1u << b;
+        int n = 0;
+#pragma unroll
+        for (int i = 0; i < NT / 64; ++i) n += __popcll(__ballot(key[i] >= next));
+        if (n >= k) at = next;
+    }
+    return at & 0x80000000u ? at : at | ((1ull << (32 - T::KEY_BITS)) - 1);  // (negative values are inverted, their later bits are set)
+}
+
+// Ranks the `n` keys of the list and keeps the first k, sorted.  Returns the value a further key has to exceed.
+template <int NT, class L>
+__device__ float keep_best(L& list, int n, int k) {
+    for (int i = threadIdx.x; i < n; i += NT) {
+        const uint64_t key = list.keys[i];
+        int rank = 0;
+        for (int j = 0; j < n; ++j) rank += list.keys[j] > key;
+        if (rank < k) list.sorted[rank] = key;
+    }
+    __syncthreads();
+    const int have = n < k ? n : k;
+    for (int i = threadIdx.x; i < have; i += NT) list.keys[i] = list.sorted[i];
+    if (threadIdx.x == 0) list.count = have;
+    __syncthreads();
+    return have < k ? -INFINITY : key_value(list.keys[k - 1]);
+}
+
+// Takes a tile's elements into the list.  floor: the value a key has to exceed (the k-th best so far: an equal one has a
+// higher class), -inf with `open` while the list holds fewer than k.
+template <class T, int NT, int NV, class L>
+__device__ __forceinline__ void take_tile(L& list, const Piece (&q)[NV], float tile_max, int base, int end, int k, float& floor, bool& open) {
+    constexpr int VEC = T::VEC, ROOM = sizeof(list.keys) / 8;
+    const int above = NT == 64 ? __popcll(__ballot(open || tile_max > floor)) : __syncthreads_count(open || tile_max > floor);
+    if (above == 0) return;
+    const int have = list.count;
+    float least = floor;     // take values above this one ...
+    bool equals = open;      // ... and equal to it
+    if (above >= k) {        // else fewer than k threads hold values above the floor: they all fit
+        list.maxima[threadIdx.x] = tile_max;
+        __syncthreads();
+        const uint32_t kth = kth_maximum<T, NT>(list.maxima, k);
+        const float v = key_value((uint64_t)kth << 32);
+        if (open || v > floor) { least = v; equals = true; }
+    }
+    if (NT != 64) __syncthreads();  // (list.count is read)
+    if (tile_max > least || (equals && tile_max == least)) {
+#pragma unroll
+        for (int i = 0; i < NV; ++i)
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) {
+                const float v = T::get(q[i], e);
+                const int j = base + (i * NT + threadIdx.x) * VEC + e;
+                if ((v > least || (equals && v == least)) && j < end) {
+                    const int n = atomicAdd(&list.count, 1);
+                    if (n < ROOM) list.keys[n] = rank_key(v, j);
+                }
+            }
+    }
+    __syncthreads();
+    int n = list.count;
+    if (n > ROOM) {
+        // More equal values than the list holds: the greater ones (fewer than k threads have any), then the equal ones of
+        // the lowest classes, piece by piece in the order of classes.
+        __syncthreads();
+        if (threadIdx.x == 0) list.count = have;
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < NV; ++i)
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) {
+                const float v = T::get(q[i], e);
+                if (v > least) {
+                    const int n = atomicAdd(&list.count, 1);
+                    if (n < ROOM) list.keys[n] = rank_key(v, base + (i * NT + threadIdx.x) * VEC + e);
+                }
+            }
+        __syncthreads();
+        n = list.count < ROOM ? list.count : ROOM;
+        int left = k < ROOM - n ? k : ROOM - n;  // equal values taken: k cover every need, keep_best cuts
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const int j = base + (i * NT + threadIdx.x) * VEC;
+            int mine = 0;
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) mine += T::get(q[i], e) == least && j + e < end;
+            int before = mine;  // inclusive prefix over the wave, then over the waves
+#pragma unroll
+            for (int o = 1; o < 64; o <<= 1) {
+                const int w = __shfl_up(before, o, 64);
+                if ((int)(threadIdx.x & 63) >= o) before += w;
+            }
+            __syncthreads();
+            if ((threadIdx.x & 63) == 63) list.wave_count[threadIdx.x >> 6] = before;
+            __syncthreads();
+            int all = 0;
+            before -= mine;
+            for (int w = 0; w < NT / 64; ++w) {
+                if (w < (int)(threadIdx.x >> 6)) before += list.wave_count[w];
+                all += list.wave_count[w];
+            }
+#pragma unroll
+            for (int e = 0; e < VEC; ++e)
+                if (T::get(q[i], e) == least && j + e < end) {
+                    if (before < left) list.keys[n + before] = rank_key(least, j + e);
+                    ++before;
+                }
+            n += all < left ? all : left;
+            left -= all < left ? all : left;
+        }
+        __syncthreads();
+    }
+    floor = keep_best<NT>(list, n, k);
+    open = list.count < k;
+}
+
+// The k best of z[first, end) by k scans, for slices that hold NaN (which compare with nothing).
+template <class T, int NT, class L>
+__device__ __noinline__ void scan_top(L& list, const typename T::E* z, int first, int end, int k) {
+    uint64_t last = ~0ull;
+    const int n = end - first < k ? end - first : k;
+    for (int i = 0; i < n; ++i) {
+        uint64_t top = 0;
+        for (int j = first + threadIdx.x; j < end; j += NT) {
+            const uint64_t key = rank_key(T::up(z[j]), j);
+            if (key < last && key > top) top = key;
+        }
+#pragma unroll
+        for (int o = 32; o > 0; o >>= 1) {
+            const uint64_t w = __shfl_xor((unsigned long long)top, o, 64);
+            top = w > top ? w : top;
+        }
+        __syncthreads();
+        if ((threadIdx.x & 63) == 0) list.sorted[threadIdx.x >> 6] = top;
+        __syncthreads();
+        for (int w = 0; w < NT / 64; ++w) top = list.sorted[w] > top ? list.sorted[w] : top;
+        last = top;
+        if (threadIdx.x == 0) list.keys[i] = top;
+    }
+    __syncthreads();
+    if (threadIdx.x == 0) list.count = n;
+    __syncthreads();
+}
+
+// A row's results from its sums and its sorted best keys (keys[i], i < k); the threads of one wave.
+template <class T, int NT>
+__device__ __forceinline__ void finish_row(const LogProbArgs& a, long p, const typename T::E* z, Sums v, const uint64_t* keys, Sums* red) {
+    const float c = a.g.c;
+    if (is_far(v.m, c)) v = far_sums<T, NT>(z, a.g.classes, v.m, c, red);
+    if (v.m == INFINITY) v.s = __builtin_nanf("");
+    const bool empty = v.m == -INFINITY && v.s == 0.f;
+    const float l2 = empty ? INFINITY : log2_(v.s);
+    if (threadIdx.x == 0) {
+        const long y = a.target[p];
+        a.log_prob[p] = y >= 0 && y < a.g.classes ? row_log_p(a.g, T::up(z[y]), v.m, l2) : 0.f;
+        a.entropy[p] = empty ? 0.f : (l2 - v.t / v.s) * LN2;
+        a.row_max[p] = v.m;
+        a.row_log_sum[p] = l2;
+    }
+    if ((int)threadIdx.x < a.k) {
+        const uint64_t key = keys[threadIdx.x];
+        a.top_class[p * a.k + threadIdx.x] = key_class(key);
+        a.top_log_prob[p * a.k + threadIdx.x] = row_log_p(a.g, key_value(key), v.m, l2);
+    }
+}
+
+// What a slice leaves for the join: its sums, then its k keys (0 where it holds fewer classes).
+__host__ __device__ inline size_t slice_bytes(int k) { return sizeof(Sums) + sizeof(uint64_t) * (size_t)k; }
+
+template <class T, int NT, int NV, bool TOP>
+__global__ __launch_bounds__(NT) void log_probs_rows_kernel(LogProbArgs a, int slices, int slice_tiles, char* parts) {
+    constexpr int VEC = T::VEC, TILE = NT * NV * VEC, ROOM = TOP ? list_room<NV * VEC>() : 1;
+    __shared__ Sums red[NT / 64];
+    __shared__ TopList<ROOM, NT> list;
+    const long p = blockIdx.x / slices;
+    const int slice = blockIdx.x % slices;
+    const typename T::E* z = (const typename T::E*)a.g.logits + p * a.g.ld;
+    const int C = a.g.classes, first = slice * slice_tiles * TILE;
+    const int end = first + slice_tiles * TILE < C ? first + slice_tiles * TILE : C;
+    const float c = a.g.c;
+    Sums v = {-INFINITY, -FAR, 0.f, 0.f};
+    float floor = -INFINITY;
+    bool open = true;
+    if (TOP) {
+        if (threadIdx.x == 0) list.count = 0;
+        __syncthreads();
+    }
+    Piece q[NV], next[NV];
+    load_tile<T, NT, NV>(q, z, first, end);
+    for (int base = first;;) {
+        const bool more = base + TILE < end;
+        if (more) load_tile<T, NT, NV>(next, z, base + TILE, end);
+        float m = T::get(q[0], 0);
+#pragma unroll
+        for (int i = 0; i < NV; ++i)
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) m = fmaxf(m, T::get(q[i], e));
+        if (m > v.m) {
+            v.m = m;
+            const float R = reference_exponent(m, c), d = v.R - R, f = exp2_(d);
+            v.t = f * (v.t + bounded(d) * v.s);
+            v.s *= f;
+            v.R = R;
+        }
+        float s = 0.f, t = 0.f;
+#pragma unroll
+        for (int i = 0; i < NV; ++i)
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) {
+                const float d = __builtin_fmaf(T::get(q[i], e), c, -v.R), x = exp2_(d);
+                s += x;
+                t = __builtin_fmaf(x, bounded(d), t);
+            }
+        v.s += s;
+        v.t += t;
+        if (TOP) take_tile<T, NT, NV>(list, q, m, base, end, a.k, floor, open);
+        if (!more) break;
+        base += TILE;
+#pragma unroll
+        for (int i = 0; i < NV; ++i) q[i] = next[i];
+    }
+    v = block_sums<NT>(v, red);
+    if (TOP && v.s != v.s) scan_top<T, NT>(list, z, first, end, a.k);
+    if (slices == 1) {
+        finish_row<T, NT>(a, p, z, v, list.keys, red);
+        return;
+    }
+    char* out = parts + (size_t)blockIdx.x * slice_bytes(a.k);
+    if (threadIdx.x == 0) *(Sums*)out = v;
+    if (TOP && (int)threadIdx.x < a.k) ((uint64_t*)(out + sizeof(Sums)))[threadIdx.x] = (int)threadIdx.x < list.count ? list.keys[threadIdx.x] : 0;
+}
+
+// Joins the slices of a row: one wave per row, lane i walks slice i's sorted keys.
+constexpr int MAX_SLICES = 64;
+template <class T>
+__global__ __launch_bounds__(64) void log_probs_join_kernel(LogProbArgs a, int slices, const char* parts) {
+    extern __shared__ uint64_t s_keys[];  // [slices][k], then the k best
+    __shared__ Sums red[1];
+    const long p = blockIdx.x;
+    const int lane = threadIdx.x, k = a.k;
+    const char* part = parts + (size_t)p * slices * slice_bytes(k);
+    Sums v = {-INFINITY, -FAR, 0.f, 0.f};
+    if (lane < slices) v = *(const Sums*)(part + lane * slice_bytes(k));
+    for (int i = lane; i < slices * k; i += 64) s_keys[i] = ((const uint64_t*)(part + (i / k) * slice_bytes(k) + sizeof(Sums)))[i % k];
+    v = wave_sums(v);
+    __syncthreads();
+    int at = 0;
+    uint64_t head = lane < slices && k ? s_keys[lane * k] : 0;
+    for (int i = 0; i < k; ++i) {
+        uint64_t top = head;
+#pragma unroll
+        for (int o = 32; o > 0; o >>= 1) {
+            const uint64_t w = __shfl_xor((unsigned long long)top, o, 64);
+            top = w > top ? w : top;
+        }
+        if (head == top && top) {  // keys are unique: one lane
+            ++at;
+            head = at < k ? s_keys[lane * k + at] : 0;
+        }
+        if (lane == 0) s_keys[slices * k + i] = top;
+    }
+    __syncthreads();
+    finish_row<T, 64>(a, p, (const typename T::E*)a.g.logits + p * a.g.ld, v, s_keys + slices * k, red);
+}
+
+// Rows, forward: a tile per workgroup.  -(gl + gh (log p + H)) p is p (A + B log2 p).
+template <class T, int NT, int NV>
+__global__ __launch_bounds__(NT) void log_probs_bwd_rows_kernel(LogProbBwdArgs a, int tiles) {
+    constexpr int VEC = T::VEC, TILE = NT * NV * VEC;
+    const long p = blockIdx.x / tiles;
+    const int base = (blockIdx.x % tiles) * TILE, C = a.g.classes;
+    const typename T::E* z = (const typename T::E*)a.g.logits + p * a.g.ld;
+    typename T::E* dz = (typename T::E*)a.d_logits + p * C;
+    Piece q[NV];
+    load_tile<T, NT, NV>(q, z, base, C);
+    const float m = a.row_max[p], l2 = a.row_log_sum[p], c = a.g.c;
+    const long y = a.target[p];
+    const float gl = a.d_log_prob && y >= 0 && y < C && l2 != INFINITY ? a.d_log_prob[p] * a.g.inv_t : 0.f;
+    const float gh = a.d_entropy ? a.d_entropy[p] * a.g.inv_t : 0.f;
+    const float A = -(gl + gh * a.entropy[p]), B = -gh * LN2;
+    const int at = y >= 0 && y < C ? (int)y : -VEC;
+    const bool far = is_far(m, c);
+    const float R = far ? 0.f : reference_exponent(m, c);
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+        const int j = base + (i * NT + threadIdx.x) * VEC;
+        if (j >= C) break;
+        float o[VEC];
+        const bool named = (unsigned)(at - j) < (unsigned)VEC;
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) {
+            const float x = T::get(q[i], e);
+            const float d = (far ? (x - m) * c : __builtin_fmaf(x, c, -R)) - l2, w = exp2_(d);
+            float g = w * __builtin_fmaf(B, bounded(d), A);
+            o[e] = named && at - j == e ? g + gl : g;
+        }
+        if (j + VEC <= C) {
+            store_piece<T>(dz + j, T::pack(o));
+        } else {
+#pragma unroll
+            for (int e = 0; e < VEC; ++e)
+                if (j + e < C) dz[j + e] = T::down(o[e]);
+        }
+    }
+}
+
+// ---- distillation of rows -------------------------------------------------------------------------------------------
+// The sums over a row leave the kept classes out (their logits become -inf in the registers); what they add comes from their
+// k logits.  So P, the mass outside, is a sum of its own and not a difference, and the gradient of every other class is one
+// factor F times its exponential:  gs (Q 2^(R' - R) / s - r / s'),  s' and R' the sums outside, s and R those of the whole row.
+struct KeptLane {  // what one wave knows of its lane's kept class
+    Kept e;
+    float z;         // the student's logit
+    float q_class;   // the class's whole share of q (it may be listed twice)
+    bool first;      // no earlier lane lists the class
+};
+template <class T>
+__device__ __forceinline__ KeptLane load_kept_lane(const DistillArgs& a, long p, const typename T::E* z, int lane) {
+    KeptLane l;
+    l.e = load_kept(a, p, lane);
+    l.z = l.e.cls >= 0 ? T::up(z[l.e.cls]) : -INFINITY;
+    l.q_class = 0.f;
+    l.first = l.e.cls >= 0;
+    for (int i = 0; i < a.k; ++i) {
+        const int cls = __shfl(l.e.cls, i, 64);
+        const float q = __shfl(l.e.q, i, 64);
+        if (cls == l.e.cls) {
+            l.q_class += q;
+            if (i < lane) l.first = false;
+        }
+    }
+    return l;
+}
+
+struct RowResult { Sums all; float factor, ref; };  // factor F, R'
+// One wave: the row from the sums outside the kept classes.  Writes the row's loss, returns the lane's class gradient in d.
+template <class T>
+__device__ __forceinline__ RowResult join_row(const DistillArgs& a, long p, float w, const KeptLane& l, const Sums& rest, float& d, int lane, bool write) {
+    const float c = a.g.c;
+    Sums v = {-INFINITY, -FAR, 0.f, 0.f};
+    if (l.first) {
+        v.m = l.z == l.z ? l.z : -INFINITY;
+        v.R = reference_exponent(v.m, c);
+        v.s = exp2_(__builtin_fmaf(l.z, c, -v.R));
+    }
+    v = join(wave_sums(v), rest);
+    if (v.m == INFINITY) v.s = __builtin_nanf("");
+    const bool empty = v.m == -INFINITY && v.s == 0.f;
+    const float l2 = empty ? INFINITY : log2_(v.s);
+    const float r = rest.s != 0.f ? l.e.rest : 0.f, Q = l.e.total + r;
+    const float gs = empty ? 0.f : w * a.g.inv_t * (a.upstream ? a.upstream[0] : 1.f);
+    if (write && a.part) {
+        float x = l.e.q != 0.f ? l.e.q * (l.e.lq - row_log_p(a.g, l.z, v.m, l2)) : 0.f;
+        x = wave_sum(x);
+        if (r != 0.f) x += r * (log2_(r) - ((rest.R - v.R) + log2_(rest.s) - l2)) * LN2;
+        if (lane == 0) a.part[p] = w * x;
+    }
+    d = gs * (exp2_(__builtin_fmaf(l.z, c, -v.R) - l2) * Q - l.q_class);
+    return {v, gs * (Q * exp2_(rest.R - v.R - l2) - (r != 0.f ? r / rest.s : 0.f)), rest.R};
+}
+
+template <class T, int NT>
+__device__ __forceinline__ void zero_row(typename T::E* dz, int first, int end) {
+    for (int j = first + (int)threadIdx.x * T::VEC; j < end; j += NT * T::VEC) {
+        if (j + T::VEC <= end) store_piece<T>(dz + j, Piece{});
+        else for (int e = j; e < end; ++e) dz[e] = T::down(0.f);
+    }
+}
+
+template <class T, int NT, int NV>
+__device__ __forceinline__ Sums tile_sums(const Piece (&q)[NV], float c) {  // one thread's
+    Sums v = {T::get(q[0], 0), 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+#pragma unroll
+        for (int e = 0; e < T::VEC; ++e) v.m = fmaxf(v.m, T::get(q[i], e));
+    if (v.m != v.m) v.m = -INFINITY;
+    v.R = reference_exponent(v.m, c);
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+        float s = 0.f;
+#pragma unroll
+        for (int e = 0; e < T::VEC; ++e) s += exp2_(__builtin_fmaf(T::get(q[i], e), c, -v.R));
+        v.s += s;
+    }
+    return v;
+}
+
+// A row held in the registers of one workgroup: read once, its gradient written once.
+template <class T, int NT, int NV>
+__global__ __launch_bounds__(NT) void distill_rows_kernel(DistillArgs a) {
+    constexpr int VEC = T::VEC;
+    __shared__ __align__(16) uint32_t flags[NT * NV / 4];  // a byte per piece: which of its elements are kept classes
+    __shared__ Sums red[NT / 64];
+    __shared__ Stats red_far[NT / 64];
+    __shared__ int s_cls[MAX_TOP];
+    __shared__ float s_d[MAX_TOP], s_row[4];
+    if (a.upstream && a.skip_unit && a.upstream[0] == 1.f) return;
+    const long p = blockIdx.x;
+    const int C = a.g.classes, lane = threadIdx.x & 63;
+    const typename T::E* z = (const typename T::E*)a.g.logits + p * a.g.ld;
+    typename T::E* dz = (typename T::E*)a.d_logits + p * C;
+    const float w = position_weight(a, p), c = a.g.c;
+    if (w == 0.f) {
+        if (a.d_logits) zero_row<T, NT>(dz, 0, C);
+        if (threadIdx.x == 0 && a.part) a.part[p] = 0.f;
+        return;
+    }
+    Piece q[NV];
+    load_tile<T, NT, NV>(q, z, 0, C);
+    for (int i = threadIdx.x; i < NT * NV / 4; i += NT) flags[i] = 0;
+    __syncthreads();
+    KeptLane l;
+    if (threadIdx.x < 64) {
+        l = load_kept_lane<T>(a, p, z, lane);
+        s_cls[lane] = l.e.cls;
+        if (l.e.cls >= 0) atomicOr(&flags[l.e.cls / VEC / 4], 1u << (l.e.cls / VEC % 4 * 8 + l.e.cls % VEC));
+    }
+    __syncthreads();
+    const uint8_t* flag = (const uint8_t*)flags;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+        const uint32_t f = flag[i * NT + threadIdx.x];
+        if (f) {
+#pragma unroll
+            for (int e = 0; e < VEC; ++e)
+                if (f >> e & 1) T::put(q[i], e, -INFINITY);
+        }
+    }
+    const Sums rest = block_sums<NT>(tile_sums<T, NT, NV>(q, c), red);
+    if (threadIdx.x < 64) {
+        float d;
+        const RowResult row = join_row<T>(a, p, w, l, rest, d, lane, true);
+        s_d[lane] = d;
+        if (lane == 0) { s_row[0] = row.factor; s_row[1] = row.ref; s_row[2] = row.all.m; }
+    }
+    __syncthreads();
+    if (is_far(s_row[2], c)) {
+        const float x = distill_position<T>(a, p, w, red_far, s_cls, s_d, s_row);
+        if (threadIdx.x == 0 && a.part) a.part[p] = x;
+        return;
+    }
+    if (!a.d_logits) return;
+    const float F = s_row[0], R = s_row[1];
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+        const int j = (i * NT + threadIdx.x) * VEC;
+        if (j >= C) break;
+        float o[VEC];
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) o[e] = F * exp2_(__builtin_fmaf(T::get(q[i], e), c, -R));
+        const uint32_t f = flag[i * NT + threadIdx.x];
+        if (f)
+            for (int k = 0; k < a.k; ++k) {
+                const int at = s_cls[k] - j;
+#pragma unroll
+                for (int e = 0; e < VEC; ++e) o[e] = at == e ? s_d[k] : o[e];
+            }
+        if (j + VEC <= C) {
+            store_piece<T>(dz + j, T::pack(o));
+        } else {
+#pragma unroll
+            for (int e = 0; e < VEC; ++e)
+                if (j + e < C) dz[j + e] = T::down(o[e]);
+        }
+    }
+}
+
+// Calls put(i, e, lane) for every kept class inside a tile: lane holds the class, i and e name the piece and element of the
+// thread that is asked about.  Uniform over the wave but for `mine`.
+template <class T, int NT, int NV, class F>
+__device__ __forceinline__ void each_kept(int cls, int base, int end, F put) {
+    uint64_t in = __ballot(cls >= base && cls < end && cls < base + NT * NV * T::VEC);
+    while (in) {
+        const int k = __builtin_ctzll(in);
+        in &= in - 1;
+        const int off = __shfl(cls, k, 64) - base, piece = off / T::VEC;
+        if (piece % NT == (int)threadIdx.x) put(piece / NT, off % T::VEC, k);
+    }
+}
+
+// Few or long rows, first pass: the sums outside the kept classes, a slice per workgroup.
+template <class T, int NT, int NV>
+__global__ __launch_bounds__(NT) void distill_slices_kernel(DistillArgs a, int slices, int slice_tiles, Sums* parts) {
+    constexpr int VEC = T::VEC, TILE = NT * NV * VEC;
+    __shared__ Sums red[NT / 64];
+    if (a.upstream && a.skip_unit && a.upstream[0] == 1.f) return;
+    const long p = blockIdx.x / slices;
+    if (position_weight(a, p) == 0.f) return;
+    const int C = a.g.classes, lane = threadIdx.x & 63, first = blockIdx.x % slices * slice_tiles * TILE;
+    const int end = first + slice_tiles * TILE < C ? first + slice_tiles * TILE : C;
+    const typename T::E* z = (const typename T::E*)a.g.logits + p * a.g.ld;
+    const long cls64 = lane < a.k ? load_class(a.top_class, a.class_bytes, p * a.k + lane) : -1;
+    const int cls = cls64 >= 0 && cls64 < C ? (int)cls64 : -1;
+    Sums v = {-INFINITY, -FAR, 0.f, 0.f};
+    Piece q[NV], next[NV];
+    load_tile<T, NT, NV>(q, z, first, end);
+    for (int base = first;;) {
+        const bool more = base + TILE < end;
+        if (more) load_tile<T, NT, NV>(next, z, base + TILE, end);
+        each_kept<T, NT, NV>(cls, base, end, [&](int pi, int pe, int) {
+#pragma unroll
+            for (int i = 0; i < NV; ++i)
+#pragma unroll
+                for (int e = 0; e < VEC; ++e)
+                    if (i == pi && e == pe) T::put(q[i], e, -INFINITY);
+        });
+        v = join(v, tile_sums<T, NT, NV>(q, a.g.c));
+        if (!more) break;
+        base += TILE;
+#pragma unroll
+        for (int i = 0; i < NV; ++i) q[i] = next[i];
+    }
+    v = block_sums<NT>(v, red);
+    if (threadIdx.x == 0) parts[blockIdx.x] = v;
+}
+
+// Second pass: the gradient, a tile per workgroup; the first tile's workgroup writes the row's loss.
+template <class T, int NT, int NV>
+__global__ __launch_bounds__(NT) void distill_tiles_kernel(DistillArgs a, int tiles, int slices, const Sums* parts) {
+    constexpr int VEC = T::VEC, TILE = NT * NV * VEC;
+    __shared__ Stats red_far[NT / 64];
+    __shared__ int s_cls[MAX_TOP];
+    __shared__ float s_d[MAX_TOP], s_row[4];
+    if (a.upstream && a.skip_unit && a.upstream[0] == 1.f) return;
+    const long p = blockIdx.x / tiles;
+    const int tile = blockIdx.x % tiles, base = tile * TILE, C = a.g.classes, lane = threadIdx.x & 63;
+    const typename T::E* z = (const typename T::E*)a.g.logits + p * a.g.ld;
+    typename T::E* dz = (typename T::E*)a.d_logits + p * C;
+    const float w = position_weight(a, p), c = a.g.c;
+    if (w == 0.f) {
+        if (a.d_logits) zero_row<T, NT>(dz, base, base + TILE < C ? base + TILE : C);
+        if (tile == 0 && threadIdx.x == 0 && a.part) a.part[p] = 0.f;
+        return;
+    }
+    Piece q[NV];
+    if (a.d_logits) load_tile<T, NT, NV>(q, z, base, C);
+    if (threadIdx.x < 64) {
+        Sums rest = {-INFINITY, -FAR, 0.f, 0.f};
+        if (lane < slices) rest = parts[p * slices + lane];
+        rest = wave_sums(rest);
+        const KeptLane l = load_kept_lane<T>(a, p, z, lane);
+        float d;
+        const RowResult row = join_row<T>(a, p, w, l, rest, d, lane, tile == 0);
+        s_cls[lane] = l.e.cls;
+        s_d[lane] = d;
+        if (lane == 0) { s_row[0] = row.factor; s_row[1] = row.ref; s_row[2] = row.all.m; }
+    }
+    __syncthreads();
+    if (is_far(s_row[2], c)) {
+        if (tile == 0) {
+            const float x = distill_position<T>(a, p, w, red_far, s_cls, s_d, s_row);
+            if (threadIdx.x == 0 && a.part) a.part[p] = x;
+        }
+        return;
+    }
+    if (!a.d_logits) return;
+    const float F = s_row[0], R = s_row[1];
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+        float o[VEC];
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) o[e] = F * exp2_(__builtin_fmaf(T::get(q[i], e), c, -R));
+        q[i] = T::pack(o);
+    }
+    each_kept<T, NT, NV>(s_cls[lane], base, C, [&](int pi, int pe, int k) {
+#pragma unroll
+        for (int i = 0; i < NV; ++i)
+#pragma unroll
+            for (int e = 0; e < VEC; ++e)
+                if (i == pi && e == pe) T::put(q[i], e, s_d[k]);
+    });
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+        const int j = base + (i * NT + threadIdx.x) * VEC;
+        if (j + VEC <= C) {
+            store_piece<T>(dz + j, q[i]);
+        } else {
+#pragma unroll
+            for (int e = 0; e < VEC; ++e)
+                if (j + e < C) dz[j + e] = T::down(T::get(q[i], e));
+        }
+    }
+}
+
+// Tiles of the row kernels: 32 elements a thread; one wave up to 2048 classes, four beyond.
+constexpr int SHORT_ROW = 2048, ROW_TILE = 8192;
+// Workgroups a row is split into: enough for every CU to hold eight, at least a tile each.
+static int row_slices(int rows, int classes) {
+    if (classes <= SHORT_ROW) return 1;
+    const int tiles = (classes + ROW_TILE - 1) / ROW_TILE, want = (2048 + rows - 1) / rows;
+    int n = want < tiles ? want : tiles;
+    if (n > MAX_SLICES) n = MAX_SLICES;
+    const int per = (tiles + n - 1) / n;
+    return (tiles + per - 1) / per;  // (no slice is empty)
+}
+
+template <class T>
+static void launch_log_probs_rows(const LogProbArgs& a, void* workspace, hipStream_t stream) {
+    constexpr int NV = 32 / T::VEC;
+    const int rows = a.g.outer, n = row_slices(rows, a.g.classes);
+#define ROWS(NT, TOP, tiles) hipLaunchKernelGGL((log_probs_rows_kernel<T, NT, NV, TOP>), dim3((unsigned)rows * n), dim3(NT), 0, stream, a, n, tiles, (char*)workspace)
+    if (a.g.classes <= SHORT_ROW) {
+        if (a.k) ROWS(64, true, 1); else ROWS(64, false, 1);
+        return;
+    }
+    const int tiles = (a.g.classes + ROW_TILE - 1) / ROW_TILE, per = (tiles + n - 1) / n;
+    if (a.k) ROWS(256, true, per); else ROWS(256, false, per);
+#undef ROWS
+    if (n > 1) hipLaunchKernelGGL(log_probs_join_kernel<T>, dim3(rows), dim3(64), sizeof(uint64_t) * (size_t)(n + 1) * a.k, stream, a, n, (const char*)workspace);
+}
+
+// Rows held in registers where a workgroup takes them; in two passes over slices where there are too few rows for the card or
+// they are longer.
+template <class T> constexpr int longest_held_row() { return T::VEC == 8 ? 131072 : 65536; }
+static bool held_rows(int rows, int classes, int dtype) {
+    if (classes <= ROW_TILE) return true;
+    return rows >= 256 && classes <= (dtype == MMAE_DT_F32 ? longest_held_row<F32>() : longest_held_row<B16>());
+}
+template <class T>
+static void launch_distill_rows(const DistillArgs& a, int dtype, Sums* parts, hipStream_t stream) {
+    const int rows = a.g.outer, C = a.g.classes;
+    constexpr int V = T::VEC;
+#define HELD(NT, EPT) hipLaunchKernelGGL((distill_rows_kernel<T, NT, EPT / V>), dim3(rows), dim3(NT), 0, stream, a)
+    if (held_rows(rows, C, dtype)) {
+        if (C <= 2048) HELD(64, 32);
+        else if (C <= 8192) HELD(256, 32);
+        else if (C <= 16384) HELD(512, 32);
+        else if (C <= 32768) HELD(1024, 32);
+        else if (C <= 65536) HELD(1024, 64);
+        else if constexpr (V == 8) HELD(1024, 128);
+        return;
+    }
+#undef HELD
+    const int tiles = (C + ROW_TILE - 1) / ROW_TILE, n = row_slices(rows, C), per = (tiles + n - 1) / n;
+    hipLaunchKernelGGL((distill_slices_kernel<T, 256, 32 / V>), dim3((unsigned)rows * n), dim3(256), 0, stream, a, n, per, parts);
+    hipLaunchKernelGGL((distill_tiles_kernel<T, 256, 32 / V>), dim3((unsigned)rows * (a.d_logits ? tiles : 1)), dim3(256), 0, stream, a,
+                       a.d_logits ? tiles : 1, n, (const Sums*)parts);
+}
+
+}  // namespace
+
+size_t log_probs_rows_workspace(int rows, int classes, int top_k) {
+    const int n = row_slices(rows, classes);
+    return n == 1 ? 0 : (size_t)rows * n * slice_bytes(top_k);
+}
+
+void log_probs_rows(int dtype, const LogProbArgs& a, void* workspace, hipStream_t stream) {
+#define CALL(T) launch_log_probs_rows<T>(a, workspace, stream)
+    BY_DTYPE(dtype, CALL);
+#undef CALL
+}
+
+int log_probs_bwd_rows(int dtype, const LogProbBwdArgs& a, hipStream_t stream) {
+    const int C = a.g.classes, tile = C <= SHORT_ROW ? SHORT_ROW : ROW_TILE, tiles = (C + tile - 1) / tile;
+    MMAE_REQUIRE((long)a.g.outer * tiles <= 0x7fffffffL, MMAE_ESHAPE, "class_log_probs_bwd: %d rows of %d classes", a.g.outer, C);
+    const unsigned grid = (unsigned)a.g.outer * tiles;
+#define CALL(T)                                                                                                                    \
+    if (C <= SHORT_ROW) hipLaunchKernelGGL((log_probs_bwd_rows_kernel<T, 64, 32 / T::VEC>), dim3(grid), dim3(64), 0, stream, a, tiles); \
+    else hipLaunchKernelGGL((log_probs_bwd_rows_kernel<T, 256, 32 / T::VEC>), dim3(grid), dim3(256), 0, stream, a, tiles)
+    BY_DTYPE(dtype, CALL);
+#undef CALL
+    return MMAE_OK;
+}
+
+size_t distill_rows_workspace(int rows, int classes) { return sizeof(Sums) * (size_t)rows * row_slices(rows, classes); }
+
+int distill_rows(int dtype, const DistillArgs& a, void* workspace, hipStream_t stream) {
+    const int C = a.g.classes;
+    MMAE_REQUIRE((long)a.g.outer * ((C + ROW_TILE - 1) / ROW_TILE) <= 0x7fffffffL, MMAE_ESHAPE, "distill: %d rows of %d classes", a.g.outer, C);
+#define CALL(T) launch_distill_rows<T>(a, dtype, (Sums*)workspace, stream)
+    BY_DTYPE(dtype, CALL);
+#undef CALL
+    return MMAE_OK;
+}
+
+}  // namespace classdist

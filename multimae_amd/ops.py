@@ -746,7 +746,7 @@ def distill(logits: torch.Tensor, top_class: torch.Tensor, top_value: torch.Tens
         _beside(_req(upstream, F32, "distill upstream"), logits, (), "distill upstream")
     loss = torch.empty((), dtype=F32, device=logits.device) if want_loss else None
     L = _L()
-    nbytes = L.mmae_distill_workspace_bytes(B, C_, inner, k)
+    nbytes = L.mmae_distill_workspace_bytes(_DT[logits.dtype], B, C_, inner, k)
     ws = torch.empty(nbytes, dtype=torch.uint8, device=logits.device)
     moved = logits.numel() * logits.element_size() * (1 if d_logits is None else 2) + B * inner * k * (top_class.element_size() + top_value.element_size())
     with _Timed("distill", 0.0, nbytes=moved):
