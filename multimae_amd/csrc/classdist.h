@@ -214,33 +214,43 @@ __device__ __forceinline__ float position_weight(const DistillArgs& a, long p) {
 
 // One wave: lane i < k holds kept class i; returns class (-1 for padding), q, log q and the totals over the wave.
 struct Kept { int cls; float q, lq; float total, rest; };
-__device__ __forceinline__ Kept load_kept(const DistillArgs& a, long p, int lane) {
+__device__ __forceinline__ void read_kept(const DistillArgs& a, long p, int lane, int& cls, float& value) {
     const long at = (p / a.g.inner) * a.k * (long)a.g.inner + p % a.g.inner + (long)lane * a.g.inner;
-    Kept e = {-1, 0.f, 0.f, 0.f, 0.f};
-    float v = -INFINITY;
+    cls = -1;
+    value = -INFINITY;
     if (lane < a.k) {
-        const long cls = load_class(a.top_class, a.class_bytes, at);
-        if (cls >= 0 && cls < a.g.classes) {
-            e.cls = (int)cls;
-            v = load_any(a.top_value, a.value_dtype, at);
+        const long c = load_class(a.top_class, a.class_bytes, at);
+        const float v = load_any(a.top_value, a.value_dtype, at);
+        if (c >= 0 && c < a.g.classes) {
+            cls = (int)c;
+            value = v;
         }
     }
+}
+__device__ __forceinline__ Kept kept_share(const DistillArgs& a, int cls, float v) {
+    Kept e = {cls, 0.f, 0.f, 0.f, 0.f};
     if (a.log_probs) {
         e.lq = v;
-        e.q = e.cls >= 0 ? expf(v) : 0.f;
-        double t = e.cls >= 0 ? exp((double)v) : 0.0;  // 64 bits: the rest is what a sum near 1 leaves
+        e.q = cls >= 0 ? expf(v) : 0.f;
+        double t = cls >= 0 ? exp((double)v) : 0.0;  // 64 bits: the rest is what a sum near 1 leaves
 #pragma unroll
         for (int o = 32; o > 0; o >>= 1) t += __shfl_xor(t, o, 64);
         e.rest = t != t ? (float)t : fmaxf((float)(1.0 - t), 0.f);
         e.total = (float)t;
     } else {
         const float m = finite_ref(wave_max(v)), c = LOG2E * a.g.inv_t;
-        const float d = (v - m) * c, x = e.cls >= 0 ? exp2_(d) : 0.f, s = wave_sum(x);
+        const float d = (v - m) * c, x = cls >= 0 ? exp2_(d) : 0.f, s = wave_sum(x);
         e.q = s > 0.f || s != s ? x / s : 0.f;
         e.lq = (v - m) * a.g.inv_t - log2_(s) * LN2;
         e.total = s > 0.f ? 1.f : (s != s ? s : 0.f);
     }
     return e;
+}
+__device__ __forceinline__ Kept load_kept(const DistillArgs& a, long p, int lane) {
+    int cls;
+    float v;
+    read_kept(a, p, lane, cls, v);
+    return kept_share(a, cls, v);
 }
 
 // One position, any layout, by a whole workgroup: class after class from memory, differences (z - m) c.  Returns its weighted loss

@@ -29,25 +29,62 @@ __device__ __noinline__ Sums far_sums(const typename T::E* z, int C, float m, fl
 }
 
 template <class T, int NT, int NV>
+__device__ __forceinline__ void load_full_tile(Piece (&q)[NV], const typename T::E* z, int base) {
+#pragma unroll
+    for (int i = 0; i < NV; ++i) q[i] = load_piece<T>(z + base + (i * NT + threadIdx.x) * T::VEC);
+}
+// The tile at `base` of a row's first `end` classes, -inf behind them.  Pieces behind the end are read
+// as the last whole one, the one that the end cuts is shifted from it: loads under conditions wait for each other.
+template <class T, int NT, int NV>
 __device__ __forceinline__ void load_tile(Piece (&q)[NV], const typename T::E* z, int base, int end) {
     constexpr int VEC = T::VEC;
     if (base + NT * NV * VEC <= end) {
+        load_full_tile<T, NT, NV>(q, z, base);
+        return;
+    }
+    const Piece none = {T::NEG_INF, T::NEG_INF, T::NEG_INF, T::NEG_INF};
+    if (end < VEC) {
 #pragma unroll
-        for (int i = 0; i < NV; ++i) q[i] = load_piece<T>(z + base + (i * NT + threadIdx.x) * VEC);
-    } else {
+        for (int i = 0; i < NV; ++i) q[i] = none;
+        if (threadIdx.x == 0 && base == 0) {
 #pragma unroll
-        for (int i = 0; i < NV; ++i) {
-            const int j = base + (i * NT + threadIdx.x) * VEC;
-            if (j + VEC <= end) {
-                q[i] = load_piece<T>(z + j);
-            } else {
-                q[i] = {T::NEG_INF, T::NEG_INF, T::NEG_INF, T::NEG_INF};
+            for (int e = 0; e < VEC; ++e)
+                if (e < end) T::put(q[0], e, T::up(z[e]));
+        }
+        return;
+    }
 #pragma unroll
-                for (int e = 0; e < VEC; ++e)
-                    if (j + e < end) T::put(q[i], e, T::up(z[j + e]));
-            }
+    for (int i = 0; i < NV; ++i) {  // all of them without a branch, inside the row
+        const int j = base + (i * NT + threadIdx.x) * VEC;
+        q[i] = load_piece<T>(z + (j + VEC <= end ? j : end - VEC));
+    }
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+        const int n = end - (base + (int)(i * NT + threadIdx.x) * VEC);
+        if (n <= 0) {
+            q[i] = none;
+        } else if (n < VEC) {
+            typedef unsigned __int128 W;
+            const int bits = (VEC - n) * (int)sizeof(typename T::E) * 8;
+            q[i] = __builtin_bit_cast(Piece, __builtin_bit_cast(W, q[i]) >> bits | __builtin_bit_cast(W, none) << (128 - bits));
         }
     }
+}
+
+// max(a, b, c) as one instruction: through fmaxf each operand that comes from memory bits is quieted first, one more each.
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float r;
+    asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
+    return r;
+}
+template <class T, int NV>
+__device__ __forceinline__ float tile_max(const Piece (&q)[NV]) {
+    float m = -INFINITY;
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+#pragma unroll
+        for (int e = 0; e < T::VEC; e += 2) m = max3(m, T::get(q[i], e), T::get(q[i], e + 1));
+    return m;
 }
 
 // Most keys a tile can append: the list's own, and those above the k-th largest of the threads' maxima, which belong to
@@ -257,16 +294,8 @@ __global__ __launch_bounds__(NT) void log_probs_rows_kernel(LogProbArgs a, int s
         if (threadIdx.x == 0) list.count = 0;
         __syncthreads();
     }
-    Piece q[NV], next[NV];
-    load_tile<T, NT, NV>(q, z, first, end);
-    for (int base = first;;) {
-        const bool more = base + TILE < end;
-        if (more) load_tile<T, NT, NV>(next, z, base + TILE, end);
-        float m = T::get(q[0], 0);
-#pragma unroll
-        for (int i = 0; i < NV; ++i)
-#pragma unroll
-            for (int e = 0; e < VEC; ++e) m = fmaxf(m, T::get(q[i], e));
+    auto process = [&](const Piece (&q)[NV], int base) {
+        const float m = tile_max<T, NV>(q);
         if (m > v.m) {
             v.m = m;
             const float R = reference_exponent(m, c), d = v.R - R, f = exp2_(d);
@@ -286,10 +315,23 @@ __global__ __launch_bounds__(NT) void log_probs_rows_kernel(LogProbArgs a, int s
         v.s += s;
         v.t += t;
         if (TOP) take_tile<T, NT, NV>(list, q, m, base, end, a.k, floor, open);
-        if (!more) break;
-        base += TILE;
+    };
+    // Whole tiles, the next one on its way while one is worked on (the last asks for itself again: a load that depended on
+    // a branch would be waited for at once); then what is left of the slice.
+    Piece q[NV], next[NV];
+    const int whole = first + (end - first) / TILE * TILE;
+    if (whole > first) {
+        load_full_tile<T, NT, NV>(q, z, first);
+        for (int base = first; base < whole; base += TILE) {
+            load_full_tile<T, NT, NV>(next, z, base + TILE < whole ? base + TILE : base);
+            process(q, base);
 #pragma unroll
-        for (int i = 0; i < NV; ++i) q[i] = next[i];
+            for (int i = 0; i < NV; ++i) q[i] = next[i];
+        }
+    }
+    if (whole < end) {
+        load_tile<T, NT, NV>(q, z, whole, end);
+        process(q, whole);
     }
     v = block_sums<NT>(v, red);
     if (TOP && v.s != v.s) scan_top<T, NT>(list, z, first, end, a.k);
@@ -387,18 +429,21 @@ struct KeptLane {  // what one wave knows of its lane's kept class
     bool first;      // no earlier lane lists the class
 };
 template <class T>
-__device__ __forceinline__ KeptLane load_kept_lane(const DistillArgs& a, long p, const typename T::E* z, int lane) {
+__device__ __forceinline__ KeptLane kept_lane(const DistillArgs& a, int cls, float value, const typename T::E* z, int lane, bool repeats) {
     KeptLane l;
-    l.e = load_kept(a, p, lane);
-    l.z = l.e.cls >= 0 ? T::up(z[l.e.cls]) : -INFINITY;
-    l.q_class = 0.f;
-    l.first = l.e.cls >= 0;
-    for (int i = 0; i < a.k; ++i) {
-        const int cls = __shfl(l.e.cls, i, 64);
-        const float q = __shfl(l.e.q, i, 64);
-        if (cls == l.e.cls) {
-            l.q_class += q;
-            if (i < lane) l.first = false;
+    l.z = cls >= 0 ? T::up(z[cls]) : -INFINITY;
+    l.e = kept_share(a, cls, value);
+    l.q_class = l.e.q;
+    l.first = cls >= 0;
+    if (repeats) {
+        l.q_class = 0.f;
+        for (int i = 0; i < a.k; ++i) {
+            const int other = __shfl(cls, i, 64);
+            const float q = __shfl(l.e.q, i, 64);
+            if (other == cls) {
+                l.q_class += q;
+                if (i < lane) l.first = false;
+            }
         }
     }
     return l;
@@ -439,15 +484,18 @@ __device__ __forceinline__ void zero_row(typename T::E* dz, int first, int end) 
     }
 }
 
+// The pieces stay as they were read: elements unpacked for one phase and kept for the next would hold twice the registers.
+template <int NV>
+__device__ __forceinline__ void keep_packed(Piece (&q)[NV]) {
+#pragma unroll
+    for (int i = 0; i < NV; ++i) asm volatile("" : "+v"(q[i].w[0]), "+v"(q[i].w[1]), "+v"(q[i].w[2]), "+v"(q[i].w[3]));
+}
+
 template <class T, int NT, int NV>
-__device__ __forceinline__ Sums tile_sums(const Piece (&q)[NV], float c) {  // one thread's
-    Sums v = {T::get(q[0], 0), 0.f, 0.f, 0.f};
-#pragma unroll
-    for (int i = 0; i < NV; ++i)
-#pragma unroll
-        for (int e = 0; e < T::VEC; ++e) v.m = fmaxf(v.m, T::get(q[i], e));
-    if (v.m != v.m) v.m = -INFINITY;
+__device__ __forceinline__ Sums tile_sums(Piece (&q)[NV], float c) {  // one thread's
+    Sums v = {tile_max<T, NV>(q), 0.f, 0.f, 0.f};
     v.R = reference_exponent(v.m, c);
+    if (NV > 8) keep_packed<NV>(q);
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
         float s = 0.f;
@@ -478,15 +526,22 @@ __global__ __launch_bounds__(NT) void distill_rows_kernel(DistillArgs a) {
         if (threadIdx.x == 0 && a.part) a.part[p] = 0.f;
         return;
     }
+    int cls = -1;
+    float value = -INFINITY;
+    if (threadIdx.x < 64) read_kept(a, p, lane, cls, value);
     Piece q[NV];
     load_tile<T, NT, NV>(q, z, 0, C);
     for (int i = threadIdx.x; i < NT * NV / 4; i += NT) flags[i] = 0;
     __syncthreads();
     KeptLane l;
     if (threadIdx.x < 64) {
-        l = load_kept_lane<T>(a, p, z, lane);
-        s_cls[lane] = l.e.cls;
-        if (l.e.cls >= 0) atomicOr(&flags[l.e.cls / VEC / 4], 1u << (l.e.cls / VEC % 4 * 8 + l.e.cls % VEC));
+        bool again = false;
+        if (cls >= 0) {
+            const uint32_t bit = 1u << (cls / VEC % 4 * 8 + cls % VEC);
+            again = atomicOr(&flags[cls / VEC / 4], bit) & bit;
+        }
+        s_cls[lane] = cls;
+        l = kept_lane<T>(a, cls, value, z, lane, __any(again));
     }
     __syncthreads();
     const uint8_t* flag = (const uint8_t*)flags;
@@ -499,7 +554,9 @@ __global__ __launch_bounds__(NT) void distill_rows_kernel(DistillArgs a) {
                 if (f >> e & 1) T::put(q[i], e, -INFINITY);
         }
     }
-    const Sums rest = block_sums<NT>(tile_sums<T, NT, NV>(q, c), red);
+    const Sums own = tile_sums<T, NT, NV>(q, c);
+    keep_packed<NV>(q);
+    const Sums rest = block_sums<NT>(own, red);
     if (threadIdx.x < 64) {
         float d;
         const RowResult row = join_row<T>(a, p, w, l, rest, d, lane, true);
@@ -562,8 +619,9 @@ __global__ __launch_bounds__(NT) void distill_slices_kernel(DistillArgs a, int s
     const int C = a.g.classes, lane = threadIdx.x & 63, first = blockIdx.x % slices * slice_tiles * TILE;
     const int end = first + slice_tiles * TILE < C ? first + slice_tiles * TILE : C;
     const typename T::E* z = (const typename T::E*)a.g.logits + p * a.g.ld;
-    const long cls64 = lane < a.k ? load_class(a.top_class, a.class_bytes, p * a.k + lane) : -1;
-    const int cls = cls64 >= 0 && cls64 < C ? (int)cls64 : -1;
+    int cls;
+    float value;
+    read_kept(a, p, lane, cls, value);
     Sums v = {-INFINITY, -FAR, 0.f, 0.f};
     Piece q[NV], next[NV];
     load_tile<T, NT, NV>(q, z, first, end);
@@ -611,7 +669,10 @@ __global__ __launch_bounds__(NT) void distill_tiles_kernel(DistillArgs a, int ti
         Sums rest = {-INFINITY, -FAR, 0.f, 0.f};
         if (lane < slices) rest = parts[p * slices + lane];
         rest = wave_sums(rest);
-        const KeptLane l = load_kept_lane<T>(a, p, z, lane);
+        int cls;
+        float value;
+        read_kept(a, p, lane, cls, value);
+        const KeptLane l = kept_lane<T>(a, cls, value, z, lane, true);
         float d;
         const RowResult row = join_row<T>(a, p, w, l, rest, d, lane, tile == 0);
         s_cls[lane] = l.e.cls;
