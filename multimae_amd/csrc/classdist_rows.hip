@@ -87,16 +87,23 @@ __device__ __forceinline__ float tile_max(const Piece (&q)[NV]) {
     return m;
 }
 
-// Most keys a tile can append: the list's own, and those above the k-th largest of the threads' maxima, which belong to
-// fewer than k threads.
-template <int EPT> constexpr int list_room() { return MAX_TOP + (MAX_TOP - 1) * EPT; }
-
-template <int ROOM, int NT>
+// The list of best keys: sorted and cut to k when it grows past SOFT, so the floor that a value has to exceed (the k-th best at
+// that time) follows slowly and most tiles only append.  A tile appends at most the values above the k-th largest of the
+// threads' maxima, which belong to fewer than k threads (and equal ones, which have a way of their own).
+constexpr int SOFT = 2 * MAX_TOP;
+template <int EPT, int NT>
 struct TopList {
-    uint64_t keys[ROOM];    // sorted up to `have` between tiles, appended behind it
+    static constexpr int ROOM = SOFT + (MAX_TOP - 1) * EPT;
+    uint64_t keys[ROOM];
     uint64_t sorted[MAX_TOP];
     float maxima[NT];
     int count, wave_count[NT / 64];
+    int added[3];  // keys appended by a tile; in turn, so that one barrier a tile is enough
+};
+struct ListState {  // the same in every thread
+    int have, turn;
+    float floor;
+    bool open;  // no floor yet: fewer than k keys
 };
 
 // ordered() of the k-th largest of the NT maxima, searched bit by bit: each wave looks at all maxima and counts by ballots, so
@@ -118,75 +125,71 @@ __device__ __forceinline__ uint32_t kth_maximum(const float* maxima, int k) {
     return at & 0x80000000u ? at : at | ((1ull << (32 - T::KEY_BITS)) - 1);  // (negative values are inverted, their later bits are set)
 }
 
-// Ranks the `n` keys of the list and keeps the first k, sorted.  Returns the value a further key has to exceed.
+// Ranks the keys of the list and keeps the first k, sorted.
 template <int NT, class L>
-__device__ float keep_best(L& list, int n, int k) {
+__device__ __forceinline__ void keep_best(L& list, ListState& st, int k) {
+    const int n = st.have;
     for (int i = threadIdx.x; i < n; i += NT) {
         const uint64_t key = list.keys[i];
         int rank = 0;
+#pragma unroll 4
         for (int j = 0; j < n; ++j) rank += list.keys[j] > key;
         if (rank < k) list.sorted[rank] = key;
     }
     __syncthreads();
-    const int have = n < k ? n : k;
-    for (int i = threadIdx.x; i < have; i += NT) list.keys[i] = list.sorted[i];
-    if (threadIdx.x == 0) list.count = have;
+    st.have = n < k ? n : k;
+    for (int i = threadIdx.x; i < st.have; i += NT) list.keys[i] = list.sorted[i];
+    if (threadIdx.x == 0) list.count = st.have;
     __syncthreads();
-    return have < k ? -INFINITY : key_value(list.keys[k - 1]);
+    st.open = st.have < k;
+    st.floor = st.open ? -INFINITY : key_value(list.keys[k - 1]);
 }
 
-// Takes a tile's elements into the list.  floor: the value a key has to exceed (the k-th best so far: an equal one has a
-// higher class), -inf with `open` while the list holds fewer than k.
+// A tile that opens the list, or holds more values above the floor than the list has room for.
 template <class T, int NT, int NV, class L>
-__device__ __forceinline__ void take_tile(L& list, const Piece (&q)[NV], float tile_max, int base, int end, int k, float& floor, bool& open) {
-    constexpr int VEC = T::VEC, ROOM = sizeof(list.keys) / 8;
-    const int above = NT == 64 ? __popcll(__ballot(open || tile_max > floor)) : __syncthreads_count(open || tile_max > floor);
-    if (above == 0) return;
-    const int have = list.count;
-    float least = floor;     // take values above this one ...
-    bool equals = open;      // ... and equal to it
-    if (above >= k) {        // else fewer than k threads hold values above the floor: they all fit
-        list.maxima[threadIdx.x] = tile_max;
-        __syncthreads();
-        const uint32_t kth = kth_maximum<T, NT>(list.maxima, k);
-        const float v = key_value((uint64_t)kth << 32);
-        if (open || v > floor) { least = v; equals = true; }
-    }
-    if (NT != 64) __syncthreads();  // (list.count is read)
+__device__ __forceinline__ void take_crowded_tile(L& list, const Piece (&q)[NV], float tile_max, int base, int end, int k, ListState& st) {
+    constexpr int VEC = T::VEC;
+    __syncthreads();
+    list.maxima[threadIdx.x] = tile_max;
+    if (threadIdx.x == 0) list.count = st.have;
+    __syncthreads();
+    const float v = key_value((uint64_t)kth_maximum<T, NT>(list.maxima, k) << 32);
+    const bool equals = st.open || v > st.floor;  // values equal to the bound are wanted too
+    const float least = equals ? v : st.floor;
     if (tile_max > least || (equals && tile_max == least)) {
 #pragma unroll
         for (int i = 0; i < NV; ++i)
 #pragma unroll
             for (int e = 0; e < VEC; ++e) {
-                const float v = T::get(q[i], e);
+                const float x = T::get(q[i], e);
                 const int j = base + (i * NT + threadIdx.x) * VEC + e;
-                if ((v > least || (equals && v == least)) && j < end) {
+                if ((x > least || (equals && x == least)) && j < end) {
                     const int n = atomicAdd(&list.count, 1);
-                    if (n < ROOM) list.keys[n] = rank_key(v, j);
+                    if (n < L::ROOM) list.keys[n] = rank_key(x, j);
                 }
             }
     }
     __syncthreads();
     int n = list.count;
-    if (n > ROOM) {
+    if (n > L::ROOM) {
         // More equal values than the list holds: the greater ones (fewer than k threads have any), then the equal ones of
         // the lowest classes, piece by piece in the order of classes.
         __syncthreads();
-        if (threadIdx.x == 0) list.count = have;
+        if (threadIdx.x == 0) list.count = st.have;
         __syncthreads();
 #pragma unroll
         for (int i = 0; i < NV; ++i)
 #pragma unroll
             for (int e = 0; e < VEC; ++e) {
-                const float v = T::get(q[i], e);
-                if (v > least) {
+                const float x = T::get(q[i], e);
+                if (x > least) {
                     const int n = atomicAdd(&list.count, 1);
-                    if (n < ROOM) list.keys[n] = rank_key(v, base + (i * NT + threadIdx.x) * VEC + e);
+                    if (n < L::ROOM) list.keys[n] = rank_key(x, base + (i * NT + threadIdx.x) * VEC + e);
                 }
             }
         __syncthreads();
-        n = list.count < ROOM ? list.count : ROOM;
-        int left = k < ROOM - n ? k : ROOM - n;  // equal values taken: k cover every need, keep_best cuts
+        n = list.count < L::ROOM ? list.count : L::ROOM;
+        int left = k < L::ROOM - n ? k : L::ROOM - n;  // equal values taken: k cover every need, keep_best cuts
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
             const int j = base + (i * NT + threadIdx.x) * VEC;
@@ -219,13 +222,48 @@ __device__ __forceinline__ void take_tile(L& list, const Piece (&q)[NV], float t
         }
         __syncthreads();
     }
-    floor = keep_best<NT>(list, n, k);
-    open = list.count < k;
+    st.have = n;
+    keep_best<NT>(list, st, k);
+}
+
+// Takes a tile's elements into the list.
+template <class T, int NT, int NV, class L>
+__device__ __forceinline__ void take_tile(L& list, const Piece (&q)[NV], float tile_max, int base, int end, int k, ListState& st) {
+    constexpr int VEC = T::VEC;
+    bool crowded = st.open;
+    if (!crowded) {
+        if (tile_max > st.floor) {
+            int mine = 0;
+#pragma unroll
+            for (int i = 0; i < NV; ++i)
+#pragma unroll
+                for (int e = 0; e < VEC; ++e) {
+                    const float x = T::get(q[i], e);
+                    if (x > st.floor) {  // (behind the end: -inf)
+                        const int n = atomicAdd(&list.count, 1);
+                        if (n < L::ROOM) list.keys[n] = rank_key(x, base + (i * NT + threadIdx.x) * VEC + e);
+                        ++mine;
+                    }
+                }
+            atomicAdd(&list.added[st.turn], mine);
+        }
+        __syncthreads();
+        const int added = list.added[st.turn], clear = st.turn == 0 ? 2 : st.turn - 1;
+        if (threadIdx.x == 0) list.added[clear] = 0;  // last read before this barrier, next used after the next one
+        st.turn = st.turn == 2 ? 0 : st.turn + 1;
+        crowded = st.have + added > L::ROOM;
+        if (!crowded) {
+            st.have += added;
+            if (st.have > SOFT) keep_best<NT>(list, st, k);
+        }
+    }
+    if (crowded) take_crowded_tile<T, NT, NV>(list, q, tile_max, base, end, k, st);
 }
 
 // The k best of z[first, end) by k scans, for slices that hold NaN (which compare with nothing).
 template <class T, int NT, class L>
 __device__ __noinline__ void scan_top(L& list, const typename T::E* z, int first, int end, int k) {
+    __syncthreads();
     uint64_t last = ~0ull;
     const int n = end - first < k ? end - first : k;
     for (int i = 0; i < n; ++i) {
@@ -251,9 +289,16 @@ __device__ __noinline__ void scan_top(L& list, const typename T::E* z, int first
     __syncthreads();
 }
 
+// The logit of the given class, asked for before the row is read: two loads that depend on each other.
+template <class T>
+__device__ __forceinline__ float named_logit(const LogProbArgs& a, long p, const typename T::E* z) {
+    const long y = a.target[p];
+    return T::up(z[y >= 0 && y < a.g.classes ? y : 0]);
+}
+
 // A row's results from its sums and its sorted best keys (keys[i], i < k); the threads of one wave.
 template <class T, int NT>
-__device__ __forceinline__ void finish_row(const LogProbArgs& a, long p, const typename T::E* z, Sums v, const uint64_t* keys, Sums* red) {
+__device__ __forceinline__ void finish_row(const LogProbArgs& a, long p, const typename T::E* z, Sums v, const uint64_t* keys, Sums* red, float named) {
     const float c = a.g.c;
     if (is_far(v.m, c)) v = far_sums<T, NT>(z, a.g.classes, v.m, c, red);
     if (v.m == INFINITY) v.s = __builtin_nanf("");
@@ -261,7 +306,7 @@ __device__ __forceinline__ void finish_row(const LogProbArgs& a, long p, const t
     const float l2 = empty ? INFINITY : log2_(v.s);
     if (threadIdx.x == 0) {
         const long y = a.target[p];
-        a.log_prob[p] = y >= 0 && y < a.g.classes ? row_log_p(a.g, T::up(z[y]), v.m, l2) : 0.f;
+        a.log_prob[p] = y >= 0 && y < a.g.classes ? row_log_p(a.g, named, v.m, l2) : 0.f;
         a.entropy[p] = empty ? 0.f : (l2 - v.t / v.s) * LN2;
         a.row_max[p] = v.m;
         a.row_log_sum[p] = l2;
@@ -278,21 +323,20 @@ __host__ __device__ inline size_t slice_bytes(int k) { return sizeof(Sums) + siz
 
 template <class T, int NT, int NV, bool TOP>
 __global__ __launch_bounds__(NT) void log_probs_rows_kernel(LogProbArgs a, int slices, int slice_tiles, char* parts) {
-    constexpr int VEC = T::VEC, TILE = NT * NV * VEC, ROOM = TOP ? list_room<NV * VEC>() : 1;
+    constexpr int VEC = T::VEC, TILE = NT * NV * VEC;
     __shared__ Sums red[NT / 64];
-    __shared__ TopList<ROOM, NT> list;
+    __shared__ TopList<NV * VEC, NT> list;
     const long p = blockIdx.x / slices;
     const int slice = blockIdx.x % slices;
     const typename T::E* z = (const typename T::E*)a.g.logits + p * a.g.ld;
     const int C = a.g.classes, first = slice * slice_tiles * TILE;
     const int end = first + slice_tiles * TILE < C ? first + slice_tiles * TILE : C;
     const float c = a.g.c;
+    const float named = slices == 1 ? named_logit<T>(a, p, z) : 0.f;
     Sums v = {-INFINITY, -FAR, 0.f, 0.f};
-    float floor = -INFINITY;
-    bool open = true;
+    ListState st = {0, 0, -INFINITY, true};
     if (TOP) {
-        if (threadIdx.x == 0) list.count = 0;
-        __syncthreads();
+        if (threadIdx.x < 3) list.added[threadIdx.x] = 0;
     }
     auto process = [&](const Piece (&q)[NV], int base) {
         const float m = tile_max<T, NV>(q);
@@ -314,7 +358,7 @@ __global__ __launch_bounds__(NT) void log_probs_rows_kernel(LogProbArgs a, int s
             }
         v.s += s;
         v.t += t;
-        if (TOP) take_tile<T, NT, NV>(list, q, m, base, end, a.k, floor, open);
+        if (TOP) take_tile<T, NT, NV>(list, q, m, base, end, a.k, st);
     };
     // Whole tiles, the next one on its way while one is worked on (the last asks for itself again: a load that depended on
     // a branch would be waited for at once); then what is left of the slice.
@@ -333,10 +377,11 @@ __global__ __launch_bounds__(NT) void log_probs_rows_kernel(LogProbArgs a, int s
         load_tile<T, NT, NV>(q, z, whole, end);
         process(q, whole);
     }
+    if (TOP && st.have > a.k) keep_best<NT>(list, st, a.k);
     v = block_sums<NT>(v, red);
     if (TOP && v.s != v.s) scan_top<T, NT>(list, z, first, end, a.k);
     if (slices == 1) {
-        finish_row<T, NT>(a, p, z, v, list.keys, red);
+        finish_row<T, NT>(a, p, z, v, list.keys, red, named);
         return;
     }
     char* out = parts + (size_t)blockIdx.x * slice_bytes(a.k);
@@ -353,6 +398,8 @@ __global__ __launch_bounds__(64) void log_probs_join_kernel(LogProbArgs a, int s
     const long p = blockIdx.x;
     const int lane = threadIdx.x, k = a.k;
     const char* part = parts + (size_t)p * slices * slice_bytes(k);
+    const typename T::E* z = (const typename T::E*)a.g.logits + p * a.g.ld;
+    const float named = named_logit<T>(a, p, z);
     Sums v = {-INFINITY, -FAR, 0.f, 0.f};
     if (lane < slices) v = *(const Sums*)(part + lane * slice_bytes(k));
     for (int i = lane; i < slices * k; i += 64) s_keys[i] = ((const uint64_t*)(part + (i / k) * slice_bytes(k) + sizeof(Sums)))[i % k];
@@ -374,7 +421,7 @@ __global__ __launch_bounds__(64) void log_probs_join_kernel(LogProbArgs a, int s
         if (lane == 0) s_keys[slices * k + i] = top;
     }
     __syncthreads();
-    finish_row<T, 64>(a, p, (const typename T::E*)a.g.logits + p * a.g.ld, v, s_keys + slices * k, red);
+    finish_row<T, 64>(a, p, z, v, s_keys + slices * k, red, named);
 }
 
 // Rows, forward: a tile per workgroup.  -(gl + gh (log p + H)) p is p (A + B log2 p).
@@ -718,29 +765,45 @@ __global__ __launch_bounds__(NT) void distill_tiles_kernel(DistillArgs a, int ti
 
 // Tiles of the row kernels: 32 elements a thread; one wave up to 2048 classes, four beyond.
 constexpr int SHORT_ROW = 2048, ROW_TILE = 8192;
-// Workgroups a row is split into: enough for every CU to hold eight, at least a tile each.
-static int row_slices(int rows, int classes) {
-    if (classes <= SHORT_ROW) return 1;
-    const int tiles = (classes + ROW_TILE - 1) / ROW_TILE, want = (2048 + rows - 1) / rows;
+#ifndef LP_EPT
+#define LP_EPT 16
+#endif
+#ifndef LP_NT
+#define LP_NT 256
+#endif
+constexpr int LP_TILE = LP_NT * LP_EPT;
+#ifndef WANT
+#define WANT 2048
+#endif
+// Workgroups a row is split into, and the tiles of each: enough for every CU to hold eight, at least a tile each, none empty.
+struct Split { int slices, tiles; };
+Split split_row(int rows, int classes, int tile) {
+    const int tiles = (classes + tile - 1) / tile, want = (WANT + rows - 1) / rows;
     int n = want < tiles ? want : tiles;
     if (n > MAX_SLICES) n = MAX_SLICES;
     const int per = (tiles + n - 1) / n;
-    return (tiles + per - 1) / per;  // (no slice is empty)
+    return {(tiles + per - 1) / per, per};
 }
+Split log_probs_split(int rows, int classes) {
+    return classes <= SHORT_ROW ? Split{1, (classes + 64 * LP_EPT - 1) / (64 * LP_EPT)} : split_row(rows, classes, LP_TILE);
+}
+int row_slices(int rows, int classes) { return split_row(rows, classes, ROW_TILE).slices; }
 
 template <class T>
 static void launch_log_probs_rows(const LogProbArgs& a, void* workspace, hipStream_t stream) {
-    constexpr int NV = 32 / T::VEC;
-    const int rows = a.g.outer, n = row_slices(rows, a.g.classes);
-#define ROWS(NT, TOP, tiles) hipLaunchKernelGGL((log_probs_rows_kernel<T, NT, NV, TOP>), dim3((unsigned)rows * n), dim3(NT), 0, stream, a, n, tiles, (char*)workspace)
+    constexpr int NV = LP_EPT / T::VEC;
+    const int rows = a.g.outer;
+    const Split d = log_probs_split(rows, a.g.classes);
+#define ROWS(NT, TOP) \
+    hipLaunchKernelGGL((log_probs_rows_kernel<T, NT, NV, TOP>), dim3((unsigned)rows * d.slices), dim3(NT), 0, stream, a, d.slices, d.tiles, (char*)workspace)
     if (a.g.classes <= SHORT_ROW) {
-        if (a.k) ROWS(64, true, 1); else ROWS(64, false, 1);
+        if (a.k) ROWS(64, true); else ROWS(64, false);
         return;
     }
-    const int tiles = (a.g.classes + ROW_TILE - 1) / ROW_TILE, per = (tiles + n - 1) / n;
-    if (a.k) ROWS(256, true, per); else ROWS(256, false, per);
+    if (a.k) ROWS(LP_NT, true); else ROWS(LP_NT, false);
 #undef ROWS
-    if (n > 1) hipLaunchKernelGGL(log_probs_join_kernel<T>, dim3(rows), dim3(64), sizeof(uint64_t) * (size_t)(n + 1) * a.k, stream, a, n, (const char*)workspace);
+    if (d.slices > 1)
+        hipLaunchKernelGGL(log_probs_join_kernel<T>, dim3(rows), dim3(64), sizeof(uint64_t) * (size_t)(d.slices + 1) * a.k, stream, a, d.slices, (const char*)workspace);
 }
 
 // Rows held in registers where a workgroup takes them; in two passes over slices where there are too few rows for the card or
@@ -765,16 +828,17 @@ static void launch_distill_rows(const DistillArgs& a, int dtype, Sums* parts, hi
         return;
     }
 #undef HELD
-    const int tiles = (C + ROW_TILE - 1) / ROW_TILE, n = row_slices(rows, C), per = (tiles + n - 1) / n;
-    hipLaunchKernelGGL((distill_slices_kernel<T, 256, 32 / V>), dim3((unsigned)rows * n), dim3(256), 0, stream, a, n, per, parts);
+    const int tiles = (C + ROW_TILE - 1) / ROW_TILE;
+    const Split d = split_row(rows, C, ROW_TILE);
+    hipLaunchKernelGGL((distill_slices_kernel<T, 256, 32 / V>), dim3((unsigned)rows * d.slices), dim3(256), 0, stream, a, d.slices, d.tiles, parts);
     hipLaunchKernelGGL((distill_tiles_kernel<T, 256, 32 / V>), dim3((unsigned)rows * (a.d_logits ? tiles : 1)), dim3(256), 0, stream, a,
-                       a.d_logits ? tiles : 1, n, (const Sums*)parts);
+                       a.d_logits ? tiles : 1, d.slices, (const Sums*)parts);
 }
 
 }  // namespace
 
 size_t log_probs_rows_workspace(int rows, int classes, int top_k) {
-    const int n = row_slices(rows, classes);
+    const int n = log_probs_split(rows, classes).slices;
     return n == 1 ? 0 : (size_t)rows * n * slice_bytes(top_k);
 }
 
