@@ -281,7 +281,7 @@ int mmae_masked_ce(const void* logits, int logits_is_bf16, const int64_t* target
  *
  * mmae_class_log_probs: log_prob = log softmax(x)[target] (0 where target is outside [0, classes), e.g. -100), entropy of
  * softmax(x), and the top_k (<= 64, <= classes) classes by z with their log probabilities: descending, equal values by the
- * lower class, NaN as +inf.  row_max / row_log_sum: what the backward pass needs.  A position whose logits are all -inf
+ * lower class, NaN as +inf.  row_max / row_log_sum: what the backward pass needs (both may be NULL).  A position whose logits are all -inf
  * has log_prob = -inf (at a valid target), entropy 0 and no gradient.  NaN and +inf logits give NaN, as in torch.
  * mmae_class_log_probs_bwd: d_logits (contiguous, the logits' dtype) for the gradients that arrive at log_prob and entropy
  * (either may be NULL). */
@@ -300,13 +300,14 @@ int mmae_class_log_probs_bwd(const void* logits, int dtype, int outer, int class
  *   loss = temperature^2 * mean of KL(q || p): over the positions in the mask of each sample, then over the samples with any
  * mask i64 [outer, (rows / patch) * (width / patch)] over inner = rows x width positions (nonzero = in the loss), or NULL: the
  * mean over all positions.  loss (f32 scalar) or d_logits (contiguous, the logits' dtype: the loss's gradient times
- * *upstream, a device scalar, or times 1 if NULL) may be NULL, not both.  skip_unit: leave everything as it is where
- * *upstream is 1. */
+ * *upstream, a device scalar, or times 1 if NULL) may be NULL, not both.  again: the workspace is as an earlier call with
+ * the same arguments up to `patch` left it, and what that call counted and summed is taken from there.  skip_unit: leave
+ * d_logits as it is where *upstream is 1. */
 size_t mmae_distill_workspace_bytes(int dtype, int outer, int classes, int inner, int k);
 int mmae_distill(const void* logits, int dtype, int outer, int classes, int inner, long ld, const void* top_class,
                  int class_bytes, const void* top_value, int value_dtype, int k, int kind, float temperature,
-                 const int64_t* mask, int width, int patch, const float* upstream, int skip_unit, float* loss, void* d_logits,
-                 void* workspace, size_t workspace_bytes, mmae_stream_t stream);
+                 const int64_t* mask, int width, int patch, const float* upstream, int again, int skip_unit, float* loss,
+                 void* d_logits, void* workspace, size_t workspace_bytes, mmae_stream_t stream);
 
 /* Truncated depth standardisation (run_pretraining_multimae.py:448-459): per sample (B rows of n values),
  * out = (x - mean) / sqrt(var + eps) with mean / unbiased var over the sorted values of ranks

@@ -65,7 +65,7 @@ SIGNATURES = {
     "mmae_class_log_probs": (_i, [_p, _i, _i, _i, _i, _l, _p, _i, _f, _p, _p, _p, _p, _p, _p, _p, _z, _p]),
     "mmae_class_log_probs_bwd": (_i, [_p, _i, _i, _i, _i, _l, _p, _f, _p, _p, _p, _p, _p, _p, _p]),
     "mmae_distill_workspace_bytes": (_z, [_i, _i, _i, _i, _i]),
-    "mmae_distill": (_i, [_p, _i, _i, _i, _i, _l, _p, _i, _p, _i, _i, _i, _f, _p, _i, _i, _p, _i, _p, _p, _p, _z, _p]),
+    "mmae_distill": (_i, [_p, _i, _i, _i, _i, _l, _p, _i, _p, _i, _i, _i, _f, _p, _i, _i, _p, _i, _i, _p, _p, _p, _z, _p]),
     "mmae_masked_loss": (_i, [_i, _i, _p, _i, _p, _p, _i, _i, _i, _i, _i, _p, _p, _p, _z, _p]),
     "mmae_masked_loss_static": (_i, [_i, _i, _p, _i, _p, _p, _i, _i, _i, _i, _i, _p, _p, _p]),
     "mmae_standardize_depth": (_i, [_p, _p, _i, _l, C.c_double, C.c_double, _f, _p]),

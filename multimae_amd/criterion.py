@@ -77,7 +77,7 @@ def class_log_probs(input, target, top_k: int = 0, temperature: float = 1.0) -> 
     differentiable.  A position whose logits are all -inf has log probability -inf, entropy 0 and no gradient."""
     if target.dtype != torch.int64:
         target = target.to(torch.int64)
-    return ClassLogProbs(*Fn.ClassLogProbsFn.apply(input, target, int(top_k), float(temperature)))
+    return ClassLogProbs(*Fn.class_log_probs(input, target, int(top_k), float(temperature)))
 
 
 class MaskedDistillationLoss(nn.Module):

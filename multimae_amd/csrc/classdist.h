@@ -320,7 +320,7 @@ size_t log_probs_rows_workspace(int rows, int classes, int top_k);
 void log_probs_rows(int dtype, const LogProbArgs& a, void* workspace, hipStream_t stream);
 int log_probs_bwd_rows(int dtype, const LogProbBwdArgs& a, hipStream_t stream);
 size_t distill_rows_workspace(int rows, int classes);
-int distill_rows(int dtype, const DistillArgs& a, void* workspace, hipStream_t stream);
+int distill_rows(int dtype, const DistillArgs& a, void* workspace, bool again, hipStream_t stream);  // again: the workspace is an earlier call's
 // classdist_maps.hip: maps, inner > 1; *_fits: the classes of 64 positions fit the LDS
 bool log_probs_map_fits(int dtype, int classes, int top_k);
 int log_probs_map(int dtype, const LogProbArgs& a, hipStream_t stream);

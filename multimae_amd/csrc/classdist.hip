@@ -28,9 +28,9 @@ __global__ __launch_bounds__(256) void log_probs_kernel(LogProbArgs a) {
         const long y = a.target[p];
         a.log_prob[p] = y >= 0 && y < C ? a.g.log_p(T::up(z[base + y * cs]), m, l2) : 0.f;
         a.entropy[p] = empty ? 0.f : (l2 - v.t / v.s) * LN2;
-        a.row_max[p] = m;
+        if (a.row_max) a.row_max[p] = m;
         // for the backward pass relative to the reference exponent it uses
-        a.row_log_sum[p] = is_far(m, c) ? l2 : l2 + __builtin_fmaf(m, c, -reference_exponent(m, c));
+        if (a.row_max) a.row_log_sum[p] = is_far(m, c) ? l2 : l2 + __builtin_fmaf(m, c, -reference_exponent(m, c));
     }
     const long at = (p / a.g.inner) * a.k * cs + p % a.g.inner;
     uint64_t last = ~0ull;
@@ -132,7 +132,7 @@ extern "C" int mmae_class_log_probs(const void* logits, int dtype, int outer, in
                                     size_t workspace_bytes, hipStream_t stream) {
     const int rc = check_logits("class_log_probs", logits, dtype, outer, classes, inner, ld, temperature);
     if (rc != MMAE_OK) return rc;
-    MMAE_REQUIRE(target && log_prob && entropy && row_max && row_log_sum && (!top_k || (top_log_prob && top_class)), MMAE_EINVAL,
+    MMAE_REQUIRE(target && log_prob && entropy && !row_max == !row_log_sum && (!top_k || (top_log_prob && top_class)), MMAE_EINVAL,
                  "class_log_probs: null pointer");
     MMAE_REQUIRE(top_k >= 0 && top_k <= MAX_TOP && top_k <= classes, MMAE_ESHAPE,
                  "class_log_probs: %d top classes of %d (at most %d)", top_k, classes, MAX_TOP);
@@ -182,7 +182,7 @@ extern "C" size_t mmae_distill_workspace_bytes(int dtype, int outer, int classes
 
 extern "C" int mmae_distill(const void* logits, int dtype, int outer, int classes, int inner, long ld, const void* top_class,
                             int class_bytes, const void* top_value, int value_dtype, int k, int kind, float temperature,
-                            const int64_t* mask, int width, int patch, const float* upstream, int skip_unit, float* loss,
+                            const int64_t* mask, int width, int patch, const float* upstream, int again, int skip_unit, float* loss,
                             void* d_logits, void* workspace, size_t workspace_bytes, hipStream_t stream) {
     const int rc = check_logits("distill", logits, dtype, outer, classes, inner, ld, temperature);
     if (rc != MMAE_OK) return rc;
@@ -203,7 +203,7 @@ extern "C" int mmae_distill(const void* logits, int dtype, int outer, int classe
     a.weight = (float)((double)temperature * temperature / ((double)outer * inner));
     a.valid = ws; a.count = ws + 4; a.part = loss ? ws + 4 + outer : nullptr;
     a.upstream = upstream; a.skip_unit = skip_unit; a.d_logits = d_logits;
-    if (mask) {
+    if (mask && !again) {
         if (a.tokens > 1) {
             hipLaunchKernelGGL(distill_count_kernel, dim3(outer), dim3(64), 0, stream, mask, outer, a.tokens, ws + 4);
             MMAE_CHECK_LAUNCH("distill_count");
@@ -214,7 +214,7 @@ extern "C" int mmae_distill(const void* logits, int dtype, int outer, int classe
     const long parts = distill_parts(dtype, outer, classes, inner, k);
     int r = MMAE_OK;
     if (inner == 1) {
-        r = distill_rows(dtype, a, ws + distill_floats(outer, parts), stream);
+        r = distill_rows(dtype, a, ws + distill_floats(outer, parts), again, stream);
     } else if (distill_map_fits(dtype, classes, k)) {
         r = distill_map(dtype, a, stream);
     } else {

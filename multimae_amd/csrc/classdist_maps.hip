@@ -170,8 +170,10 @@ __global__ __launch_bounds__(64 * most_waves(K)) void log_probs_map_kernel(LogPr
         const long y = a.target[p];
         a.log_prob[p] = y >= 0 && y < C ? row_log_p(a.g, T::up(tile[y * POS + lane]), v.m, l2) : 0.f;
         a.entropy[p] = empty ? 0.f : (l2 - v.t / v.s) * LN2;
-        a.row_max[p] = v.m;
-        a.row_log_sum[p] = l2;
+        if (a.row_max) {
+            a.row_max[p] = v.m;
+            a.row_log_sum[p] = l2;
+        }
     }
     if constexpr (K > 0) {
 #pragma unroll

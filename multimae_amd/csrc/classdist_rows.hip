@@ -308,8 +308,10 @@ __device__ __forceinline__ void finish_row(const LogProbArgs& a, long p, const t
         const long y = a.target[p];
         a.log_prob[p] = y >= 0 && y < a.g.classes ? row_log_p(a.g, named, v.m, l2) : 0.f;
         a.entropy[p] = empty ? 0.f : (l2 - v.t / v.s) * LN2;
-        a.row_max[p] = v.m;
-        a.row_log_sum[p] = l2;
+        if (a.row_max) {
+            a.row_max[p] = v.m;
+            a.row_log_sum[p] = l2;
+        }
     }
     if ((int)threadIdx.x < a.k) {
         const uint64_t key = keys[threadIdx.x];
@@ -814,7 +816,7 @@ static bool held_rows(int rows, int classes, int dtype) {
     return rows >= 256 && classes <= (dtype == MMAE_DT_F32 ? longest_held_row<F32>() : longest_held_row<B16>());
 }
 template <class T>
-static void launch_distill_rows(const DistillArgs& a, int dtype, Sums* parts, hipStream_t stream) {
+static void launch_distill_rows(const DistillArgs& a, int dtype, Sums* parts, bool again, hipStream_t stream) {
     const int rows = a.g.outer, C = a.g.classes;
     constexpr int V = T::VEC;
 #define HELD(NT, EPT) hipLaunchKernelGGL((distill_rows_kernel<T, NT, EPT / V>), dim3(rows), dim3(NT), 0, stream, a)
@@ -830,7 +832,7 @@ static void launch_distill_rows(const DistillArgs& a, int dtype, Sums* parts, hi
 #undef HELD
     const int tiles = (C + ROW_TILE - 1) / ROW_TILE;
     const Split d = split_row(rows, C, ROW_TILE);
-    hipLaunchKernelGGL((distill_slices_kernel<T, 256, 32 / V>), dim3((unsigned)rows * d.slices), dim3(256), 0, stream, a, d.slices, d.tiles, parts);
+    if (!again) hipLaunchKernelGGL((distill_slices_kernel<T, 256, 32 / V>), dim3((unsigned)rows * d.slices), dim3(256), 0, stream, a, d.slices, d.tiles, parts);
     hipLaunchKernelGGL((distill_tiles_kernel<T, 256, 32 / V>), dim3((unsigned)rows * (a.d_logits ? tiles : 1)), dim3(256), 0, stream, a,
                        a.d_logits ? tiles : 1, d.slices, (const Sums*)parts);
 }
@@ -862,10 +864,10 @@ int log_probs_bwd_rows(int dtype, const LogProbBwdArgs& a, hipStream_t stream) {
 
 size_t distill_rows_workspace(int rows, int classes) { return sizeof(Sums) * (size_t)rows * row_slices(rows, classes); }
 
-int distill_rows(int dtype, const DistillArgs& a, void* workspace, hipStream_t stream) {
+int distill_rows(int dtype, const DistillArgs& a, void* workspace, bool again, hipStream_t stream) {
     const int C = a.g.classes;
     MMAE_REQUIRE((long)a.g.outer * ((C + ROW_TILE - 1) / ROW_TILE) <= 0x7fffffffL, MMAE_ESHAPE, "distill: %d rows of %d classes", a.g.outer, C);
-#define CALL(T) launch_distill_rows<T>(a, dtype, (Sums*)workspace, stream)
+#define CALL(T) launch_distill_rows<T>(a, dtype, (Sums*)workspace, again, stream)
     BY_DTYPE(dtype, CALL);
 #undef CALL
     return MMAE_OK;

@@ -900,6 +900,13 @@ def _class_scores(x: torch.Tensor) -> torch.Tensor:
     return x if x.dim() < 2 or ops.class_geometry(x) is not None else x.contiguous()
 
 
+def class_log_probs(logits, target, top_k, temperature):
+    """ClassLogProbsFn, without a node where no gradient is asked for."""
+    if torch.is_grad_enabled() and logits.requires_grad:
+        return ClassLogProbsFn.apply(logits, target, top_k, temperature)
+    return ops.class_log_probs(_class_scores(logits), target.contiguous(), top_k, temperature, want_stats=False)[:4]
+
+
 class ClassLogProbsFn(torch.autograd.Function):
     """(log probability of the given class, entropy, top log probabilities, top classes) of each position's distribution;
     the first two carry gradients."""
@@ -907,11 +914,13 @@ class ClassLogProbsFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, target, top_k, temperature):
         logits = _class_scores(logits)
-        log_prob, entropy, top_log_prob, top_class, stats = ops.class_log_probs(logits, target.contiguous(), top_k, temperature)
+        target = target.contiguous()
+        log_prob, entropy, top_log_prob, top_class, stats = ops.class_log_probs(logits, target, top_k, temperature)
         ctx.temperature = temperature
         ctx.set_materialize_grads(False)
-        ctx.mark_non_differentiable(*(t for t in (top_log_prob, top_class) if t is not None))
-        ctx.save_for_backward(logits, target.contiguous(), entropy, stats)
+        if top_k:
+            ctx.mark_non_differentiable(top_log_prob, top_class)
+        ctx.save_for_backward(logits, target, entropy, stats)
         return log_prob, entropy, top_log_prob, top_class
 
     @staticmethod
@@ -933,24 +942,24 @@ class DistillFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, top_class, top_value, mask, patch, temperature, log_probs):
         logits, top_class, top_value = _class_scores(logits), top_class.contiguous(), top_value.contiguous()
-        ctx.d_logits = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device) if ctx.needs_input_grad[0] else None
-        loss = ops.distill(logits, top_class, top_value, mask, patch, temperature, log_probs, d_logits=ctx.d_logits)
-        if ctx.d_logits is not None:
-            ctx.save_for_backward(logits, top_class, top_value, mask)
-            ctx.options = (patch, temperature, log_probs)
-        return loss
+        call = ops.Distillation(logits, top_class, top_value, mask, patch, temperature, log_probs)
+        if not ctx.needs_input_grad[0]:
+            return call.run()
+        ctx.save_for_backward(logits, top_class, top_value, mask)
+        ctx.call, ctx.d_logits = call, torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
+        return call.run(ctx.d_logits)
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, g):
         d_logits, ctx.d_logits = ctx.d_logits, None
         if d_logits is None or not getattr(ctx, "unit_upstream", False):
-            logits, top_class, top_value, mask = ctx.saved_tensors
-            first = d_logits is not None
-            if not first:
-                d_logits = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
-            ops.distill(logits, top_class, top_value, mask, *ctx.options, want_loss=False, d_logits=d_logits, upstream=g.float().contiguous(),
-                        skip_unit=first)
+            logits = ctx.saved_tensors[0]  # (refused if an input was changed since)
+            g = g if g.dtype == torch.float32 else g.float()
+            if d_logits is None:
+                d_logits = ctx.call.scale(torch.empty(logits.shape, dtype=logits.dtype, device=logits.device), g)
+            else:
+                ctx.call.scale(d_logits, g, skip_unit=True)
         return d_logits, None, None, None, None, None, None
 
 

@@ -608,6 +608,9 @@ def class_geometry(t: torch.Tensor):
     shape = t.shape
     if t.numel() == 0:
         return (0, shape[1], 1, shape[1])
+    if t.is_contiguous():
+        n = t.numel() // (shape[0] * shape[1])
+        return (shape[0], shape[1], n, shape[1] * n)
     inner = 1
     for i in range(len(shape) - 1, 1, -1):
         if shape[i] != 1 and t.stride(i) != inner:
@@ -636,53 +639,63 @@ def _beside(t: torch.Tensor, other: torch.Tensor, shape, name: str):
     """t is a contiguous tensor of `shape` on the device of `other`."""
     if not t.is_cuda or t.device != other.device:
         raise _lib.MmaeError(f"{name}: expected a tensor on {other.device}, got {t.device}")
-    if tuple(t.shape) != tuple(shape):
+    if t.shape != shape:
         raise _lib.MmaeError(f"{name}: shape {tuple(t.shape)} != {tuple(shape)}")
     if not t.is_contiguous():
         raise _lib.MmaeError(f"{name}: expected a contiguous tensor")
     return t
 
 
-def _launch(what: str, fn, device, *args):
-    """fn(*args, the current stream of `device`), with `device` current."""
+def _launch(what: str, fn, device, nbytes, *args):
+    """fn(*args, the current stream of `device`), with `device` current; nbytes: what the call cannot avoid to move."""
     idx = device.index
-    if idx == torch._C._cuda_getDevice():
+    if PROFILE is None and idx == torch._C._cuda_getDevice():
         rc = fn(*args, _raw_stream(idx))
     else:
-        with torch.cuda.device(idx):
+        with torch.cuda.device(idx), _Timed(what, 0.0, nbytes=nbytes):
             rc = fn(*args, _raw_stream(idx))
-    _lib.check(rc, what)
+    if rc:
+        _lib.check(rc, what)
 
 
 def _addr(t: Optional[torch.Tensor]):
     return None if t is None else t.data_ptr()
 
 
-def class_log_probs(logits: torch.Tensor, target: torch.Tensor, top_k: int = 0, temperature: float = 1.0):
+def _class_call(logits: torch.Tensor, geo):
+    """The arguments that describe logits in every call."""
+    return (logits.data_ptr(), _DT[logits.dtype], *geo)
+
+
+def class_log_probs(logits: torch.Tensor, target: torch.Tensor, top_k: int = 0, temperature: float = 1.0, want_stats: bool = True):
     """logits [B, C, ...], target int64 [B, ...] -> (log_prob f32 [B, ...], entropy f32 [B, ...], top_log_prob f32 [B, k, ...],
-    top_class int64 [B, k, ...] (None, None for top_k = 0), stats f32 [2, B, ...] for class_log_probs_bwd)."""
-    _, C_, inner, ld = _class_scores(logits, "class_log_probs")
-    B, space = logits.shape[0], tuple(logits.shape[2:])
+    top_class int64 [B, k, ...] (None, None for top_k = 0), stats f32 [2, B, ...] for class_log_probs_bwd (None unless
+    want_stats))."""
+    geo = _class_scores(logits, "class_log_probs")
+    shape = logits.shape
+    batch = shape[:1] + shape[2:]
     if target.dtype != torch.int64:
         raise _lib.MmaeError(f"class_log_probs target: expected dtype torch.int64, got {target.dtype}")
-    _beside(target, logits, (B,) + space, "class_log_probs target")
-    if not 0 <= top_k <= min(C_, MAX_TOP_CLASSES):
-        raise _lib.MmaeError(f"class_log_probs: {top_k} top classes of {C_} (at most {MAX_TOP_CLASSES})")
+    _beside(target, logits, batch, "class_log_probs target")
+    if not 0 <= top_k <= min(shape[1], MAX_TOP_CLASSES):
+        raise _lib.MmaeError(f"class_log_probs: {top_k} top classes of {shape[1]} (at most {MAX_TOP_CLASSES})")
     dev = logits.device
-    log_prob = torch.empty((B,) + space, dtype=F32, device=dev)
-    entropy = torch.empty((B,) + space, dtype=F32, device=dev)
-    stats = torch.empty((2, B) + space, dtype=F32, device=dev)
-    top_log_prob = torch.empty((B, top_k) + space, dtype=F32, device=dev) if top_k else None
-    top_class = torch.empty((B, top_k) + space, dtype=torch.int64, device=dev) if top_k else None
-    if logits.numel():
+    log_prob = torch.empty(batch, dtype=F32, device=dev)
+    entropy = torch.empty_like(log_prob)
+    stats = torch.empty((2,) + batch, dtype=F32, device=dev) if want_stats else None
+    top_log_prob = top_class = None
+    if top_k:
+        top_log_prob = torch.empty(shape[:1] + (top_k,) + shape[2:], dtype=F32, device=dev)
+        top_class = torch.empty_like(top_log_prob, dtype=torch.int64)
+    if geo[0]:
         L = _L()
-        nbytes = L.mmae_class_log_probs_workspace_bytes(B, C_, inner, top_k)
+        nbytes = L.mmae_class_log_probs_workspace_bytes(geo[0], geo[1], geo[2], top_k)
         ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
-        at = stats.data_ptr()
-        with _Timed("class_log_probs", 0.0, nbytes=logits.numel() * logits.element_size() + B * inner * (24 + 12 * top_k)):
-            _launch("class_log_probs", L.mmae_class_log_probs, dev, logits.data_ptr(), _DT[logits.dtype], B, C_, inner, ld,
-                    target.data_ptr(), top_k, temperature, log_prob.data_ptr(), entropy.data_ptr(), at, at + 4 * B * inner,
-                    _addr(top_log_prob), _addr(top_class), _addr(ws), nbytes)
+        n = geo[0] * geo[2]
+        at = stats.data_ptr() if want_stats else 0
+        _launch("class_log_probs", L.mmae_class_log_probs, dev, logits.numel() * logits.element_size() + n * (24 + 12 * top_k),
+                *_class_call(logits, geo), target.data_ptr(), top_k, temperature, log_prob.data_ptr(), entropy.data_ptr(),
+                at or None, at + 4 * n if at else None, _addr(top_log_prob), _addr(top_class), _addr(ws), nbytes)
     return log_prob, entropy, top_log_prob, top_class, stats
 
 
@@ -690,70 +703,86 @@ def class_log_probs_bwd(logits: torch.Tensor, target: torch.Tensor, entropy: tor
                         d_log_prob: Optional[torch.Tensor], d_entropy: Optional[torch.Tensor], temperature: float = 1.0):
     """Gradient of the logits (contiguous, their dtype) for the gradients of log_prob and entropy (f32 [B, ...] or None);
     entropy and stats as class_log_probs returned them."""
-    _, C_, inner, ld = _class_scores(logits, "class_log_probs_bwd")
-    B = logits.shape[0]
-    shape = (B,) + tuple(logits.shape[2:])
+    geo = _class_scores(logits, "class_log_probs_bwd")
+    shape = logits.shape[:1] + logits.shape[2:]
     if target.dtype != torch.int64:
         raise _lib.MmaeError(f"class_log_probs_bwd target: expected dtype torch.int64, got {target.dtype}")
-    for t, s, n in ((target, shape, "target"), (entropy, shape, "entropy"), (stats, (2,) + shape, "stats"), (d_log_prob, shape, "d_log_prob"),
-                    (d_entropy, shape, "d_entropy")):
+    _beside(target, logits, shape, "class_log_probs_bwd target")
+    for t, s, n in ((entropy, shape, "entropy"), (stats, (2,) + shape, "stats"), (d_log_prob, shape, "d_log_prob"), (d_entropy, shape, "d_entropy")):
         if t is not None:
-            _beside(t, logits, s, f"class_log_probs_bwd {n}")
-            if n != "target":
-                _req(t, F32, f"class_log_probs_bwd {n}")
+            _beside(_req(t, F32, f"class_log_probs_bwd {n}"), logits, s, f"class_log_probs_bwd {n}")
     d_logits = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
-    if logits.numel():
-        at = stats.data_ptr()
-        with _Timed("class_log_probs_bwd", 0.0, nbytes=2 * logits.numel() * logits.element_size() + B * inner * 28):
-            _launch("class_log_probs_bwd", _L().mmae_class_log_probs_bwd, logits.device, logits.data_ptr(), _DT[logits.dtype], B, C_, inner,
-                    ld, target.data_ptr(), temperature, entropy.data_ptr(), at, at + 4 * B * inner, _addr(d_log_prob), _addr(d_entropy),
-                    d_logits.data_ptr())
+    if geo[0]:
+        n, at = geo[0] * geo[2], stats.data_ptr()
+        _launch("class_log_probs_bwd", _L().mmae_class_log_probs_bwd, logits.device, 2 * logits.numel() * logits.element_size() + n * 28,
+                *_class_call(logits, geo), target.data_ptr(), temperature, entropy.data_ptr(), at, at + 4 * n, _addr(d_log_prob),
+                _addr(d_entropy), d_logits.data_ptr())
     return d_logits
 
 
+class Distillation:
+    """One distillation call: loss and gradient of logits [B, C, ...] against the teacher's top classes (int32 / int64
+    [B, k, ...]) and their logits, or with log_probs their log probabilities.  mask int64 [B, tokens] (nonzero = in the loss):
+    tokens are patch x patch squares of the last two dimensions, or single positions with patch = 1.
+
+    run() computes the f32 scalar loss and, into d_logits (contiguous, the logits' dtype), its gradient.  scale() then makes
+    the gradient again, times an f32 scalar on the device, from what run() left in the workspace."""
+
+    def __init__(self, logits: torch.Tensor, top_class: torch.Tensor, top_value: torch.Tensor, mask: Optional[torch.Tensor] = None,
+                 patch: int = 1, temperature: float = 1.0, log_probs: bool = False):
+        geo = _class_scores(logits, "distill")
+        shape = logits.shape
+        B, space = shape[0], shape[2:]
+        if not geo[0]:
+            raise _lib.MmaeError("distill: empty input")
+        if top_class.dtype not in (torch.int64, torch.int32):
+            raise _lib.MmaeError(f"distill top_class: expected int32 or int64, got {top_class.dtype}")
+        if top_value.dtype not in _DT:
+            raise _lib.MmaeError(f"distill top_value: expected float32, bfloat16 or float16, got {top_value.dtype}")
+        k = top_class.shape[1] if top_class.dim() > 1 else 0
+        if not 1 <= k <= MAX_TOP_CLASSES:
+            raise _lib.MmaeError(f"distill: {k} kept classes, between 1 and {MAX_TOP_CLASSES} are taken")
+        _beside(top_class, logits, (B, k) + space, "distill top_class")
+        _beside(top_value, logits, (B, k) + space, "distill top_value")
+        width = space[-1] if space else 1
+        if mask is not None:
+            if patch < 1 or (patch > 1 and len(space) != 2) or width % patch or (geo[2] // width) % patch:
+                raise _lib.MmaeError(f"distill: positions {tuple(space)} are not whole patches of {patch} x {patch}")
+            if mask.dtype != torch.int64:
+                raise _lib.MmaeError(f"distill mask: expected dtype torch.int64, got {mask.dtype}")
+            _beside(mask, logits, (B, geo[2] // (patch * patch)), "distill mask")
+        self.logits = logits
+        nbytes = _L().mmae_distill_workspace_bytes(_DT[logits.dtype], *geo[:3], k)
+        self.workspace = torch.empty(nbytes, dtype=torch.uint8, device=logits.device)
+        self.args = (*_class_call(logits, geo), top_class.data_ptr(), top_class.element_size(), top_value.data_ptr(), _DT[top_value.dtype],
+                     k, int(log_probs), temperature, _addr(mask), width, patch if mask is not None else 1)
+        self.beside_bytes = geo[0] * geo[2] * k * (top_class.element_size() + top_value.element_size())
+
+    def _launch(self, upstream, again, skip_unit, loss, d_logits):
+        bytes_ = self.logits.numel() * self.logits.element_size() * (1 if d_logits is None else 2) + self.beside_bytes
+        _launch("distill", _L().mmae_distill, self.logits.device, bytes_, *self.args, _addr(upstream), again, skip_unit, _addr(loss),
+                _addr(d_logits), self.workspace.data_ptr(), self.workspace.numel())
+
+    def _gradient(self, d_logits):
+        _beside(d_logits, self.logits, self.logits.shape, "distill d_logits")
+        return _req(d_logits, self.logits.dtype, "distill d_logits")
+
+    def run(self, d_logits: Optional[torch.Tensor] = None) -> torch.Tensor:
+        loss = torch.empty((), dtype=F32, device=self.logits.device)
+        self._launch(None, 0, 0, loss, None if d_logits is None else self._gradient(d_logits))
+        return loss
+
+    def scale(self, d_logits: torch.Tensor, upstream: torch.Tensor, skip_unit: bool = False) -> torch.Tensor:
+        """skip_unit: d_logits holds run()'s gradient and is left alone where the scalar is 1."""
+        _beside(_req(upstream, F32, "distill upstream"), self.logits, (), "distill upstream")
+        self._launch(upstream, 1, int(skip_unit), None, self._gradient(d_logits))
+        return d_logits
+
+
 def distill(logits: torch.Tensor, top_class: torch.Tensor, top_value: torch.Tensor, mask: Optional[torch.Tensor] = None, patch: int = 1,
-            temperature: float = 1.0, log_probs: bool = False, want_loss: bool = True, d_logits: Optional[torch.Tensor] = None,
-            upstream: Optional[torch.Tensor] = None, skip_unit: bool = False):
-    """Distillation loss of logits [B, C, ...] against the teacher's top classes (int32 / int64 [B, k, ...]) and their logits,
-    or with log_probs their log probabilities: the f32 scalar loss (None unless want_loss).  d_logits (contiguous, the
-    logits' dtype) receives the gradient, times the f32 scalar `upstream` if given; with skip_unit nothing is written where
-    that scalar is 1.  mask int64 [B, tokens] (nonzero = in the loss): tokens are patch x patch squares of the last two
-    dimensions, or single positions with patch = 1."""
-    B, C_, inner, ld = _class_scores(logits, "distill")
-    space = tuple(logits.shape[2:])
-    if B * inner == 0:
-        raise _lib.MmaeError("distill: empty input")
-    if top_class.dtype not in (torch.int32, torch.int64):
-        raise _lib.MmaeError(f"distill top_class: expected int32 or int64, got {top_class.dtype}")
-    if top_value.dtype not in _DT:
-        raise _lib.MmaeError(f"distill top_value: expected float32, bfloat16 or float16, got {top_value.dtype}")
-    k = top_class.shape[1] if top_class.dim() > 1 else 0
-    if not 1 <= k <= MAX_TOP_CLASSES:
-        raise _lib.MmaeError(f"distill: {k} kept classes, between 1 and {MAX_TOP_CLASSES} are taken")
-    _beside(top_class, logits, (B, k) + space, "distill top_class")
-    _beside(top_value, logits, (B, k) + space, "distill top_value")
-    width = space[-1] if space else 1
-    if mask is not None:
-        if patch < 1 or (patch > 1 and len(space) != 2) or width % patch or (inner // width) % patch:
-            raise _lib.MmaeError(f"distill: positions {space} are not whole patches of {patch} x {patch}")
-        if mask.dtype != torch.int64:
-            raise _lib.MmaeError(f"distill mask: expected dtype torch.int64, got {mask.dtype}")
-        _beside(mask, logits, (B, inner // (patch * patch)), "distill mask")
-    if d_logits is not None:
-        _beside(d_logits, logits, logits.shape, "distill d_logits")
-        _req(d_logits, logits.dtype, "distill d_logits")
-    if upstream is not None:
-        _beside(_req(upstream, F32, "distill upstream"), logits, (), "distill upstream")
-    loss = torch.empty((), dtype=F32, device=logits.device) if want_loss else None
-    L = _L()
-    nbytes = L.mmae_distill_workspace_bytes(_DT[logits.dtype], B, C_, inner, k)
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=logits.device)
-    moved = logits.numel() * logits.element_size() * (1 if d_logits is None else 2) + B * inner * k * (top_class.element_size() + top_value.element_size())
-    with _Timed("distill", 0.0, nbytes=moved):
-        _launch("distill", L.mmae_distill, logits.device, logits.data_ptr(), _DT[logits.dtype], B, C_, inner, ld, top_class.data_ptr(),
-                top_class.element_size(), top_value.data_ptr(), _DT[top_value.dtype], k, int(log_probs), temperature, _addr(mask), width,
-                patch if mask is not None else 1, _addr(upstream), int(skip_unit), _addr(loss), _addr(d_logits), ws.data_ptr(), nbytes)
-    return loss
+            temperature: float = 1.0, log_probs: bool = False, d_logits: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Distillation.run: the f32 scalar loss; d_logits receives the gradient."""
+    return Distillation(logits, top_class, top_value, mask, patch, temperature, log_probs).run(d_logits)
 
 
 def standardize_depth(depth: torch.Tensor, lo_frac: float = 0.1, hi_frac: float = 0.9, eps: float = 1e-6,

@@ -447,7 +447,7 @@ def test_distillation_refusals(M):
                 lambda: fn(z.cpu(), (cls.cpu(), val.cpu())), lambda: fn(z[:, :, :6], (cls[:, :, :6], val[:, :, :6]), mask=mask),
                 lambda: M.MaskedDistillationLoss(16, 4, temperature=0.0)(z, (cls, val)), lambda: fn(z[:0], (cls[:0], val[:0])),
                 lambda: fn(z.double(), (cls, val)), lambda: ops.distill(z, cls, val, d_logits=torch.empty(4, 9, 8, 8, device="cuda").bfloat16()),
-                lambda: ops.distill(z, cls, val, want_loss=False)):
+                lambda: ops.Distillation(z, cls, val).scale(torch.empty_like(z), torch.ones(2, device="cuda"))):
         with pytest.raises(MmaeError):
             bad()
     with pytest.raises(ValueError):
