@@ -21,6 +21,13 @@ typedef _Float16 f16;
 
 // 16 bytes of a row: VEC elements.  Loads and stores take any alignment of the element type.
 struct __attribute__((may_alias)) Piece { uint32_t w[4]; };
+__device__ __forceinline__ void clear_halves(Piece& q, uint32_t f, uint32_t fill) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        const uint32_t m = ((0u - (f >> (2 * e) & 1u)) & 0xffffu) | ((0u - (f >> (2 * e + 1) & 1u)) & 0xffff0000u);
+        q.w[e] = (q.w[e] & ~m) | (fill & m);
+    }
+}
 // KEY_BITS: leading bits of ordered(v) that tell all values of the type apart
 struct F32 {
     typedef float E;
@@ -30,6 +37,10 @@ struct F32 {
     static __device__ __forceinline__ float down(float v) { return v; }
     static __device__ __forceinline__ float get(const Piece& q, int e) { return __uint_as_float(q.w[e]); }
     static __device__ __forceinline__ void put(Piece& q, int e, float v) { q.w[e] = __float_as_uint(v); }
+    static __device__ __forceinline__ void clear(Piece& q, uint32_t f) {  // -inf into the elements whose bits are set
+#pragma unroll
+        for (int e = 0; e < 4; ++e) q.w[e] = f >> e & 1 ? NEG_INF : q.w[e];
+    }
     static __device__ __forceinline__ Piece pack(const float (&v)[4]) { return {__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3])}; }
 };
 struct B16 {
@@ -43,6 +54,7 @@ struct B16 {
         const uint32_t b = __builtin_bit_cast(uint16_t, (bf16)v);
         q.w[e >> 1] = e & 1 ? (q.w[e >> 1] & 0xffffu) | b << 16 : (q.w[e >> 1] & 0xffff0000u) | b;
     }
+    static __device__ __forceinline__ void clear(Piece& q, uint32_t f) { clear_halves(q, f, NEG_INF); }
     static __device__ __forceinline__ Piece pack(const float (&v)[8]) {
         typedef __attribute__((ext_vector_type(8))) bf16 V;
         V r;
@@ -64,6 +76,7 @@ struct H16 {
         const uint32_t b = __builtin_bit_cast(uint16_t, (f16)v);
         q.w[e >> 1] = e & 1 ? (q.w[e >> 1] & 0xffffu) | b << 16 : (q.w[e >> 1] & 0xffff0000u) | b;
     }
+    static __device__ __forceinline__ void clear(Piece& q, uint32_t f) { clear_halves(q, f, NEG_INF); }
     static __device__ __forceinline__ Piece pack(const float (&v)[8]) {
         typedef __attribute__((ext_vector_type(8))) f16 V;
         V r;
@@ -227,16 +240,27 @@ __device__ __forceinline__ void read_kept(const DistillArgs& a, long p, int lane
         }
     }
 }
+// exp v with the product's rounding put back: relative error of the exponential instruction, not of v.
+__device__ __forceinline__ float exp_(float v) {
+    const float d = v * LOG2E, lost = __builtin_fmaf(v, LOG2E, -d) + v * 1.9259629e-8f;  // log2(e) - LOG2E
+    const float x = exp2_(d);
+    return fabsf(d) < 1e4f ? __builtin_fmaf(x, lost * LN2, x) : x;
+}
+// The lane's share of the teacher's distribution; SUMS: the totals over the wave too (in 64 bits where the rest is what a sum
+// near 1 leaves), else those of logits only.
+template <bool SUMS = true>
 __device__ __forceinline__ Kept kept_share(const DistillArgs& a, int cls, float v) {
     Kept e = {cls, 0.f, 0.f, 0.f, 0.f};
     if (a.log_probs) {
         e.lq = v;
-        e.q = cls >= 0 ? expf(v) : 0.f;
-        double t = cls >= 0 ? exp((double)v) : 0.0;  // 64 bits: the rest is what a sum near 1 leaves
+        e.q = cls >= 0 ? exp_(v) : 0.f;
+        if (SUMS) {
+            double t = cls >= 0 ? exp((double)v) : 0.0;
 #pragma unroll
-        for (int o = 32; o > 0; o >>= 1) t += __shfl_xor(t, o, 64);
-        e.rest = t != t ? (float)t : fmaxf((float)(1.0 - t), 0.f);
-        e.total = (float)t;
+            for (int o = 32; o > 0; o >>= 1) t += __shfl_xor(t, o, 64);
+            e.rest = t != t ? (float)t : fmaxf((float)(1.0 - t), 0.f);
+            e.total = (float)t;
+        }
     } else {
         const float m = finite_ref(wave_max(v)), c = LOG2E * a.g.inv_t;
         const float d = (v - m) * c, x = cls >= 0 ? exp2_(d) : 0.f, s = wave_sum(x);

@@ -33,31 +33,13 @@ __device__ __forceinline__ void load_full_tile(Piece (&q)[NV], const typename T:
 #pragma unroll
     for (int i = 0; i < NV; ++i) q[i] = load_piece<T>(z + base + (i * NT + threadIdx.x) * T::VEC);
 }
-// The tile at `base` of a row's first `end` classes, -inf behind them.  Pieces behind the end are read
-// as the last whole one, the one that the end cuts is shifted from it: loads under conditions wait for each other.
+// The tile at `base` of a row's first `end` classes, -inf behind them: read without a branch and inside the row (pieces behind
+// the end as the last whole one; loads under conditions wait for each other), then mended: the piece that the end cuts is shifted.
 template <class T, int NT, int NV>
-__device__ __forceinline__ void load_tile(Piece (&q)[NV], const typename T::E* z, int base, int end) {
+__device__ __forceinline__ void mend_tile(Piece (&q)[NV], int base, int end) {
     constexpr int VEC = T::VEC;
-    if (base + NT * NV * VEC <= end) {
-        load_full_tile<T, NT, NV>(q, z, base);
-        return;
-    }
+    if (base + NT * NV * VEC <= end) return;
     const Piece none = {T::NEG_INF, T::NEG_INF, T::NEG_INF, T::NEG_INF};
-    if (end < VEC) {
-#pragma unroll
-        for (int i = 0; i < NV; ++i) q[i] = none;
-        if (threadIdx.x == 0 && base == 0) {
-#pragma unroll
-            for (int e = 0; e < VEC; ++e)
-                if (e < end) T::put(q[0], e, T::up(z[e]));
-        }
-        return;
-    }
-#pragma unroll
-    for (int i = 0; i < NV; ++i) {  // all of them without a branch, inside the row
-        const int j = base + (i * NT + threadIdx.x) * VEC;
-        q[i] = load_piece<T>(z + (j + VEC <= end ? j : end - VEC));
-    }
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
         const int n = end - (base + (int)(i * NT + threadIdx.x) * VEC);
@@ -67,6 +49,30 @@ __device__ __forceinline__ void load_tile(Piece (&q)[NV], const typename T::E* z
             typedef unsigned __int128 W;
             const int bits = (VEC - n) * (int)sizeof(typename T::E) * 8;
             q[i] = __builtin_bit_cast(Piece, __builtin_bit_cast(W, q[i]) >> bits | __builtin_bit_cast(W, none) << (128 - bits));
+        }
+    }
+}
+template <class T, int NT>
+__device__ __forceinline__ Piece load_inside(const typename T::E* z, int i, int base, int end) {
+    const int j = base + (i * NT + (int)threadIdx.x) * T::VEC;
+    return load_piece<T>(z + (j + T::VEC <= end ? j : end - T::VEC));
+}
+template <class T, int NT, int NV>
+__device__ __forceinline__ void load_tile(Piece (&q)[NV], const typename T::E* z, int base, int end) {
+    constexpr int VEC = T::VEC;
+    if (base + NT * NV * VEC <= end) {
+        load_full_tile<T, NT, NV>(q, z, base);
+    } else if (end >= VEC) {
+#pragma unroll
+        for (int i = 0; i < NV; ++i) q[i] = load_inside<T, NT>(z, i, base, end);
+        mend_tile<T, NT, NV>(q, base, end);
+    } else {
+#pragma unroll
+        for (int i = 0; i < NV; ++i) q[i] = {T::NEG_INF, T::NEG_INF, T::NEG_INF, T::NEG_INF};
+        if (threadIdx.x == 0 && base == 0) {
+#pragma unroll
+            for (int e = 0; e < VEC; ++e)
+                if (e < end) T::put(q[0], e, T::up(z[e]));
         }
     }
 }
@@ -477,11 +483,11 @@ struct KeptLane {  // what one wave knows of its lane's kept class
     float q_class;   // the class's whole share of q (it may be listed twice)
     bool first;      // no earlier lane lists the class
 };
-template <class T>
+template <class T, bool SUMS = true>
 __device__ __forceinline__ KeptLane kept_lane(const DistillArgs& a, int cls, float value, const typename T::E* z, int lane, bool repeats) {
     KeptLane l;
     l.z = cls >= 0 ? T::up(z[cls]) : -INFINITY;
-    l.e = kept_share(a, cls, value);
+    l.e = kept_share<SUMS>(a, cls, value);
     l.q_class = l.e.q;
     l.first = cls >= 0;
     if (repeats) {
@@ -554,6 +560,8 @@ __device__ __forceinline__ Sums tile_sums(Piece (&q)[NV], float c) {  // one thr
     }
     return v;
 }
+
+__device__ __forceinline__ float uniform(float v) { return __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(v))); }
 
 // A row held in the registers of one workgroup: read once, its gradient written once.
 template <class T, int NT, int NV>
@@ -642,6 +650,170 @@ __global__ __launch_bounds__(NT) void distill_rows_kernel(DistillArgs a) {
                 if (j + e < C) dz[j + e] = T::down(o[e]);
         }
     }
+}
+
+// The long rows, of which a CU holds only one: a workgroup takes row after row, and while the pieces of one row's gradient
+// leave, the next row's come into the registers they free, so that reading and writing overlap.  Every piece but the last
+// begins at a multiple of NT * VEC elements and the last one ends with the row, so that a piece is a uniform address and the
+// thread's own offset.  The elements that the last piece shares with the one before are -inf in the last one,
+// which writes its zeros first.
+template <class T, int NT>
+struct LongRow {
+    static constexpr int VEC = T::VEC, SPAN = NT * VEC;
+    int C, last;  // classes (at least SPAN); the piece that ends with the row
+    __device__ __forceinline__ explicit LongRow(int classes) : C(classes), last((classes - 1) / SPAN) {}
+    // (the pieces' starts are a few scalar instructions; kept from row to row they would take the registers)
+    __device__ __forceinline__ LongRow again() const {
+        LongRow r = *this;
+        r.C = __builtin_amdgcn_readfirstlane(C);
+        r.last = __builtin_amdgcn_readfirstlane(last);
+        asm volatile("" : "+s"(r.C), "+s"(r.last));
+        return r;
+    }
+    __device__ __forceinline__ int start(int i) const { return i < last ? i * SPAN : C - SPAN; }
+    __device__ __forceinline__ uint32_t shared() const {  // bits of the thread's elements of the last piece that the one before holds
+        const int n = last * SPAN - (C - SPAN + (int)threadIdx.x * VEC);
+        return n <= 0 ? 0u : n >= VEC ? 0xffu : (1u << n) - 1;
+    }
+    __device__ __forceinline__ int place(int cls) const {  // the class's element, counted piece by piece and thread by thread
+        const int piece = cls / SPAN;
+        return piece * SPAN + cls - start(piece);
+    }
+    __device__ __forceinline__ Piece load(const typename T::E* z, int i) const { return load_piece<T>(z + start(i) + (unsigned)(threadIdx.x * VEC)); }
+};
+
+// What goes from kernel to kernel with a long row: the teacher's totals, made before (in 64 bits, whose constants would take
+// registers from the pieces), and whether the row is beyond FAR.
+struct RowNote { float total, rest; int far, unused; };
+static_assert(sizeof(RowNote) == sizeof(Sums), "both live in the rows' workspace");
+__global__ __launch_bounds__(64) void distill_notes_kernel(DistillArgs a, RowNote* notes) {
+    const long p = blockIdx.x;
+    const Kept e = load_kept(a, p, threadIdx.x);
+    if (threadIdx.x == 0) notes[p] = {e.total, e.rest, 0, 0};
+}
+
+// The next row in the loss from `p` on, the rows outside it zeroed; `rows` behind the last.
+template <class T, int NT>
+__device__ __forceinline__ int next_row(const DistillArgs& a, int p, float& w) {
+    const int rows = a.g.outer, C = a.g.classes;
+    for (; p < rows; p += gridDim.x) {
+        w = uniform(position_weight(a, p));
+        if (w != 0.f) break;
+        zero_row<T, NT>((typename T::E*)a.d_logits + (long)p * C, 0, C);
+        if (threadIdx.x == 0 && a.part) a.part[p] = 0.f;
+    }
+    return p;
+}
+
+// Workgroups of 512 threads that the registers of a CU hold at NV pieces a thread.
+constexpr int long_groups(int NV) { return NV <= 16 ? 2 : 1; }
+
+template <class T, int NT, int NV>
+__global__ __launch_bounds__(NT, 2 * long_groups(NV)) void distill_long_rows_kernel(DistillArgs a, RowNote* notes) {
+    constexpr int VEC = T::VEC;
+    __shared__ __align__(16) uint32_t flags[NT * NV / 4];  // a byte per piece: which of its elements are kept classes
+    __shared__ Sums red[NT / 64];
+    __shared__ int s_cls[MAX_TOP];
+    __shared__ float s_d[MAX_TOP], s_row[2];
+    if (a.upstream && a.skip_unit && a.upstream[0] == 1.f) return;
+    const int C = a.g.classes, lane = threadIdx.x & 63, rows = a.g.outer;
+    const float c = a.g.c;
+    const LongRow<T, NT> row_at(C);
+    const uint8_t* flag = (const uint8_t*)flags;
+    for (int i = threadIdx.x; i < NT * NV / 4; i += NT) flags[i] = 0;
+    __syncthreads();
+    float w = 0.f;
+    int p = next_row<T, NT>(a, blockIdx.x, w);
+    if (p >= rows) return;
+    int cls = -1;
+    float value = -INFINITY;
+    if (threadIdx.x < 64) read_kept(a, p, lane, cls, value);
+    const typename T::E* z = (const typename T::E*)a.g.logits + (long)p * a.g.ld;
+    Piece q[NV];
+#pragma unroll
+    for (int i = 0; i < NV; ++i) q[i] = row_at.load(z, i);
+    while (p < rows) {
+        float next_w = 0.f;
+        const int next = next_row<T, NT>(a, p + gridDim.x, next_w);
+        const typename T::E* next_z = (const typename T::E*)a.g.logits + (long)(next < rows ? next : p) * a.g.ld;  // (at the end: once more)
+        int word = 0;
+        KeptLane l;
+        if (threadIdx.x < 64) {
+            bool again = false;
+            if (cls >= 0) {
+                const int place = row_at.place(cls), byte = place / VEC;
+                const uint32_t bit = 1u << (byte % 4 * 8 + place % VEC);
+                word = byte / 4;
+                again = atomicOr(&flags[word], bit) & bit;
+            }
+            s_cls[lane] = cls;
+            l = kept_lane<T, false>(a, cls, value, z, lane, __any(again));
+            if (a.log_probs) {
+                l.e.total = notes[p].total;
+                l.e.rest = notes[p].rest;
+            }
+        }
+        __syncthreads();
+        const int last = row_at.last;
+        const uint32_t shared = row_at.shared();
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            uint32_t f = flag[i * NT + threadIdx.x];
+            if (i >= last) f = i > last ? 0xffu : f | shared;
+            if (__any(f != 0)) T::clear(q[i], f);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        const Sums own = tile_sums<T, NT, NV>(q, c);
+        keep_packed<NV>(q);
+        const Sums rest = block_sums<NT>(own, red);
+        if (threadIdx.x < 64) {
+            float d;
+            const RowResult row = join_row<T>(a, p, w, l, rest, d, lane, true);
+            s_d[lane] = d;
+            if (lane == 0) {
+                s_row[0] = row.factor;
+                s_row[1] = row.ref;
+                if (is_far(row.all.m, c)) notes[p].far = 1;
+            }
+        }
+        int next_cls = -1;
+        float next_value = -INFINITY;
+        if (threadIdx.x < 64 && next < rows) read_kept(a, next, lane, next_cls, next_value);
+        __syncthreads();
+        typename T::E* dz = (typename T::E*)a.d_logits + (long)p * C;
+        const float F = s_row[0], R = s_row[1];
+#pragma unroll
+        for (int i = NV - 1; i >= 0; --i) {
+            const LongRow<T, NT> at = row_at.again();
+            float o[VEC];
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) o[e] = F * exp2_(__builtin_fmaf(T::get(q[i], e), c, -R));
+            if (i <= at.last) store_piece<T>(dz + at.start(i) + (unsigned)(threadIdx.x * VEC), T::pack(o));
+            q[i] = at.load(next_z, i);
+            if (i == at.last) __syncthreads();  // (the shared elements: the piece before writes them after this one's zeros)
+            __builtin_amdgcn_sched_barrier(0);  // (moved up, the loads would hold a second row's registers)
+        }
+        __syncthreads();
+        if (cls >= 0) {  // the first wave: over the pieces' values there; it marks the next row's classes, too
+            flags[word] = 0;
+            dz[cls] = T::down(s_d[lane]);
+        }
+        p = next; w = next_w; z = next_z; cls = next_cls; value = next_value;
+    }
+}
+
+// The rows that distill_long_rows_kernel found beyond FAR, anew (a kernel of its own: what it keeps would take registers from the
+// long rows' pieces).
+template <class T>
+__global__ __launch_bounds__(256) void distill_far_rows_kernel(DistillArgs a, const RowNote* notes) {
+    __shared__ Stats red[4];
+    __shared__ int s_cls[MAX_TOP];
+    __shared__ float s_q[MAX_TOP], s_tot[2];
+    if (a.upstream && a.skip_unit && a.upstream[0] == 1.f) return;
+    const long p = blockIdx.x;
+    if (!notes[p].far) return;
+    const float x = distill_position<T>(a, p, position_weight(a, p), red, s_cls, s_q, s_tot);
+    if (threadIdx.x == 0 && a.part) a.part[p] = x;
 }
 
 // Calls put(i, e, lane) for every kept class inside a tile: lane holds the class, i and e name the piece and element of the
@@ -766,7 +938,8 @@ __global__ __launch_bounds__(NT) void distill_tiles_kernel(DistillArgs a, int ti
 }
 
 // Tiles of the row kernels: 32 elements a thread; one wave up to 2048 classes, four beyond.
-constexpr int SHORT_ROW = 2048, ROW_TILE = 8192;
+constexpr int SHORT_ROW = 2048, ROW_TILE = 8192, CUS = 256;
+constexpr int LONG_NT = 512;  // threads of a long row: with 1024, what a thread keeps beside the pieces counts twice
 #ifndef LP_EPT
 #define LP_EPT 16
 #endif
@@ -820,16 +993,25 @@ static void launch_distill_rows(const DistillArgs& a, int dtype, Sums* parts, bo
     const int rows = a.g.outer, C = a.g.classes;
     constexpr int V = T::VEC;
 #define HELD(NT, EPT) hipLaunchKernelGGL((distill_rows_kernel<T, NT, EPT / V>), dim3(rows), dim3(NT), 0, stream, a)
-    if (held_rows(rows, C, dtype)) {
+#define LONG(EPT)                                                                                                              \
+    do {                                                                                                                       \
+        RowNote* notes = (RowNote*)parts;                                                                                      \
+        const int groups = CUS * long_groups(EPT / V);                                                                         \
+        if (!again) hipLaunchKernelGGL(distill_notes_kernel, dim3(rows), dim3(64), 0, stream, a, notes);                         \
+        hipLaunchKernelGGL((distill_long_rows_kernel<T, LONG_NT, EPT / V>), dim3(rows < groups ? rows : groups), dim3(LONG_NT), 0, stream, a, notes); \
+        hipLaunchKernelGGL((distill_far_rows_kernel<T>), dim3(rows), dim3(256), 0, stream, a, (const RowNote*)notes);            \
+    } while (0)
+    if (held_rows(rows, C, dtype) && (C <= 32768 || a.d_logits)) {  // (without a gradient one pass over slices does)
         if (C <= 2048) HELD(64, 32);
         else if (C <= 8192) HELD(256, 32);
         else if (C <= 16384) HELD(512, 32);
         else if (C <= 32768) HELD(1024, 32);
-        else if (C <= 65536) HELD(1024, 64);
-        else if constexpr (V == 8) HELD(1024, 128);
+        else if (C <= 65536) LONG(128);
+        else if constexpr (V == 8) LONG(256);
         return;
     }
 #undef HELD
+#undef LONG
     const int tiles = (C + ROW_TILE - 1) / ROW_TILE;
     const Split d = split_row(rows, C, ROW_TILE);
     if (!again) hipLaunchKernelGGL((distill_slices_kernel<T, 256, 32 / V>), dim3((unsigned)rows * d.slices), dim3(256), 0, stream, a, d.slices, d.tiles, parts);
