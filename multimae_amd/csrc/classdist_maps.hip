@@ -482,6 +482,336 @@ __global__ __launch_bounds__(1024) void distill_map_kernel(DistillArgs a, int ti
     }
 }
 
+// ---- many positions, up to 136 classes: a wave per tile, the logits in its registers ------------------------------------
+// The tile in the LDS bounds the maps' kernels above by latency: 34 KiB of 133 fp32 classes leave three workgroups on a CU,
+// each in one phase at a time.  Held in registers the same tile takes no LDS and no other wave: 12 waves a CU that wait for
+// nobody.  CP: classes held (the first MIN of them exist).
+constexpr int REG_CLASSES = 136, REG_TOP = 16;
+// Waves per SIMD that the registers have to allow.
+constexpr int reg_waves(int CP) { return CP <= 32 ? 3 : 3; }
+
+// Class after class of a map: a uniform address that one scalar addition moves on, and the lane's offset beside it (as vector
+// addresses, 136 classes would take the registers).
+template <class E> using Global = __attribute__((address_space(1))) E;
+template <class E>
+__device__ __forceinline__ void step(Global<E>*& row, int inner) {
+    row += inner;
+    asm volatile("" : "+s"(row));
+}
+template <class T, int CP, int MIN>
+__device__ __forceinline__ void load_classes(float (&x)[CP], const typename T::E* z, unsigned px, int C, int inner) {
+    typedef typename T::E E;
+    Global<const E>* row = (Global<const E>*)z;
+    E raw[CP];  // (all of them on their way before the first is converted)
+#pragma unroll
+    for (int j = 0; j < CP; ++j) {  // (behind the last class: the last one again; under a branch each load would be waited for)
+        raw[j] = row[px];
+        step(row, j + 1 < MIN || j + 1 < C ? inner : 0);
+    }
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int j = 0; j < CP; ++j) {
+        x[j] = T::up(raw[j]);
+        if (j >= MIN && j >= C) x[j] = -INFINITY;
+        if (sizeof(E) == 2) asm("" : "+v"(x[j]));  // (one register a class from here on: not the 16 bits and the fp32 value)
+    }
+}
+template <int CP>
+__device__ __forceinline__ float max_of(const float (&x)[CP]) {
+    static_assert(CP % 2 == 0, "in pairs");
+    float m = -INFINITY;
+#pragma unroll
+    for (int j = 0; j < CP; j += 2) asm("v_max3_f32 %0, %1, %2, %3" : "=v"(m) : "v"(m), "v"(x[j]), "v"(x[j + 1]));  // (fmaxf quiets each operand first)
+    return m;
+}
+
+template <class T, int CP, int MIN, int K>
+__global__ __launch_bounds__(64, reg_waves(CP)) void log_probs_map_regs_kernel(LogProbArgs a, int tiles) {
+    __shared__ float s_x[K ? (QUEUE + 1) * POS : 1];       // the queue: values and classes; the place behind it takes the overflow
+    __shared__ uint32_t s_c[K ? (QUEUE + 1) * POS : 1], s_slot[K ? K * POS : 1];
+    const int C = a.g.classes, inner = a.g.inner, k = a.k, lane = threadIdx.x;
+    const int b = blockIdx.x / tiles, i0 = blockIdx.x % tiles * POS, n = inner - i0 < POS ? inner - i0 : POS;
+    const unsigned px = lane < n ? lane : 0;
+    const typename T::E* z = (const typename T::E*)a.g.logits + b * a.g.ld + i0;
+    const long p = (long)b * inner + i0 + px;
+    const float c = a.g.c;
+    const long y = a.target[p];
+    float x[CP];
+    load_classes<T, CP, MIN>(x, z, px, C, inner);
+    const float named = T::up(z[(y >= 0 && y < C ? y : 0) * inner + px]);
+    const float m = max_of(x), R = reference_exponent(m, c);
+    float s = 0.f, t = 0.f;
+#pragma unroll
+    for (int j = 0; j < CP; j += 8) {
+        float s8 = 0.f, t8 = 0.f;
+#pragma unroll
+        for (int u = 0; u < 8; ++u) {
+            const float d = __builtin_fmaf(x[j + u], c, -R), e = exp2_(d);
+            s8 += e;
+            t8 = __builtin_fmaf(e, bounded(d), t8);
+        }
+        s += s8;
+        t += t8;
+    }
+    const bool nan = s != s;
+    if (__any(is_far(m, c) && !nan)) {
+        float fs = 0.f, ft = 0.f;
+#pragma unroll
+        for (int j = 0; j < CP; ++j) {
+            const float d = (x[j] - m) * c, e = exp2_(d);
+            fs += e;
+            ft += e * bounded(d);
+        }
+        if (is_far(m, c) && !nan) { s = fs; t = ft; }
+    }
+    if (m == INFINITY) s = __builtin_nanf("");
+    const bool empty = m == -INFINITY && s == 0.f;
+    const float l2 = empty ? INFINITY : log2_(s);
+    if (lane < n) {
+        a.log_prob[p] = y >= 0 && y < C ? row_log_p(a.g, named, m, l2) : 0.f;
+        a.entropy[p] = empty ? 0.f : (l2 - t / s) * LN2;
+        if (a.row_max) {
+            a.row_max[p] = m;
+            a.row_log_sum[p] = l2;
+        }
+    }
+    if constexpr (K > 0) {
+        const bool any_nan = __any(nan);
+        if (any_nan) {  // NaN ranks as +inf
+#pragma unroll
+            for (int j = 0; j < CP; ++j) x[j] = x[j] != x[j] ? INFINITY : x[j];
+        }
+        float best[K];
+#pragma unroll
+        for (int i = 0; i < K; ++i) {
+            best[i] = -INFINITY;
+            s_slot[i * POS + lane] = NONE;
+        }
+#pragma unroll
+        for (int j = 0; j < CP; ++j) list_add(best, x[j]);
+        float least = best[0];
+#pragma unroll
+        for (int i = 1; i < K; ++i) least = i == k - 1 ? best[i] : least;
+        int queued = 0;
+        auto drain = [&]() {
+            for (int i = 0; __any(i < queued); ++i)
+                if (i < queued) {
+                    const float v = s_x[i * POS + lane];
+                    uint32_t cls = s_c[i * POS + lane];
+                    int rank = 0, end = 0;
+#pragma unroll
+                    for (int r = 0; r < K; ++r) {
+                        rank += best[r] > v;
+                        end += best[r] >= v;
+                    }
+                    if (end > k) end = k;
+                    for (int q = rank; q < end && cls != NONE; ++q) {  // equal values: the lower class first
+                        const uint32_t old = s_slot[q * POS + lane];
+                        if (cls < old) {
+                            s_slot[q * POS + lane] = cls;
+                            cls = old;
+                        }
+                    }
+                }
+            queued = 0;
+        };
+#pragma unroll
+        for (int j = 0; j < CP; ++j)
+            if (x[j] >= least && (j < MIN || j < C)) {
+                const int at = (queued < QUEUE ? queued : QUEUE) * POS + lane;
+                s_x[at] = x[j];
+                s_c[at] = j;
+                ++queued;
+            }
+        if (__any(queued > QUEUE)) {  // many equal values: class after class, a full queue emptied at once
+            queued = 0;
+            for (int j = 0; j < C; ++j) {
+                float v = T::up(z[(long)j * inner + px]);
+                if (v != v) v = INFINITY;
+                if (v >= least) {
+                    s_x[queued * POS + lane] = v;
+                    s_c[queued++ * POS + lane] = j;
+                }
+                if (__any(queued == QUEUE)) drain();
+            }
+        }
+        drain();
+        if (lane < n) {
+#pragma unroll
+            for (int i = 0; i < K; ++i)
+                if (i < k) {
+                    const long at = ((long)b * k + i) * inner + i0 + lane;
+                    a.top_class[at] = s_slot[i * POS + lane];
+                    a.top_log_prob[at] = row_log_p(a.g, best[i], m, l2);
+                }
+        }
+    }
+}
+
+// Distillation.  The kept classes of a position are bits of a mask; the gradient leaves from the registers, and what belongs to
+// the kept classes is written over it by the same lane.
+template <class T, int CP, int MIN, bool REST>
+__global__ __launch_bounds__(64, reg_waves(CP)) void distill_map_regs_kernel(DistillArgs a, int tiles) {
+    constexpr int WORDS = (CP + 31) / 32;
+    extern __shared__ __align__(16) char smem[];
+    if (a.upstream && a.skip_unit && a.upstream[0] == 1.f) return;
+    typedef typename T::E E;
+    const int C = a.g.classes, inner = a.g.inner, k = a.k, lane = threadIdx.x;
+    int* s_cls = (int*)smem;              // [k][POS]: the class, -1 for padding and for entries listed before
+    float* s_q = (float*)(s_cls + k * POS);  // its share of q, later its gradient
+    float* s_z = s_q + k * POS;           // the student's logit
+    const int b = blockIdx.x / tiles, i0 = blockIdx.x % tiles * POS, n = inner - i0 < POS ? inner - i0 : POS;
+    const unsigned px = lane < n ? lane : 0;
+    const E* z = (const E*)a.g.logits + b * a.g.ld + i0;
+    E* dz = (E*)a.d_logits + (long)b * C * inner + i0;
+    const float c = a.g.c, w = lane < n ? position_weight(a, (long)b * inner + i0 + lane) : 0.f;
+    const bool write = a.d_logits && lane < n;
+    if (!__any(w != 0.f)) {
+        if (write)
+            for (int j = 0; j < C; ++j) dz[(long)j * inner + px] = T::down(0.f);
+        if (lane == 0 && a.part) a.part[blockIdx.x] = 0.f;
+        return;
+    }
+    const long at = (long)b * k * inner + i0 + px;
+    float top = -INFINITY;
+    uint32_t kept[WORDS] = {};
+    bool again = false;
+    for (int i = 0; i < k; ++i) {
+        const long named = load_class(a.top_class, a.class_bytes, at + (long)i * inner);
+        const float v = load_any(a.top_value, a.value_dtype, at + (long)i * inner);
+        const bool in = named >= 0 && named < C;
+        const int cls = in ? (int)named : -1;
+        s_cls[i * POS + lane] = cls;
+        s_q[i * POS + lane] = in ? v : -INFINITY;
+        if (in) top = fmaxf(top, v);
+#pragma unroll
+        for (int u = 0; u < WORDS; ++u) {
+            const uint32_t bit = in && cls / 32 == u ? 1u << cls % 32 : 0u;
+            again |= (kept[u] & bit) != 0;
+            kept[u] |= bit;
+        }
+    }
+    float x[CP];
+    load_classes<T, CP, MIN>(x, z, px, C, inner);
+#pragma unroll 4
+    for (int i = 0; i < k; ++i) {
+        const int cls = s_cls[i * POS + lane];
+        s_z[i * POS + lane] = cls >= 0 ? T::up(z[(long)cls * inner + px]) : -INFINITY;
+    }
+    float total, left = 0.f, loss = 0.f;  // sum of q, what it leaves, the position's loss
+    if (REST) {
+        double sum = 0.0;  // 64 bits: the rest is what a sum near 1 leaves
+#pragma unroll 1
+        for (int i = 0; i < k; ++i) {
+            const float v = s_q[i * POS + lane], q = exp_(v);
+            sum += exp((double)v);
+            if (q != 0.f) loss += q * v;
+            s_q[i * POS + lane] = q;
+        }
+        total = (float)sum;
+        left = sum != sum ? total : fmaxf((float)(1.0 - sum), 0.f);
+    } else {
+        top = finite_ref(top);
+        float sum = 0.f;
+#pragma unroll 1
+        for (int i = 0; i < k; ++i) {
+            const float d = s_q[i * POS + lane] - top, q = exp2_(d * c);
+            sum += q;
+            if (q != 0.f) loss += q * d;
+            s_q[i * POS + lane] = q;
+        }
+        const float inv = sum != 0.f ? 1.f / sum : 0.f;
+#pragma unroll 1
+        for (int i = 0; i < k; ++i) s_q[i * POS + lane] *= inv;
+        total = sum > 0.f ? 1.f : (sum != sum ? sum : 0.f);
+        loss = sum != 0.f ? loss * inv * a.g.inv_t - log2_(sum) * LN2 : 0.f;
+    }
+    if (__any(again)) {
+        for (int i = 1; i < k; ++i)
+            for (int j = 0; j < i; ++j) {
+                const int cls = s_cls[i * POS + lane];
+                if (cls >= 0 && s_cls[j * POS + lane] == cls) {
+                    s_q[j * POS + lane] += s_q[i * POS + lane];
+                    s_cls[i * POS + lane] = -1;
+                }
+            }
+    }
+    if (REST) {
+#pragma unroll
+        for (int j = 0; j < CP; ++j) x[j] = kept[j / 32] >> j % 32 & 1 ? -INFINITY : x[j];
+    }
+    Sums rest = {max_of(x), 0.f, 0.f, 0.f};
+    rest.R = reference_exponent(rest.m, c);
+#pragma unroll
+    for (int j = 0; j < CP; j += 8) {
+        float s8 = 0.f;
+#pragma unroll
+        for (int u = 0; u < 8; ++u) {
+            x[j + u] = exp2_(__builtin_fmaf(x[j + u], c, -rest.R));
+            s8 += x[j + u];
+        }
+        rest.s += s8;
+    }
+    Sums v = rest;  // the whole position
+    if (REST)
+#pragma unroll 1
+        for (int i = 0; i < k; ++i)
+            if (s_cls[i * POS + lane] >= 0) {
+                const float one[1] = {s_z[i * POS + lane]};
+                add_logits<1, false>(v, one, c);
+            }
+    // A wave with a position beyond FAR goes by (z - m) c, class after class from memory.
+    const bool far = __any(is_far(v.m, c));
+    const float m = finite_ref(v.m);
+    if (far) {
+        rest.s = v.s = 0.f;
+        for (int j = 0; j < C; ++j) {
+            const float e = exp2_((T::up(z[(long)j * inner + px]) - m) * c);
+            bool out = REST;
+            for (int i = 0; i < k && out; ++i) out = s_cls[i * POS + lane] != j;
+            v.s += e;
+            if (!REST || out) rest.s += e;
+        }
+    }
+    if (v.m == INFINITY) v.s = __builtin_nanf("");
+    const bool empty = v.m == -INFINITY && v.s == 0.f;
+    const float own_l2 = empty ? INFINITY : log2_(v.s);  // relative to what the sums are relative to, and to R
+    const float l2 = far && !is_far(v.m, c) ? own_l2 + __builtin_fmaf(m, c, -v.R) : own_l2;
+    const float r = REST && rest.s != 0.f ? left : 0.f, Q = total + r, rest_R = far ? v.R : rest.R;
+    const float gs = empty ? 0.f : w * a.g.inv_t * (a.upstream ? a.upstream[0] : 1.f);
+#pragma unroll 1
+    for (int i = 0; i < k; ++i) {
+        const int cls = s_cls[i * POS + lane];
+        if (cls < 0) continue;
+        const float q = s_q[i * POS + lane], zk = s_z[i * POS + lane];
+        if (q != 0.f) loss -= q * row_log_p(a.g, zk, v.m, l2);
+        const float d = far ? (zk - m) * c : __builtin_fmaf(zk, c, -v.R);
+        s_q[i * POS + lane] = w != 0.f ? gs * (exp2_(d - own_l2) * Q - q) : 0.f;
+    }
+    if (r != 0.f) loss += r * (log2_(r) - ((rest_R - v.R) + log2_(rest.s) - own_l2)) * LN2;
+    loss = wave_sum(w != 0.f ? w * loss : 0.f);
+    if (lane == 0 && a.part) a.part[blockIdx.x] = loss;
+    if (!write) return;
+    const float F = w != 0.f ? gs * (Q * exp2_(rest_R - v.R - own_l2) - (r != 0.f ? r / rest.s : 0.f)) : 0.f;
+    if (far) {
+        for (int j = 0; j < C; ++j) {
+            const float e = exp2_((T::up(z[(long)j * inner + px]) - m) * c);
+            dz[(long)j * inner + px] = T::down(F != 0.f ? F * e : 0.f);
+        }
+    } else {
+        Global<E>* row = (Global<E>*)dz;
+#pragma unroll
+        for (int j = 0; j < CP; ++j) {
+            if (j < MIN || j < C) row[px] = T::down(F != 0.f ? F * x[j] : 0.f);  // (outside the loss a logit may be anything)
+            step(row, inner);
+        }
+    }
+    for (int i = 0; i < k; ++i) {
+        const int cls = s_cls[i * POS + lane];
+        if (cls >= 0) dz[(long)cls * inner + px] = T::down(s_q[i * POS + lane]);
+    }
+}
+
 // Waves of a workgroup: enough that the workgroups whose tiles fit a CU bring 16, more where the map has few tiles.
 int map_waves(long tiles, int bytes, int classes) {
     const int on_cu = LDS_BYTES / bytes < 1 ? 1 : LDS_BYTES / bytes;
@@ -521,8 +851,36 @@ int launch_log_probs_map(const LogProbArgs& a, hipStream_t stream) {
     hipLaunchKernelGGL((log_probs_map_kernel<T, K>), dim3((unsigned)((long)a.g.outer * tiles)), dim3(64 * waves), bytes, stream, a, tiles);
     return MMAE_OK;
 }
+// The register kernels: enough tiles that every CU has its 12 waves, classes and alternatives that fit.  Fewer tiles are shared
+// by the waves of a workgroup instead.
+#ifndef REG_TILES
+#define REG_TILES 2048
+#endif
+bool in_registers(long tiles, int classes, int k) { return tiles >= REG_TILES && classes <= REG_CLASSES && k <= REG_TOP; }
+
+#define BY_CLASSES(C, CALL)             \
+    do {                                \
+        if ((C) <= 32) CALL(32, 0);     \
+        else if ((C) <= 64) CALL(64, 32); \
+        else if ((C) <= 104) CALL(104, 64); \
+        else CALL(136, 104);            \
+    } while (0)
+
 template <class T>
 int launch_log_probs_map(const LogProbArgs& a, hipStream_t stream) {
+    const int tiles = map_tiles(a.g.inner);
+    const long all = (long)a.g.outer * tiles;
+    if (in_registers(all, a.g.classes, a.k)) {
+#define CALL(CP, MIN)                                                                                                              \
+    do {                                                                                                                           \
+        if (a.k == 0) hipLaunchKernelGGL((log_probs_map_regs_kernel<T, CP, MIN, 0>), dim3((unsigned)all), dim3(64), 0, stream, a, tiles); \
+        else if (a.k <= 8) hipLaunchKernelGGL((log_probs_map_regs_kernel<T, CP, MIN, 8>), dim3((unsigned)all), dim3(64), 0, stream, a, tiles); \
+        else hipLaunchKernelGGL((log_probs_map_regs_kernel<T, CP, MIN, 16>), dim3((unsigned)all), dim3(64), 0, stream, a, tiles);     \
+    } while (0)
+        BY_CLASSES(a.g.classes, CALL);
+#undef CALL
+        return MMAE_OK;
+    }
     switch (list_slots(a.k)) {
         case 0: return launch_log_probs_map<T, 0>(a, stream);
         case 8: return launch_log_probs_map<T, 8>(a, stream);
@@ -535,6 +893,13 @@ int launch_log_probs_map(const LogProbArgs& a, hipStream_t stream) {
 template <class T, bool REST>
 int launch_distill_map(const DistillArgs& a, hipStream_t stream) {
     const int tiles = map_tiles(a.g.inner), C = a.g.classes, k = a.k;
+    const long all = (long)a.g.outer * tiles;
+    if (in_registers(all, C, k)) {
+#define CALL(CP, MIN) hipLaunchKernelGGL((distill_map_regs_kernel<T, CP, MIN, REST>), dim3((unsigned)all), dim3(64), 3 * k * POS * 4, stream, a, tiles)
+        BY_CLASSES(C, CALL);
+#undef CALL
+        return MMAE_OK;
+    }
     const int waves = fitting_waves((long)a.g.outer * tiles, C, [&](int w) { return distill_map_bytes(sizeof(typename T::E), C, k, w); },
                                     LDS_BYTES - DISTILL_STATIC, 16);
     const int bytes = distill_map_bytes(sizeof(typename T::E), C, k, waves);
