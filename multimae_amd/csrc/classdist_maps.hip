@@ -51,6 +51,28 @@ __device__ __forceinline__ void load_map_tile(typename T::E* tile, const typenam
     }
 }
 
+// Reads a position's kept entries in groups, every load of a group on its way before the first is used: take(i, class or -1, value).
+template <class F>
+__device__ __forceinline__ void read_entries(const DistillArgs& a, long at, bool live, F take) {
+    constexpr int G = 8;
+    for (int i0 = 0; i0 < a.k; i0 += G) {
+        long cls[G];
+        float v[G];
+#pragma unroll
+        for (int u = 0; u < G; ++u) {
+            const long e = at + (long)(i0 + u < a.k ? i0 + u : a.k - 1) * a.g.inner;
+            cls[u] = load_class(a.top_class, a.class_bytes, e);
+            v[u] = load_any(a.top_value, a.value_dtype, e);
+        }
+#pragma unroll
+        for (int u = 0; u < G; ++u)
+            if (i0 + u < a.k) {
+                const bool in = live && cls[u] >= 0 && cls[u] < a.g.classes;
+                take(i0 + u, in ? (int)cls[u] : -1, in ? v[u] : -INFINITY);
+            }
+    }
+}
+
 // Adds the exponentials of N logits to a lane's running sums.
 template <int N, bool ENTROPY>
 __device__ __forceinline__ void add_logits(Sums& v, const float (&x)[N], float c) {
@@ -80,7 +102,29 @@ __device__ __forceinline__ void add_logits(Sums& v, const float (&x)[N], float c
 // The waves' lists are joined (the larger ends of two sorted lists, sorted again by halving strides).  A second pass finds
 // the classes: those that reach the k-th best value wait in a short queue per lane and go to the slot their rank names;
 // equal values share a run of slots, which atomic minima keep in the order of classes whatever wave comes first.
+//
+// The 16-bit types leave the low bits of an fp32 number free: there a value carries its class along, so that the sorted list is
+// the answer and the second pass falls away.
 constexpr int QUEUE = 16;
+constexpr int CODE_BITS = 12;                   // of a carried class: the mantissa bits that bf16 (16) and f16 (13) leave
+constexpr uint32_t CODES = (1u << CODE_BITS) - 1, CARRIED_INF = 0x7f800000u - (1u << CODE_BITS);  // above the largest finite value of both
+template <class T> constexpr bool carries() { return sizeof(typename T::E) == 2; }
+
+// As fp32 numbers, larger values come first and equal ones by the lower class; +-inf (and NaN, as +inf) stay finite.
+__device__ __forceinline__ float carry(float v, uint32_t cls) {
+    const float big = __uint_as_float(CARRIED_INF);
+    const uint32_t b = __float_as_uint(__builtin_amdgcn_fmed3f(v + 0.0f, -big, big));
+    const uint32_t negative = (uint32_t)((int32_t)b >> 31);
+    return __uint_as_float(b | ((negative & CODES) ^ (CODES ^ cls)));
+}
+__device__ __forceinline__ uint32_t carried_class(float key) {
+    const uint32_t b = __float_as_uint(key), negative = (uint32_t)((int32_t)b >> 31);
+    return (b ^ (negative & CODES) ^ CODES) & CODES;
+}
+__device__ __forceinline__ float carried_value(float key) {
+    const uint32_t b = __float_as_uint(key) & ~CODES;
+    return (b & 0x7fffffffu) == CARRIED_INF ? __uint_as_float((b & 0x80000000u) | 0x7f800000u) : __uint_as_float(b);
+}
 
 template <int K>
 __device__ __forceinline__ void list_add(float (&a)[K], float x) {
@@ -94,8 +138,9 @@ __host__ __device__ constexpr int most_waves(int slots) { return slots == 64 ? 8
 __host__ __device__ inline int list_slots(int k) { return k == 0 ? 0 : k <= 8 ? 8 : k <= 16 ? 16 : k <= 32 ? 32 : 64; }
 // Bytes behind the tile: the waves' sums; their lists, later their queues; the slots.
 inline int log_probs_map_bytes(int element, int classes, int k, int waves) {
-    const int lists = waves * POS * list_slots(k) * 4, queues = k ? waves * POS * QUEUE * 4 : 0;
-    return (classes * POS * element + 15) / 16 * 16 + waves * POS * (int)sizeof(Sums) + (lists > queues ? lists : queues) + k * POS * 4;
+    const bool second = k && element == 4;  // queues and slots
+    const int lists = waves * POS * list_slots(k) * 4, queues = second ? waves * POS * QUEUE * 4 : 0;
+    return (classes * POS * element + 15) / 16 * 16 + waves * POS * (int)sizeof(Sums) + (lists > queues ? lists : queues) + (second ? k * POS * 4 : 0);
 }
 
 template <class T, int K>
@@ -112,7 +157,8 @@ __global__ __launch_bounds__(64 * most_waves(K)) void log_probs_map_kernel(LogPr
     const typename T::E* z = (const typename T::E*)a.g.logits + b * a.g.ld + i0;
     const float c = a.g.c;
     load_map_tile<T>(tile, z, C, inner, n);
-    for (int i = threadIdx.x; i < k * POS; i += blockDim.x) s_slot[i] = NONE;
+    if (!carries<T>())
+        for (int i = threadIdx.x; i < k * POS; i += blockDim.x) s_slot[i] = NONE;
     __syncthreads();
 
     const int c0 = (int)((long)C * wave / waves), c1 = (int)((long)C * (wave + 1) / waves);
@@ -127,7 +173,7 @@ __global__ __launch_bounds__(64 * most_waves(K)) void log_probs_map_kernel(LogPr
         add_logits<8, true>(v, x, c);
         if constexpr (K > 0) {
 #pragma unroll
-            for (int u = 0; u < 8; ++u) list_add(best, x[u]);
+            for (int u = 0; u < 8; ++u) list_add(best, carries<T>() ? (j + u < c1 ? carry(x[u], j + u) : -INFINITY) : x[u]);
         }
     }
     if constexpr (K > 0) {
@@ -140,7 +186,7 @@ __global__ __launch_bounds__(64 * most_waves(K)) void log_probs_map_kernel(LogPr
                     x = INFINITY;
                     tile[j * POS + lane] = T::down(x);
                 }
-                list_add(best, x);
+                list_add(best, carries<T>() ? carry(x, j) : x);
             }
         }
     }
@@ -190,6 +236,18 @@ __global__ __launch_bounds__(64 * most_waves(K)) void log_probs_map_kernel(LogPr
                         best[i] = hi;
                         best[i + o] = lo;
                     }
+        }
+        if constexpr (carries<T>()) {
+            if (lane < n) {
+#pragma unroll
+                for (int i = 0; i < K; ++i)
+                    if (i < k && i % waves == wave) {
+                        const long at = ((long)b * k + i) * inner + i0 + lane;
+                        a.top_class[at] = carried_class(best[i]);
+                        a.top_log_prob[at] = row_log_p(a.g, carried_value(best[i]), v.m, l2);
+                    }
+            }
+            return;
         }
         float least = best[0];  // the k-th best
 #pragma unroll
@@ -340,20 +398,13 @@ __global__ __launch_bounds__(1024) void distill_map_kernel(DistillArgs a, int ti
     load_map_tile<T>(tile, z, C, inner, n);
     float total = 0.f, left = 0.f, loss = 0.f;  // sum of q, what it leaves, the position's loss
     if (wave == 0) {
-        const long at = (long)b * k * inner + i0 + lane;
+        const long at = (long)b * k * inner + i0 + (lane < n ? lane : 0);
         float m = -INFINITY;
-        for (int i = 0; i < k; ++i) {
-            long cls = -1;
-            float x = -INFINITY;
-            if (lane < n) {
-                cls = load_class(a.top_class, a.class_bytes, at + (long)i * inner);
-                if (cls < 0 || cls >= C) cls = -1;
-                else x = load_any(a.top_value, a.value_dtype, at + (long)i * inner);
-            }
-            s_cls[i * POS + lane] = (int)cls;
+        read_entries(a, at, lane < n, [&](int i, int cls, float x) {
+            s_cls[i * POS + lane] = cls;
             s_q[i * POS + lane] = x;
             m = fmaxf(m, x);
-        }
+        });
         if (REST) {
             double sum = 0.0;  // 64 bits: the rest is what a sum near 1 leaves
             for (int i = 0; i < k; ++i) {
@@ -527,8 +578,9 @@ __device__ __forceinline__ float max_of(const float (&x)[CP]) {
 
 template <class T, int CP, int MIN, int K>
 __global__ __launch_bounds__(64, reg_waves(CP)) void log_probs_map_regs_kernel(LogProbArgs a, int tiles) {
-    __shared__ float s_x[K ? (QUEUE + 1) * POS : 1];       // the queue: values and classes; the place behind it takes the overflow
-    __shared__ uint32_t s_c[K ? (QUEUE + 1) * POS : 1], s_slot[K ? K * POS : 1];
+    constexpr int PLACES = K && !carries<T>() ? K + 4 : 0;  // of the queue: values and classes; the place behind it takes the overflow
+    __shared__ float s_x[PLACES ? (PLACES + 1) * POS : 1];
+    __shared__ uint32_t s_c[PLACES ? (PLACES + 1) * POS : 1], s_slot[PLACES ? K * POS : 1];
     const int C = a.g.classes, inner = a.g.inner, k = a.k, lane = threadIdx.x;
     const int b = blockIdx.x / tiles, i0 = blockIdx.x % tiles * POS, n = inner - i0 < POS ? inner - i0 : POS;
     const unsigned px = lane < n ? lane : 0;
@@ -583,10 +635,29 @@ __global__ __launch_bounds__(64, reg_waves(CP)) void log_probs_map_regs_kernel(L
         }
         float best[K];
 #pragma unroll
-        for (int i = 0; i < K; ++i) {
-            best[i] = -INFINITY;
-            s_slot[i * POS + lane] = NONE;
+        for (int i = 0; i < K; ++i) best[i] = -INFINITY;
+        if constexpr (carries<T>()) {
+#pragma unroll
+            for (int j = 0; j < CP; ++j) {  // (behind the last class: -inf of a higher class, which ranks behind all others)
+                list_add(best, carry(x[j], j));
+                if (j % 8 == 7) {  // (the list stands here: put off, it would keep all keys beside the values)
+#pragma unroll
+                    for (int i = 0; i < K; ++i) asm volatile("" : "+v"(best[i]));
+                }
+            }
+            if (lane < n) {
+#pragma unroll
+                for (int i = 0; i < K; ++i)
+                    if (i < k) {
+                        const long at = ((long)b * k + i) * inner + i0 + lane;
+                        a.top_class[at] = carried_class(best[i]);
+                        a.top_log_prob[at] = row_log_p(a.g, carried_value(best[i]), m, l2);
+                    }
+            }
+            return;
         }
+#pragma unroll
+        for (int i = 0; i < K; ++i) s_slot[i * POS + lane] = NONE;
 #pragma unroll
         for (int j = 0; j < CP; ++j) list_add(best, x[j]);
         float least = best[0];
@@ -618,12 +689,12 @@ __global__ __launch_bounds__(64, reg_waves(CP)) void log_probs_map_regs_kernel(L
 #pragma unroll
         for (int j = 0; j < CP; ++j)
             if (x[j] >= least && (j < MIN || j < C)) {
-                const int at = (queued < QUEUE ? queued : QUEUE) * POS + lane;
+                const int at = (queued < PLACES ? queued : PLACES) * POS + lane;
                 s_x[at] = x[j];
                 s_c[at] = j;
                 ++queued;
             }
-        if (__any(queued > QUEUE)) {  // many equal values: class after class, a full queue emptied at once
+        if (__any(queued > PLACES)) {  // many equal values: class after class, a full queue emptied at once
             queued = 0;
             for (int j = 0; j < C; ++j) {
                 float v = T::up(z[(long)j * inner + px]);
@@ -632,7 +703,7 @@ __global__ __launch_bounds__(64, reg_waves(CP)) void log_probs_map_regs_kernel(L
                     s_x[queued * POS + lane] = v;
                     s_c[queued++ * POS + lane] = j;
                 }
-                if (__any(queued == QUEUE)) drain();
+                if (__any(queued == PLACES)) drain();
             }
         }
         drain();
@@ -676,27 +747,29 @@ __global__ __launch_bounds__(64, reg_waves(CP)) void distill_map_regs_kernel(Dis
     float top = -INFINITY;
     uint32_t kept[WORDS] = {};
     bool again = false;
-    for (int i = 0; i < k; ++i) {
-        const long named = load_class(a.top_class, a.class_bytes, at + (long)i * inner);
-        const float v = load_any(a.top_value, a.value_dtype, at + (long)i * inner);
-        const bool in = named >= 0 && named < C;
-        const int cls = in ? (int)named : -1;
+    read_entries(a, at, true, [&](int i, int cls, float v) {
         s_cls[i * POS + lane] = cls;
-        s_q[i * POS + lane] = in ? v : -INFINITY;
-        if (in) top = fmaxf(top, v);
+        s_q[i * POS + lane] = v;
+        top = fmaxf(top, v);
 #pragma unroll
         for (int u = 0; u < WORDS; ++u) {
-            const uint32_t bit = in && cls / 32 == u ? 1u << cls % 32 : 0u;
+            const uint32_t bit = cls >= 0 && cls / 32 == u ? 1u << cls % 32 : 0u;
             again |= (kept[u] & bit) != 0;
             kept[u] |= bit;
         }
-    }
+    });
     float x[CP];
     load_classes<T, CP, MIN>(x, z, px, C, inner);
-#pragma unroll 4
-    for (int i = 0; i < k; ++i) {
-        const int cls = s_cls[i * POS + lane];
-        s_z[i * POS + lane] = cls >= 0 ? T::up(z[(long)cls * inner + px]) : -INFINITY;
+    for (int i0 = 0; i0 < k; i0 += 8) {
+        float zk[8];
+#pragma unroll
+        for (int u = 0; u < 8; ++u) {
+            const int cls = i0 + u < k ? s_cls[(i0 + u) * POS + lane] : 0;
+            zk[u] = T::up(z[(long)(cls < 0 ? 0 : cls) * inner + px]);
+        }
+#pragma unroll
+        for (int u = 0; u < 8; ++u)
+            if (i0 + u < k) s_z[(i0 + u) * POS + lane] = zk[u];
     }
     float total, left = 0.f, loss = 0.f;  // sum of q, what it leaves, the position's loss
     if (REST) {
