@@ -538,8 +538,6 @@ __global__ __launch_bounds__(1024) void distill_map_kernel(DistillArgs a, int ti
 // each in one phase at a time.  Held in registers the same tile takes no LDS and no other wave: 12 waves a CU that wait for
 // nobody.  CP: classes held (the first MIN of them exist).
 constexpr int REG_CLASSES = 136, REG_TOP = 16;
-// Waves per SIMD that the registers have to allow.
-constexpr int reg_waves(int CP) { return CP <= 32 ? 3 : 3; }
 
 // Class after class of a map: a uniform address that one scalar addition moves on, and the lane's offset beside it (as vector
 // addresses, 136 classes would take the registers).
@@ -577,7 +575,7 @@ __device__ __forceinline__ float max_of(const float (&x)[CP]) {
 }
 
 template <class T, int CP, int MIN, int K>
-__global__ __launch_bounds__(64, reg_waves(CP)) void log_probs_map_regs_kernel(LogProbArgs a, int tiles) {
+__global__ __launch_bounds__(64, 3) void log_probs_map_regs_kernel(LogProbArgs a, int tiles) {
     constexpr int PLACES = K && !carries<T>() ? K + 4 : 0;  // of the queue: values and classes; the place behind it takes the overflow
     __shared__ float s_x[PLACES ? (PLACES + 1) * POS : 1];
     __shared__ uint32_t s_c[PLACES ? (PLACES + 1) * POS : 1], s_slot[PLACES ? K * POS : 1];
@@ -587,10 +585,11 @@ __global__ __launch_bounds__(64, reg_waves(CP)) void log_probs_map_regs_kernel(L
     const typename T::E* z = (const typename T::E*)a.g.logits + b * a.g.ld + i0;
     const long p = (long)b * inner + i0 + px;
     const float c = a.g.c;
-    const long y = a.target[p];
+    const long target = a.target[p];
+    const int y = target >= 0 && target < C ? (int)target : -1;
     float x[CP];
     load_classes<T, CP, MIN>(x, z, px, C, inner);
-    const float named = T::up(z[(y >= 0 && y < C ? y : 0) * inner + px]);
+    const float named = T::up(z[(long)(y < 0 ? 0 : y) * inner + px]);
     const float m = max_of(x), R = reference_exponent(m, c);
     float s = 0.f, t = 0.f;
 #pragma unroll
@@ -620,7 +619,7 @@ __global__ __launch_bounds__(64, reg_waves(CP)) void log_probs_map_regs_kernel(L
     const bool empty = m == -INFINITY && s == 0.f;
     const float l2 = empty ? INFINITY : log2_(s);
     if (lane < n) {
-        a.log_prob[p] = y >= 0 && y < C ? row_log_p(a.g, named, m, l2) : 0.f;
+        a.log_prob[p] = y >= 0 ? row_log_p(a.g, named, m, l2) : 0.f;
         a.entropy[p] = empty ? 0.f : (l2 - t / s) * LN2;
         if (a.row_max) {
             a.row_max[p] = m;
@@ -719,18 +718,20 @@ __global__ __launch_bounds__(64, reg_waves(CP)) void log_probs_map_regs_kernel(L
     }
 }
 
-// Distillation.  The kept classes of a position are bits of a mask; the gradient leaves from the registers, and what belongs to
-// the kept classes is written over it by the same lane.
+// Distillation.  The kept classes of a position are bits of a mask; a kept class has a place in the LDS, the number of kept
+// classes below it, which a walk over the classes counts along.  So its logit gets there and its gradient back without a
+// load or store of its own, each of which would move a line per position.
 template <class T, int CP, int MIN, bool REST>
-__global__ __launch_bounds__(64, reg_waves(CP)) void distill_map_regs_kernel(DistillArgs a, int tiles) {
+__global__ __launch_bounds__(64, 2) void distill_map_regs_kernel(DistillArgs a, int tiles) {
     constexpr int WORDS = (CP + 31) / 32;
     extern __shared__ __align__(16) char smem[];
     if (a.upstream && a.skip_unit && a.upstream[0] == 1.f) return;
     typedef typename T::E E;
     const int C = a.g.classes, inner = a.g.inner, k = a.k, lane = threadIdx.x;
-    int* s_cls = (int*)smem;              // [k][POS]: the class, -1 for padding and for entries listed before
-    float* s_q = (float*)(s_cls + k * POS);  // its share of q, later its gradient
-    float* s_z = s_q + k * POS;           // the student's logit
+    int* s_cls = (int*)smem + lane;        // [k][POS], entry by entry: the class or -1, later with its place << 16
+    float* s_q = (float*)smem + k * POS + lane;      // the entry's q
+    float* s_z = s_q + k * POS;            // [k + 1][POS], place by place: the student's logit
+    float* s_d = s_z + (k + 1) * POS;      // the class's share of q, then its gradient
     const int b = blockIdx.x / tiles, i0 = blockIdx.x % tiles * POS, n = inner - i0 < POS ? inner - i0 : POS;
     const unsigned px = lane < n ? lane : 0;
     const E* z = (const E*)a.g.logits + b * a.g.ld + i0;
@@ -743,43 +744,27 @@ __global__ __launch_bounds__(64, reg_waves(CP)) void distill_map_regs_kernel(Dis
         if (lane == 0 && a.part) a.part[blockIdx.x] = 0.f;
         return;
     }
-    const long at = (long)b * k * inner + i0 + px;
     float top = -INFINITY;
     uint32_t kept[WORDS] = {};
-    bool again = false;
-    read_entries(a, at, true, [&](int i, int cls, float v) {
-        s_cls[i * POS + lane] = cls;
-        s_q[i * POS + lane] = v;
+    read_entries(a, (long)b * k * inner + i0 + px, true, [&](int i, int cls, float v) {
+        s_cls[i * POS] = cls;
+        s_q[i * POS] = v;
+        s_d[i * POS] = 0.f;
         top = fmaxf(top, v);
 #pragma unroll
-        for (int u = 0; u < WORDS; ++u) {
-            const uint32_t bit = cls >= 0 && cls / 32 == u ? 1u << cls % 32 : 0u;
-            again |= (kept[u] & bit) != 0;
-            kept[u] |= bit;
-        }
+        for (int u = 0; u < WORDS; ++u) kept[u] |= cls >= 0 && cls / 32 == u ? 1u << cls % 32 : 0u;
     });
     float x[CP];
     load_classes<T, CP, MIN>(x, z, px, C, inner);
-    for (int i0 = 0; i0 < k; i0 += 8) {
-        float zk[8];
-#pragma unroll
-        for (int u = 0; u < 8; ++u) {
-            const int cls = i0 + u < k ? s_cls[(i0 + u) * POS + lane] : 0;
-            zk[u] = T::up(z[(long)(cls < 0 ? 0 : cls) * inner + px]);
-        }
-#pragma unroll
-        for (int u = 0; u < 8; ++u)
-            if (i0 + u < k) s_z[(i0 + u) * POS + lane] = zk[u];
-    }
     float total, left = 0.f, loss = 0.f;  // sum of q, what it leaves, the position's loss
     if (REST) {
         double sum = 0.0;  // 64 bits: the rest is what a sum near 1 leaves
 #pragma unroll 1
         for (int i = 0; i < k; ++i) {
-            const float v = s_q[i * POS + lane], q = exp_(v);
+            const float v = s_q[i * POS], q = exp_(v);
             sum += exp((double)v);
             if (q != 0.f) loss += q * v;
-            s_q[i * POS + lane] = q;
+            s_q[i * POS] = q;
         }
         total = (float)sum;
         left = sum != sum ? total : fmaxf((float)(1.0 - sum), 0.f);
@@ -788,30 +773,39 @@ __global__ __launch_bounds__(64, reg_waves(CP)) void distill_map_regs_kernel(Dis
         float sum = 0.f;
 #pragma unroll 1
         for (int i = 0; i < k; ++i) {
-            const float d = s_q[i * POS + lane] - top, q = exp2_(d * c);
+            const float d = s_q[i * POS] - top, q = exp2_(d * c);
             sum += q;
             if (q != 0.f) loss += q * d;
-            s_q[i * POS + lane] = q;
+            s_q[i * POS] = q;
         }
         const float inv = sum != 0.f ? 1.f / sum : 0.f;
 #pragma unroll 1
-        for (int i = 0; i < k; ++i) s_q[i * POS + lane] *= inv;
+        for (int i = 0; i < k; ++i) s_q[i * POS] *= inv;
         total = sum > 0.f ? 1.f : (sum != sum ? sum : 0.f);
         loss = sum != 0.f ? loss * inv * a.g.inv_t - log2_(sum) * LN2 : 0.f;
     }
-    if (__any(again)) {
-        for (int i = 1; i < k; ++i)
-            for (int j = 0; j < i; ++j) {
-                const int cls = s_cls[i * POS + lane];
-                if (cls >= 0 && s_cls[j * POS + lane] == cls) {
-                    s_q[j * POS + lane] += s_q[i * POS + lane];
-                    s_cls[i * POS + lane] = -1;
-                }
-            }
-    }
-    if (REST) {
+    int places = 0;
 #pragma unroll
-        for (int j = 0; j < CP; ++j) x[j] = kept[j / 32] >> j % 32 & 1 ? -INFINITY : x[j];
+    for (int u = 0; u < WORDS; ++u) places += __popc(kept[u]);
+#pragma unroll 1
+    for (int i = 0; i < k; ++i) {
+        const int cls = s_cls[i * POS];
+        if (cls < 0) continue;
+        int place = 0;
+#pragma unroll
+        for (int u = 0; u < WORDS; ++u) place += __popc(kept[u] & (cls / 32 > u ? ~0u : cls / 32 == u ? (1u << cls % 32) - 1 : 0u));
+        s_cls[i * POS] = cls | place << 16;
+        s_d[place * POS] += s_q[i * POS];
+    }
+    {
+        float* at = s_z;  // every class is written, a kept one moves on: what stands at a place is the kept class's
+#pragma unroll
+        for (int j = 0; j < CP; ++j) {
+            const uint32_t bit = kept[j / 32] >> j % 32 & 1;
+            *at = x[j];
+            at += bit * POS;
+            if (REST) x[j] = bit ? -INFINITY : x[j];
+        }
     }
     Sums rest = {max_of(x), 0.f, 0.f, 0.f};
     rest.R = reference_exponent(rest.m, c);
@@ -828,11 +822,10 @@ __global__ __launch_bounds__(64, reg_waves(CP)) void distill_map_regs_kernel(Dis
     Sums v = rest;  // the whole position
     if (REST)
 #pragma unroll 1
-        for (int i = 0; i < k; ++i)
-            if (s_cls[i * POS + lane] >= 0) {
-                const float one[1] = {s_z[i * POS + lane]};
-                add_logits<1, false>(v, one, c);
-            }
+        for (int i = 0; i < places; ++i) {
+            const float one[1] = {s_z[i * POS]};
+            add_logits<1, false>(v, one, c);
+        }
     // A wave with a position beyond FAR goes by (z - m) c, class after class from memory.
     const bool far = __any(is_far(v.m, c));
     const float m = finite_ref(v.m);
@@ -840,8 +833,9 @@ __global__ __launch_bounds__(64, reg_waves(CP)) void distill_map_regs_kernel(Dis
         rest.s = v.s = 0.f;
         for (int j = 0; j < C; ++j) {
             const float e = exp2_((T::up(z[(long)j * inner + px]) - m) * c);
-            bool out = REST;
-            for (int i = 0; i < k && out; ++i) out = s_cls[i * POS + lane] != j;
+            bool out = true;
+            for (int i = 0; i < k; ++i)
+                if (s_cls[i * POS] >= 0 && (s_cls[i * POS] & 0xffff) == j) out = false;
             v.s += e;
             if (!REST || out) rest.s += e;
         }
@@ -853,13 +847,11 @@ __global__ __launch_bounds__(64, reg_waves(CP)) void distill_map_regs_kernel(Dis
     const float r = REST && rest.s != 0.f ? left : 0.f, Q = total + r, rest_R = far ? v.R : rest.R;
     const float gs = empty ? 0.f : w * a.g.inv_t * (a.upstream ? a.upstream[0] : 1.f);
 #pragma unroll 1
-    for (int i = 0; i < k; ++i) {
-        const int cls = s_cls[i * POS + lane];
-        if (cls < 0) continue;
-        const float q = s_q[i * POS + lane], zk = s_z[i * POS + lane];
+    for (int i = 0; i < places; ++i) {
+        const float q = s_d[i * POS], zk = s_z[i * POS];
         if (q != 0.f) loss -= q * row_log_p(a.g, zk, v.m, l2);
         const float d = far ? (zk - m) * c : __builtin_fmaf(zk, c, -v.R);
-        s_q[i * POS + lane] = w != 0.f ? gs * (exp2_(d - own_l2) * Q - q) : 0.f;
+        s_d[i * POS] = w != 0.f ? gs * (exp2_(d - own_l2) * Q - q) : 0.f;
     }
     if (r != 0.f) loss += r * (log2_(r) - ((rest_R - v.R) + log2_(rest.s) - own_l2)) * LN2;
     loss = wave_sum(w != 0.f ? w * loss : 0.f);
@@ -871,17 +863,30 @@ __global__ __launch_bounds__(64, reg_waves(CP)) void distill_map_regs_kernel(Dis
             const float e = exp2_((T::up(z[(long)j * inner + px]) - m) * c);
             dz[(long)j * inner + px] = T::down(F != 0.f ? F * e : 0.f);
         }
-    } else {
-        Global<E>* row = (Global<E>*)dz;
+        for (int i = 0; i < k; ++i)
+            if (s_cls[i * POS] >= 0) dz[(long)(s_cls[i * POS] & 0xffff) * inner + px] = T::down(s_d[(s_cls[i * POS] >> 16) * POS]);
+        return;
+    }
+    Global<E>* row = (Global<E>*)dz;
+    const float* at = s_d;
 #pragma unroll
-        for (int j = 0; j < CP; ++j) {
-            if (j < MIN || j < C) row[px] = T::down(F != 0.f ? F * x[j] : 0.f);  // (outside the loss a logit may be anything)
+    for (int u = 0; u < WORDS; ++u) asm volatile("" : "+v"(kept[u]));  // (the walk anew: its addresses kept would take a register a class)
+#pragma unroll
+    for (int j0 = 0; j0 < CP; j0 += 8) {  // (eight places asked for at once)
+        float place[8];
+#pragma unroll
+        for (int u = 0; u < 8; ++u) {
+            place[u] = *at;
+            at += (kept[(j0 + u) / 32] >> (j0 + u) % 32 & 1) * POS;
+        }
+#pragma unroll
+        for (int u = 0; u < 8; ++u) {
+            const int j = j0 + u;
+            float d = F != 0.f ? F * x[j] : 0.f;  // (outside the loss a logit may be anything)
+            d = kept[j / 32] >> j % 32 & 1 ? place[u] : d;
+            if (j < MIN || j < C) row[px] = T::down(d);
             step(row, inner);
         }
-    }
-    for (int i = 0; i < k; ++i) {
-        const int cls = s_cls[i * POS + lane];
-        if (cls >= 0) dz[(long)cls * inner + px] = T::down(s_q[i * POS + lane]);
     }
 }
 
@@ -968,7 +973,7 @@ int launch_distill_map(const DistillArgs& a, hipStream_t stream) {
     const int tiles = map_tiles(a.g.inner), C = a.g.classes, k = a.k;
     const long all = (long)a.g.outer * tiles;
     if (in_registers(all, C, k)) {
-#define CALL(CP, MIN) hipLaunchKernelGGL((distill_map_regs_kernel<T, CP, MIN, REST>), dim3((unsigned)all), dim3(64), 3 * k * POS * 4, stream, a, tiles)
+#define CALL(CP, MIN) hipLaunchKernelGGL((distill_map_regs_kernel<T, CP, MIN, REST>), dim3((unsigned)all), dim3(64), (4 * k + 2) * POS * 4, stream, a, tiles)
         BY_CLASSES(C, CALL);
 #undef CALL
         return MMAE_OK;
