@@ -194,6 +194,7 @@ extern "C" int mmae_distill(const void* logits, int dtype, int outer, int classe
     MMAE_REQUIRE(!mask || (width >= 1 && patch >= 1 && inner % width == 0 && width % patch == 0 && inner / width % patch == 0), MMAE_ESHAPE,
                  "distill: %d positions in rows of %d are not whole patches of %d", inner, width, patch);
     MMAE_REQUIRE(workspace_bytes >= mmae_distill_workspace_bytes(dtype, outer, classes, inner, k), MMAE_EWORKSPACE, "distill: workspace too small");
+    MMAE_REQUIRE(!again || !loss, MMAE_EINVAL, "distill: the loss comes from the first call");
     float* ws = (float*)workspace;
     DistillArgs a = {{logits, ld, outer, classes, inner, LOG2E / temperature, 1.f / temperature}, top_class, top_value, class_bytes, value_dtype, k, kind, mask};
     a.W = width; a.patch = mask ? patch : 1;

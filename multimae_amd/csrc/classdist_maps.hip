@@ -929,12 +929,11 @@ int launch_log_probs_map(const LogProbArgs& a, hipStream_t stream) {
     hipLaunchKernelGGL((log_probs_map_kernel<T, K>), dim3((unsigned)((long)a.g.outer * tiles)), dim3(64 * waves), bytes, stream, a, tiles);
     return MMAE_OK;
 }
-// The register kernels: enough tiles that every CU has its 12 waves, classes and alternatives that fit.  Fewer tiles are shared
-// by the waves of a workgroup instead.
-#ifndef REG_TILES
-#define REG_TILES 2048
-#endif
-bool in_registers(long tiles, int classes, int k) { return tiles >= REG_TILES && classes <= REG_CLASSES && k <= REG_TOP; }
+// The register kernels take what fits them.  Distillation alone shares a tile of a small map among the waves of a workgroup: its
+// walk over the classes is longer (8 x 133 x 56 x 56 fp32, 392 tiles: 23.1 us in registers, 19.6 us in the LDS; 784 tiles: 26.6
+// and 32.6 us).
+constexpr long REG_TILES = 512;
+bool in_registers(int classes, int k) { return classes <= REG_CLASSES && k <= REG_TOP; }
 
 #define BY_CLASSES(C, CALL)             \
     do {                                \
@@ -948,7 +947,7 @@ template <class T>
 int launch_log_probs_map(const LogProbArgs& a, hipStream_t stream) {
     const int tiles = map_tiles(a.g.inner);
     const long all = (long)a.g.outer * tiles;
-    if (in_registers(all, a.g.classes, a.k)) {
+    if (in_registers(a.g.classes, a.k)) {
 #define CALL(CP, MIN)                                                                                                              \
     do {                                                                                                                           \
         if (a.k == 0) hipLaunchKernelGGL((log_probs_map_regs_kernel<T, CP, MIN, 0>), dim3((unsigned)all), dim3(64), 0, stream, a, tiles); \
@@ -972,7 +971,7 @@ template <class T, bool REST>
 int launch_distill_map(const DistillArgs& a, hipStream_t stream) {
     const int tiles = map_tiles(a.g.inner), C = a.g.classes, k = a.k;
     const long all = (long)a.g.outer * tiles;
-    if (in_registers(all, C, k)) {
+    if (all >= REG_TILES && in_registers(C, k)) {
 #define CALL(CP, MIN) hipLaunchKernelGGL((distill_map_regs_kernel<T, CP, MIN, REST>), dim3((unsigned)all), dim3(64), (4 * k + 2) * POS * 4, stream, a, tiles)
         BY_CLASSES(C, CALL);
 #undef CALL

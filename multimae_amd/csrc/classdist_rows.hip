@@ -705,11 +705,12 @@ __device__ __forceinline__ int next_row(const DistillArgs& a, int p, float& w) {
     return p;
 }
 
-// Workgroups of 512 threads that the registers of a CU hold at NV pieces a thread.
-constexpr int long_groups(int NV) { return NV <= 16 ? 2 : 1; }
+// Waves per SIMD that the registers of NV pieces a thread leave, and the workgroups of a CU.
+constexpr int long_waves(int NT, int NV) { return NT == 256 ? (NV <= 4 ? 5 : 4) : NV <= 16 ? 4 : 2; }
+constexpr int long_groups(int NT, int NV) { return long_waves(NT, NV) * 256 / NT; }
 
 template <class T, int NT, int NV>
-__global__ __launch_bounds__(NT, 2 * long_groups(NV)) void distill_long_rows_kernel(DistillArgs a, RowNote* notes) {
+__global__ __launch_bounds__(NT, long_waves(NT, NV)) void distill_long_rows_kernel(DistillArgs a, RowNote* notes) {
     constexpr int VEC = T::VEC;
     __shared__ __align__(16) uint32_t flags[NT * NV / 4];  // a byte per piece: which of its elements are kept classes
     __shared__ Sums red[NT / 64];
@@ -937,23 +938,16 @@ __global__ __launch_bounds__(NT) void distill_tiles_kernel(DistillArgs a, int ti
     }
 }
 
-// Tiles of the row kernels: 32 elements a thread; one wave up to 2048 classes, four beyond.
-constexpr int SHORT_ROW = 2048, ROW_TILE = 8192, CUS = 256;
-constexpr int LONG_NT = 512;  // threads of a long row: with 1024, what a thread keeps beside the pieces counts twice
-#ifndef LP_EPT
-#define LP_EPT 16
-#endif
-#ifndef LP_NT
-#define LP_NT 256
-#endif
-constexpr int LP_TILE = LP_NT * LP_EPT;
-#ifndef WANT
-#define WANT 2048
-#endif
+constexpr int CUS = 256;
+constexpr int SHORT_ROW = 2048;  // up to here a row is one wave's
+// Elements of a tile, a workgroup of 256 threads: in the log probabilities' forward pass, which holds a second tile on its way,
+// 16 a thread (4096 x 150016 bf16, 8 alternatives: 234 us; 8 a thread 259 us, 32 a thread 249 us; 512 threads, which wait for
+// each other at the lists' barriers, 345 us), 32 elsewhere.
+constexpr int LP_NT = 256, LP_EPT = 16, LP_TILE = LP_NT * LP_EPT, ROW_TILE = 8192;
 // Workgroups a row is split into, and the tiles of each: enough for every CU to hold eight, at least a tile each, none empty.
 struct Split { int slices, tiles; };
 Split split_row(int rows, int classes, int tile) {
-    const int tiles = (classes + tile - 1) / tile, want = (WANT + rows - 1) / rows;
+    const int tiles = (classes + tile - 1) / tile, want = (8 * CUS + rows - 1) / rows;
     int n = want < tiles ? want : tiles;
     if (n > MAX_SLICES) n = MAX_SLICES;
     const int per = (tiles + n - 1) / n;
@@ -981,33 +975,56 @@ static void launch_log_probs_rows(const LogProbArgs& a, void* workspace, hipStre
         hipLaunchKernelGGL(log_probs_join_kernel<T>, dim3(rows), dim3(64), sizeof(uint64_t) * (size_t)(d.slices + 1) * a.k, stream, a, d.slices, (const char*)workspace);
 }
 
-// Rows held in registers where a workgroup takes them; in two passes over slices where there are too few rows for the card or
-// they are longer.
-template <class T> constexpr int longest_held_row() { return T::VEC == 8 ? 131072 : 65536; }
-static bool held_rows(int rows, int classes, int dtype) {
-    if (classes <= ROW_TILE) return true;
-    return rows >= 256 && classes <= (dtype == MMAE_DT_F32 ? longest_held_row<F32>() : longest_held_row<B16>());
+// Three ways.  Many rows are walked, each workgroup holding one and the next one on its way.  Fewer rows, if short, are held by
+// one workgroup each; few and long ones are cut into slices and read twice, the second time mostly from the caches.
+// Walked against held: 16-bit rows gain at every length (bf16, 4096 rows of 4000: 37 and 47 us, of 8000: 44 and 64 us, of
+// 32000: 141 and 196 us; 2048 rows of 4000: 26 and 29 us).  fp32 rows fill the same registers with half the classes and gain up
+// to 4096 of them (4096 x 4000: 40 and 48 us; 16384 x 16000: 429 and 405 us).  A row of more than 32768 classes takes half
+// a CU or all of it, and no second workgroup covers its loads: walked from one row per CU on.
+bool walked_rows(int rows, int classes, int dtype) {
+    if (classes <= SHORT_ROW) return false;
+    if (dtype == MMAE_DT_F32) return classes <= 65536 && (classes > 32768 ? rows >= CUS : classes <= 4096 && rows >= 8 * CUS);
+    return classes <= 131072 && rows >= (classes > 32768 ? CUS : 8 * CUS);
 }
+bool held_rows(int rows, int classes) { return classes <= ROW_TILE || (rows >= 256 && classes <= 32768); }
+
 template <class T>
 static void launch_distill_rows(const DistillArgs& a, int dtype, Sums* parts, bool again, hipStream_t stream) {
     const int rows = a.g.outer, C = a.g.classes;
     constexpr int V = T::VEC;
 #define HELD(NT, EPT) hipLaunchKernelGGL((distill_rows_kernel<T, NT, EPT / V>), dim3(rows), dim3(NT), 0, stream, a)
-#define LONG(EPT)                                                                                                              \
+#define LONG(NT, NV)                                                                                                           \
     do {                                                                                                                       \
         RowNote* notes = (RowNote*)parts;                                                                                      \
-        const int groups = CUS * long_groups(EPT / V);                                                                         \
+        const int groups = CUS * long_groups(NT, NV);                                                                          \
         if (!again) hipLaunchKernelGGL(distill_notes_kernel, dim3(rows), dim3(64), 0, stream, a, notes);                         \
-        hipLaunchKernelGGL((distill_long_rows_kernel<T, LONG_NT, EPT / V>), dim3(rows < groups ? rows : groups), dim3(LONG_NT), 0, stream, a, notes); \
+        hipLaunchKernelGGL((distill_long_rows_kernel<T, NT, NV>), dim3(rows < groups ? rows : groups), dim3(NT), 0, stream, a, notes); \
         hipLaunchKernelGGL((distill_far_rows_kernel<T>), dim3(rows), dim3(256), 0, stream, a, (const RowNote*)notes);            \
+        return;                                                                                                                \
     } while (0)
-    if (held_rows(rows, C, dtype) && (C <= 32768 || a.d_logits)) {  // (without a gradient one pass over slices does)
+    if (a.d_logits && walked_rows(rows, C, dtype)) {
+        if constexpr (V == 8) {
+            if (C <= 4096) LONG(256, 2);
+            else if (C <= 8192) LONG(256, 4);
+            else if (C <= 16384) LONG(256, 8);
+            else if (C <= 32768) LONG(512, 8);
+            else if (C <= 49152) LONG(512, 12);
+            else if (C <= 65536) LONG(512, 16);
+            else if (C <= 81920) LONG(512, 20);
+            else if (C <= 98304) LONG(512, 24);
+            else if (C <= 114688) LONG(512, 28);
+            else LONG(512, 32);
+        } else {
+            if (C <= 4096) LONG(256, 4);
+            else if (C <= 49152) LONG(512, 24);
+            else LONG(512, 32);
+        }
+    }
+    if (held_rows(rows, C)) {
         if (C <= 2048) HELD(64, 32);
         else if (C <= 8192) HELD(256, 32);
         else if (C <= 16384) HELD(512, 32);
-        else if (C <= 32768) HELD(1024, 32);
-        else if (C <= 65536) LONG(128);
-        else if constexpr (V == 8) LONG(256);
+        else HELD(1024, 32);
         return;
     }
 #undef HELD
