@@ -301,8 +301,8 @@ int mmae_class_log_probs_bwd(const void* logits, int dtype, int outer, int class
  * mask i64 [outer, (rows / patch) * (width / patch)] over inner = rows x width positions (nonzero = in the loss), or NULL: the
  * mean over all positions.  loss (f32 scalar) or d_logits (contiguous, the logits' dtype: the loss's gradient times
  * *upstream, a device scalar, or times 1 if NULL) may be NULL, not both.  again: the workspace is as an earlier call with
- * the same arguments up to `patch` left it, and what that call counted and summed is taken from there.  skip_unit: leave
- * d_logits as it is where *upstream is 1. */
+ * the same arguments up to `patch`, and a d_logits too, left it, and what that call counted and summed is taken from there; loss
+ * is NULL then.  skip_unit: leave d_logits as it is where *upstream is 1. */
 size_t mmae_distill_workspace_bytes(int dtype, int outer, int classes, int inner, int k);
 int mmae_distill(const void* logits, int dtype, int outer, int classes, int inner, long ld, const void* top_class,
                  int class_bytes, const void* top_value, int value_dtype, int k, int kind, float temperature,

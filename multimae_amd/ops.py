@@ -726,7 +726,7 @@ class Distillation:
     tokens are patch x patch squares of the last two dimensions, or single positions with patch = 1.
 
     run() computes the f32 scalar loss and, into d_logits (contiguous, the logits' dtype), its gradient.  scale() then makes
-    the gradient again, times an f32 scalar on the device, from what run() left in the workspace."""
+    the gradient again, times an f32 scalar on the device, from what a run() with a gradient left in the workspace."""
 
     def __init__(self, logits: torch.Tensor, top_class: torch.Tensor, top_value: torch.Tensor, mask: Optional[torch.Tensor] = None,
                  patch: int = 1, temperature: float = 1.0, log_probs: bool = False):
@@ -756,6 +756,7 @@ class Distillation:
         self.workspace = torch.empty(nbytes, dtype=torch.uint8, device=logits.device)
         self.args = (*_class_call(logits, geo), top_class.data_ptr(), top_class.element_size(), top_value.data_ptr(), _DT[top_value.dtype],
                      k, int(log_probs), temperature, _addr(mask), width, patch if mask is not None else 1)
+        self.scalable = False  # (a run() for the loss alone lays the workspace out otherwise)
         self.beside_bytes = geo[0] * geo[2] * k * (top_class.element_size() + top_value.element_size())
 
     def _launch(self, upstream, again, skip_unit, loss, d_logits):
@@ -768,12 +769,15 @@ class Distillation:
         return _req(d_logits, self.logits.dtype, "distill d_logits")
 
     def run(self, d_logits: Optional[torch.Tensor] = None) -> torch.Tensor:
+        self.scalable = d_logits is not None
         loss = torch.empty((), dtype=F32, device=self.logits.device)
         self._launch(None, 0, 0, loss, None if d_logits is None else self._gradient(d_logits))
         return loss
 
     def scale(self, d_logits: torch.Tensor, upstream: torch.Tensor, skip_unit: bool = False) -> torch.Tensor:
         """skip_unit: d_logits holds run()'s gradient and is left alone where the scalar is 1."""
+        if not self.scalable:
+            raise _lib.MmaeError("distill: scale() needs a run() that made the gradient")
         _beside(_req(upstream, F32, "distill upstream"), self.logits, (), "distill upstream")
         self._launch(upstream, 1, int(skip_unit), None, self._gradient(d_logits))
         return d_logits

@@ -493,6 +493,124 @@ def test_distillation_beyond_32_bit_offsets(M):
     assert (grad[:-3] == 0).all()
 
 
+def check_repeated(M, base, cls, val, rows, log_probs, temperature=1.0):
+    """Many rows, repetitions of a few (the oracle's work is that of the few), a third of them outside the loss and NaN there."""
+    n = base.shape[0]
+    which = torch.arange(rows) % n
+    mask = (torch.rand(rows, generator=torch.Generator().manual_seed(1)) > 0.33).long()
+    mask[rows - 1] = 1
+    z = base[which.cuda()]
+    z[mask.cuda() == 0] = float("nan")
+    leaf = z.requires_grad_(True)
+    fn = loss_module(M, 1, temperature, log_probs)
+    loss = fn(leaf, (cls[which.cuda()], val[which.cuda()]), mask=mask.view(-1, 1).cuda())
+    (grad,) = torch.autograd.grad(loss, leaf, retain_graph=True)
+    (scaled,) = torch.autograd.grad(loss, leaf, torch.tensor(-3.0, device="cuda"))
+    with torch.no_grad():
+        alone = fn(leaf, (cls[which.cuda()], val[which.cuda()]), mask=mask.view(-1, 1).cuda())
+    c, count = base.shape[1], mask.sum().item()
+    rel = 2 * CHAIN + 16 * U * (1 + math.log(c)) + (cls.shape[1] + 16) * U
+    total, sizes = 0.0, 0.0
+    for j in range(n):
+        want, size, want_grad, grad_size = reference_distill(base[j:j + 1], cls[j:j + 1], val[j:j + 1], None, 1, temperature, log_probs)
+        times = (mask[which == j] != 0).sum().item()
+        total, sizes = total + want * times / count, sizes + size * times / count
+        at = ((which == j) & (mask != 0)).nonzero().view(-1)
+        mine = grad[at.cuda()]
+        assert torch.equal(mine, mine[:1].expand_as(mine)), ("one row, two gradients", j)
+        size = grad_size * (rel + 8 * U * 30)
+        close(mine[:1], want_grad / count, half_step(base.dtype, want_grad / count) + size / count, f"grad of row {j}")
+        mine = scaled[at.cuda()]
+        assert torch.equal(mine, mine[:1].expand_as(mine)), ("one row, two gradients, upstream -3", j)
+        close(mine[:1], -3 * want_grad / count, half_step(base.dtype, 3 * want_grad / count) + 3 * size / count, f"grad of row {j}, upstream -3")
+    assert (grad[(mask == 0).cuda()] == 0).all() and (scaled[(mask == 0).cuda()] == 0).all()
+    for got in (loss, alone):
+        close(got, total, torch.as_tensor(sizes * (rel + 2 * 16 * U)), "loss")
+
+
+MANY_ROWS = [(2100, c, d) for d in ("bf16", "f16") for c in (2049, 4095, 4104, 8191, 9000, 16384, 20001, 32768)] \
+    + [(2100, c, "f32") for c in (2049, 3001, 4096)] \
+    + [(600, c, "bf16") for c in (32769, 49152, 50001, 70000, 90007, 100000, 114696, 131072)] \
+    + [(300, c, "f32") for c in (32770, 50001, 65536)]
+
+
+@pytest.mark.parametrize("log_probs", [False, True], ids=["logits", "log_probs"])
+@pytest.mark.parametrize("rows,c,dtype", MANY_ROWS, ids=str)
+def test_distillation_of_many_rows(M, rows, c, dtype, log_probs):
+    """More rows than the card takes at once: masked classes, padding, duplicates, empty rows and rows at the lowest value among
+    them, so that one kind follows another."""
+    base = scores((8, c), dtype, seed=c)
+    cls, val = teacher_top((8, c), 9, 5, log_probs, 1.5)
+    cls[0, 3:] = -1
+    cls[1, ::2] = c + 5
+    cls[2] = -100
+    cls[3, 4] = cls[3, 2]; cls[3, 8] = cls[3, 2]
+    cls[3, 0], cls[3, 1], cls[3, 3] = 0, c - 1, (c // 2048) * 2048 - 1    # the ends, and where the pieces meet
+    val[4, 5:] = NINF
+    base[5, : c // 2] = NINF
+    cls[5] = torch.where(cls[5] < c // 2, cls[5] + (c + 1) // 2, cls[5]).clamp(max=c - 1)
+    base[6] = torch.finfo(base.dtype).min
+    check_repeated(M, base, cls, val, rows, log_probs, 1.5)
+    base[1] = NINF
+    fn = loss_module(M, 1, 1.5, log_probs)
+    leaf = base[(torch.arange(rows) % 8).cuda()].requires_grad_(True)
+    loss = fn(leaf, (cls.repeat(rows // 8 + 1, 1)[:rows], val.repeat(rows // 8 + 1, 1)[:rows]))
+    (grad,) = torch.autograd.grad(loss, leaf)
+    # (a row without a class left: no gradient, and an infinite loss wherever the teacher's mass is above zero)
+    assert loss.item() == math.inf and (grad[1::8] == 0).all() and torch.isfinite(grad).all()
+
+
+@pytest.mark.parametrize("log_probs", [False, True], ids=["logits", "log_probs"])
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("c", [1, 7, 32, 33, 64, 65, 104, 105, 133, 136, 137])
+def test_distillation_of_many_small_maps(M, c, dtype, log_probs):
+    """As many tiles of positions as the card has waves, few classes: masks with NaN outside, padding, duplicates, -inf and the
+    lowest value, up to 16 kept classes and more."""
+    shape = (530, c, 4, 6)
+    z = scores(shape, dtype, seed=c)
+    mask = (classes((530, 6), 4, 5) > 0).long()
+    mask[7] = 0
+    for k in (min(16, c), min(3, c), min(17, c)):
+        cls, val = teacher_top(shape, k, 3, log_probs, 1.5, "bf16" if k == 3 else "f32", torch.int32 if k == 3 else torch.int64)
+        cls[0, k // 2:] = -1
+        cls[1] = c
+        cls[2, -1] = cls[2, 0]; cls[2, k // 2] = cls[2, 0]
+        val[3, k // 2:] = NINF
+        z[4] = torch.finfo(z.dtype).min
+        z[5, c // 2:] = torch.finfo(z.dtype).min
+        z[6, 1::2] = torch.finfo(z.dtype).min
+        check_distill(M, z, cls, val, None, 1, 1.5, log_probs)
+        off = (mask == 0).view(530, 1, 2, 3).repeat_interleave(2, 2).repeat_interleave(2, 3).expand(shape)
+        check_distill(M, torch.where(off, float("nan"), z), cls, val, mask, 2, 1.5, log_probs)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+def test_distillation_of_large_maps(M, dtype):
+    shape = (5, 133, 90, 91)
+    for log_probs in (False, True):
+        check_distill(M, scores(shape, dtype, 1), *teacher_top(shape, 8, 2, log_probs, 2.0), temperature=2.0, log_probs=log_probs)
+
+
+def test_scaling_needs_a_gradient_to_scale(M):
+    from multimae_amd import ops
+    from multimae_amd._lib import MmaeError
+    z = scores((300, 40000), "bf16", 1)
+    call = ops.Distillation(z, *teacher_top((300, 40000), 8, 2, True, 1.0), log_probs=True)
+    one, two, d = torch.ones((), device="cuda"), torch.full((), 2.0, device="cuda"), torch.empty_like(z)
+    with pytest.raises(MmaeError):
+        call.scale(d, one)
+    loss = call.run()
+    with pytest.raises(MmaeError):
+        call.scale(d, one)
+    assert torch.equal(call.run(d), loss) or abs(call.run(d).item() - loss.item()) < 4 * CHAIN * (abs(loss.item()) + 1)
+    first = d.clone()
+    assert torch.equal(call.scale(d, one), first)
+    assert torch.equal(call.scale(d, two), 2 * first)  # (a power of two: exact; none of the gradients is subnormal in bf16)
+    call.run()
+    with pytest.raises(MmaeError):
+        call.scale(d, one)
+
+
 # ------------------------------------------------------------------------------------------------ as they are used
 def test_class_distribution_calls_are_bitwise_reproducible_and_stay_in_their_buffers(M):
     from multimae_amd import ops
