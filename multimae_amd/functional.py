@@ -907,6 +907,12 @@ def class_log_probs(logits, target, top_k, temperature):
     return ops.class_log_probs(_class_scores(logits), target.contiguous(), top_k, temperature, want_stats=False)[:4]
 
 
+def _once(backward):
+    """torch's once_differentiable, whose bookkeeping a pass without create_graph does without."""
+    checked = torch.autograd.function.once_differentiable(backward)
+    return lambda ctx, *g: checked(ctx, *g) if torch.is_grad_enabled() else backward(ctx, *g)
+
+
 class ClassLogProbsFn(torch.autograd.Function):
     """(log probability of the given class, entropy, top log probabilities, top classes) of each position's distribution;
     the first two carry gradients."""
@@ -916,21 +922,21 @@ class ClassLogProbsFn(torch.autograd.Function):
         logits = _class_scores(logits)
         target = target.contiguous()
         log_prob, entropy, top_log_prob, top_class, stats = ops.class_log_probs(logits, target, top_k, temperature)
-        ctx.temperature = temperature
+        ctx.stats, ctx.temperature = stats, temperature
         ctx.set_materialize_grads(False)
         if top_k:
             ctx.mark_non_differentiable(top_log_prob, top_class)
-        ctx.save_for_backward(logits, target, entropy, stats)
+        ctx.save_for_backward(logits, target, entropy)
         return log_prob, entropy, top_log_prob, top_class
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
+    @_once
     def backward(ctx, g_log_prob, g_entropy, _top_log_prob, _top_class):
         if g_log_prob is None and g_entropy is None:
             return None, None, None, None
-        logits, target, entropy, stats = ctx.saved_tensors
-        g = [None if t is None else t.float().contiguous() for t in (g_log_prob, g_entropy)]
-        return ops.class_log_probs_bwd(logits, target, entropy, stats, *g, ctx.temperature), None, None, None
+        logits, target, entropy = ctx.saved_tensors
+        g = [None if t is None else t.contiguous() for t in (g_log_prob, g_entropy)]  # (fp32, as the outputs: autograd sees to it)
+        return ops._class_log_probs_bwd(logits, ops.class_geometry(logits), target, entropy, ctx.stats, *g, ctx.temperature), None, None, None
 
 
 class DistillFn(torch.autograd.Function):
@@ -950,12 +956,11 @@ class DistillFn(torch.autograd.Function):
         return call.run(ctx.d_logits)
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
+    @_once
     def backward(ctx, g):
         d_logits, ctx.d_logits = ctx.d_logits, None
         if d_logits is None or not getattr(ctx, "unit_upstream", False):
             logits = ctx.saved_tensors[0]  # (refused if an input was changed since)
-            g = g if g.dtype == torch.float32 else g.float()
             if d_logits is None:
                 d_logits = ctx.call.scale(torch.empty(logits.shape, dtype=logits.dtype, device=logits.device), g)
             else:

@@ -650,7 +650,7 @@ def _launch(what: str, fn, device, nbytes, *args):
     """fn(*args, the current stream of `device`), with `device` current; nbytes: what the call cannot avoid to move."""
     idx = device.index
     if PROFILE is None and idx == torch._C._cuda_getDevice():
-        rc = fn(*args, _raw_stream(idx))
+        rc = fn(*args, torch._C._cuda_getCurrentRawStream(idx))
     else:
         with torch.cuda.device(idx), _Timed(what, 0.0, nbytes=nbytes):
             rc = fn(*args, _raw_stream(idx))
@@ -711,12 +711,18 @@ def class_log_probs_bwd(logits: torch.Tensor, target: torch.Tensor, entropy: tor
     for t, s, n in ((entropy, shape, "entropy"), (stats, (2,) + shape, "stats"), (d_log_prob, shape, "d_log_prob"), (d_entropy, shape, "d_entropy")):
         if t is not None:
             _beside(_req(t, F32, f"class_log_probs_bwd {n}"), logits, s, f"class_log_probs_bwd {n}")
-    d_logits = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
+    return _class_log_probs_bwd(logits, geo, target, entropy, stats, d_log_prob, d_entropy, temperature)
+
+
+def _class_log_probs_bwd(logits, geo, target, entropy, stats, d_log_prob, d_entropy, temperature):
+    """class_log_probs_bwd of a call that was checked before (host time counts in the backward pass of a small one)."""
+    dev = logits.device
+    d_logits = torch.empty(logits.shape, dtype=logits.dtype, device=dev)
     if geo[0]:
         n, at = geo[0] * geo[2], stats.data_ptr()
-        _launch("class_log_probs_bwd", _L().mmae_class_log_probs_bwd, logits.device, 2 * logits.numel() * logits.element_size() + n * 28,
-                *_class_call(logits, geo), target.data_ptr(), temperature, entropy.data_ptr(), at, at + 4 * n, _addr(d_log_prob),
-                _addr(d_entropy), d_logits.data_ptr())
+        _launch("class_log_probs_bwd", _L().mmae_class_log_probs_bwd, dev, 2 * d_logits.nbytes + n * 28, *_class_call(logits, geo),
+                target.data_ptr(), temperature, entropy.data_ptr(), at, at + 4 * n, None if d_log_prob is None else d_log_prob.data_ptr(),
+                None if d_entropy is None else d_entropy.data_ptr(), d_logits.data_ptr())
     return d_logits
 
 

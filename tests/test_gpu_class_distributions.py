@@ -700,6 +700,31 @@ def test_outputs_can_be_changed_in_place_and_one_of_them_used(M):
         assert not M.MaskedDistillationLoss()(z, (target.view(5, 1), torch.zeros(5, 1, device="cuda"))).requires_grad
 
 
+def test_gradients_of_gradients_are_refused_and_other_gradient_types_taken(M):
+    z = scores((6, 500), "bf16", 1).requires_grad_(True)
+    target = classes((6,), 500, 2)
+    loss = M.MaskedDistillationLoss()(z, (target.view(6, 1), torch.zeros(6, 1, device="cuda")))
+    out = M.class_log_probs(z, target)
+    for value in (loss, out.entropy.sum()):
+        (first,) = torch.autograd.grad(value, z, retain_graph=True)
+        (grad,) = torch.autograd.grad(value, z, create_graph=True)
+        assert torch.equal(grad, first)
+        with pytest.raises(RuntimeError):
+            torch.autograd.grad(grad.sum(), z)
+    # gradients that are expanded, strided or of another type
+    gl = torch.randn(12, generator=torch.Generator().manual_seed(3)).cuda()[::2]
+    (want,) = torch.autograd.grad(out.log_prob, z, gl.contiguous(), retain_graph=True)
+    (got,) = torch.autograd.grad(out.log_prob, z, gl, retain_graph=True)
+    assert torch.equal(got, want)
+    half = gl.bfloat16()
+    (want,) = torch.autograd.grad(out.log_prob, z, half.float(), retain_graph=True)
+    (got,) = torch.autograd.grad(out.log_prob, z, half, retain_graph=True)
+    assert torch.equal(got, want)
+    (want,) = torch.autograd.grad(loss, z, torch.tensor(0.5, device="cuda"), retain_graph=True)
+    (got,) = torch.autograd.grad(loss, z, torch.tensor(0.5, device="cuda", dtype=torch.float64))
+    assert torch.equal(got, want)
+
+
 def test_a_teacher_labels_and_the_pretraining_step_distils(M):
     """As they are used together: the teacher decoder's alternatives become the target of the semseg task in PretrainStep, with
     the semseg domain's mask; the gradients are those of the plain definition through the same model."""
