@@ -332,6 +332,17 @@ __device__ float distill_position(const DistillArgs& a, long p, float w, Stats* 
     return l;
 }
 
+// A launch holds fewer than 2^32 threads.
+inline int fits_grid(const char* name, long blocks, int threads) {
+    MMAE_REQUIRE(blocks * threads <= 0xffffffffL, MMAE_ESHAPE, "%s: %ld workgroups of %d threads are more than one launch holds", name, blocks, threads);
+    return MMAE_OK;
+}
+#define REQUIRE_GRID(name, blocks, threads)                          \
+    do {                                                             \
+        const int rc__ = fits_grid(name, (long)(blocks), threads);   \
+        if (rc__ != MMAE_OK) return rc__;                            \
+    } while (0)
+
 #define BY_DTYPE(dtype, CALL)            \
     do {                                 \
         if ((dtype) == MMAE_DT_F32) { CALL(F32); } \
@@ -341,7 +352,7 @@ __device__ float distill_position(const DistillArgs& a, long p, float w, Stats* 
 
 // classdist_rows.hip: rows, inner = 1
 size_t log_probs_rows_workspace(int rows, int classes, int top_k);
-void log_probs_rows(int dtype, const LogProbArgs& a, void* workspace, hipStream_t stream);
+int log_probs_rows(int dtype, const LogProbArgs& a, void* workspace, hipStream_t stream);
 int log_probs_bwd_rows(int dtype, const LogProbBwdArgs& a, hipStream_t stream);
 size_t distill_rows_workspace(int rows, int classes);
 int distill_rows(int dtype, const DistillArgs& a, void* workspace, bool again, hipStream_t stream);  // again: the workspace is an earlier call's

@@ -111,7 +111,7 @@ int check_logits(const char* name, const void* logits, int dtype, int outer, int
     MMAE_REQUIRE(dtype >= MMAE_DT_F32 && dtype <= MMAE_DT_F16, MMAE_EINVAL, "%s: dtype code %d", name, dtype);
     MMAE_REQUIRE(outer > 0 && classes > 0 && inner > 0, MMAE_ESHAPE, "%s: empty input (%d x %d x %d)", name, outer, classes, inner);
     MMAE_REQUIRE(classes <= 1 << 30, MMAE_ESHAPE, "%s: %d classes", name, classes);
-    MMAE_REQUIRE((long)outer * inner <= 0x7fffffffL, MMAE_ESHAPE, "%s: %d x %d positions are more than 2^31 - 1", name, outer, inner);
+    MMAE_REQUIRE((long)outer * inner <= 0x7fffffc0L, MMAE_ESHAPE, "%s: %d x %d positions are more than 2^31 - 64", name, outer, inner);
     MMAE_REQUIRE(ld >= (long)classes * inner, MMAE_ESHAPE, "%s: samples %ld elements apart hold %d x %d values", name, ld, classes, inner);
     MMAE_REQUIRE(temperature > 0.f && temperature < INFINITY, MMAE_EINVAL, "%s: temperature %g is not positive and finite", name, temperature);
     return MMAE_OK;
@@ -140,16 +140,18 @@ extern "C" int mmae_class_log_probs(const void* logits, int dtype, int outer, in
                      row_log_sum, top_log_prob, top_class};
     MMAE_REQUIRE(workspace_bytes >= mmae_class_log_probs_workspace_bytes(outer, classes, inner, top_k) && (workspace || !workspace_bytes),
                  MMAE_EWORKSPACE, "class_log_probs: workspace too small");
+    int r = MMAE_OK;
     if (inner == 1) {
-        log_probs_rows(dtype, a, workspace, stream);
+        r = log_probs_rows(dtype, a, workspace, stream);
     } else if (log_probs_map_fits(dtype, classes, top_k)) {
-        const int r = log_probs_map(dtype, a, stream);
-        if (r != MMAE_OK) return r;
+        r = log_probs_map(dtype, a, stream);
     } else {
+        REQUIRE_GRID("class_log_probs", (long)outer * inner, 256);
 #define CALL(T) hipLaunchKernelGGL(log_probs_kernel<T>, dim3(outer * inner), dim3(256), 0, stream, a)
         BY_DTYPE(dtype, CALL);
 #undef CALL
     }
+    if (r != MMAE_OK) return r;
     MMAE_CHECK_LAUNCH("class_log_probs");
     return MMAE_OK;
 }
@@ -195,6 +197,7 @@ extern "C" int mmae_distill(const void* logits, int dtype, int outer, int classe
                  "distill: %d positions in rows of %d are not whole patches of %d", inner, width, patch);
     MMAE_REQUIRE(workspace_bytes >= mmae_distill_workspace_bytes(dtype, outer, classes, inner, k), MMAE_EWORKSPACE, "distill: workspace too small");
     MMAE_REQUIRE(!again || !loss, MMAE_EINVAL, "distill: the loss comes from the first call");
+    REQUIRE_GRID("distill", outer, 64);  // (the count of masked positions)
     float* ws = (float*)workspace;
     DistillArgs a = {{logits, ld, outer, classes, inner, LOG2E / temperature, 1.f / temperature}, top_class, top_value, class_bytes, value_dtype, k, kind, mask};
     a.W = width; a.patch = mask ? patch : 1;
@@ -219,6 +222,7 @@ extern "C" int mmae_distill(const void* logits, int dtype, int outer, int classe
     } else if (distill_map_fits(dtype, classes, k)) {
         r = distill_map(dtype, a, stream);
     } else {
+        REQUIRE_GRID("distill", (long)outer * inner, 256);
 #define CALL(T) hipLaunchKernelGGL(distill_kernel<T>, dim3(outer * inner), dim3(256), 0, stream, a)
         BY_DTYPE(dtype, CALL);
 #undef CALL

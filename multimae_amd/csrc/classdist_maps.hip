@@ -905,7 +905,7 @@ int allow_lds(const void* kernel, int bytes, const char* name) {
 }
 
 int element_bytes(int dtype) { return dtype == MMAE_DT_F32 ? 4 : 2; }
-int map_tiles(int inner) { return (inner + POS - 1) / POS; }
+int map_tiles(int inner) { return inner / POS + (inner % POS != 0); }
 constexpr int DISTILL_STATIC = 1024;  // the distillation kernel's fixed arrays (an upper bound)
 
 // The largest number of waves that map_waves may ask for and that fits.
@@ -926,6 +926,7 @@ int launch_log_probs_map(const LogProbArgs& a, hipStream_t stream) {
         const int rc = allow_lds((const void*)log_probs_map_kernel<T, K>, bytes, "class_log_probs");
         if (rc != MMAE_OK) return rc;
     }
+    REQUIRE_GRID("class_log_probs", (long)a.g.outer * tiles, 64 * waves);
     hipLaunchKernelGGL((log_probs_map_kernel<T, K>), dim3((unsigned)((long)a.g.outer * tiles)), dim3(64 * waves), bytes, stream, a, tiles);
     return MMAE_OK;
 }
@@ -948,6 +949,7 @@ int launch_log_probs_map(const LogProbArgs& a, hipStream_t stream) {
     const int tiles = map_tiles(a.g.inner);
     const long all = (long)a.g.outer * tiles;
     if (in_registers(a.g.classes, a.k)) {
+        REQUIRE_GRID("class_log_probs", all, 64);
 #define CALL(CP, MIN)                                                                                                              \
     do {                                                                                                                           \
         if (a.k == 0) hipLaunchKernelGGL((log_probs_map_regs_kernel<T, CP, MIN, 0>), dim3((unsigned)all), dim3(64), 0, stream, a, tiles); \
@@ -972,6 +974,7 @@ int launch_distill_map(const DistillArgs& a, hipStream_t stream) {
     const int tiles = map_tiles(a.g.inner), C = a.g.classes, k = a.k;
     const long all = (long)a.g.outer * tiles;
     if (all >= REG_TILES && in_registers(C, k)) {
+        REQUIRE_GRID("distill", all, 64);
 #define CALL(CP, MIN) hipLaunchKernelGGL((distill_map_regs_kernel<T, CP, MIN, REST>), dim3((unsigned)all), dim3(64), (4 * k + 2) * POS * 4, stream, a, tiles)
         BY_CLASSES(C, CALL);
 #undef CALL
@@ -984,6 +987,7 @@ int launch_distill_map(const DistillArgs& a, hipStream_t stream) {
         const int rc = allow_lds((const void*)distill_map_kernel<T, REST>, bytes, "distill");
         if (rc != MMAE_OK) return rc;
     }
+    REQUIRE_GRID("distill", all, 64 * waves);
     hipLaunchKernelGGL((distill_map_kernel<T, REST>), dim3((unsigned)((long)a.g.outer * tiles)), dim3(64 * waves), bytes, stream, a, tiles);
     return MMAE_OK;
 }
@@ -1008,7 +1012,7 @@ int log_probs_bwd_map(int dtype, const LogProbBwdArgs& a, hipStream_t stream) {
     const long all = (long)a.g.outer * tiles;
     int splits = 1;  // workgroups that share a tile's classes, where there are few tiles
     while (splits < 16 && all * splits < 2048 && splits * 64 < a.g.classes) splits *= 2;
-    MMAE_REQUIRE(all * splits <= 0x7fffffffL, MMAE_ESHAPE, "class_log_probs_bwd: %d x %d positions", a.g.outer, a.g.inner);
+    REQUIRE_GRID("class_log_probs_bwd", all * splits, 256);
 #define CALL(T) hipLaunchKernelGGL(log_probs_bwd_map_kernel<T>, dim3((unsigned)(all * splits)), dim3(256), 0, stream, a, tiles, splits)
     BY_DTYPE(dtype, CALL);
 #undef CALL

@@ -1043,15 +1043,18 @@ size_t log_probs_rows_workspace(int rows, int classes, int top_k) {
     return n == 1 ? 0 : (size_t)rows * n * slice_bytes(top_k);
 }
 
-void log_probs_rows(int dtype, const LogProbArgs& a, void* workspace, hipStream_t stream) {
+int log_probs_rows(int dtype, const LogProbArgs& a, void* workspace, hipStream_t stream) {
+    const int slices = log_probs_split(a.g.outer, a.g.classes).slices;
+    REQUIRE_GRID("class_log_probs", (long)a.g.outer * slices, a.g.classes <= SHORT_ROW ? 64 : LP_NT);
 #define CALL(T) launch_log_probs_rows<T>(a, workspace, stream)
     BY_DTYPE(dtype, CALL);
 #undef CALL
+    return MMAE_OK;
 }
 
 int log_probs_bwd_rows(int dtype, const LogProbBwdArgs& a, hipStream_t stream) {
     const int C = a.g.classes, tile = C <= SHORT_ROW ? SHORT_ROW : ROW_TILE, tiles = (C + tile - 1) / tile;
-    MMAE_REQUIRE((long)a.g.outer * tiles <= 0x7fffffffL, MMAE_ESHAPE, "class_log_probs_bwd: %d rows of %d classes", a.g.outer, C);
+    REQUIRE_GRID("class_log_probs_bwd", (long)a.g.outer * tiles, C <= SHORT_ROW ? 64 : 256);
     const unsigned grid = (unsigned)a.g.outer * tiles;
 #define CALL(T)                                                                                                                    \
     if (C <= SHORT_ROW) hipLaunchKernelGGL((log_probs_bwd_rows_kernel<T, 64, 32 / T::VEC>), dim3(grid), dim3(64), 0, stream, a, tiles); \
@@ -1065,7 +1068,7 @@ size_t distill_rows_workspace(int rows, int classes) { return sizeof(Sums) * (si
 
 int distill_rows(int dtype, const DistillArgs& a, void* workspace, bool again, hipStream_t stream) {
     const int C = a.g.classes;
-    MMAE_REQUIRE((long)a.g.outer * ((C + ROW_TILE - 1) / ROW_TILE) <= 0x7fffffffL, MMAE_ESHAPE, "distill: %d rows of %d classes", a.g.outer, C);
+    REQUIRE_GRID("distill", (long)a.g.outer * ((C + ROW_TILE - 1) / ROW_TILE), C <= SHORT_ROW ? 64 : C <= ROW_TILE ? 256 : 1024);
 #define CALL(T) launch_distill_rows<T>(a, dtype, (Sums*)workspace, again, stream)
     BY_DTYPE(dtype, CALL);
 #undef CALL
