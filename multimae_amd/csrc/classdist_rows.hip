@@ -131,6 +131,26 @@ __device__ __forceinline__ uint32_t kth_maximum(const float* maxima, int k) {
     return at & 0x80000000u ? at : at | ((1ull << (32 - T::KEY_BITS)) - 1);  // (negative values are inverted, their later bits are set)
 }
 
+// ordered() of the k-th largest element of one wave's tile: the bound that the maxima give leaves up to 5 k values above it where
+// k is near the number of lanes that hold any (1024 x 1000 bf16, 64 alternatives: 16 us instead of 119).
+template <class T, int NV>
+__device__ __forceinline__ uint32_t kth_element(const Piece (&q)[NV], int k) {
+    uint32_t at = 0;
+    for (int b = 31; b >= 32 - T::KEY_BITS; --b) {
+        const uint32_t next = at | 1u << b;
+        // (the later bits are those of the least value that begins so; what lies beyond the infinities is NaN, no element reaches it)
+        const float least = key_value((uint64_t)(next & 0x80000000u ? next : next | ((1ull << (32 - T::KEY_BITS)) - 1)) << 32);
+        int n = 0;
+#pragma unroll
+        for (int i = 0; i < NV; ++i)
+#pragma unroll
+            for (int e = 0; e < T::VEC; ++e) n += __popcll(__ballot(T::get(q[i], e) >= least));
+        if (n >= k) at = next;
+    }
+    at = at & 0x80000000u ? at : at | ((1ull << (32 - T::KEY_BITS)) - 1);
+    return at < 0x007fffffu ? 0x007fffffu : at;  // (-inf)
+}
+
 // Ranks the keys of the list and keeps the first k, sorted.
 template <int NT, class L>
 __device__ __forceinline__ void keep_best(L& list, ListState& st, int k) {
@@ -138,7 +158,7 @@ __device__ __forceinline__ void keep_best(L& list, ListState& st, int k) {
     for (int i = threadIdx.x; i < n; i += NT) {
         const uint64_t key = list.keys[i];
         int rank = 0;
-#pragma unroll 4
+#pragma unroll 8
         for (int j = 0; j < n; ++j) rank += list.keys[j] > key;
         if (rank < k) list.sorted[rank] = key;
     }
@@ -159,7 +179,10 @@ __device__ __forceinline__ void take_crowded_tile(L& list, const Piece (&q)[NV],
     list.maxima[threadIdx.x] = tile_max;
     if (threadIdx.x == 0) list.count = st.have;
     __syncthreads();
-    const float v = key_value((uint64_t)kth_maximum<T, NT>(list.maxima, k) << 32);
+    uint32_t bound;
+    if (NT == 64 && 2 * k > (end - base < 64 * VEC ? (end - base) / VEC : 64)) bound = kth_element<T, NV>(q, k);
+    else bound = kth_maximum<T, NT>(list.maxima, k);
+    const float v = key_value((uint64_t)bound << 32);
     const bool equals = st.open || v > st.floor;  // values equal to the bound are wanted too
     const float least = equals ? v : st.floor;
     if (tile_max > least || (equals && tile_max == least)) {
@@ -953,8 +976,13 @@ Split split_row(int rows, int classes, int tile) {
     const int per = (tiles + n - 1) / n;
     return {(tiles + per - 1) / per, per};
 }
-Split log_probs_split(int rows, int classes) {
-    return classes <= SHORT_ROW ? Split{1, (classes + 64 * LP_EPT - 1) / (64 * LP_EPT)} : split_row(rows, classes, LP_TILE);
+// A row of the log probabilities' forward pass is one wave's, which waits for no other, up to SHORT_ROW classes, and where every CU
+// has eight rows up to 8192 (bf16, 4096 x 5000: 13 us, a workgroup of four waves 20; 8192 x 8000: 27 and 34).  The list of
+// alternatives is where one wave is slow: up to 4096 with 16 of them (4096 x 4000, 8 alternatives: 24 and 27 us;
+// 4096 x 6000: 36 and 36; 20 alternatives, 4096 x 4000: 32 and 30).
+bool one_wave(int rows, int classes, int k) { return classes <= (rows < 8 * CUS || k > 16 ? SHORT_ROW : k ? 4096 : 8192); }
+Split log_probs_split(int rows, int classes, int k) {
+    return one_wave(rows, classes, k) ? Split{1, (classes + 64 * LP_EPT - 1) / (64 * LP_EPT)} : split_row(rows, classes, LP_TILE);
 }
 int row_slices(int rows, int classes) { return split_row(rows, classes, ROW_TILE).slices; }
 
@@ -962,10 +990,10 @@ template <class T>
 static void launch_log_probs_rows(const LogProbArgs& a, void* workspace, hipStream_t stream) {
     constexpr int NV = LP_EPT / T::VEC;
     const int rows = a.g.outer;
-    const Split d = log_probs_split(rows, a.g.classes);
+    const Split d = log_probs_split(rows, a.g.classes, a.k);
 #define ROWS(NT, TOP) \
     hipLaunchKernelGGL((log_probs_rows_kernel<T, NT, NV, TOP>), dim3((unsigned)rows * d.slices), dim3(NT), 0, stream, a, d.slices, d.tiles, (char*)workspace)
-    if (a.g.classes <= SHORT_ROW) {
+    if (one_wave(rows, a.g.classes, a.k)) {
         if (a.k) ROWS(64, true); else ROWS(64, false);
         return;
     }
@@ -1039,13 +1067,13 @@ static void launch_distill_rows(const DistillArgs& a, int dtype, Sums* parts, bo
 }  // namespace
 
 size_t log_probs_rows_workspace(int rows, int classes, int top_k) {
-    const int n = log_probs_split(rows, classes).slices;
+    const int n = log_probs_split(rows, classes, top_k).slices;
     return n == 1 ? 0 : (size_t)rows * n * slice_bytes(top_k);
 }
 
 int log_probs_rows(int dtype, const LogProbArgs& a, void* workspace, hipStream_t stream) {
-    const int slices = log_probs_split(a.g.outer, a.g.classes).slices;
-    REQUIRE_GRID("class_log_probs", (long)a.g.outer * slices, a.g.classes <= SHORT_ROW ? 64 : LP_NT);
+    const int slices = log_probs_split(a.g.outer, a.g.classes, a.k).slices;
+    REQUIRE_GRID("class_log_probs", (long)a.g.outer * slices, one_wave(a.g.outer, a.g.classes, a.k) ? 64 : LP_NT);
 #define CALL(T) launch_log_probs_rows<T>(a, workspace, stream)
     BY_DTYPE(dtype, CALL);
 #undef CALL

@@ -186,6 +186,23 @@ def test_equal_logits_rank_by_the_lower_class(M, shape, dtype):
             check_log_probs(M, z, target, k, 1.0, backward=False)
 
 
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("c", [5, 100, 1000, 2049, 4095, 8191])
+def test_log_probs_of_many_rows(M, c, dtype):
+    """A wave a row; lists of any length from a tile that fills few lanes, levels with many equal values, mostly -inf."""
+    z = scores((2051, c), dtype, seed=c)
+    z[3] = torch.randint(0, 3, (c,), generator=torch.Generator().manual_seed(1)).to(z.dtype)
+    z[4] = -z[3]
+    z[5, 3:] = NINF
+    z[6] = NINF
+    z[7] = torch.finfo(z.dtype).min
+    z[8, : c // 2] = torch.finfo(z.dtype).min
+    z[9] = 0.0; z[9, 1::3] = -0.0
+    target = classes((2051,), c, 1)
+    for k in (0, 5, 16, 33, 64):
+        check_log_probs(M, z, target, min(k, c), 1.5, backward=k in (0, 33))
+
+
 def test_targets_outside_the_classes_are_ignored(M):
     for shape in ((6, 50), (6, 5000), (6, 50, 2, 3)):
         z = scores(shape, "f32", seed=1)
