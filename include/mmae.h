@@ -286,7 +286,7 @@ int mmae_masked_ce(const void* logits, int logits_is_bf16, const int64_t* target
  * mmae_class_log_probs_bwd: d_logits (contiguous, the logits' dtype) for the gradients that arrive at log_prob and entropy
  * (either may be NULL). */
 enum { MMAE_DT_F32 = 0, MMAE_DT_BF16 = 1, MMAE_DT_F16 = 2 };
-size_t mmae_class_log_probs_workspace_bytes(int outer, int classes, int inner, int top_k);
+size_t mmae_class_log_probs_workspace_bytes(int dtype, int outer, int classes, int inner, int top_k);
 int mmae_class_log_probs(const void* logits, int dtype, int outer, int classes, int inner, long ld, const int64_t* target,
                          int top_k, float temperature, float* log_prob, float* entropy, float* row_max, float* row_log_sum,
                          float* top_log_prob, int64_t* top_class, void* workspace, size_t workspace_bytes, mmae_stream_t stream);

@@ -61,7 +61,7 @@ SIGNATURES = {
     "mmae_masked_loss_workspace_bytes": (_z, [_i, _i, _i, _i, _i]),
     "mmae_masked_ce_workspace_bytes": (_z, [_i, _i, _i]),
     "mmae_masked_ce": (_i, [_p, _i, _p, _p, _i, _i, _i, _i, _i, _f, _p, _p, _p, _z, _p]),
-    "mmae_class_log_probs_workspace_bytes": (_z, [_i, _i, _i, _i]),
+    "mmae_class_log_probs_workspace_bytes": (_z, [_i, _i, _i, _i, _i]),
     "mmae_class_log_probs": (_i, [_p, _i, _i, _i, _i, _l, _p, _i, _f, _p, _p, _p, _p, _p, _p, _p, _z, _p]),
     "mmae_class_log_probs_bwd": (_i, [_p, _i, _i, _i, _i, _l, _p, _f, _p, _p, _p, _p, _p, _p, _p]),
     "mmae_distill_workspace_bytes": (_z, [_i, _i, _i, _i, _i]),

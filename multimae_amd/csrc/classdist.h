@@ -332,6 +332,83 @@ __device__ float distill_position(const DistillArgs& a, long p, float w, Stats* 
     return l;
 }
 
+// ---- maps: a lane per position ------------------------------------------------------------------------------------------
+constexpr int POS = 64;  // positions of a tile: one wave
+
+// Reads a position's kept entries in groups, every load of a group on its way before the first is used: take(i, class or -1, value).
+template <class F>
+__device__ __forceinline__ void read_entries(const DistillArgs& a, long at, bool live, F take) {
+    constexpr int G = 8;
+    for (int i0 = 0; i0 < a.k; i0 += G) {
+        long cls[G];
+        float v[G];
+#pragma unroll
+        for (int u = 0; u < G; ++u) {
+            const long e = at + (long)(i0 + u < a.k ? i0 + u : a.k - 1) * a.g.inner;
+            cls[u] = load_class(a.top_class, a.class_bytes, e);
+            v[u] = load_any(a.top_value, a.value_dtype, e);
+        }
+#pragma unroll
+        for (int u = 0; u < G; ++u)
+            if (i0 + u < a.k) {
+                const bool in = live && cls[u] >= 0 && cls[u] < a.g.classes;
+                take(i0 + u, in ? (int)cls[u] : -1, in ? v[u] : -INFINITY);
+            }
+    }
+}
+
+// Adds the exponentials of N logits to a lane's running sums.
+template <int N, bool ENTROPY>
+__device__ __forceinline__ void add_logits(Sums& v, const float (&x)[N], float c) {
+    float m = x[0];
+#pragma unroll
+    for (int i = 1; i < N; ++i) m = fmaxf(m, x[i]);
+    if (m > v.m) {
+        v.m = m;
+        const float R = reference_exponent(m, c), d = v.R - R, f = exp2_(d);
+        if (ENTROPY) v.t = f * (v.t + bounded(d) * v.s);
+        v.s *= f;
+        v.R = R;
+    }
+    float s = 0.f, t = 0.f;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        const float d = __builtin_fmaf(x[i], c, -v.R), e = exp2_(d);
+        s += e;
+        if (ENTROPY) t = __builtin_fmaf(e, bounded(d), t);
+    }
+    v.s += s;
+    if (ENTROPY) v.t += t;
+}
+
+// A lane per position, its k kept values at q[i * POS]: their probabilities in place; total: their sum, left: what it leaves of 1,
+// loss: sum q log q.
+__device__ __forceinline__ void shares_of_log_probs(float* q, int k, float& total, float& left, float& loss) {
+    double sum = 0.0;  // 64 bits: the rest is what a sum near 1 leaves
+    for (int i = 0; i < k; ++i) {
+        const float x = q[i * POS], e = expf(x);
+        sum += exp((double)x);
+        if (e != 0.f) loss += e * x;
+        q[i * POS] = e;
+    }
+    total = (float)sum;
+    left = sum != sum ? total : fmaxf((float)(1.0 - sum), 0.f);
+}
+__device__ __forceinline__ void shares_of_logits(float* q, int k, float m, float c, float inv_t, float& total, float& loss) {
+    m = finite_ref(m);  // (the largest)
+    float sum = 0.f;
+    for (int i = 0; i < k; ++i) {
+        const float d = q[i * POS] - m, e = exp2_(d * c);
+        sum += e;
+        if (e != 0.f) loss += e * d;
+        q[i * POS] = e;
+    }
+    const float inv = sum != 0.f ? 1.f / sum : 0.f;
+    for (int i = 0; i < k; ++i) q[i * POS] *= inv;
+    total = sum > 0.f ? 1.f : (sum != sum ? sum : 0.f);
+    loss = sum != 0.f ? loss * inv * inv_t - log2_(sum) * LN2 : 0.f;
+}
+
 // A launch holds fewer than 2^32 threads.
 inline int fits_grid(const char* name, long blocks, int threads) {
     MMAE_REQUIRE(blocks * threads <= 0xffffffffL, MMAE_ESHAPE, "%s: %ld workgroups of %d threads are more than one launch holds", name, blocks, threads);
@@ -356,12 +433,21 @@ int log_probs_rows(int dtype, const LogProbArgs& a, void* workspace, hipStream_t
 int log_probs_bwd_rows(int dtype, const LogProbBwdArgs& a, hipStream_t stream);
 size_t distill_rows_workspace(int rows, int classes);
 int distill_rows(int dtype, const DistillArgs& a, void* workspace, bool again, hipStream_t stream);  // again: the workspace is an earlier call's
-// classdist_maps.hip: maps, inner > 1; *_fits: the classes of 64 positions fit the LDS
-bool log_probs_map_fits(int dtype, int classes, int top_k);
-int log_probs_map(int dtype, const LogProbArgs& a, hipStream_t stream);
+// Maps, inner > 1, whose classes are worked on in slices (count 1: all at once).  A slice leaves its sums and its k best keys (0: none)
+// of every position, sums[slice][position] and keys[slice][i][position].
+struct MapSlices { int count, width; Sums* sums; uint64_t* keys; };
+inline int map_tiles(int inner) { return inner / POS + (inner % POS != 0); }
+inline long map_blocks(const Geometry& g) { return (long)g.outer * map_tiles(g.inner); }
+// classdist_maps.hip
+int log_probs_map(int dtype, const LogProbArgs& a, const MapSlices& slices, hipStream_t stream);
 int log_probs_bwd_map(int dtype, const LogProbBwdArgs& a, hipStream_t stream);
-bool distill_map_fits(int dtype, int classes, int k);
-long distill_map_parts(int outer, int inner);
 int distill_map(int dtype, const DistillArgs& a, hipStream_t stream);
+// classdist_slices.hip
+MapSlices log_probs_map_slices(int dtype, int classes, int top_k);  // (without buffers)
+MapSlices distill_map_slices(int dtype, int classes);
+size_t log_probs_slices_workspace(const MapSlices& s, int outer, int inner, int top_k);
+int log_probs_slices(int dtype, const LogProbArgs& a, MapSlices s, void* workspace, hipStream_t stream);
+size_t distill_slices_workspace(const MapSlices& s, int outer, int inner, int k);
+int distill_slices(int dtype, const DistillArgs& a, const MapSlices& s, void* workspace, bool again, hipStream_t stream);
 
 }  // namespace classdist

@@ -1,80 +1,8 @@
-// Class distributions: entry points, the kernels that take any layout, and the mask's counts.
+// Class distributions: entry points and the mask's counts.
 #include "classdist.h"
 
 namespace classdist {
 namespace {
-
-// ---- log probabilities, one workgroup per position: class maps whose classes do not fit the LDS ----------------------
-template <class T>
-__global__ __launch_bounds__(256) void log_probs_kernel(LogProbArgs a) {
-    __shared__ Stats red[4];
-    __shared__ uint64_t best[4];
-    const typename T::E* z = (const typename T::E*)a.g.logits;
-    const long p = blockIdx.x, base = a.g.base(p), cs = a.g.inner;
-    const int C = a.g.classes;
-    const float c = a.g.c;
-    Stats v = {-INFINITY, 0.f, 0.f};
-    for (int j = threadIdx.x; j < C; j += 256) v.m = fmaxf(v.m, T::up(z[base + j * cs]));
-    const float r = finite_ref(v.m);
-    for (int j = threadIdx.x; j < C; j += 256) {
-        const float d = (T::up(z[base + j * cs]) - r) * c, e = exp2_(d);
-        v.s += e;
-        v.t += e * bounded(d);
-    }
-    v = block_stats(v, c, red);
-    const bool empty = v.m == -INFINITY && v.s == 0.f;
-    const float l2 = empty ? INFINITY : log2_(v.s), m = finite_ref(v.m);  // +inf: every log probability is -inf
-    if (threadIdx.x == 0) {
-        const long y = a.target[p];
-        a.log_prob[p] = y >= 0 && y < C ? a.g.log_p(T::up(z[base + y * cs]), m, l2) : 0.f;
-        a.entropy[p] = empty ? 0.f : (l2 - v.t / v.s) * LN2;
-        if (a.row_max) a.row_max[p] = m;
-        // for the backward pass relative to the reference exponent it uses
-        if (a.row_max) a.row_log_sum[p] = is_far(m, c) ? l2 : l2 + __builtin_fmaf(m, c, -reference_exponent(m, c));
-    }
-    const long at = (p / a.g.inner) * a.k * cs + p % a.g.inner;
-    uint64_t last = ~0ull;
-    for (int i = 0; i < a.k; ++i) {  // the largest key below the last one found
-        uint64_t top = 0;
-        for (int j = threadIdx.x; j < C; j += 256) {
-            const uint64_t key = rank_key(T::up(z[base + j * cs]), j);
-            if (key < last && key > top) top = key;
-        }
-#pragma unroll
-        for (int o = 32; o > 0; o >>= 1) {
-            const uint64_t w = __shfl_xor((unsigned long long)top, o, 64);
-            top = w > top ? w : top;
-        }
-        __syncthreads();
-        if ((threadIdx.x & 63) == 0) best[threadIdx.x >> 6] = top;
-        __syncthreads();
-        for (int w = 0; w < 4; ++w) top = best[w] > top ? best[w] : top;
-        last = top;
-        if (threadIdx.x == 0) {
-            const uint32_t j = 0xffffffffu - (uint32_t)top;
-            a.top_class[at + i * cs] = j;
-            a.top_log_prob[at + i * cs] = a.g.log_p(T::up(z[base + j * cs]), m, l2);
-        }
-    }
-}
-
-template <class T>
-__global__ __launch_bounds__(256) void distill_kernel(DistillArgs a) {
-    __shared__ Stats red[4];
-    __shared__ int s_cls[MAX_TOP];
-    __shared__ float s_q[MAX_TOP], s_tot[2];
-    if (a.upstream && a.skip_unit && a.upstream[0] == 1.f) return;
-    const long p = blockIdx.x, cs = a.g.inner;
-    const float w = position_weight(a, p);
-    if (w == 0.f) {
-        typename T::E* dz = (typename T::E*)a.d_logits + (p / cs) * a.g.classes * cs + p % cs;
-        if (a.d_logits) for (int j = threadIdx.x; j < a.g.classes; j += 256) dz[j * cs] = T::down(0.f);
-        if (threadIdx.x == 0 && a.part) a.part[p] = 0.f;
-        return;
-    }
-    const float l = distill_position<T>(a, p, w, red, s_cls, s_q, s_tot);
-    if (threadIdx.x == 0 && a.part) a.part[p] = l;
-}
 
 // Masked tokens per sample; then the number of samples that have any (of rows, and of samples of one token: from the mask).
 __global__ __launch_bounds__(64) void distill_count_kernel(const int64_t* mask, int outer, int tokens, float* count) {
@@ -122,8 +50,9 @@ int check_logits(const char* name, const void* logits, int dtype, int outer, int
 
 using namespace classdist;
 
-extern "C" size_t mmae_class_log_probs_workspace_bytes(int outer, int classes, int inner, int top_k) {
-    return inner != 1 || outer < 1 || classes < 1 || top_k < 0 ? 0 : log_probs_rows_workspace(outer, classes, top_k);
+extern "C" size_t mmae_class_log_probs_workspace_bytes(int dtype, int outer, int classes, int inner, int top_k) {
+    if (outer < 1 || classes < 1 || inner < 1 || top_k < 0) return 0;
+    return inner == 1 ? log_probs_rows_workspace(outer, classes, top_k) : log_probs_slices_workspace(log_probs_map_slices(dtype, classes, top_k), outer, inner, top_k);
 }
 
 extern "C" int mmae_class_log_probs(const void* logits, int dtype, int outer, int classes, int inner, long ld, const int64_t* target,
@@ -138,19 +67,9 @@ extern "C" int mmae_class_log_probs(const void* logits, int dtype, int outer, in
                  "class_log_probs: %d top classes of %d (at most %d)", top_k, classes, MAX_TOP);
     LogProbArgs a = {{logits, ld, outer, classes, inner, LOG2E / temperature, 1.f / temperature}, target, top_k, log_prob, entropy, row_max,
                      row_log_sum, top_log_prob, top_class};
-    MMAE_REQUIRE(workspace_bytes >= mmae_class_log_probs_workspace_bytes(outer, classes, inner, top_k) && (workspace || !workspace_bytes),
+    MMAE_REQUIRE(workspace_bytes >= mmae_class_log_probs_workspace_bytes(dtype, outer, classes, inner, top_k) && (workspace || !workspace_bytes),
                  MMAE_EWORKSPACE, "class_log_probs: workspace too small");
-    int r = MMAE_OK;
-    if (inner == 1) {
-        r = log_probs_rows(dtype, a, workspace, stream);
-    } else if (log_probs_map_fits(dtype, classes, top_k)) {
-        r = log_probs_map(dtype, a, stream);
-    } else {
-        REQUIRE_GRID("class_log_probs", (long)outer * inner, 256);
-#define CALL(T) hipLaunchKernelGGL(log_probs_kernel<T>, dim3(outer * inner), dim3(256), 0, stream, a)
-        BY_DTYPE(dtype, CALL);
-#undef CALL
-    }
+    const int r = inner == 1 ? log_probs_rows(dtype, a, workspace, stream) : log_probs_slices(dtype, a, log_probs_map_slices(dtype, classes, top_k), workspace, stream);
     if (r != MMAE_OK) return r;
     MMAE_CHECK_LAUNCH("class_log_probs");
     return MMAE_OK;
@@ -171,15 +90,14 @@ extern "C" int mmae_class_log_probs_bwd(const void* logits, int dtype, int outer
     return MMAE_OK;
 }
 
-// Parts of the loss that are added at the end: one per row, per tile of a map, or per position.
-static long distill_parts(int dtype, int outer, int classes, int inner, int k) {
-    return inner == 1 ? outer : distill_map_fits(dtype, classes, k) ? distill_map_parts(outer, inner) : (long)outer * inner;
-}
+// Parts of the loss that are added at the end: one per row, or per tile of a map.
+static long distill_parts(int outer, int inner) { return inner == 1 ? outer : (long)outer * map_tiles(inner); }
 static size_t distill_floats(int outer, long parts) { return (4 + (size_t)outer + (size_t)parts + 3) / 4 * 4; }
 
 extern "C" size_t mmae_distill_workspace_bytes(int dtype, int outer, int classes, int inner, int k) {
     if (outer < 1 || classes < 1 || inner < 1) return 0;
-    return sizeof(float) * distill_floats(outer, distill_parts(dtype, outer, classes, inner, k)) + (inner == 1 ? distill_rows_workspace(outer, classes) : 0);
+    return sizeof(float) * distill_floats(outer, distill_parts(outer, inner)) +
+           (inner == 1 ? distill_rows_workspace(outer, classes) : distill_slices_workspace(distill_map_slices(dtype, classes), outer, inner, k));
 }
 
 extern "C" int mmae_distill(const void* logits, int dtype, int outer, int classes, int inner, long ld, const void* top_class,
@@ -215,18 +133,11 @@ extern "C" int mmae_distill(const void* logits, int dtype, int outer, int classe
         hipLaunchKernelGGL(distill_valid_kernel, dim3(1), dim3(1024), 0, stream, ws + 4, a.tokens > 1 ? nullptr : mask, outer, ws);
         MMAE_CHECK_LAUNCH("distill_valid");
     }
-    const long parts = distill_parts(dtype, outer, classes, inner, k);
-    int r = MMAE_OK;
-    if (inner == 1) {
-        r = distill_rows(dtype, a, ws + distill_floats(outer, parts), again, stream);
-    } else if (distill_map_fits(dtype, classes, k)) {
-        r = distill_map(dtype, a, stream);
-    } else {
-        REQUIRE_GRID("distill", (long)outer * inner, 256);
-#define CALL(T) hipLaunchKernelGGL(distill_kernel<T>, dim3(outer * inner), dim3(256), 0, stream, a)
-        BY_DTYPE(dtype, CALL);
-#undef CALL
-    }
+    const long parts = distill_parts(outer, inner);
+    void* room = ws + distill_floats(outer, parts);
+    const MapSlices s = distill_map_slices(dtype, classes);
+    const int r = inner == 1 ? distill_rows(dtype, a, room, again, stream)
+                             : s.count == 1 ? distill_map(dtype, a, stream) : distill_slices(dtype, a, s, room, again, stream);
     if (r != MMAE_OK) return r;
     MMAE_CHECK_LAUNCH("distill");
     if (loss) {

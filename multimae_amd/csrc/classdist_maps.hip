@@ -7,7 +7,6 @@
 namespace classdist {
 namespace {
 
-constexpr int POS = 64;            // positions of a tile: one wave
 constexpr int LDS_BYTES = 160 * 1024;
 constexpr uint32_t NONE = 0xffffffffu;
 
@@ -49,52 +48,6 @@ __device__ __forceinline__ void load_map_tile(typename T::E* tile, const typenam
             if (id < pieces) *(Piece*)(tile + (size_t)id * T::VEC) = q[u];
         }
     }
-}
-
-// Reads a position's kept entries in groups, every load of a group on its way before the first is used: take(i, class or -1, value).
-template <class F>
-__device__ __forceinline__ void read_entries(const DistillArgs& a, long at, bool live, F take) {
-    constexpr int G = 8;
-    for (int i0 = 0; i0 < a.k; i0 += G) {
-        long cls[G];
-        float v[G];
-#pragma unroll
-        for (int u = 0; u < G; ++u) {
-            const long e = at + (long)(i0 + u < a.k ? i0 + u : a.k - 1) * a.g.inner;
-            cls[u] = load_class(a.top_class, a.class_bytes, e);
-            v[u] = load_any(a.top_value, a.value_dtype, e);
-        }
-#pragma unroll
-        for (int u = 0; u < G; ++u)
-            if (i0 + u < a.k) {
-                const bool in = live && cls[u] >= 0 && cls[u] < a.g.classes;
-                take(i0 + u, in ? (int)cls[u] : -1, in ? v[u] : -INFINITY);
-            }
-    }
-}
-
-// Adds the exponentials of N logits to a lane's running sums.
-template <int N, bool ENTROPY>
-__device__ __forceinline__ void add_logits(Sums& v, const float (&x)[N], float c) {
-    float m = x[0];
-#pragma unroll
-    for (int i = 1; i < N; ++i) m = fmaxf(m, x[i]);
-    if (m > v.m) {
-        v.m = m;
-        const float R = reference_exponent(m, c), d = v.R - R, f = exp2_(d);
-        if (ENTROPY) v.t = f * (v.t + bounded(d) * v.s);
-        v.s *= f;
-        v.R = R;
-    }
-    float s = 0.f, t = 0.f;
-#pragma unroll
-    for (int i = 0; i < N; ++i) {
-        const float d = __builtin_fmaf(x[i], c, -v.R), e = exp2_(d);
-        s += e;
-        if (ENTROPY) t = __builtin_fmaf(e, bounded(d), t);
-    }
-    v.s += s;
-    if (ENTROPY) v.t += t;
 }
 
 // ---- log probabilities ----------------------------------------------------------------------------------------------
@@ -144,17 +97,20 @@ inline int log_probs_map_bytes(int element, int classes, int k, int waves) {
 }
 
 template <class T, int K>
-__global__ __launch_bounds__(64 * most_waves(K)) void log_probs_map_kernel(LogProbArgs a, int tiles) {
+__global__ __launch_bounds__(64 * most_waves(K)) void log_probs_map_kernel(LogProbArgs a, int tiles, MapSlices sl) {
     extern __shared__ __align__(16) char smem[];
-    const int C = a.g.classes, inner = a.g.inner, k = a.k, waves = blockDim.x / 64, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int slice = blockIdx.x / tiles % sl.count, first = slice * sl.width, C = a.g.classes - first < sl.width ? a.g.classes - first : sl.width;
+    const int inner = a.g.inner, k = a.k, waves = blockDim.x / 64, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     typename T::E* tile = (typename T::E*)smem;
     Sums* s_sums = (Sums*)(smem + (C * POS * sizeof(typename T::E) + 15) / 16 * 16);
     float* s_list = (float*)(s_sums + waves * POS);
     uint32_t* s_queue = (uint32_t*)s_list;
     constexpr int REGION = K * 4 > QUEUE * 4 ? K * 4 : QUEUE * 4;
     uint32_t* s_slot = (uint32_t*)((char*)s_list + (K ? waves * POS * REGION : 0));
-    const int b = blockIdx.x / tiles, i0 = blockIdx.x % tiles * POS, n = inner - i0 < POS ? inner - i0 : POS;
-    const typename T::E* z = (const typename T::E*)a.g.logits + b * a.g.ld + i0;
+    const int b = blockIdx.x / tiles / sl.count, i0 = blockIdx.x % tiles * POS, n = inner - i0 < POS ? inner - i0 : POS;
+    const typename T::E* z = (const typename T::E*)a.g.logits + b * a.g.ld + (long)first * inner + i0;
+    const long positions = (long)a.g.outer * inner;
+    const bool whole = sl.count == 1;
     const float c = a.g.c;
     load_map_tile<T>(tile, z, C, inner, n);
     if (!carries<T>())
@@ -198,7 +154,9 @@ __global__ __launch_bounds__(64 * most_waves(K)) void log_probs_map_kernel(LogPr
     __syncthreads();
     v = s_sums[lane];
     for (int w = 1; w < waves; ++w) v = join(v, s_sums[w * POS + lane]);
-    const bool far = is_far(v.m, c) && v.s == v.s;
+    const long p = (long)b * inner + i0 + lane;
+    if (!whole && wave == 0 && lane < n) sl.sums[slice * positions + p] = v;
+    const bool far = whole && is_far(v.m, c) && v.s == v.s;
     if (__any(far)) {
         float s = 0.f, t = 0.f;
         for (int j = 0; j < C; ++j) {
@@ -211,8 +169,7 @@ __global__ __launch_bounds__(64 * most_waves(K)) void log_probs_map_kernel(LogPr
     if (v.m == INFINITY) v.s = __builtin_nanf("");
     const bool empty = v.m == -INFINITY && v.s == 0.f;
     const float l2 = empty ? INFINITY : log2_(v.s);
-    const long p = (long)b * inner + i0 + lane;
-    if (wave == 0 && lane < n) {
+    if (whole && wave == 0 && lane < n) {
         const long y = a.target[p];
         a.log_prob[p] = y >= 0 && y < C ? row_log_p(a.g, T::up(tile[y * POS + lane]), v.m, l2) : 0.f;
         a.entropy[p] = empty ? 0.f : (l2 - v.t / v.s) * LN2;
@@ -243,8 +200,14 @@ __global__ __launch_bounds__(64 * most_waves(K)) void log_probs_map_kernel(LogPr
                 for (int i = 0; i < K; ++i)
                     if (i < k && i % waves == wave) {
                         const long at = ((long)b * k + i) * inner + i0 + lane;
-                        a.top_class[at] = carried_class(best[i]);
-                        a.top_log_prob[at] = row_log_p(a.g, carried_value(best[i]), v.m, l2);
+                        const int cls = carried_class(best[i]);
+                        const float x = carried_value(best[i]);
+                        if (whole) {
+                            a.top_class[at] = cls;
+                            a.top_log_prob[at] = row_log_p(a.g, x, v.m, l2);
+                        } else {
+                            sl.keys[((long)slice * k + i) * positions + p] = i < C ? rank_key(x, first + cls) : 0;
+                        }
                     }
             }
             return;
@@ -284,8 +247,12 @@ __global__ __launch_bounds__(64 * most_waves(K)) void log_probs_map_kernel(LogPr
             for (int i = wave; i < k; i += waves) {
                 const uint32_t cls = s_slot[i * POS + lane];
                 const long at = ((long)b * k + i) * inner + i0 + lane;
-                a.top_class[at] = cls;
-                a.top_log_prob[at] = row_log_p(a.g, T::up(tile[cls * POS + lane]), v.m, l2);
+                if (whole) {
+                    a.top_class[at] = cls;
+                    a.top_log_prob[at] = row_log_p(a.g, T::up(tile[cls * POS + lane]), v.m, l2);
+                } else {
+                    sl.keys[((long)slice * k + i) * positions + p] = i < C ? rank_key(T::up(tile[cls * POS + lane]), first + cls) : 0;
+                }
             }
     }
 }
@@ -405,30 +372,8 @@ __global__ __launch_bounds__(1024) void distill_map_kernel(DistillArgs a, int ti
             s_q[i * POS + lane] = x;
             m = fmaxf(m, x);
         });
-        if (REST) {
-            double sum = 0.0;  // 64 bits: the rest is what a sum near 1 leaves
-            for (int i = 0; i < k; ++i) {
-                const float x = s_q[i * POS + lane], q = expf(x);
-                sum += exp((double)x);
-                if (q != 0.f) loss += q * x;
-                s_q[i * POS + lane] = q;
-            }
-            total = (float)sum;
-            left = sum != sum ? total : fmaxf((float)(1.0 - sum), 0.f);
-        } else {
-            m = finite_ref(m);
-            float sum = 0.f;
-            for (int i = 0; i < k; ++i) {
-                const float d = s_q[i * POS + lane] - m, q = exp2_(d * c);
-                sum += q;
-                if (q != 0.f) loss += q * d;
-                s_q[i * POS + lane] = q;
-            }
-            const float inv = sum != 0.f ? 1.f / sum : 0.f;
-            for (int i = 0; i < k; ++i) s_q[i * POS + lane] *= inv;
-            total = sum > 0.f ? 1.f : (sum != sum ? sum : 0.f);
-            loss = sum != 0.f ? loss * inv * a.g.inv_t - log2_(sum) * LN2 : 0.f;
-        }
+        if (REST) shares_of_log_probs(s_q + lane, k, total, left, loss);
+        else shares_of_logits(s_q + lane, k, m, c, a.g.inv_t, total, loss);
     }
     __syncthreads();
     if (wave == 0) {
@@ -904,8 +849,6 @@ int allow_lds(const void* kernel, int bytes, const char* name) {
     return MMAE_OK;
 }
 
-int element_bytes(int dtype) { return dtype == MMAE_DT_F32 ? 4 : 2; }
-int map_tiles(int inner) { return inner / POS + (inner % POS != 0); }
 constexpr int DISTILL_STATIC = 1024;  // the distillation kernel's fixed arrays (an upper bound)
 
 // The largest number of waves that map_waves may ask for and that fits.
@@ -918,16 +861,17 @@ int fitting_waves(long tiles, int classes, F bytes, int room, int most) {
 }
 
 template <class T, int K>
-int launch_log_probs_map(const LogProbArgs& a, hipStream_t stream) {
-    const int tiles = map_tiles(a.g.inner), C = a.g.classes, k = a.k;
-    const int waves = fitting_waves((long)a.g.outer * tiles, C, [&](int w) { return log_probs_map_bytes(sizeof(typename T::E), C, k, w); }, LDS_BYTES, most_waves(K));
+int launch_log_probs_map(const LogProbArgs& a, const MapSlices& s, hipStream_t stream) {
+    const int tiles = map_tiles(a.g.inner), C = s.width, k = a.k;
+    const long all = (long)a.g.outer * tiles * s.count;
+    const int waves = fitting_waves(all, C, [&](int w) { return log_probs_map_bytes(sizeof(typename T::E), C, k, w); }, LDS_BYTES, most_waves(K));
     const int bytes = log_probs_map_bytes(sizeof(typename T::E), C, k, waves);
     if (bytes > 65536) {
         const int rc = allow_lds((const void*)log_probs_map_kernel<T, K>, bytes, "class_log_probs");
         if (rc != MMAE_OK) return rc;
     }
-    REQUIRE_GRID("class_log_probs", (long)a.g.outer * tiles, 64 * waves);
-    hipLaunchKernelGGL((log_probs_map_kernel<T, K>), dim3((unsigned)((long)a.g.outer * tiles)), dim3(64 * waves), bytes, stream, a, tiles);
+    REQUIRE_GRID("class_log_probs", all, 64 * waves);
+    hipLaunchKernelGGL((log_probs_map_kernel<T, K>), dim3((unsigned)all), dim3(64 * waves), bytes, stream, a, tiles, s);
     return MMAE_OK;
 }
 // The register kernels take what fits them.  Distillation alone shares a tile of a small map among the waves of a workgroup: its
@@ -945,7 +889,7 @@ bool in_registers(int classes, int k) { return classes <= REG_CLASSES && k <= RE
     } while (0)
 
 template <class T>
-int launch_log_probs_map(const LogProbArgs& a, hipStream_t stream) {
+int launch_log_probs_map(const LogProbArgs& a, const MapSlices& s, hipStream_t stream) {
     const int tiles = map_tiles(a.g.inner);
     const long all = (long)a.g.outer * tiles;
     if (in_registers(a.g.classes, a.k)) {
@@ -961,11 +905,11 @@ int launch_log_probs_map(const LogProbArgs& a, hipStream_t stream) {
         return MMAE_OK;
     }
     switch (list_slots(a.k)) {
-        case 0: return launch_log_probs_map<T, 0>(a, stream);
-        case 8: return launch_log_probs_map<T, 8>(a, stream);
-        case 16: return launch_log_probs_map<T, 16>(a, stream);
-        case 32: return launch_log_probs_map<T, 32>(a, stream);
-        default: return launch_log_probs_map<T, 64>(a, stream);
+        case 0: return launch_log_probs_map<T, 0>(a, s, stream);
+        case 8: return launch_log_probs_map<T, 8>(a, s, stream);
+        case 16: return launch_log_probs_map<T, 16>(a, s, stream);
+        case 32: return launch_log_probs_map<T, 32>(a, s, stream);
+        default: return launch_log_probs_map<T, 64>(a, s, stream);
     }
 }
 
@@ -994,17 +938,9 @@ int launch_distill_map(const DistillArgs& a, hipStream_t stream) {
 
 }  // namespace
 
-bool log_probs_map_fits(int dtype, int classes, int top_k) {
-    return classes <= 4096 && log_probs_map_bytes(element_bytes(dtype), classes, top_k, 1) <= LDS_BYTES;
-}
-bool distill_map_fits(int dtype, int classes, int k) {
-    return classes <= 4096 && distill_map_bytes(element_bytes(dtype), classes, k, 1) <= LDS_BYTES - DISTILL_STATIC;
-}
-long distill_map_parts(int outer, int inner) { return (long)outer * map_tiles(inner); }
-
-int log_probs_map(int dtype, const LogProbArgs& a, hipStream_t stream) {
-    return dtype == MMAE_DT_F32 ? launch_log_probs_map<F32>(a, stream)
-                                : dtype == MMAE_DT_BF16 ? launch_log_probs_map<B16>(a, stream) : launch_log_probs_map<H16>(a, stream);
+int log_probs_map(int dtype, const LogProbArgs& a, const MapSlices& s, hipStream_t stream) {
+    return dtype == MMAE_DT_F32 ? launch_log_probs_map<F32>(a, s, stream)
+                                : dtype == MMAE_DT_BF16 ? launch_log_probs_map<B16>(a, s, stream) : launch_log_probs_map<H16>(a, s, stream);
 }
 
 int log_probs_bwd_map(int dtype, const LogProbBwdArgs& a, hipStream_t stream) {

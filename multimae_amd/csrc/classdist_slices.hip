@@ -1,0 +1,314 @@
+// Class distributions over maps [B, C, inner] of more classes than a workgroup's LDS holds well: slices of the classes, whose sums
+// (and best classes) are joined per position.  Read once for the log probabilities, twice for distillation with its gradient.
+//
+// A wave's load is one class of 64 neighbouring positions.  131 x 1000 x 32 x 32 fp32 (537 MB): log probabilities 119 us (4.5 TB/s),
+// with 8 alternatives 560 us, where the lists' arithmetic bounds them, distillation with its gradient 440 us (three passes, 3.7 TB/s);
+// a workgroup per position, which reads a line for each of its logits, takes 1270, 9121 and 4030 us.  Maps of few positions a
+// sample (2 x 2) leave most lanes idle.
+#include "classdist.h"
+
+namespace classdist {
+namespace {
+
+constexpr int U = 8;  // loads on their way
+
+// The slices' sums of one position.
+__device__ __forceinline__ Sums join_slices(const Sums* sums, int count, long positions) {
+    Sums v = {-INFINITY, -FAR, 0.f, 0.f};
+    for (int s0 = 0; s0 < count; s0 += U) {
+        Sums x[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) x[u] = sums[(s0 + u < count ? s0 + u : count - 1) * positions];
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+            if (s0 + u < count) v = join(v, x[u]);
+    }
+    return v;
+}
+
+// A lane per position: joins the sums and walks the slices' sorted keys, each into the list of the best so far (in the LDS, sorted)
+// as long as they reach it.
+template <class T>
+__global__ __launch_bounds__(64) void log_probs_map_join_kernel(LogProbArgs a, int tiles, MapSlices sl) {
+    extern __shared__ uint64_t s_best[];  // [k][POS]
+    const int inner = a.g.inner, k = a.k, lane = threadIdx.x;
+    const int b = blockIdx.x / tiles, i0 = blockIdx.x % tiles * POS, n = inner - i0 < POS ? inner - i0 : POS;
+    if (lane >= n) return;
+    const long positions = (long)a.g.outer * inner, p = (long)b * inner + i0 + lane;
+    const typename T::E* z = (const typename T::E*)a.g.logits + b * a.g.ld + i0 + lane;
+    const float c = a.g.c;
+    const long y = a.target[p];
+    const bool named = y >= 0 && y < a.g.classes;
+    const float zy = T::up(z[(named ? y : 0) * inner]);
+    Sums v = join_slices(sl.sums + p, sl.count, positions);
+    if (is_far(v.m, c) && v.s == v.s) {
+        v.s = v.t = 0.f;
+        for (int j = 0; j < a.g.classes; ++j) {
+            const float d = (T::up(z[(long)j * inner]) - v.m) * c, e = exp2_(d);
+            v.s += e;
+            v.t += e * bounded(d);
+        }
+    }
+    if (v.m == INFINITY) v.s = __builtin_nanf("");
+    const bool empty = v.m == -INFINITY && v.s == 0.f;
+    const float l2 = empty ? INFINITY : log2_(v.s);
+    a.log_prob[p] = named ? row_log_p(a.g, zy, v.m, l2) : 0.f;
+    a.entropy[p] = empty ? 0.f : (l2 - v.t / v.s) * LN2;
+    if (a.row_max) {
+        a.row_max[p] = v.m;
+        a.row_log_sum[p] = l2;
+    }
+    if (!k) return;
+    uint64_t* best = s_best + lane;
+    const uint64_t* keys = sl.keys + p;
+    for (int i = 0; i < k; ++i) best[i * POS] = keys[i * positions];  // the first slice's are sorted already
+    uint64_t worst = best[(k - 1) * POS];
+    for (int s = 1; s < sl.count; ++s) {
+        const uint64_t* from = keys + (long)s * k * positions;
+        bool more = true;
+        for (int i0 = 0; i0 < k && more; i0 += U) {
+            uint64_t key[U];
+#pragma unroll
+            for (int u = 0; u < U; ++u) key[u] = from[(i0 + u < k ? i0 + u : k - 1) * positions];
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                more = more && i0 + u < k && key[u] > worst;
+                if (more) {
+                    int j = k - 1;
+                    for (; j > 0; --j) {
+                        const uint64_t above = best[(j - 1) * POS];
+                        if (above > key[u]) break;
+                        best[j * POS] = above;
+                    }
+                    best[j * POS] = key[u];
+                    worst = best[(k - 1) * POS];
+                }
+            }
+        }
+    }
+    for (int i = 0; i < k; ++i) {
+        const uint64_t key = best[i * POS];
+        const long at = ((long)b * k + i) * inner + i0 + lane;
+        a.top_class[at] = key_class(key);
+        a.top_log_prob[at] = row_log_p(a.g, key_value(key), v.m, l2);
+    }
+}
+
+// ---- distillation -------------------------------------------------------------------------------------------------------
+// First the sums over the classes that are not kept, a bit per class and position of the slice says which are; then a lane per
+// position joins them, adds the kept classes and leaves the factors of the gradient; then the gradient, slice by slice.
+constexpr int SLICE_BYTES = 64 * 1024, MOST_WIDTH = SLICE_BYTES / (POS * 2);  // a CU holds two such tiles
+
+struct SliceNotes {  // per position: gradient = F 2^(x c - R) where not kept; the kept classes' gradients beside
+    float *F, *R;
+    int* cls;   // [k][positions], -1: none
+    float* g;
+};
+__device__ __forceinline__ bool settled(float R) { return R != R; }  // the position's gradient is written
+
+__device__ __forceinline__ bool skip_call(const DistillArgs& a) { return a.upstream && a.skip_unit && a.upstream[0] == 1.f; }
+
+template <class T>
+__global__ __launch_bounds__(256) void distill_map_sums_kernel(DistillArgs a, int tiles, int count, int width, Sums* sums) {
+    __shared__ uint32_t kept[MOST_WIDTH * 2];
+    __shared__ Sums part[4 * POS];
+    const int slice = blockIdx.x / tiles % count, first = slice * width, C = a.g.classes - first < width ? a.g.classes - first : width;
+    const int b = blockIdx.x / tiles / count, i0 = blockIdx.x % tiles * POS, inner = a.g.inner, n = inner - i0 < POS ? inner - i0 : POS;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, i = i0 + (lane < n ? lane : n - 1);
+    const long p = (long)b * inner + i;
+    const float w = position_weight(a, p), c = a.g.c;
+    if (!__any(w != 0.f)) return;  // (the same in every wave)
+    for (int j = threadIdx.x; j < 2 * C; j += 256) kept[j] = 0;
+    __syncthreads();
+    for (int e = wave; e < a.k; e += 4) {
+        const long cls = load_class(a.top_class, a.class_bytes, ((long)b * a.k + e) * inner + i) - first;
+        if (cls >= 0 && cls < C && lane < n) atomicOr(&kept[cls * 2 + (lane >> 5)], 1u << (lane & 31));
+    }
+    __syncthreads();
+    const typename T::E* z = (const typename T::E*)a.g.logits + b * a.g.ld + (long)first * inner + i;
+    const int c0 = C * wave / 4, c1 = C * (wave + 1) / 4;
+    Sums v = {-INFINITY, -FAR, 0.f, 0.f};
+    for (int j = c0; j < c1; j += U) {
+        float x[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) x[u] = T::up(z[(long)(j + u < c1 ? j + u : c1 - 1) * inner]);
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const bool in = j + u < c1 && !(kept[(j + u < c1 ? j + u : c1 - 1) * 2 + (lane >> 5)] >> (lane & 31) & 1);
+            x[u] = in ? x[u] : -INFINITY;
+        }
+        add_logits<U, false>(v, x, c);
+    }
+    part[threadIdx.x] = v;
+    __syncthreads();
+    if (wave == 0 && lane < n) {
+        for (int o = 1; o < 4; ++o) v = join(v, part[o * POS + lane]);
+        sums[(long)slice * a.g.outer * inner + p] = v;
+    }
+}
+
+template <class T>
+__global__ __launch_bounds__(64) void distill_map_join_kernel(DistillArgs a, int tiles, int count, const Sums* sums, SliceNotes notes) {
+    extern __shared__ int s_cls[];  // [k][POS], then q (later the gradient) and the student's logits alike
+    __shared__ Stats red_far[4];
+    __shared__ int far_cls[MAX_TOP];
+    __shared__ float far_q[MAX_TOP], far_tot[2];
+    if (skip_call(a)) return;
+    const int inner = a.g.inner, k = a.k, lane = threadIdx.x;
+    const int b = blockIdx.x / tiles, i0 = blockIdx.x % tiles * POS, n = inner - i0 < POS ? inner - i0 : POS;
+    const int i = i0 + (lane < n ? lane : n - 1);
+    const long positions = (long)a.g.outer * inner, p = (long)b * inner + i;
+    const float c = a.g.c, w = lane < n ? position_weight(a, p) : 0.f;
+    const uint64_t live = __ballot(w != 0.f);
+    if (!live) {
+        if (lane == 0 && a.part) a.part[blockIdx.x] = 0.f;
+        return;
+    }
+    const typename T::E* z = (const typename T::E*)a.g.logits + b * a.g.ld + i;
+    float* s_q = (float*)s_cls + k * POS;
+    float* s_z = s_q + k * POS;
+    float m = -INFINITY, total = 0.f, left = 0.f, loss = 0.f;
+    read_entries(a, (long)b * k * inner + i, w != 0.f, [&](int e, int cls, float x) {
+        s_cls[e * POS + lane] = cls;
+        s_q[e * POS + lane] = x;
+        s_z[e * POS + lane] = cls >= 0 ? T::up(z[(long)cls * inner]) : -INFINITY;
+        m = fmaxf(m, x);
+    });
+    if (a.log_probs) shares_of_log_probs(s_q + lane, k, total, left, loss);
+    else shares_of_logits(s_q + lane, k, m, c, a.g.inv_t, total, loss);
+    for (int e = 1; e < k; ++e) {  // an entry listed before adds its q to that one
+        const int cls = s_cls[e * POS + lane];
+        for (int o = 0; o < e && cls >= 0; ++o)
+            if (s_cls[o * POS + lane] == cls) {
+                s_q[o * POS + lane] += s_q[e * POS + lane];
+                s_cls[e * POS + lane] = -1;
+                break;
+            }
+    }
+    const Sums rest = join_slices(sums + p, count, positions);
+    Sums v = rest;
+    for (int e = 0; e < k; ++e)
+        if (s_cls[e * POS + lane] >= 0) {
+            const float x[1] = {s_z[e * POS + lane]};
+            add_logits<1, false>(v, x, c);
+        }
+    if (v.m == INFINITY) v.s = __builtin_nanf("");
+    const bool empty = v.m == -INFINITY && v.s == 0.f;
+    const float l2 = empty ? INFINITY : log2_(v.s);
+    const float r = a.log_probs && rest.s != 0.f ? left : 0.f, Q = total + r;
+    const float gs = empty ? 0.f : w * a.g.inv_t * (a.upstream ? a.upstream[0] : 1.f);
+    const bool far = w != 0.f && is_far(v.m, c);
+    for (int e = 0; e < k; ++e) {
+        int cls = s_cls[e * POS + lane];
+        const float q = s_q[e * POS + lane], x = s_z[e * POS + lane];
+        if (cls >= 0 && q != 0.f) loss -= q * row_log_p(a.g, x, v.m, l2);
+        if (a.d_logits && lane < n) {
+            notes.cls[e * positions + p] = w != 0.f && !far ? cls : -1;
+            notes.g[e * positions + p] = gs * (exp2_(__builtin_fmaf(x, c, -v.R) - l2) * Q - q);
+        }
+    }
+    if (r != 0.f) loss += r * (log2_(r) - ((rest.R - v.R) + log2_(rest.s) - l2)) * LN2;
+    loss = wave_sum(w != 0.f && !far ? w * loss : 0.f);
+    if (a.d_logits && lane < n) {
+        notes.F[p] = w != 0.f ? gs * (Q * exp2_(rest.R - v.R - l2) - (r != 0.f ? r / rest.s : 0.f)) : 0.f;
+        notes.R[p] = far ? __builtin_nanf("") : rest.R;
+    }
+    for (uint64_t f = __ballot(far); f; f &= f - 1) {
+        const long at = (long)b * inner + i0 + __builtin_ctzll(f);
+        __syncthreads();
+        loss += distill_position<T>(a, at, position_weight(a, at), red_far, far_cls, far_q, far_tot);
+    }
+    if (lane == 0 && a.part) a.part[blockIdx.x] = loss;
+}
+
+template <class T>
+__global__ __launch_bounds__(256) void distill_map_gradient_kernel(DistillArgs a, int tiles, int count, int width, SliceNotes notes) {
+    if (skip_call(a)) return;
+    const int slice = blockIdx.x / tiles % count, first = slice * width, C = a.g.classes - first < width ? a.g.classes - first : width;
+    const int b = blockIdx.x / tiles / count, i0 = blockIdx.x % tiles * POS, inner = a.g.inner, n = inner - i0 < POS ? inner - i0 : POS;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, i = i0 + (lane < n ? lane : n - 1);
+    const long p = (long)b * inner + i, positions = (long)a.g.outer * inner;
+    const float w = position_weight(a, p), c = a.g.c;
+    const bool any = __any(w != 0.f);  // (the same in every wave; else the notes are not written)
+    const float F = any ? notes.F[p] : 0.f, R = any ? notes.R[p] : 0.f;
+    const bool mine = lane < n && !settled(R);
+    const typename T::E* z = (const typename T::E*)a.g.logits + b * a.g.ld + (long)first * inner + i;
+    typename T::E* dz = (typename T::E*)a.d_logits + ((long)b * a.g.classes + first) * inner + i;
+    const int c0 = C * wave / 4, c1 = C * (wave + 1) / 4;
+    for (int j = c0; j < c1; j += U) {
+        float x[U];
+        if (any) {
+#pragma unroll
+            for (int u = 0; u < U; ++u) x[u] = T::up(z[(long)(j + u < c1 ? j + u : c1 - 1) * inner]);
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+            if (mine && j + u < c1) dz[(long)(j + u) * inner] = T::down(any && F != 0.f ? F * exp2_(__builtin_fmaf(x[u], c, -R)) : 0.f);
+    }
+    if (!any) return;
+    __syncthreads();
+    for (int e = wave; e < a.k; e += 4) {
+        const int cls = notes.cls[e * positions + p];
+        const float g = notes.g[e * positions + p];
+        if (mine && cls >= first && cls < first + C) dz[(long)(cls - first) * inner] = T::down(g);
+    }
+}
+
+SliceNotes slice_notes(char* at, long positions, int k) {
+    float* f = (float*)at;
+    return {f, f + positions, (int*)(f + 2 * positions), f + (2 + k) * positions};
+}
+
+}  // namespace
+
+static MapSlices map_slices(int dtype, int classes, int whole) {
+    const int bytes = POS * (dtype == MMAE_DT_F32 ? 4 : 2), most = SLICE_BYTES / bytes;
+    const int count = (long)classes * bytes <= whole ? 1 : (classes + most - 1) / most, width = (classes + count - 1) / count;
+    return {(classes + width - 1) / width, width, nullptr, nullptr};
+}
+// Whole up to a tile of 80 KiB where slices cost more than they overlap: distillation, which reads them twice (109 x 300 x 64 x 64
+// fp32: 431 us whole, 541 us sliced), and long lists of alternatives (64: 1878 and 3765 us; 8: 508 and 363 us, none: 192 and
+// 127 us).
+constexpr int WHOLE_BYTES = 80 * 1024;
+MapSlices log_probs_map_slices(int dtype, int classes, int top_k) { return map_slices(dtype, classes, top_k > 16 ? WHOLE_BYTES : SLICE_BYTES); }
+MapSlices distill_map_slices(int dtype, int classes) { return map_slices(dtype, classes, WHOLE_BYTES); }
+
+size_t log_probs_slices_workspace(const MapSlices& s, int outer, int inner, int top_k) {
+    return s.count == 1 ? 0 : (size_t)outer * inner * s.count * (sizeof(Sums) + sizeof(uint64_t) * (size_t)top_k);
+}
+
+int log_probs_slices(int dtype, const LogProbArgs& a, MapSlices s, void* workspace, hipStream_t stream) {
+    s.sums = (Sums*)workspace;
+    s.keys = (uint64_t*)(s.sums + (size_t)a.g.outer * a.g.inner * s.count);
+    const int rc = log_probs_map(dtype, a, s, stream);
+    if (rc != MMAE_OK || s.count == 1) return rc;
+    const int tiles = map_tiles(a.g.inner);
+#define CALL(T) hipLaunchKernelGGL(log_probs_map_join_kernel<T>, dim3((unsigned)map_blocks(a.g)), dim3(64), a.k * POS * sizeof(uint64_t), stream, a, tiles, s)
+    BY_DTYPE(dtype, CALL);
+#undef CALL
+    return MMAE_OK;
+}
+
+size_t distill_slices_workspace(const MapSlices& s, int outer, int inner, int k) {
+    return s.count == 1 ? 0 : (size_t)outer * inner * (s.count * sizeof(Sums) + (2 + 2 * (size_t)k) * sizeof(float));
+}
+
+int distill_slices(int dtype, const DistillArgs& a, const MapSlices& s, void* workspace, bool again, hipStream_t stream) {
+    const int tiles = map_tiles(a.g.inner);
+    const long all = map_blocks(a.g), positions = (long)a.g.outer * a.g.inner;
+    REQUIRE_GRID("distill", all * s.count, 256);
+    Sums* sums = (Sums*)workspace;
+    const SliceNotes notes = slice_notes((char*)(sums + positions * s.count), positions, a.k);
+#define CALL(T)                                                                                                                          \
+    do {                                                                                                                                 \
+        if (!again) hipLaunchKernelGGL(distill_map_sums_kernel<T>, dim3((unsigned)(all * s.count)), dim3(256), 0, stream, a, tiles, s.count, s.width, sums); \
+        hipLaunchKernelGGL(distill_map_join_kernel<T>, dim3((unsigned)all), dim3(64), 3 * a.k * POS * 4, stream, a, tiles, s.count, (const Sums*)sums, notes); \
+        if (a.d_logits)                                                                                                                  \
+            hipLaunchKernelGGL(distill_map_gradient_kernel<T>, dim3((unsigned)(all * s.count)), dim3(256), 0, stream, a, tiles, s.count, s.width, notes); \
+    } while (0)
+    BY_DTYPE(dtype, CALL);
+#undef CALL
+    return MMAE_OK;
+}
+
+}  // namespace classdist

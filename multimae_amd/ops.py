@@ -689,7 +689,7 @@ def class_log_probs(logits: torch.Tensor, target: torch.Tensor, top_k: int = 0, 
         top_class = torch.empty_like(top_log_prob, dtype=torch.int64)
     if geo[0]:
         L = _L()
-        nbytes = L.mmae_class_log_probs_workspace_bytes(geo[0], geo[1], geo[2], top_k)
+        nbytes = L.mmae_class_log_probs_workspace_bytes(_DT[logits.dtype], geo[0], geo[1], geo[2], top_k)
         ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
         n = geo[0] * geo[2]
         at = stats.data_ptr() if want_stats else 0

@@ -51,12 +51,14 @@ def test_calls_are_refused_on_the_host(name, args, case):
 
 def test_workspaces():
     lib = _lib.load()
-    assert lib.mmae_class_log_probs_workspace_bytes(4, 100, 1, 5) == 0         # a row is one wave's
-    assert lib.mmae_class_log_probs_workspace_bytes(1, 100000, 1, 64) > lib.mmae_class_log_probs_workspace_bytes(1, 100000, 1, 0) > 0
-    assert lib.mmae_class_log_probs_workspace_bytes(4096, 100000, 1, 5) == 0   # a row is one workgroup's
-    assert lib.mmae_class_log_probs_workspace_bytes(2, 133, 64, 5) == 0        # maps
+    assert lib.mmae_class_log_probs_workspace_bytes(0, 4, 100, 1, 5) == 0         # a row is one wave's
+    assert lib.mmae_class_log_probs_workspace_bytes(0, 1, 100000, 1, 64) > lib.mmae_class_log_probs_workspace_bytes(0, 1, 100000, 1, 0) > 0
+    assert lib.mmae_class_log_probs_workspace_bytes(1, 4096, 100000, 1, 5) == 0   # a row is one workgroup's
+    assert lib.mmae_class_log_probs_workspace_bytes(0, 2, 133, 64, 5) == 0        # a map's tile fits
+    assert lib.mmae_class_log_probs_workspace_bytes(0, 2, 32000, 64, 5) >= 2 * 64 * (16 + 5 * 8)
+    assert lib.mmae_distill_workspace_bytes(0, 2, 32000, 64, 5) > lib.mmae_distill_workspace_bytes(0, 2, 133, 64, 5)
     for bad in ((0, 1, 1, 0), (1, 0, 1, 0), (1, 1, 1, -1)):
-        assert lib.mmae_class_log_probs_workspace_bytes(*bad) == 0
+        assert lib.mmae_class_log_probs_workspace_bytes(0, *bad) == 0
     assert lib.mmae_distill_workspace_bytes(0, 0, 1, 1, 1) == 0
     for rows in (1, 1000):
         for classes in (10, 5000, 300000):

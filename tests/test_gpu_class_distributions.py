@@ -132,7 +132,7 @@ def check_log_probs(M, z, target, k, temperature, backward=True):
 ROWS = [(1, 1), (1, 2), (3, 5), (64, 63), (65, 64), (130, 133), (7, 511), (5, 512), (6, 513), (4, 1000), (3, 2049), (2, 8191), (2, 8192),
         (3, 8200), (1, 16387), (2, 50001), (1, 131072), (3, 150016), (1, 262147)]
 MAPS = [(2, 133, 56, 56), (1, 5, 4, 4), (3, 7, 1, 1), (2, 150, 5, 7), (1, 1000, 3, 5), (2, 40, 11), (1, 2, 1, 130), (1, 6007, 2, 3), (4, 257, 9),
-        (1, 1, 8, 8), (2, 700, 1, 65)]
+        (1, 1, 8, 8), (2, 700, 1, 65), (2, 640, 6, 7), (1, 641, 70), (1, 321, 70), (1, 32000, 66), (1, 5001, 1, 3)]
 
 
 @pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
@@ -144,7 +144,7 @@ def test_log_probs_of_rows_and_maps(M, shape, dtype):
         check_log_probs(M, z, target, k, temperature, backward=k != 0)
 
 
-@pytest.mark.parametrize("shape", [(6, 70), (6, 700), (6, 9000), (6, 40007), (6, 70, 3, 5)], ids=str)
+@pytest.mark.parametrize("shape", [(6, 70), (6, 700), (6, 9000), (6, 40007), (6, 70, 3, 5), (6, 1700, 3, 5)], ids=str)
 @pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
 def test_log_probs_of_masked_rows(M, shape, dtype):
     """-inf and the type's lowest value in masked places, rows with one class or none left, NaN and +inf."""
@@ -171,7 +171,7 @@ def test_log_probs_of_masked_rows(M, shape, dtype):
     assert not out.entropy[1:5].isnan().any()
 
 
-@pytest.mark.parametrize("shape", [(3, 70), (3, 700), (3, 9000), (2, 40007), (3, 140, 3, 5)], ids=str)
+@pytest.mark.parametrize("shape", [(3, 70), (3, 700), (3, 9000), (2, 40007), (3, 140, 3, 5), (3, 1400, 3, 5)], ids=str)
 @pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
 def test_equal_logits_rank_by_the_lower_class(M, shape, dtype):
     few = classes(shape, 4, seed=8).to(DTYPES[dtype]) - 1.0        # four levels, one of them zero
@@ -221,6 +221,9 @@ def test_log_probs_of_strided_logits(M, dtype):
     check_log_probs(M, wide.t()[:77].t(), classes((9,), 77, 3), 5, 1.0)     # (the same rows, cut)
     check_log_probs(M, wide.t(), classes((1300,), 9, 3), 5, 1.0)            # classes far apart: copied
     check_log_probs(M, wide[:1].expand(4, 1300), classes((4,), 1300, 3), 5, 1.0)
+    large = scores((4, 1001, 3, 5), dtype, seed=4)
+    check_log_probs(M, large[::2], classes((2, 3, 5), 1001, 5), 5, 1.0)
+    check_log_probs(M, large[:, 3:], classes((4, 3, 5), 998, 5), 5, 1.0)
     maps = scores((4, 20, 6, 9), dtype, seed=4)
     t = classes((4, 6, 9), 20, 5)
     check_log_probs(M, maps.contiguous(memory_format=torch.channels_last), t, 5, 1.0)
@@ -380,7 +383,7 @@ def test_distillation_of_rows_and_maps(M, shape, log_probs, dtype):
 
 @pytest.mark.parametrize("log_probs", [False, True], ids=["logits", "log_probs"])
 @pytest.mark.parametrize("shape,patch", [((5, 133, 56, 56), 4), ((4, 12, 8, 4), 4), ((3, 150, 6, 10), 2), ((4, 9, 5, 3), 1), ((130, 40), 1),
-                                         ((33, 3000), 1), ((9, 20000), 1), ((6, 21, 50), 1)], ids=str)
+                                         ((33, 3000), 1), ((9, 20000), 1), ((6, 21, 50), 1), ((4, 1500, 6, 10), 2), ((4, 900, 130), 1)], ids=str)
 @pytest.mark.parametrize("dtype", ["f32", "bf16"])
 def test_distillation_with_a_mask(M, shape, patch, log_probs, dtype):
     z = scores(shape, dtype, seed=2)
@@ -400,7 +403,7 @@ def test_distillation_with_a_mask(M, shape, patch, log_probs, dtype):
 
 
 @pytest.mark.parametrize("log_probs", [False, True], ids=["logits", "log_probs"])
-@pytest.mark.parametrize("shape", [(7, 70), (7, 3000), (7, 40007), (7, 70, 2, 3)], ids=str)
+@pytest.mark.parametrize("shape", [(7, 70), (7, 3000), (7, 40007), (7, 70, 2, 3), (7, 1300, 2, 3)], ids=str)
 @pytest.mark.parametrize("dtype", ["f32", "bf16"])
 def test_distillation_padding_duplicates_and_masked_classes(M, shape, log_probs, dtype):
     c = shape[1]
@@ -631,7 +634,7 @@ def test_scaling_needs_a_gradient_to_scale(M):
 # ------------------------------------------------------------------------------------------------ as they are used
 def test_class_distribution_calls_are_bitwise_reproducible_and_stay_in_their_buffers(M):
     from multimae_amd import ops
-    for shape in ((5, 133, 9, 7), (300, 133), (40, 3000), (3, 100003)):
+    for shape in ((5, 133, 9, 7), (300, 133), (40, 3000), (3, 100003), (3, 2000, 9, 9)):
         z = scores(shape, "bf16", seed=1)
         target = classes(shape[:1] + shape[2:], shape[1], 2)
         cls, val = teacher_top(shape, 8, 3, True, 1.0)
@@ -665,7 +668,7 @@ def test_class_distributions_on_another_stream_and_two_at_once(M):
         assert all(torch.equal(a, b) for a, b in zip(out, want[0])) and torch.equal(loss, want[1])
 
 
-@pytest.mark.parametrize("shape", [(40, 133), (24, 9000), (2, 140000), (3, 133, 8, 12)], ids=str)
+@pytest.mark.parametrize("shape", [(40, 133), (24, 9000), (2, 140000), (3, 133, 8, 12), (2, 1111, 8, 12)], ids=str)
 def test_class_distributions_in_captured_graphs(M, shape):
     """A teacher's alternatives, the student's loss and its gradient captured as one graph, two such graphs, replayed in turn
     with new logits and eager calls in between."""
