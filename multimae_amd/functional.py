@@ -951,20 +951,25 @@ class DistillFn(torch.autograd.Function):
         call = ops.Distillation(logits, top_class, top_value, mask, patch, temperature, log_probs)
         if not ctx.needs_input_grad[0]:
             return call.run()
-        ctx.save_for_backward(logits, top_class, top_value, mask)
-        ctx.call, ctx.d_logits = call, torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
-        return call.run(ctx.d_logits)
+        d_logits = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
+        loss = call.run(d_logits)
+        # what the call reads again lives as long as the graph keeps its tensors, however long the loss is kept
+        ctx.save_for_backward(logits, top_class, top_value, mask, call.workspace)
+        call.tensors = call.workspace = None
+        ctx.call, ctx.d_logits = call, d_logits
+        return loss
 
     @staticmethod
     @_once
     def backward(ctx, g):
         d_logits, ctx.d_logits = ctx.d_logits, None
         if d_logits is None or not getattr(ctx, "unit_upstream", False):
-            logits = ctx.saved_tensors[0]  # (refused if an input was changed since)
-            if d_logits is None:
-                d_logits = ctx.call.scale(torch.empty(logits.shape, dtype=logits.dtype, device=logits.device), g)
-            else:
-                ctx.call.scale(d_logits, g, skip_unit=True)
+            call, first = ctx.call, d_logits is not None
+            call.workspace = ctx.saved_tensors[4]  # (refused if an input was changed since, or the graph is freed)
+            if not first:
+                d_logits = torch.empty(call.shape, dtype=call.dtype, device=call.device)
+            call.scale(d_logits, g, skip_unit=first)
+            call.workspace = None
         return d_logits, None, None, None, None, None, None
 
 

@@ -757,7 +757,8 @@ class Distillation:
             if mask.dtype != torch.int64:
                 raise _lib.MmaeError(f"distill mask: expected dtype torch.int64, got {mask.dtype}")
             _beside(mask, logits, (B, geo[2] // (patch * patch)), "distill mask")
-        self.logits = logits
+        self.shape, self.dtype, self.device, self.bytes = shape, logits.dtype, logits.device, logits.nbytes
+        self.tensors = (logits, top_class, top_value, mask)  # (what args point to)
         nbytes = _L().mmae_distill_workspace_bytes(_DT[logits.dtype], *geo[:3], k)
         self.workspace = torch.empty(nbytes, dtype=torch.uint8, device=logits.device)
         self.args = (*_class_call(logits, geo), top_class.data_ptr(), top_class.element_size(), top_value.data_ptr(), _DT[top_value.dtype],
@@ -766,26 +767,27 @@ class Distillation:
         self.beside_bytes = geo[0] * geo[2] * k * (top_class.element_size() + top_value.element_size())
 
     def _launch(self, upstream, again, skip_unit, loss, d_logits):
-        bytes_ = self.logits.numel() * self.logits.element_size() * (1 if d_logits is None else 2) + self.beside_bytes
-        _launch("distill", _L().mmae_distill, self.logits.device, bytes_, *self.args, _addr(upstream), again, skip_unit, _addr(loss),
+        bytes_ = self.bytes * (1 if d_logits is None else 2) + self.beside_bytes
+        _launch("distill", _L().mmae_distill, self.device, bytes_, *self.args, _addr(upstream), again, skip_unit, _addr(loss),
                 _addr(d_logits), self.workspace.data_ptr(), self.workspace.numel())
 
-    def _gradient(self, d_logits):
-        _beside(d_logits, self.logits, self.logits.shape, "distill d_logits")
-        return _req(d_logits, self.logits.dtype, "distill d_logits")
+    def _check(self, t, dtype, shape, name):
+        if _req(t, dtype, f"distill {name}").device != self.device or t.shape != shape:
+            raise _lib.MmaeError(f"distill {name}: expected shape {tuple(shape)} on {self.device}, got {tuple(t.shape)} on {t.device}")
+        return t
 
     def run(self, d_logits: Optional[torch.Tensor] = None) -> torch.Tensor:
         self.scalable = d_logits is not None
-        loss = torch.empty((), dtype=F32, device=self.logits.device)
-        self._launch(None, 0, 0, loss, None if d_logits is None else self._gradient(d_logits))
+        loss = torch.empty((), dtype=F32, device=self.device)
+        self._launch(None, 0, 0, loss, None if d_logits is None else self._check(d_logits, self.dtype, self.shape, "d_logits"))
         return loss
 
     def scale(self, d_logits: torch.Tensor, upstream: torch.Tensor, skip_unit: bool = False) -> torch.Tensor:
         """skip_unit: d_logits holds run()'s gradient and is left alone where the scalar is 1."""
         if not self.scalable:
             raise _lib.MmaeError("distill: scale() needs a run() that made the gradient")
-        _beside(_req(upstream, F32, "distill upstream"), self.logits, (), "distill upstream")
-        self._launch(upstream, 1, int(skip_unit), None, self._gradient(d_logits))
+        self._check(upstream, F32, (), "upstream")
+        self._launch(upstream, 1, int(skip_unit), None, self._check(d_logits, self.dtype, self.shape, "d_logits"))
         return d_logits
 
 

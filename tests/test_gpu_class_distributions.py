@@ -720,6 +720,41 @@ def test_outputs_can_be_changed_in_place_and_one_of_them_used(M):
         assert not M.MaskedDistillationLoss()(z, (target.view(5, 1), torch.zeros(5, 1, device="cuda"))).requires_grad
 
 
+def test_what_a_call_points_to_lives_as_long_as_it_is_needed(M):
+    """ops.Distillation keeps its arguments; a loss that is kept after the backward pass keeps none of them."""
+    import gc
+    from multimae_amd import ops
+    z = scores((300, 40000), "bf16", 1)
+    cls, val = teacher_top((300, 40000), 8, 2, True, 1.0)
+    d = torch.empty_like(z)
+    want = ops.distill(z, cls, val, log_probs=True, d_logits=d)
+    call = ops.Distillation(z.clone(), cls.clone(), val.clone(), log_probs=True)
+    trash = [torch.full_like(t, 1) for t in (z, cls, val)]
+    got = torch.empty_like(z)
+    assert torch.equal(call.run(got), want) and torch.equal(got, d)
+    trash += [torch.full_like(t, 1) for t in (z, cls, val)]
+    assert torch.equal(call.scale(got, torch.ones((), device="cuda")), d)
+    del call, trash, got
+    gc.collect()
+    fn = M.MaskedDistillationLoss(teacher="log_probs")
+    leaf = z.clone().requires_grad_(True)  # (the graph keeps its leaf, and the leaf its gradient: not what is counted)
+    before = torch.cuda.memory_allocated()
+    loss = fn(leaf * 1.0, (cls.clone(), val.clone()))
+    loss.backward()
+    with pytest.raises(RuntimeError):  # the graph is freed
+        loss.backward()
+    leaf.grad = None
+    gc.collect()
+    assert torch.cuda.memory_allocated() - before < 4096  # the loss itself
+    # changed since: refused, as for any tensor that autograd saved
+    leaf = z.clone().requires_grad_(True)
+    x = leaf * 1.0
+    loss = fn(x, (cls, val))
+    x.mul_(2.0)
+    with pytest.raises(RuntimeError):
+        loss.backward()
+
+
 def test_gradients_of_gradients_are_refused_and_other_gradient_types_taken(M):
     z = scores((6, 500), "bf16", 1).requires_grad_(True)
     target = classes((6,), 500, 2)
