@@ -241,9 +241,16 @@ __global__ __launch_bounds__(64 * most_waves(K)) void log_probs_map_kernel(LogPr
                 }
             queued = 0;
         };
-        for (int j = c0; j < c1; ++j) {
-            if (lane < n && T::up(tile[j * POS + lane]) >= least) queue[queued++ * POS] = j;
-            if (__any(queued == QUEUE)) drain();
+        for (int j = c0; j < c1; j += 8) {
+            float x[8];
+#pragma unroll
+            for (int u = 0; u < 8; ++u) x[u] = T::up(tile[(j + u < c1 ? j + u : c1 - 1) * POS + lane]);
+            if (__any(queued > QUEUE - 8)) drain();
+#pragma unroll
+            for (int u = 0; u < 8; ++u) {  // (written in any case: most classes are wanted by some lane)
+                queue[queued * POS] = j + u;
+                queued += lane < n && j + u < c1 && x[u] >= least;
+            }
         }
         drain();
         __syncthreads();
