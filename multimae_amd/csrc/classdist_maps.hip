@@ -60,8 +60,8 @@ __device__ __forceinline__ void load_map_tile(typename T::E* tile, const typenam
 // The 16-bit types leave the low bits of an fp32 number free: there a value carries its class along, so that the sorted list is
 // the answer and the second pass falls away.
 //
-// 167 x 255 x 56 x 56: fp32 114 us (4.7 TB/s), bf16 73 us; with 8 alternatives 516 and 189 us, the list's three instructions a slot
-// and logit.
+// 256 x 150 x 56 x 56: fp32 115 us (4.2 TB/s), with 8 alternatives 284 us; 167 x 255 x 56 x 56 bf16 73 and 188 us: the lists'
+// arithmetic and, fp32, the second pass.
 constexpr int QUEUE = 16;
 constexpr int CODE_BITS = 12;                   // of a carried class: the mantissa bits that bf16 (16) and f16 (13) leave
 constexpr uint32_t CODES = (1u << CODE_BITS) - 1, CARRIED_INF = 0x7f800000u - (1u << CODE_BITS);  // above the largest finite value of both
@@ -96,7 +96,7 @@ __host__ __device__ inline int list_slots(int k) { return k == 0 ? 0 : k <= 4 ? 
 // Bytes behind the tile: the waves' sums; their lists, later their queues; the slots.
 inline int log_probs_map_bytes(int element, int classes, int k, int waves) {
     const bool second = k && element == 4;  // queues and slots
-    const int lists = waves * POS * list_slots(k) * 4, queues = second ? waves * POS * QUEUE * 4 : 0;
+    const int lists = waves * POS * list_slots(k) * 4, queues = second ? waves * POS * QUEUE * 2 : 0;
     return (classes * POS * element + 15) / 16 * 16 + waves * POS * (int)sizeof(Sums) + (lists > queues ? lists : queues) + (second ? k * POS * 4 : 0);
 }
 
@@ -108,8 +108,8 @@ __global__ __launch_bounds__(64 * most_waves(K)) void log_probs_map_kernel(LogPr
     typename T::E* tile = (typename T::E*)smem;
     Sums* s_sums = (Sums*)(smem + (C * POS * sizeof(typename T::E) + 15) / 16 * 16);
     float* s_list = (float*)(s_sums + waves * POS);
-    uint32_t* s_queue = (uint32_t*)s_list;
-    constexpr int REGION = K * 4 > QUEUE * 4 ? K * 4 : QUEUE * 4;
+    uint16_t* s_queue = (uint16_t*)s_list;
+    constexpr int REGION = K * 4 > QUEUE * 2 ? K * 4 : QUEUE * 2;
     uint32_t* s_slot = (uint32_t*)((char*)s_list + (K ? waves * POS * REGION : 0));
     const int b = blockIdx.x / tiles / sl.count, i0 = blockIdx.x % tiles * POS, n = inner - i0 < POS ? inner - i0 : POS;
     const typename T::E* z = (const typename T::E*)a.g.logits + b * a.g.ld + (long)first * inner + i0;
@@ -220,7 +220,7 @@ __global__ __launch_bounds__(64 * most_waves(K)) void log_probs_map_kernel(LogPr
 #pragma unroll
         for (int i = 1; i < K; ++i) least = i == k - 1 ? best[i] : least;
         __syncthreads();  // the lists are read: their room is the queues' now
-        uint32_t* queue = s_queue + wave * QUEUE * POS + lane;
+        uint16_t* queue = s_queue + wave * QUEUE * POS + lane;
         int queued = 0;
         auto drain = [&]() {
             for (int i = 0; __any(i < queued); ++i)

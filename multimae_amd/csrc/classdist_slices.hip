@@ -2,7 +2,7 @@
 // (and best classes) are joined per position.  Read once for the log probabilities, twice for distillation with its gradient.
 //
 // A wave's load is one class of 64 neighbouring positions.  131 x 1000 x 32 x 32 fp32 (537 MB): log probabilities 119 us (4.5 TB/s),
-// with 8 alternatives 560 us, where the lists' arithmetic bounds them, distillation with its gradient 440 us (three passes, 3.7 TB/s);
+// with 8 alternatives 314 us, where the lists bound them, distillation with its gradient 440 us (three passes, 3.7 TB/s);
 // a workgroup per position, which reads a line for each of its logits, takes 1270, 9121 and 4030 us.  Maps of few positions a
 // sample (2 x 2) leave most lanes idle.
 #include "classdist.h"
@@ -96,8 +96,8 @@ __global__ __launch_bounds__(64) void log_probs_map_join_kernel(LogProbArgs a, i
 
 // The same with a wave per position, a lane per slice: k times the largest of the lanes' heads, whose lane takes its next key.  The
 // last lane holds the best of the slices before, 63 at a time.  Each key costs six exchanges instead of insertions that wait for
-// each other: 16 x 32000 x 16 x 16 bf16, 63 slices, with 8 alternatives 236 us instead of 338, with 64 739 instead of 2351.  4 slices
-// fill 4 lanes only: 131 x 1000 x 32 x 32 fp32 with 8 742 us instead of 569; from 8 to 16 slices both take the same.
+// each other: 16 x 32000 x 16 x 16 bf16, 63 slices, with 8 alternatives 236 us instead of 338, with 64 739 instead of 2351.  4
+// slices fill 4 lanes only (131 x 1000 x 32 x 32 fp32 with 8: 742 us instead of 569); from 8 to 16 both take the same.
 template <class T>
 __global__ __launch_bounds__(256) void log_probs_map_merge_kernel(LogProbArgs a, MapSlices sl) {
     const int inner = a.g.inner, k = a.k, lane = threadIdx.x & 63;
@@ -337,17 +337,22 @@ SliceNotes slice_notes(char* at, long positions, int k) {
 
 }  // namespace
 
-static MapSlices map_slices(int dtype, int classes, int whole) {
-    const int bytes = POS * (dtype == MMAE_DT_F32 ? 4 : 2), most = SLICE_BYTES / bytes;
+static MapSlices map_slices(int dtype, int classes, int whole, int slice) {
+    const int bytes = POS * (dtype == MMAE_DT_F32 ? 4 : 2), most = slice / bytes;
     const int count = (long)classes * bytes <= whole ? 1 : (classes + most - 1) / most, width = (classes + count - 1) / count;
     return {(classes + width - 1) / width, width, nullptr, nullptr};
 }
 // Whole up to a tile of 80 KiB where slices cost more than they overlap: distillation, which reads them twice (109 x 300 x 64 x 64
-// fp32: 431 us whole, 541 us sliced), and long lists of alternatives (64: 1878 and 3765 us; 8: 508 and 363 us, none: 192 and
-// 127 us).
+// fp32: 431 us whole, 541 us sliced), and long lists of alternatives (64: 1878 and 3765 us; none: 192 and 127 us).  Short lists
+// gain by more and smaller workgroups on a CU (8 alternatives, 131 x 1000 x 32 x 32: fp32 392 us with slices of 64 KiB, 314 us
+// of 48, 360 us of 32; bf16 252 us of 64, 196 us of 48, 213 us of 32, but with 16 488, 410 and 327 us).
 constexpr int WHOLE_BYTES = 80 * 1024;
-MapSlices log_probs_map_slices(int dtype, int classes, int top_k) { return map_slices(dtype, classes, top_k > 16 ? WHOLE_BYTES : SLICE_BYTES); }
-MapSlices distill_map_slices(int dtype, int classes) { return map_slices(dtype, classes, WHOLE_BYTES); }
+MapSlices log_probs_map_slices(int dtype, int classes, int top_k) {
+    if (top_k > 16) return map_slices(dtype, classes, WHOLE_BYTES, SLICE_BYTES);
+    const int most = !top_k ? SLICE_BYTES : dtype == MMAE_DT_F32 ? 48 * 1024 : 32 * 1024;
+    return map_slices(dtype, classes, most, most);
+}
+MapSlices distill_map_slices(int dtype, int classes) { return map_slices(dtype, classes, WHOLE_BYTES, SLICE_BYTES); }
 
 size_t log_probs_slices_workspace(const MapSlices& s, int outer, int inner, int top_k) {
     return s.count == 1 ? 0 : (size_t)outer * inner * s.count * (sizeof(Sums) + sizeof(uint64_t) * (size_t)top_k);
