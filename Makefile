@@ -11,7 +11,13 @@ LIB   := multimae_amd/libmmae_hip.so
 FLAGS := --offload-arch=$(ARCH) -O3 -fPIC -std=c++17 -Wall -Wno-unused-variable -Wno-unused-but-set-variable \
          -Xclang -target-feature -Xclang -packed-fp32-ops
 
-all: $(LIB)
+# The autograd nodes that are C++ link to torch: a module of the package's own beside the library, which knows no torch.
+PYTHON ?= python3
+TORCH  := $(shell $(PYTHON) -c "import importlib.util as u; print(u.find_spec('torch').submodule_search_locations[0])")
+PYINC  := $(shell $(PYTHON) -c "import sysconfig; print(sysconfig.get_paths()['include'])")
+NODES  := multimae_amd/_nodes.so
+
+all: $(LIB) $(NODES)
 
 $(OBJ)/%.o: $(CSRC)/%.hip $(CSRC)/common.h $(CSRC)/ln_rows.h $(CSRC)/classdist.h include/mmae.h Makefile
 	@mkdir -p $(OBJ)
@@ -28,6 +34,14 @@ $(OBJ)/comm.o: $(CSRC)/comm.cpp include/mmae.h Makefile
 $(LIB): $(OBJS)
 	$(HIPCC) --offload-arch=$(ARCH) -shared -fPIC -o $@ $(OBJS) -ldl
 
+$(OBJ)/classdist_nodes.o: $(CSRC)/classdist_nodes.cpp include/mmae.h Makefile
+	@mkdir -p $(OBJ)
+	g++ -O2 -fPIC -std=c++17 -fvisibility=hidden -D__HIP_PLATFORM_AMD__=1 -DUSE_ROCM=1 -DTORCH_EXTENSION_NAME=_nodes -isystem $(TORCH)/include \
+	    -isystem $(TORCH)/include/torch/csrc/api/include -isystem $(PYINC) -isystem /opt/rocm/include -c $< -o $@
+
+$(NODES): $(OBJ)/classdist_nodes.o $(LIB)
+	g++ -shared -o $@ $< -Lmultimae_amd -lmmae_hip -Wl,-rpath,'$$ORIGIN' -L$(TORCH)/lib -lc10 -lc10_hip -ltorch -ltorch_cpu -ltorch_python
+
 clean:
-	rm -rf build $(LIB)
+	rm -rf build $(LIB) $(NODES)
 .PHONY: all clean

@@ -111,4 +111,4 @@ class MaskedDistillationLoss(nn.Module):
                 mask = mask.to(torch.int64)
             mask = mask.reshape(input.shape[0], -1).contiguous()
         patch = self.scale_factor if input.dim() == 4 else 1
-        return Fn.DistillFn.apply(input, top_class, top_value, mask, patch, float(self.temperature), self.teacher == "log_probs")
+        return Fn.distill(input, top_class, top_value, mask, patch, float(self.temperature), self.teacher == "log_probs")

@@ -6,6 +6,7 @@ accumulates in fp32.  Each function saves exactly what its backward kernels read
 from typing import Dict, List, Optional, Sequence, Tuple
 
 import os
+import sys
 
 import torch
 
@@ -900,11 +901,36 @@ def _class_scores(x: torch.Tensor) -> torch.Tensor:
     return x if x.dim() < 2 or ops.class_geometry(x) is not None else x.contiguous()
 
 
+_NODES = __package__ + "._nodes"
+
+
+def _nodes():
+    """The C++ nodes (csrc/classdist_nodes.cpp), None while launches are timed, which the Python nodes' are."""
+    if ops.PROFILE is not None:
+        return None
+    ops._L()  # (names the library where it is missing)
+    from . import _nodes as module
+    return module
+
+
 def class_log_probs(logits, target, top_k, temperature):
-    """ClassLogProbsFn, without a node where no gradient is asked for."""
+    """Log probability of the given class, entropy and top classes; a node only where a gradient is asked for."""
+    nodes = _nodes()
+    out = nodes and nodes.class_log_probs(logits, target, top_k, temperature)
+    if out is not None:
+        return out
     if torch.is_grad_enabled() and logits.requires_grad:
         return ClassLogProbsFn.apply(logits, target, top_k, temperature)
     return ops.class_log_probs(_class_scores(logits), target.contiguous(), top_k, temperature, want_stats=False)[:4]
+
+
+def distill(logits, top_class, top_value, mask, patch, temperature, log_probs):
+    """The distillation loss; its gradient comes with it."""
+    nodes = _nodes()
+    loss = nodes and nodes.distill(logits, top_class, top_value, mask, patch, temperature, log_probs)
+    if loss is None:  # (the teacher has no gradient)
+        loss = DistillFn.apply(logits, top_class, top_value.detach(), mask, patch, temperature, log_probs)
+    return loss
 
 
 def _once(backward):
@@ -982,6 +1008,8 @@ def mark_unit_upstream(losses) -> None:
         node = getattr(t, "grad_fn", None)
         if isinstance(node, (MaskedLossFn._backward_cls, MaskedCEFn._backward_cls, DistillFn._backward_cls)):
             node.unit_upstream = True
+        elif node is not None and _NODES in sys.modules:  # (a C++ node only where its module is loaded)
+            sys.modules[_NODES].mark_unit_upstream(t)
 
 
 class MaskedLossFn(torch.autograd.Function):

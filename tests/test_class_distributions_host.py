@@ -65,6 +65,15 @@ def test_workspaces():
             assert lib.mmae_distill_workspace_bytes(1, rows, classes, 1, 8) >= 4 * (4 + 2 * rows)
 
 
+def test_the_nodes_leave_what_they_do_not_take():
+    """Anything but contiguous tensors on the GPU is answered with None, before anything is launched."""
+    from multimae_amd import _nodes
+    z, t, v = torch.randn(4, 9), torch.zeros(4, dtype=torch.long), torch.zeros(4, 1)
+    assert _nodes.class_log_probs(z, t, 2, 1.0) is None
+    assert _nodes.distill(z, t.view(4, 1), v, None, 1, 1.0, False) is None
+    assert not _nodes.mark_unit_upstream(z) and not _nodes.mark_unit_upstream(z.requires_grad_(True).sum())
+
+
 def test_the_entry_points_take_tensors_on_the_gpu_only():
     import multimae_amd as M
     z, t = torch.randn(4, 9), torch.zeros(4, dtype=torch.long)

@@ -720,6 +720,48 @@ def test_outputs_can_be_changed_in_place_and_one_of_them_used(M):
         assert not M.MaskedDistillationLoss()(z, (target.view(5, 1), torch.zeros(5, 1, device="cuda"))).requires_grad
 
 
+@pytest.mark.parametrize("shape", [(40, 133), (24, 9000), (700, 40007), (3, 133, 8, 12), (2, 1111, 8, 12), (5, 21, 50)], ids=str)
+def test_timed_calls_go_through_the_python_nodes_with_the_same_results(M, shape, monkeypatch):
+    from multimae_amd import functional, ops
+    target = classes(shape[:1] + shape[2:], shape[1], 3)
+    cls, val = teacher_top(shape, 8, 2, True, 1.5)
+    mask = torch.ones(shape[0], math.prod(shape[2:]), dtype=torch.long, device="cuda")
+    mask[1] = 0
+    fn = loss_module(M, 1, 1.5, True)
+    rows = []
+    for profile in (None, []):
+        monkeypatch.setattr(ops, "PROFILE", profile)
+        z = scores(shape, "bf16", 1).requires_grad_(True)
+        out = M.class_log_probs(z, target, top_k=5, temperature=1.5)
+        (g,) = torch.autograd.grad(out[:2], z, [torch.ones_like(out.entropy), out.entropy.detach()], retain_graph=True)
+        loss = fn(z, (cls, val), mask=mask)
+        mine = []
+        for up in (1.0, 1.0, 0.3):
+            mine += torch.autograd.grad(loss, z, torch.tensor(up, device="cuda"), retain_graph=True)
+        assert mine[0].data_ptr() != mine[1].data_ptr()
+        marked = fn(z, (cls, val), mask=mask)
+        functional.mark_unit_upstream([marked])
+        (unit,) = torch.autograd.grad(marked, z, torch.tensor(5.0, device="cuda"))  # (taken at its word)
+        with torch.no_grad():
+            plain = (*M.class_log_probs(z, target, top_k=3), fn(z, (cls, val), mask=mask))
+        rows.append([*out, g, loss, *mine, unit, *plain])
+        assert (type(loss.grad_fn).__name__ == "DistillFnBackward") == (profile is not None)
+    assert all(torch.equal(a, b) for a, b in zip(*rows)) and torch.equal(rows[0][9], rows[0][6])  # (unit, the first of mine)
+
+
+def test_the_teacher_has_no_gradient(M, monkeypatch):
+    from multimae_amd import ops
+    z = scores((6, 500), "f32", 1)
+    cls, val = teacher_top((6, 500), 4, 2, False, 1.0)
+    fn = M.MaskedDistillationLoss()
+    for profile in (None, []):
+        monkeypatch.setattr(ops, "PROFILE", profile)
+        leaf, teacher = z.clone().requires_grad_(True), val.clone().requires_grad_(True)
+        assert not fn(z, (cls, teacher)).requires_grad
+        fn(leaf, (cls, teacher)).backward()
+        assert leaf.grad is not None and teacher.grad is None
+
+
 def test_what_a_call_points_to_lives_as_long_as_it_is_needed(M):
     """ops.Distillation keeps its arguments; a loss that is kept after the backward pass keeps none of them."""
     import gc
