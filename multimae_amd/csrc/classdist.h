@@ -108,6 +108,24 @@ __device__ __forceinline__ float key_value(uint64_t key) {
 }
 __device__ __forceinline__ uint32_t key_class(uint64_t key) { return 0xffffffffu - (uint32_t)key; }
 
+// The largest key of a wave, in every lane: along the rows of 16 lanes and from row to row without the LDS's exchanges.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ uint64_t max_with(uint64_t v) {  // lanes without a partner keep their own
+    const uint32_t lo = (uint32_t)v, hi = (uint32_t)(v >> 32);
+    const uint64_t w = (uint64_t)(uint32_t)__builtin_amdgcn_update_dpp((int)hi, (int)hi, CTRL, ROWS, 0xf, false) << 32 |
+                       (uint32_t)__builtin_amdgcn_update_dpp((int)lo, (int)lo, CTRL, ROWS, 0xf, false);
+    return w > v ? w : v;
+}
+__device__ __forceinline__ uint64_t wave_max_key(uint64_t v) {
+    v = max_with<0x111, 0xf>(v);  // from 1, 2, 4 and 8 lanes below in the row
+    v = max_with<0x112, 0xf>(v);
+    v = max_with<0x114, 0xf>(v);
+    v = max_with<0x118, 0xf>(v);
+    v = max_with<0x142, 0xa>(v);  // the last lane of rows 0 and 2 to the rows above them
+    v = max_with<0x143, 0xc>(v);  // lane 31 to the upper half
+    return (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(v >> 32), 63) << 32 | (uint32_t)__builtin_amdgcn_readlane((int)v, 63);
+}
+
 __device__ __forceinline__ float load_any(const void* p, int dtype, long i) {
     if (dtype == MMAE_DT_F32) return ((const float*)p)[i];
     if (dtype == MMAE_DT_BF16) return (float)((const bf16*)p)[i];

@@ -424,32 +424,40 @@ __global__ __launch_bounds__(NT) void log_probs_rows_kernel(LogProbArgs a, int s
     if (TOP && (int)threadIdx.x < a.k) ((uint64_t*)(out + sizeof(Sums)))[threadIdx.x] = (int)threadIdx.x < list.count ? list.keys[threadIdx.x] : 0;
 }
 
-// Joins the slices of a row: one wave per row, lane i walks slice i's sorted keys.  Latency: k steps of six exchanges (32 slices of
-// 20 alternatives 12 us, beside 10 us for the slices of 24 x 131072).
-constexpr int MAX_SLICES = 64;
+// Joins the slices of a row: four waves fetch the keys, then one goes on: lane i walks slice i's sorted keys.  Latency: the fetch, and
+// k largest of the lanes' heads (24 x 131072 bf16, 32 slices of 20 alternatives: 19 us with the slices; fetched by one wave, and the
+// largest found by exchanges through the LDS, 24 us).
+constexpr int MAX_SLICES = 64, JOIN_NT = 256;
 template <class T>
-__global__ __launch_bounds__(64) void log_probs_join_kernel(LogProbArgs a, int slices, const char* parts) {
+__global__ __launch_bounds__(JOIN_NT) void log_probs_join_kernel(LogProbArgs a, int slices, const char* parts) {
     extern __shared__ uint64_t s_keys[];  // [slices][k], then the k best
     __shared__ Sums red[1];
     const long p = blockIdx.x;
-    const int lane = threadIdx.x, k = a.k;
+    const int lane = threadIdx.x & 63, k = a.k;
     const char* part = parts + (size_t)p * slices * slice_bytes(k);
     const typename T::E* z = (const typename T::E*)a.g.logits + p * a.g.ld;
     const float named = named_logit<T>(a, p, z);
     Sums v = {-INFINITY, -FAR, 0.f, 0.f};
     if (lane < slices) v = *(const Sums*)(part + lane * slice_bytes(k));
-    for (int i = lane; i < slices * k; i += 64) s_keys[i] = ((const uint64_t*)(part + (i / k) * slice_bytes(k) + sizeof(Sums)))[i % k];
-    v = wave_sums(v);
+    constexpr int U = 4;  // (64 slices of 16 alternatives on their way at once)
+    for (int i0 = threadIdx.x; i0 < slices * k; i0 += U * JOIN_NT) {
+        uint64_t key[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int i = i0 + u * JOIN_NT < slices * k ? i0 + u * JOIN_NT : slices * k - 1;
+            key[u] = ((const uint64_t*)(part + (i / k) * slice_bytes(k) + sizeof(Sums)))[i % k];
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+            if (i0 + u * JOIN_NT < slices * k) s_keys[i0 + u * JOIN_NT] = key[u];
+    }
     __syncthreads();
+    if (threadIdx.x >= 64) return;
+    v = wave_sums(v);
     int at = 0;
     uint64_t head = lane < slices && k ? s_keys[lane * k] : 0;
     for (int i = 0; i < k; ++i) {
-        uint64_t top = head;
-#pragma unroll
-        for (int o = 32; o > 0; o >>= 1) {
-            const uint64_t w = __shfl_xor((unsigned long long)top, o, 64);
-            top = w > top ? w : top;
-        }
+        const uint64_t top = wave_max_key(head);
         if (head == top && top) {  // keys are unique: one lane
             ++at;
             head = at < k ? s_keys[lane * k + at] : 0;
@@ -1009,7 +1017,7 @@ static void launch_log_probs_rows(const LogProbArgs& a, void* workspace, hipStre
     if (a.k) ROWS(LP_NT, true); else ROWS(LP_NT, false);
 #undef ROWS
     if (d.slices > 1)
-        hipLaunchKernelGGL(log_probs_join_kernel<T>, dim3(rows), dim3(64), sizeof(uint64_t) * (size_t)(d.slices + 1) * a.k, stream, a, d.slices, (const char*)workspace);
+        hipLaunchKernelGGL(log_probs_join_kernel<T>, dim3(rows), dim3(JOIN_NT), sizeof(uint64_t) * (size_t)(d.slices + 1) * a.k, stream, a, d.slices, (const char*)workspace);
 }
 
 // Three ways.  Many rows are walked, each workgroup holding one and the next one on its way.  Fewer rows, if short, are held by

@@ -144,12 +144,7 @@ __global__ __launch_bounds__(256) void log_probs_map_merge_kernel(LogProbArgs a,
         if (lane == 63) head = first;
         int at = 0;  // of the lane's head
         for (int i = 0; i < k; ++i) {
-            uint64_t top = head;
-#pragma unroll
-            for (int o = 32; o > 0; o >>= 1) {
-                const uint64_t w = __shfl_xor((unsigned long long)top, o, 64);
-                top = w > top ? w : top;
-            }
+            const uint64_t top = wave_max_key(head);
             if (lane == i) fresh = top;
             if (!top) break;
             const bool mine = head == top;  // keys are unique: one lane
