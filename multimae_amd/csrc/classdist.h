@@ -172,10 +172,13 @@ __device__ Stats block_stats(Stats v, float c, Stats* red) {
 }
 
 // Sums in the base-2 domain against a reference exponent R: s = sum 2^(z c - R), t = sum (z c - R) 2^(z c - R), m = max z.
-// z c - R is one fused multiply-add without intermediate overflow; R = m c, held to +-FAR, is the same rounded number wherever
-// it is used, so its rounding cancels.  Beyond FAR (every class left at the type's lowest value, say) the row's sums are
-// formed anew from (z - m) c.
-constexpr float FAR = 1e38f;
+// z c - R is one fused multiply-add without intermediate overflow.  R = m c, held to +-FAR, is a rounded number, and the multiply-add
+// sees what the rounding lost as a whole: up to FAR = 2^24 that is at most 1/2, a factor between 2^-1/2 and 2^1/2 that s, t and every
+// term have in common, and R is the same number wherever it is used, so it cancels.  (At 2^33 it would be up to 2^8: s of 0 or
+// infinity.)  Sums of values that all lie below -FAR, classes that are switched off, are 0 beside any other; a row whose maximum lies
+// beyond FAR (every class left is one of those) has its sums formed anew from (z - m) c, and so has the mass of the classes that a
+// teacher does not keep where their maximum does.
+constexpr float FAR = 16777216.f;
 struct Sums { float m, R, s, t; };
 __device__ __forceinline__ float reference_exponent(float m, float c) { return __builtin_amdgcn_fmed3f(m * c, -FAR, FAR); }
 __device__ __forceinline__ Sums join(const Sums& a, const Sums& b) {

@@ -438,7 +438,7 @@ __global__ __launch_bounds__(1024) void distill_map_kernel(DistillArgs a, int ti
         const float l2 = empty ? INFINITY : log2_(v.s);
         const float r = REST && rest.s != 0.f ? left : 0.f, Q = total + r;
         const float gs = empty ? 0.f : w * a.g.inv_t * (a.upstream ? a.upstream[0] : 1.f);
-        const bool far = w != 0.f && is_far(v.m, c);
+        const bool far = w != 0.f && (is_far(v.m, c) || (REST && is_far(rest.m, c)));
         const uint64_t fars = __ballot(far);
         for (int i = 0; i < k; ++i) {
             const int cls = s_cls[i * POS + lane];
@@ -786,25 +786,26 @@ __global__ __launch_bounds__(64, 2) void distill_map_regs_kernel(DistillArgs a, 
             const float one[1] = {s_z[i * POS]};
             add_logits<1, false>(v, one, c);
         }
-    // A wave with a position beyond FAR goes by (z - m) c, class after class from memory.
-    const bool far = __any(is_far(v.m, c));
-    const float m = finite_ref(v.m);
+    // A wave with a position beyond FAR goes by (z - m) c, class after class from memory, and with a rest by its own maximum.
+    const bool far = __any(is_far(v.m, c) || (REST && is_far(rest.m, c)));
+    const float m = finite_ref(v.m), rest_m = finite_ref(rest.m);
     if (far) {
         rest.s = v.s = 0.f;
         for (int j = 0; j < C; ++j) {
-            const float e = exp2_((T::up(z[(long)j * inner + px]) - m) * c);
+            const float one = T::up(z[(long)j * inner + px]);
+            v.s += exp2_((one - m) * c);
+            if (!REST) continue;
             bool out = true;
             for (int i = 0; i < k; ++i)
                 if (s_cls[i * POS] >= 0 && (s_cls[i * POS] & 0xffff) == j) out = false;
-            v.s += e;
-            if (!REST || out) rest.s += e;
+            if (out) rest.s += exp2_((one - rest_m) * c);
         }
     }
     if (v.m == INFINITY) v.s = __builtin_nanf("");
     const bool empty = v.m == -INFINITY && v.s == 0.f;
     const float own_l2 = empty ? INFINITY : log2_(v.s);  // relative to what the sums are relative to, and to R
     const float l2 = far && !is_far(v.m, c) ? own_l2 + __builtin_fmaf(m, c, -v.R) : own_l2;
-    const float r = REST && rest.s != 0.f ? left : 0.f, Q = total + r, rest_R = far ? v.R : rest.R;
+    const float r = REST && rest.s != 0.f ? left : 0.f, Q = total + r;
     const float gs = empty ? 0.f : w * a.g.inv_t * (a.upstream ? a.upstream[0] : 1.f);
 #pragma unroll 1
     for (int i = 0; i < places; ++i) {
@@ -813,20 +814,22 @@ __global__ __launch_bounds__(64, 2) void distill_map_regs_kernel(DistillArgs a, 
         const float d = far ? (zk - m) * c : __builtin_fmaf(zk, c, -v.R);
         s_d[i * POS] = w != 0.f ? gs * (exp2_(d - own_l2) * Q - q) : 0.f;
     }
-    if (r != 0.f) loss += r * (log2_(r) - ((rest_R - v.R) + log2_(rest.s) - own_l2)) * LN2;
+    const float rest_l2 = log2_(rest.s);
+    if (r != 0.f) loss += far ? r * ((log2_(r) - (rest_l2 - own_l2)) * LN2 - (rest_m - m) * a.g.inv_t) : r * (log2_(r) - ((rest.R - v.R) + rest_l2 - own_l2)) * LN2;
     loss = wave_sum(w != 0.f ? w * loss : 0.f);
     if (lane == 0 && a.part) a.part[blockIdx.x] = loss;
     if (!write) return;
-    const float F = w != 0.f ? gs * (Q * exp2_(rest_R - v.R - own_l2) - (r != 0.f ? r / rest.s : 0.f)) : 0.f;
     if (far) {
         for (int j = 0; j < C; ++j) {
-            const float e = exp2_((T::up(z[(long)j * inner + px]) - m) * c);
-            dz[(long)j * inner + px] = T::down(F != 0.f ? F * e : 0.f);
+            const float one = T::up(z[(long)j * inner + px]);
+            const float d = exp2_((one - m) * c - own_l2) * Q - (r != 0.f ? r * exp2_((one - rest_m) * c - rest_l2) : 0.f);
+            dz[(long)j * inner + px] = T::down(w != 0.f ? gs * d : 0.f);  // (outside the loss a logit may be anything)
         }
         for (int i = 0; i < k; ++i)
             if (s_cls[i * POS] >= 0) dz[(long)(s_cls[i * POS] & 0xffff) * inner + px] = T::down(s_d[(s_cls[i * POS] >> 16) * POS]);
         return;
     }
+    const float F = w != 0.f ? gs * (Q * exp2_(rest.R - v.R - own_l2) - (r != 0.f ? r / rest.s : 0.f)) : 0.f;
     Global<E>* row = (Global<E>*)dz;
     const float* at = s_d;
 #pragma unroll

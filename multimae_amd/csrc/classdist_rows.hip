@@ -541,7 +541,7 @@ __device__ __forceinline__ KeptLane kept_lane(const DistillArgs& a, int cls, flo
     return l;
 }
 
-struct RowResult { Sums all; float factor, ref; };  // factor F, R'
+struct RowResult { float factor, ref; bool far; };  // factor F, R'; beyond FAR: to be formed anew
 // One wave: the row from the sums outside the kept classes.  Writes the row's loss, returns the lane's class gradient in d.
 template <class T>
 __device__ __forceinline__ RowResult join_row(const DistillArgs& a, long p, float w, const KeptLane& l, const Sums& rest, float& d, int lane, bool write) {
@@ -565,7 +565,7 @@ __device__ __forceinline__ RowResult join_row(const DistillArgs& a, long p, floa
         if (lane == 0) a.part[p] = w * x;
     }
     d = gs * (exp2_(__builtin_fmaf(l.z, c, -v.R) - l2) * Q - l.q_class);
-    return {v, gs * (Q * exp2_(rest.R - v.R - l2) - (r != 0.f ? r / rest.s : 0.f)), rest.R};
+    return {gs * (Q * exp2_(rest.R - v.R - l2) - (r != 0.f ? r / rest.s : 0.f)), rest.R, is_far(v.m, c) || (a.log_probs && is_far(rest.m, c))};
 }
 
 template <class T, int NT>
@@ -609,7 +609,8 @@ __global__ __launch_bounds__(NT) void distill_rows_kernel(DistillArgs a) {
     __shared__ Sums red[NT / 64];
     __shared__ Stats red_far[NT / 64];
     __shared__ int s_cls[MAX_TOP];
-    __shared__ float s_d[MAX_TOP], s_row[4];
+    __shared__ float s_d[MAX_TOP], s_row[2];
+    __shared__ int s_far;
     if (a.upstream && a.skip_unit && a.upstream[0] == 1.f) return;
     const long p = blockIdx.x;
     const int C = a.g.classes, lane = threadIdx.x & 63;
@@ -656,10 +657,10 @@ __global__ __launch_bounds__(NT) void distill_rows_kernel(DistillArgs a) {
         float d;
         const RowResult row = join_row<T>(a, p, w, l, rest, d, lane, true);
         s_d[lane] = d;
-        if (lane == 0) { s_row[0] = row.factor; s_row[1] = row.ref; s_row[2] = row.all.m; }
+        if (lane == 0) { s_row[0] = row.factor; s_row[1] = row.ref; s_far = row.far; }
     }
     __syncthreads();
-    if (is_far(s_row[2], c)) {
+    if (s_far) {
         const float x = distill_position<T>(a, p, w, red_far, s_cls, s_d, s_row);
         if (threadIdx.x == 0 && a.part) a.part[p] = x;
         return;
@@ -722,7 +723,7 @@ struct LongRow {
 };
 
 // What goes from kernel to kernel with a long row: the teacher's totals, made before (in 64 bits, whose constants would take
-// registers from the pieces), and whether the row is beyond FAR.
+// registers from the pieces), and whether the row, or what the teacher does not keep of it, is beyond FAR.
 struct RowNote { float total, rest; int far, unused; };
 static_assert(sizeof(RowNote) == sizeof(Sums), "both live in the rows' workspace");
 __global__ __launch_bounds__(64) void distill_notes_kernel(DistillArgs a, RowNote* notes) {
@@ -813,7 +814,7 @@ __global__ __launch_bounds__(NT, long_waves(NT, NV)) void distill_long_rows_kern
             if (lane == 0) {
                 s_row[0] = row.factor;
                 s_row[1] = row.ref;
-                if (is_far(row.all.m, c)) notes[p].far = 1;
+                if (row.far) notes[p].far = 1;
             }
         }
         int next_cls = -1;
@@ -913,7 +914,8 @@ __global__ __launch_bounds__(NT) void distill_tiles_kernel(DistillArgs a, int ti
     constexpr int VEC = T::VEC, TILE = NT * NV * VEC;
     __shared__ Stats red_far[NT / 64];
     __shared__ int s_cls[MAX_TOP];
-    __shared__ float s_d[MAX_TOP], s_row[4];
+    __shared__ float s_d[MAX_TOP], s_row[2];
+    __shared__ int s_far;
     if (a.upstream && a.skip_unit && a.upstream[0] == 1.f) return;
     const long p = blockIdx.x / tiles;
     const int tile = blockIdx.x % tiles, base = tile * TILE, C = a.g.classes, lane = threadIdx.x & 63;
@@ -939,10 +941,10 @@ __global__ __launch_bounds__(NT) void distill_tiles_kernel(DistillArgs a, int ti
         const RowResult row = join_row<T>(a, p, w, l, rest, d, lane, tile == 0);
         s_cls[lane] = l.e.cls;
         s_d[lane] = d;
-        if (lane == 0) { s_row[0] = row.factor; s_row[1] = row.ref; s_row[2] = row.all.m; }
+        if (lane == 0) { s_row[0] = row.factor; s_row[1] = row.ref; s_far = row.far; }
     }
     __syncthreads();
-    if (is_far(s_row[2], c)) {
+    if (s_far) {
         if (tile == 0) {
             const float x = distill_position<T>(a, p, w, red_far, s_cls, s_d, s_row);
             if (threadIdx.x == 0 && a.part) a.part[p] = x;

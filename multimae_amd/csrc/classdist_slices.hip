@@ -268,7 +268,7 @@ __global__ __launch_bounds__(64) void distill_map_join_kernel(DistillArgs a, int
     const float l2 = empty ? INFINITY : log2_(v.s);
     const float r = a.log_probs && rest.s != 0.f ? left : 0.f, Q = total + r;
     const float gs = empty ? 0.f : w * a.g.inv_t * (a.upstream ? a.upstream[0] : 1.f);
-    const bool far = w != 0.f && is_far(v.m, c);
+    const bool far = w != 0.f && (is_far(v.m, c) || (a.log_probs && is_far(rest.m, c)));
     for (int e = 0; e < k; ++e) {
         int cls = s_cls[e * POS + lane];
         const float q = s_q[e * POS + lane], x = s_z[e * POS + lane];
