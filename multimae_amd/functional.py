@@ -979,10 +979,9 @@ class DistillFn(torch.autograd.Function):
             return call.run()
         d_logits = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
         loss = call.run(d_logits)
-        # what the call reads again lives as long as the graph keeps its tensors, however long the loss is kept
+        # what the backward pass reads again lives as long as the graph keeps its tensors, however long the loss is kept
         ctx.save_for_backward(logits, top_class, top_value, mask, call.workspace)
-        call.tensors = call.workspace = None
-        ctx.call, ctx.d_logits = call, d_logits
+        ctx.how, ctx.d_logits = (patch, temperature, log_probs), d_logits
         return loss
 
     @staticmethod
@@ -990,12 +989,15 @@ class DistillFn(torch.autograd.Function):
     def backward(ctx, g):
         d_logits, ctx.d_logits = ctx.d_logits, None
         if d_logits is None or not getattr(ctx, "unit_upstream", False):
-            call, first = ctx.call, d_logits is not None
-            call.workspace = ctx.saved_tensors[4]  # (refused if an input was changed since, or the graph is freed)
+            # (refused if an input was changed since, or the graph is freed; where saved tensors are packed, or computed anew, they come
+            # back at another address, and their layout is the hook's)
+            logits, top_class, top_value, mask, workspace = ctx.saved_tensors
+            call = ops.Distillation(_class_scores(logits), top_class.contiguous(), top_value.contiguous(), None if mask is None else mask.contiguous(),
+                                    *ctx.how, workspace=workspace)
+            first = d_logits is not None
             if not first:
                 d_logits = torch.empty(call.shape, dtype=call.dtype, device=call.device)
             call.scale(d_logits, g, skip_unit=first)
-            call.workspace = None
         return d_logits, None, None, None, None, None, None
 
 

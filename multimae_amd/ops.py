@@ -732,10 +732,11 @@ class Distillation:
     tokens are patch x patch squares of the last two dimensions, or single positions with patch = 1.
 
     run() computes the f32 scalar loss and, into d_logits (contiguous, the logits' dtype), its gradient.  scale() then makes
-    the gradient again, times an f32 scalar on the device, from what a run() with a gradient left in the workspace."""
+    the gradient again, times an f32 scalar on the device, from what a run() with a gradient left in the workspace.  workspace: that
+    of an earlier such call on equal tensors (in any layout), which scale() of this one goes on from."""
 
     def __init__(self, logits: torch.Tensor, top_class: torch.Tensor, top_value: torch.Tensor, mask: Optional[torch.Tensor] = None,
-                 patch: int = 1, temperature: float = 1.0, log_probs: bool = False):
+                 patch: int = 1, temperature: float = 1.0, log_probs: bool = False, workspace: Optional[torch.Tensor] = None):
         geo = _class_scores(logits, "distill")
         shape = logits.shape
         B, space = shape[0], shape[2:]
@@ -760,10 +761,13 @@ class Distillation:
         self.shape, self.dtype, self.device, self.bytes = shape, logits.dtype, logits.device, logits.nbytes
         self.tensors = (logits, top_class, top_value, mask)  # (what args point to)
         nbytes = _L().mmae_distill_workspace_bytes(_DT[logits.dtype], *geo[:3], k)
-        self.workspace = torch.empty(nbytes, dtype=torch.uint8, device=logits.device)
+        if workspace is None:
+            self.workspace = torch.empty(nbytes, dtype=torch.uint8, device=logits.device)
+        else:
+            self.workspace = _beside(_req(workspace, torch.uint8, "distill workspace"), logits, (nbytes,), "distill workspace")
         self.args = (*_class_call(logits, geo), top_class.data_ptr(), top_class.element_size(), top_value.data_ptr(), _DT[top_value.dtype],
                      k, int(log_probs), temperature, _addr(mask), width, patch if mask is not None else 1)
-        self.scalable = False  # (a run() for the loss alone lays the workspace out otherwise)
+        self.scalable = workspace is not None  # (a run() for the loss alone lays the workspace out otherwise)
         self.beside_bytes = geo[0] * geo[2] * k * (top_class.element_size() + top_value.element_size())
 
     def _launch(self, upstream, again, skip_unit, loss, d_logits):

@@ -1,0 +1,63 @@
+"""The autograd nodes of the class distributions without a GPU: the launches are recorded instead of made, so no address is followed."""
+import pytest
+import torch
+from torch.utils.checkpoint import checkpoint
+
+from multimae_amd import functional, ops
+
+
+@pytest.fixture
+def launches(monkeypatch):
+    """(name, arguments) of every launch; tensors on the CPU are taken."""
+    seen = []
+    monkeypatch.setattr(ops, "_launch", lambda what, fn, device, nbytes, *args: seen.append((what, args)))
+    monkeypatch.setattr(ops, "_req", lambda t, *a, **k: t)
+    monkeypatch.setattr(ops, "_beside", lambda t, *a: t)
+    return seen
+
+
+def distill_args():
+    logits = torch.randn(6, 40)[:, 3:33].requires_grad_(True)  # rows further apart: the Python node
+    return logits, torch.randint(0, 30, (6, 4)), torch.randn(6, 4), torch.ones(6, 1, dtype=torch.long)
+
+
+class Unpacked(torch.autograd.graph.saved_tensors_hooks):
+    """Saved tensors live elsewhere when they come back, in the layout that `like` gives them."""
+
+    def __init__(self, like=torch.clone):
+        self.given = []
+
+        def unpack(t):
+            self.given.append(like(t))
+            return self.given[-1]
+        super().__init__(lambda t: t.detach().clone(), unpack)
+
+
+def test_distillation_backward_points_to_the_unpacked_tensors(launches):
+    logits, cls, val, mask = distill_args()
+    hooks = Unpacked()
+    with hooks:
+        loss = functional.distill(logits, cls, val, mask, 1, 1.0, True)
+    for again in range(2):
+        hooks.given.clear()
+        torch.autograd.grad(loss, logits, torch.tensor(3.0), retain_graph=True)
+        args = launches[-1][1]
+        at = {t.data_ptr() for t in hooks.given}
+        assert len(hooks.given) == 5
+        for place, what in ((0, "logits"), (6, "classes"), (8, "values"), (13, "mask"), (-2, "workspace")):
+            assert args[place] in at, (what, again)
+        assert args[5] == hooks.given[0].stride(0)
+
+
+def test_distillation_backward_after_recomputation_points_to_the_recomputed_tensors(launches):
+    logits, cls, val, mask = distill_args()
+    made = []
+
+    def body(x):
+        made.append((x * 2.0).t().contiguous().t()[:, :29])
+        return functional.distill(made[-1], cls % 29, val, mask, 1, 1.0, False)
+    loss = checkpoint(body, logits, use_reentrant=False)
+    made.clear()  # what the first forward pass made is gone
+    torch.autograd.grad(loss, logits, torch.tensor(3.0))
+    first, again, last = (args[0] for _, args in launches)
+    assert len(made) == 1 and last == again != first

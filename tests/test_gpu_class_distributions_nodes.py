@@ -1,0 +1,65 @@
+"""The autograd nodes of the class distributions under what autograd does with saved tensors: packed and unpacked by hooks, kept on
+the host, freed and computed anew.  Results are those of a plain backward pass, bit by bit."""
+import pytest
+import torch
+from torch.utils.checkpoint import checkpoint
+
+from tests.test_gpu_class_distributions import M, classes, loss_module, scores, teacher_top  # noqa: F401  (M: the fixture)
+
+pytestmark = pytest.mark.gpu
+
+# contiguous logits (the C++ nodes), rows and maps cut from larger ones and channels_last (the Python nodes)
+LAYOUTS = {"rows": lambda x: x, "cut rows": lambda x: torch.cat([x, x], 1)[:, : x.shape[1]], "maps": lambda x: x.view(4, -1, 4, 6),
+           "channels_last": lambda x: x.view(4, -1, 4, 6).contiguous(memory_format=torch.channels_last),
+           "large maps": lambda x: torch.cat([x.view(2, -1, 2, 2)] * 2, 1)[:, : x.numel() // 8]}
+
+
+def trash():
+    """What the allocator has free is overwritten."""
+    torch.cuda.synchronize()
+    for n in (1 << 20, 1 << 16, 1 << 14, 1 << 10):
+        [torch.full((n,), 1e3, device="cuda") for _ in range(4)]
+
+
+def losses(M, z, log_probs):  # noqa: F811
+    """Of z [B, C, ...]: a distillation loss and a sum of log probabilities and entropies."""
+    shape = tuple(z.shape)
+    cls, val = teacher_top(shape, 6, 3, log_probs, 1.5)
+    mask = torch.ones(shape[0], z[0, 0].numel(), dtype=torch.long, device="cuda")
+    mask[1] = 0
+    loss = loss_module(M, 1, 1.5, log_probs)(z, (cls, val), mask=mask)
+    out = M.class_log_probs(z, classes(shape[:1] + shape[2:], shape[1], 4), temperature=1.5)
+    return loss, out.log_prob.sum() - out.entropy.square().sum()
+
+
+def gradients(leaf, values):
+    """With upstream gradients of 3 and 1, twice the same graph."""
+    found = []
+    for v in values:
+        for up in (3.0, 1.0, 0.5):
+            trash()
+            found += torch.autograd.grad(v, leaf, torch.tensor(up, device="cuda"), retain_graph=True)
+    return found
+
+
+@pytest.mark.parametrize("log_probs", [False, True], ids=["logits", "log_probs"])
+@pytest.mark.parametrize("layout", LAYOUTS)
+def test_gradients_with_saved_tensors_packed_and_recomputed(M, layout, log_probs):  # noqa: F811
+    leaf = scores((8, 12000), "bf16", 1).requires_grad_(True)
+
+    def body(x):
+        return losses(M, LAYOUTS[layout](x * 1.5), log_probs)
+    want = gradients(leaf, body(leaf))
+    assert all(torch.isfinite(g).all() and g.abs().sum() > 0 for g in want)
+    with torch.autograd.graph.save_on_cpu():
+        values = body(leaf)
+    assert all(torch.equal(a, b) for a, b in zip(want, gradients(leaf, values)))
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: (t.detach().clone(),), lambda t: t[0].clone()):
+        values = body(leaf)
+    assert all(torch.equal(a, b) for a, b in zip(want, gradients(leaf, values)))
+    got = []
+    for i, up in ((0, 3.0), (0, 1.0), (0, 0.5), (1, 3.0), (1, 1.0), (1, 0.5)):  # (a recomputed graph is used once)
+        value = checkpoint(body, leaf, use_reentrant=False)[i]
+        trash()
+        got += torch.autograd.grad(value, leaf, torch.tensor(up, device="cuda"))
+    assert all(torch.equal(a, b) for a, b in zip(want, got))
