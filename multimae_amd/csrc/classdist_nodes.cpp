@@ -42,6 +42,30 @@ bool beside(const Tensor& t, const Tensor& logits, int64_t k) {
     return true;
 }
 
+// What a distillation call points to.
+bool fits(const Tensor& logits, const Tensor& top_class, const Tensor& top_value, const Tensor& mask, int64_t patch, Geometry& g) {
+    if (!plain_logits(logits, g) || top_class.dim() < 2) return false;
+    const int64_t k = top_class.size(1);
+    const auto kind = top_class.scalar_type();
+    if (k < 1 || k > 64 || (kind != at::kLong && kind != at::kInt) || dtype_code(top_value) < 0 || !beside(top_class, logits, k) || !beside(top_value, logits, k)) return false;
+    if (!mask.defined()) return true;
+    const int64_t width = logits.dim() > 2 ? logits.size(-1) : 1;
+    if (patch < 1 || (patch > 1 && logits.dim() != 4) || width % patch || g.inner / width % patch) return false;
+    return mask.is_cuda() && mask.device() == logits.device() && mask.scalar_type() == at::kLong && mask.is_contiguous() && mask.dim() == 2 &&
+           mask.size(0) == g.outer && mask.size(1) == g.inner / (patch * patch);
+}
+// The tensors that a backward pass gets back: as they were saved, or what a hook made of them, in any layout.  Whatever else the hook
+// changed is refused.
+variable_list unpacked(AutogradContext* ctx) {
+    at::AutoGradMode off(false);
+    auto saved = ctx->get_saved_variables();
+    for (auto& t : saved)
+        if (t.defined()) t = t.contiguous();
+    return saved;
+}
+bool floats(const Tensor& t, const Tensor& like, int64_t n) { return t.device() == like.device() && t.scalar_type() == at::kFloat && t.numel() == n; }
+#define UNPACKED(as_saved) TORCH_CHECK(as_saved, "class distributions: a saved tensor came back with another shape, type or device")
+
 mmae_stream_t stream_of(const Tensor& t) { return (mmae_stream_t)c10::hip::getCurrentHIPStream(t.device().index()).stream(); }
 void check(int rc) { TORCH_CHECK(rc == MMAE_OK, mmae_last_error()); }
 
@@ -92,10 +116,11 @@ struct LogProbs : torch::autograd::Function<LogProbs> {
     }
     static variable_list backward(AutogradContext* ctx, variable_list grads) {
         if (!grads[0].defined() && !grads[1].defined()) return {Tensor(), Tensor(), Tensor(), Tensor()};
-        const auto saved = ctx->get_saved_variables();
+        const auto saved = unpacked(ctx);
         const Tensor &logits = saved[0], &target = saved[1];
         Geometry g;
-        plain_logits(logits, g);
+        UNPACKED(plain_logits(logits, g) && target.scalar_type() == at::kLong && beside(target, logits, 0) && floats(saved[2], logits, target.numel()) &&
+                 floats(saved[3], logits, 2 * target.numel()));
         Tensor d[2], d_logits;
         {
             at::AutoGradMode off(false);
@@ -155,8 +180,11 @@ struct Distill : torch::autograd::Function<Distill> {
         }
         const bool made = d_logits.defined();
         if (!made || !d.count("unit")) {
-            const auto saved = ctx->get_saved_variables();  // (refused if an input was changed since, or the graph is freed)
+            const auto saved = unpacked(ctx);  // (refused if an input was changed since, or the graph is freed)
             at::AutoGradMode off(false);
+            Geometry g;
+            UNPACKED(fits(saved[0], saved[1], saved[2], saved[3], d["patch"].toInt(), g) && saved[4].device() == saved[0].device() &&
+                     saved[4].scalar_type() == at::kByte && (!made || (d_logits.sizes() == saved[0].sizes() && d_logits.scalar_type() == saved[0].scalar_type())));
             if (!made) d_logits = at::empty(saved[0].sizes(), saved[0].options());
             const Tensor upstream = grads[0].contiguous();
             Distillation{saved[0], saved[1], saved[2], saved[3], saved[4], d["patch"].toInt(), d["temperature"].toDouble(), d["log_probs"].toBool()}.run(
@@ -189,19 +217,8 @@ pybind11::object distill(const Tensor& logits, const Tensor& top_class, const Te
                          double temperature, bool log_probs) {
     Geometry g;
     const Tensor mask = mask_ ? *mask_ : Tensor();
-    if (!plain_logits(logits, g) || !(temperature > 0) || temperature > 1e30 || top_class.dim() < 2) return pybind11::none();
-    const int64_t k = top_class.size(1);
-    const auto kind = top_class.scalar_type();
-    if (k < 1 || k > 64 || (kind != at::kLong && kind != at::kInt) || dtype_code(top_value) < 0 || !beside(top_class, logits, k) || !beside(top_value, logits, k))
-        return pybind11::none();
-    if (mask.defined()) {
-        const int64_t width = logits.dim() > 2 ? logits.size(-1) : 1;
-        if (patch < 1 || (patch > 1 && logits.dim() != 4) || width % patch || g.inner / width % patch) return pybind11::none();
-        if (!mask.is_cuda() || mask.device() != logits.device() || mask.scalar_type() != at::kLong || !mask.is_contiguous() || mask.dim() != 2 ||
-            mask.size(0) != g.outer || mask.size(1) != g.inner / (patch * patch))
-            return pybind11::none();
-    }
-    const size_t bytes = mmae_distill_workspace_bytes(dtype_code(logits), g.outer, g.classes, g.inner, (int)k);
+    if (!fits(logits, top_class, top_value, mask, patch, g) || !(temperature > 0) || temperature > 1e30) return pybind11::none();
+    const size_t bytes = mmae_distill_workspace_bytes(dtype_code(logits), g.outer, g.classes, g.inner, (int)top_class.size(1));
     const Tensor workspace = at::empty({(int64_t)bytes}, logits.options().dtype(at::kByte).requires_grad(false));
     if (at::GradMode::is_enabled() && logits.requires_grad())
         return pybind11::cast(Distill::apply(logits, top_class, top_value, mask_, workspace, patch, temperature, log_probs));

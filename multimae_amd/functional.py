@@ -962,7 +962,8 @@ class ClassLogProbsFn(torch.autograd.Function):
             return None, None, None, None
         logits, target, entropy = ctx.saved_tensors
         g = [None if t is None else t.contiguous() for t in (g_log_prob, g_entropy)]  # (fp32, as the outputs: autograd sees to it)
-        return ops._class_log_probs_bwd(logits, ops.class_geometry(logits), target, entropy, ctx.stats, *g, ctx.temperature), None, None, None
+        # (what a hook unpacks has a layout of its own)
+        return ops.class_log_probs_bwd(_class_scores(logits), target.contiguous(), entropy.contiguous(), ctx.stats, *g, ctx.temperature), None, None, None
 
 
 class DistillFn(torch.autograd.Function):
@@ -993,7 +994,7 @@ class DistillFn(torch.autograd.Function):
             # back at another address, and their layout is the hook's)
             logits, top_class, top_value, mask, workspace = ctx.saved_tensors
             call = ops.Distillation(_class_scores(logits), top_class.contiguous(), top_value.contiguous(), None if mask is None else mask.contiguous(),
-                                    *ctx.how, workspace=workspace)
+                                    *ctx.how, workspace=workspace.contiguous())
             first = d_logits is not None
             if not first:
                 d_logits = torch.empty(call.shape, dtype=call.dtype, device=call.device)

@@ -711,11 +711,6 @@ def class_log_probs_bwd(logits: torch.Tensor, target: torch.Tensor, entropy: tor
     for t, s, n in ((entropy, shape, "entropy"), (stats, (2,) + shape, "stats"), (d_log_prob, shape, "d_log_prob"), (d_entropy, shape, "d_entropy")):
         if t is not None:
             _beside(_req(t, F32, f"class_log_probs_bwd {n}"), logits, s, f"class_log_probs_bwd {n}")
-    return _class_log_probs_bwd(logits, geo, target, entropy, stats, d_log_prob, d_entropy, temperature)
-
-
-def _class_log_probs_bwd(logits, geo, target, entropy, stats, d_log_prob, d_entropy, temperature):
-    """class_log_probs_bwd of a call that was checked before (host time counts in the backward pass of a small one)."""
     dev = logits.device
     d_logits = torch.empty(logits.shape, dtype=logits.dtype, device=dev)
     if geo[0]:

@@ -21,6 +21,11 @@ def distill_args():
     return logits, torch.randint(0, 30, (6, 4)), torch.randn(6, 4), torch.ones(6, 1, dtype=torch.long)
 
 
+def strided(t):
+    """t with its elements two apart."""
+    return torch.stack([t, t], -1)[..., 0]
+
+
 class Unpacked(torch.autograd.graph.saved_tensors_hooks):
     """Saved tensors live elsewhere when they come back, in the layout that `like` gives them."""
 
@@ -61,3 +66,28 @@ def test_distillation_backward_after_recomputation_points_to_the_recomputed_tens
     torch.autograd.grad(loss, logits, torch.tensor(3.0))
     first, again, last = (args[0] for _, args in launches)
     assert len(made) == 1 and last == again != first
+
+
+def test_backward_passes_take_any_layout_from_the_hooks(launches):
+    logits, cls, val, mask = distill_args()
+    hooks = Unpacked(strided)
+    target = torch.randint(0, 30, (6,))
+    with hooks:
+        loss = functional.distill(logits, cls, val, mask, 1, 1.0, True)
+        log_prob, entropy, _, _ = functional.class_log_probs(logits, target, 0, 1.0)
+    contiguous = []
+    launch = ops._launch
+
+    def look(what, fn, device, nbytes, *args):  # (while the tensors live)
+        import ctypes
+        if what == "class_log_probs_bwd":
+            contiguous.append([ctypes.c_int64.from_address(args[6] + 8 * i).value for i in range(6)] == target.tolist())
+            contiguous.append([ctypes.c_float.from_address(args[0] + 4 * i).value for i in range(30)] == logits[0].tolist())
+        elif what == "distill":
+            contiguous.append([ctypes.c_int64.from_address(args[6] + 8 * i).value for i in range(24)] == cls.flatten().tolist())
+            contiguous.append([ctypes.c_float.from_address(args[8] + 4 * i).value for i in range(24)] == val.flatten().tolist())
+        launch(what, fn, device, nbytes, *args)
+    ops._launch = look
+    torch.autograd.grad(loss, logits, torch.tensor(3.0))
+    torch.autograd.grad((log_prob, entropy), logits, (torch.ones(6), torch.ones(6)))
+    assert contiguous == [True] * 4

@@ -63,3 +63,30 @@ def test_gradients_with_saved_tensors_packed_and_recomputed(M, layout, log_probs
         trash()
         got += torch.autograd.grad(value, leaf, torch.tensor(up, device="cuda"))
     assert all(torch.equal(a, b) for a, b in zip(want, got))
+
+
+@pytest.mark.parametrize("layout", LAYOUTS)
+def test_gradients_with_another_layout_from_the_hooks(M, layout):  # noqa: F811
+    """What an unpack hook returns may have strides of its own; another shape, type or place is refused."""
+    leaf = scores((8, 12000), "bf16", 1).requires_grad_(True)
+
+    def body(x):
+        return losses(M, LAYOUTS[layout](x * 1.5), True)
+    want = gradients(leaf, body(leaf))
+
+    def strided(t):
+        return torch.stack([t, t], -1)[..., 0]
+
+    def last(t):
+        return t.contiguous(memory_format=torch.channels_last) if t.dim() == 4 else t.clone()
+    for like in (strided, last):
+        with torch.autograd.graph.saved_tensors_hooks(lambda t: t.detach(), like):
+            values = body(leaf)
+        assert all(torch.equal(a, b) for a, b in zip(want, gradients(leaf, values)))
+    x = LAYOUTS[layout](leaf.detach() * 1.5).requires_grad_(True)
+    for like in (lambda t: t.cpu(), lambda t: t[:1], lambda t: t.double()):
+        with torch.autograd.graph.saved_tensors_hooks(lambda t: t.detach(), like):
+            values = losses(M, x, False)
+        for v in values:
+            with pytest.raises(RuntimeError):
+                torch.autograd.grad(v, x, torch.tensor(3.0, device="cuda"))
