@@ -74,7 +74,7 @@ def class_log_probs(input, target, top_k: int = 0, temperature: float = 1.0) -> 
     the distribution is softmax(input / temperature) over dimension 1.  A target outside [0, C) (-100: an ignored pixel) has
     log probability 0 and no gradient.  Up to 64 alternatives in descending order, equal logits by the lower class; these
     carry no gradient (they are what MaskedDistillationLoss takes from a teacher).  log_prob and entropy are fp32 and
-    differentiable.  A position whose logits are all -inf has log probability -inf, entropy 0 and no gradient."""
+    differentiable once, in reverse mode; forward mode and tracing are refused.  A position whose logits are all -inf has log probability -inf, entropy 0 and no gradient."""
     if target.dtype != torch.int64:
         target = target.to(torch.int64)
     return ClassLogProbs(*Fn.class_log_probs(input, target, int(top_k), float(temperature)))
@@ -88,7 +88,7 @@ class MaskedDistillationLoss(nn.Module):
     teacher="logits": the target's values are the teacher's logits of the kept classes, and its distribution is
     softmax(values / temperature) over these.  teacher="log_probs": they are its log probabilities at this temperature (the
     top_log_prob of class_log_probs), and what the kept classes leave of 1 is compared with the student's probability of
-    all other classes together."""
+    all other classes together.  Differentiable once, in the student's logits, in reverse mode; forward mode and tracing are refused."""
 
     def __init__(self, patch_size: int = 16, stride: int = 1, temperature: float = 1.0, teacher: str = "logits"):
         super().__init__()

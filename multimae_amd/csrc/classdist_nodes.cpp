@@ -2,10 +2,12 @@
 // make, without the interpreter in the backward pass, which runs on autograd's own thread and finds cold caches there.  On one host,
 // log probabilities and gradient of 512 x 1000 fp32: 63 us a step, 112 us with the Python nodes; distillation of 16 x 32000 bf16 68
 // and 119 us; log probabilities of 1 x 32000 bf16 10 and 21 us.  (44 us of the steps are autograd's: log_softmax and its gradient.)
-// A call that is anything else (another layout, type or device, a wrong argument) is answered with None: the Python side copies,
-// or refuses it by name.
+// A call that is anything else (another layout, type or device, a wrong argument, a mode that does not see the kernels) is answered
+// with None: the Python side copies, or refuses it by name.
+#include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/jit/frontend/tracer.h>
 #include <torch/extension.h>
 
 #include "../../include/mmae.h"
@@ -22,6 +24,12 @@ int dtype_code(const Tensor& t) {
 }
 
 struct Geometry { int outer, classes, inner; };
+
+// Forward-mode derivatives and traces do not see what the kernels write.
+bool passed_by(const Tensor& logits) {
+    return logits._fw_grad(0).defined() || torch::jit::tracer::isTracing() ||
+           c10::impl::TorchDispatchModeTLS::get_mode(c10::impl::TorchDispatchModeKey::PROXY).has_value();
+}
 
 // Logits [B, C, ...] as they are in most calls: contiguous, not empty, on the current device.
 bool plain_logits(const Tensor& t, Geometry& g) {
@@ -198,7 +206,7 @@ struct Distill : torch::autograd::Function<Distill> {
 
 pybind11::object class_log_probs(const Tensor& logits, const Tensor& target, int64_t k, double temperature) {
     Geometry g;
-    if (!plain_logits(logits, g) || target.scalar_type() != at::kLong || !beside(target, logits, 0) || k < 0 || k > 64 || k > g.classes || !(temperature > 0) ||
+    if (passed_by(logits) || !plain_logits(logits, g) || target.scalar_type() != at::kLong || !beside(target, logits, 0) || k < 0 || k > 64 || k > g.classes || !(temperature > 0) ||
         temperature > 1e30)
         return pybind11::none();
     const auto give = [](const Tensor& a, const Tensor& b, const Tensor& c, const Tensor& e) {
@@ -217,7 +225,7 @@ pybind11::object distill(const Tensor& logits, const Tensor& top_class, const Te
                          double temperature, bool log_probs) {
     Geometry g;
     const Tensor mask = mask_ ? *mask_ : Tensor();
-    if (!fits(logits, top_class, top_value, mask, patch, g) || !(temperature > 0) || temperature > 1e30) return pybind11::none();
+    if (passed_by(logits) || !fits(logits, top_class, top_value, mask, patch, g) || !(temperature > 0) || temperature > 1e30) return pybind11::none();
     const size_t bytes = mmae_distill_workspace_bytes(dtype_code(logits), g.outer, g.classes, g.inner, (int)top_class.size(1));
     const Tensor workspace = at::empty({(int64_t)bytes}, logits.options().dtype(at::kByte).requires_grad(false));
     if (at::GradMode::is_enabled() && logits.requires_grad())

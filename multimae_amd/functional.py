@@ -10,7 +10,7 @@ import sys
 
 import torch
 
-from . import ops
+from . import _lib, ops
 
 # ---------------------------------------------------------------------------------------------
 # bf16 copies of the fp32 master weights ([out,in] for the forward / dW, [in,out] for dA)
@@ -913,12 +913,22 @@ def _nodes():
     return module
 
 
+def _seen_by_autograd(logits: torch.Tensor, name: str):
+    """Refuses what does not see the kernels: forward-mode derivatives would be zero, and a trace would hold nothing but the
+    outputs' allocations."""
+    if torch.autograd.forward_ad.unpack_dual(logits).tangent is not None:
+        raise _lib.MmaeError(f"{name}: forward-mode derivatives are not there")
+    if torch.jit.is_tracing() or torch._C._get_dispatch_mode(torch._C._TorchDispatchModeKey.PROXY) is not None:
+        raise _lib.MmaeError(f"{name}: cannot be traced")
+
+
 def class_log_probs(logits, target, top_k, temperature):
     """Log probability of the given class, entropy and top classes; a node only where a gradient is asked for."""
     nodes = _nodes()
     out = nodes and nodes.class_log_probs(logits, target, top_k, temperature)
     if out is not None:
         return out
+    _seen_by_autograd(logits, "class_log_probs")
     if torch.is_grad_enabled() and logits.requires_grad:
         return ClassLogProbsFn.apply(logits, target, top_k, temperature)
     return ops.class_log_probs(_class_scores(logits), target.contiguous(), top_k, temperature, want_stats=False)[:4]
@@ -929,6 +939,7 @@ def distill(logits, top_class, top_value, mask, patch, temperature, log_probs):
     nodes = _nodes()
     loss = nodes and nodes.distill(logits, top_class, top_value, mask, patch, temperature, log_probs)
     if loss is None:  # (the teacher has no gradient)
+        _seen_by_autograd(logits, "distill")
         loss = DistillFn.apply(logits, top_class, top_value.detach(), mask, patch, temperature, log_probs)
     return loss
 

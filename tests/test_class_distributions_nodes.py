@@ -91,3 +91,25 @@ def test_backward_passes_take_any_layout_from_the_hooks(launches):
     torch.autograd.grad(loss, logits, torch.tensor(3.0))
     torch.autograd.grad((log_prob, entropy), logits, (torch.ones(6), torch.ones(6)))
     assert contiguous == [True] * 4
+
+
+def test_forward_mode_and_tracing_are_refused_by_name():
+    """Neither sees the kernels: a derivative of zero, a graph that holds nothing but the outputs' allocations."""
+    import multimae_amd as M
+    from torch.autograd import forward_ad
+    from torch.fx.experimental.proxy_tensor import make_fx
+    from multimae_amd._lib import MmaeError
+    z, t, v = torch.randn(6, 30), torch.randint(0, 30, (6,)), torch.randn(6, 1)
+    calls = [lambda x: M.class_log_probs(x, t).log_prob, lambda x: M.MaskedDistillationLoss()(x, (t.view(6, 1), v))]
+    for call in calls:
+        with forward_ad.dual_level():
+            with pytest.raises(MmaeError, match="forward-mode"):
+                call(forward_ad.make_dual(z, torch.ones_like(z)))
+            with pytest.raises(MmaeError, match="GPU"):  # (no tangent: an ordinary call)
+                call(z)
+        with pytest.raises(MmaeError, match="traced"):
+            torch.jit.trace(call, z, check_trace=False)
+        with pytest.raises(MmaeError, match="traced"):
+            make_fx(call)(z)
+        with pytest.raises(MmaeError, match="GPU"):
+            call(z)

@@ -90,3 +90,25 @@ def test_gradients_with_another_layout_from_the_hooks(M, layout):  # noqa: F811
         for v in values:
             with pytest.raises(RuntimeError):
                 torch.autograd.grad(v, x, torch.tensor(3.0, device="cuda"))
+
+
+@pytest.mark.parametrize("profile", [None, []], ids=["C++", "Python"])
+def test_forward_mode_and_tracing_are_refused(M, profile, monkeypatch):  # noqa: F811
+    from torch.autograd import forward_ad
+    from torch.fx.experimental.proxy_tensor import make_fx
+    from multimae_amd import ops
+    from multimae_amd._lib import MmaeError
+    monkeypatch.setattr(ops, "PROFILE", profile)
+    z, t, v = scores((6, 300), "f32", 1), classes((6,), 300, 2), torch.zeros(6, 1, device="cuda")
+    for call in (lambda x: M.class_log_probs(x, t).log_prob, lambda x: M.MaskedDistillationLoss()(x, (t.view(6, 1), v))):
+        want = call(z)
+        for x in (z, z.clone().requires_grad_(True)):
+            with forward_ad.dual_level():
+                with pytest.raises(MmaeError, match="forward-mode"):
+                    call(forward_ad.make_dual(x, torch.ones_like(x)))
+                assert torch.equal(call(x), want)
+            with pytest.raises(MmaeError, match="traced"):
+                torch.jit.trace(call, x, check_trace=False)
+            with pytest.raises(MmaeError, match="traced"):
+                make_fx(call)(x)
+        assert torch.equal(call(z), want)
