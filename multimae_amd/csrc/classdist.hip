@@ -34,12 +34,18 @@ __global__ __launch_bounds__(1024) void distill_sum_kernel(const float* part, lo
     }
 }
 
+// Sizes that the launches take (the products below stay inside their types); a workspace is asked for before they are looked at.
+constexpr int MOST_CLASSES = 1 << 30;
+constexpr long MOST_POSITIONS = 0x7fffffc0L;
+bool sizes_taken(int outer, int classes, int inner, int k) {
+    return outer > 0 && classes > 0 && inner > 0 && classes <= MOST_CLASSES && (long)outer * inner <= MOST_POSITIONS && k >= 0 && k <= MAX_TOP;
+}
 int check_logits(const char* name, const void* logits, int dtype, int outer, int classes, int inner, long ld, float temperature) {
     MMAE_REQUIRE(logits, MMAE_EINVAL, "%s: null pointer", name);
     MMAE_REQUIRE(dtype >= MMAE_DT_F32 && dtype <= MMAE_DT_F16, MMAE_EINVAL, "%s: dtype code %d", name, dtype);
     MMAE_REQUIRE(outer > 0 && classes > 0 && inner > 0, MMAE_ESHAPE, "%s: empty input (%d x %d x %d)", name, outer, classes, inner);
-    MMAE_REQUIRE(classes <= 1 << 30, MMAE_ESHAPE, "%s: %d classes", name, classes);
-    MMAE_REQUIRE((long)outer * inner <= 0x7fffffc0L, MMAE_ESHAPE, "%s: %d x %d positions are more than 2^31 - 64", name, outer, inner);
+    MMAE_REQUIRE(classes <= MOST_CLASSES, MMAE_ESHAPE, "%s: %d classes", name, classes);
+    MMAE_REQUIRE((long)outer * inner <= MOST_POSITIONS, MMAE_ESHAPE, "%s: %d x %d positions are more than 2^31 - 64", name, outer, inner);
     MMAE_REQUIRE(ld >= (long)classes * inner, MMAE_ESHAPE, "%s: samples %ld elements apart hold %d x %d values", name, ld, classes, inner);
     MMAE_REQUIRE(temperature > 0.f && temperature < INFINITY, MMAE_EINVAL, "%s: temperature %g is not positive and finite", name, temperature);
     return MMAE_OK;
@@ -51,7 +57,7 @@ int check_logits(const char* name, const void* logits, int dtype, int outer, int
 using namespace classdist;
 
 extern "C" size_t mmae_class_log_probs_workspace_bytes(int dtype, int outer, int classes, int inner, int top_k) {
-    if (outer < 1 || classes < 1 || inner < 1 || top_k < 0) return 0;
+    if (!sizes_taken(outer, classes, inner, top_k)) return 0;
     return inner == 1 ? log_probs_rows_workspace(outer, classes, top_k) : log_probs_slices_workspace(log_probs_map_slices(dtype, classes, top_k), outer, inner, top_k);
 }
 
@@ -95,7 +101,7 @@ static long distill_parts(int outer, int inner) { return inner == 1 ? outer : (l
 static size_t distill_floats(int outer, long parts) { return (4 + (size_t)outer + (size_t)parts + 3) / 4 * 4; }
 
 extern "C" size_t mmae_distill_workspace_bytes(int dtype, int outer, int classes, int inner, int k) {
-    if (outer < 1 || classes < 1 || inner < 1) return 0;
+    if (!sizes_taken(outer, classes, inner, k)) return 0;
     return sizeof(float) * distill_floats(outer, distill_parts(outer, inner)) +
            (inner == 1 ? distill_rows_workspace(outer, classes) : distill_slices_workspace(distill_map_slices(dtype, classes), outer, inner, k));
 }

@@ -989,7 +989,7 @@ constexpr int LP_NT = 256, LP_EPT = 16, LP_TILE = LP_NT * LP_EPT, ROW_TILE = 819
 // Workgroups a row is split into, and the tiles of each: enough for every CU to hold eight, at least a tile each, none empty.
 struct Split { int slices, tiles; };
 Split split_row(int rows, int classes, int tile) {
-    const int tiles = (classes + tile - 1) / tile, want = (8 * CUS + rows - 1) / rows;
+    const int tiles = (classes + tile - 1) / tile, want = rows < 8 * CUS ? (8 * CUS + rows - 1) / rows : 1;
     int n = want < tiles ? want : tiles;
     if (n > MAX_SLICES) n = MAX_SLICES;
     const int per = (tiles + n - 1) / n;
