@@ -13,11 +13,16 @@ FLAGS := --offload-arch=$(ARCH) -O3 -fPIC -std=c++17 -Wall -Wno-unused-variable 
 
 # The autograd nodes that are C++ link to torch: a module of the package's own beside the library, which knows no torch.
 PYTHON ?= python3
-TORCH  := $(shell $(PYTHON) -c "import importlib.util as u; print(u.find_spec('torch').submodule_search_locations[0])")
+TORCH  := $(shell $(PYTHON) -c "import importlib.util as u; s = u.find_spec('torch'); print(s.submodule_search_locations[0] if s else '')")
 PYINC  := $(shell $(PYTHON) -c "import sysconfig; print(sysconfig.get_paths()['include'])")
 NODES  := multimae_amd/_nodes.so
 
-all: $(LIB) $(NODES)
+all: lib $(if $(TORCH),nodes)
+lib: $(LIB)
+nodes: $(NODES)
+ifeq ($(TORCH),)
+$(warning $(PYTHON) has no torch: $(NODES) is left out, the Python autograd nodes serve its calls)
+endif
 
 $(OBJ)/%.o: $(CSRC)/%.hip $(CSRC)/common.h $(CSRC)/ln_rows.h $(CSRC)/classdist.h include/mmae.h Makefile
 	@mkdir -p $(OBJ)
@@ -44,4 +49,4 @@ $(NODES): $(OBJ)/classdist_nodes.o $(LIB)
 
 clean:
 	rm -rf build $(LIB) $(NODES)
-.PHONY: all clean
+.PHONY: all lib nodes clean

@@ -6,7 +6,7 @@ accumulates in fp32.  Each function saves exactly what its backward kernels read
 from typing import Dict, List, Optional, Sequence, Tuple
 
 import os
-import sys
+import warnings
 
 import torch
 
@@ -902,15 +902,24 @@ def _class_scores(x: torch.Tensor) -> torch.Tensor:
 
 
 _NODES = __package__ + "._nodes"
+_node_module = False  # (not asked for yet)
 
 
 def _nodes():
-    """The C++ nodes (csrc/classdist_nodes.cpp), None while launches are timed, which the Python nodes' are."""
+    """The C++ nodes (csrc/classdist_nodes.cpp), None while launches are timed, which the Python nodes' are, and where the module is
+    not built or does not fit this torch: the Python nodes make the same calls of the library, with more time on the host."""
+    global _node_module
     if ops.PROFILE is not None:
         return None
-    ops._L()  # (names the library where it is missing)
-    from . import _nodes as module
-    return module
+    if _node_module is False:
+        ops._L()  # (names the library where it is missing)
+        try:
+            from . import _nodes as module
+        except ImportError as e:
+            module = None
+            warnings.warn(f"{_NODES} is not usable ({e}): the Python nodes serve its calls, with more time on the host; `make` builds it")
+        _node_module = module
+    return _node_module
 
 
 def _seen_by_autograd(logits: torch.Tensor, name: str):
@@ -1022,8 +1031,8 @@ def mark_unit_upstream(losses) -> None:
         node = getattr(t, "grad_fn", None)
         if isinstance(node, (MaskedLossFn._backward_cls, MaskedCEFn._backward_cls, DistillFn._backward_cls)):
             node.unit_upstream = True
-        elif node is not None and _NODES in sys.modules:  # (a C++ node only where its module is loaded)
-            sys.modules[_NODES].mark_unit_upstream(t)
+        elif node is not None and _node_module:  # (a C++ node only where its module is loaded)
+            _node_module.mark_unit_upstream(t)
 
 
 class MaskedLossFn(torch.autograd.Function):

@@ -113,3 +113,20 @@ def test_forward_mode_and_tracing_are_refused_by_name():
             make_fx(call)(z)
         with pytest.raises(MmaeError, match="GPU"):
             call(z)
+
+
+def test_without_the_module_the_python_nodes_serve(launches, monkeypatch, recwarn):
+    import sys
+
+    import multimae_amd
+    monkeypatch.setitem(sys.modules, "multimae_amd._nodes", None)  # (an import error)
+    monkeypatch.delattr(multimae_amd, "_nodes", raising=False)
+    monkeypatch.setattr(functional, "_node_module", False)
+    logits, cls, val, mask = distill_args()
+    for _ in range(2):
+        loss = functional.distill(logits, cls, val, mask, 1, 1.0, True)
+        functional.mark_unit_upstream([loss, logits.sum()])
+        functional.class_log_probs(logits, cls[:, 0], 2, 1.0)
+    assert [what for what, _ in launches] == ["distill", "class_log_probs"] * 2
+    assert type(loss.grad_fn).__name__ == "DistillFnBackward" and loss.grad_fn.unit_upstream
+    assert sum("_nodes" in str(w.message) for w in recwarn) == 1
