@@ -6,6 +6,7 @@
 // with None: the Python side copies, or refuses it by name.
 #include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/hip/HIPStream.h>
+#include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/jit/frontend/tracer.h>
 #include <torch/extension.h>
@@ -17,6 +18,13 @@ namespace {
 using at::Tensor;
 using torch::autograd::AutogradContext;
 using torch::autograd::variable_list;
+
+// The package's own error: what a backward pass throws reaches the caller of backward() as this type.
+PyObject* error_type = nullptr;
+struct Refused : torch::PyTorchError {
+    using PyTorchError::PyTorchError;
+    PyObject* python_type() override { return error_type; }
+};
 
 int dtype_code(const Tensor& t) {
     const auto s = t.scalar_type();
@@ -72,10 +80,14 @@ variable_list unpacked(AutogradContext* ctx) {
     return saved;
 }
 bool floats(const Tensor& t, const Tensor& like, int64_t n) { return t.device() == like.device() && t.scalar_type() == at::kFloat && t.numel() == n; }
-#define UNPACKED(as_saved) TORCH_CHECK(as_saved, "class distributions: a saved tensor came back with another shape, type or device")
+void require_unpacked(bool as_saved) {
+    if (!as_saved) throw Refused("class distributions: a saved tensor came back with another shape, type or device");
+}
 
 mmae_stream_t stream_of(const Tensor& t) { return (mmae_stream_t)c10::hip::getCurrentHIPStream(t.device().index()).stream(); }
-void check(int rc) { TORCH_CHECK(rc == MMAE_OK, mmae_last_error()); }
+void check(int rc) {
+    if (rc != MMAE_OK) throw Refused(mmae_last_error());
+}
 
 // What a backward pass hands out: a gradient of it is refused, not taken for zero.
 Tensor once(const Tensor& grad) {
@@ -127,8 +139,8 @@ struct LogProbs : torch::autograd::Function<LogProbs> {
         const auto saved = unpacked(ctx);
         const Tensor &logits = saved[0], &target = saved[1];
         Geometry g;
-        UNPACKED(plain_logits(logits, g) && target.scalar_type() == at::kLong && beside(target, logits, 0) && floats(saved[2], logits, target.numel()) &&
-                 floats(saved[3], logits, 2 * target.numel()));
+        require_unpacked(plain_logits(logits, g) && target.scalar_type() == at::kLong && beside(target, logits, 0) && floats(saved[2], logits, target.numel()) &&
+                         floats(saved[3], logits, 2 * target.numel()));
         Tensor d[2], d_logits;
         {
             at::AutoGradMode off(false);
@@ -191,8 +203,8 @@ struct Distill : torch::autograd::Function<Distill> {
             const auto saved = unpacked(ctx);  // (refused if an input was changed since, or the graph is freed)
             at::AutoGradMode off(false);
             Geometry g;
-            UNPACKED(fits(saved[0], saved[1], saved[2], saved[3], d["patch"].toInt(), g) && saved[4].device() == saved[0].device() &&
-                     saved[4].scalar_type() == at::kByte && (!made || (d_logits.sizes() == saved[0].sizes() && d_logits.scalar_type() == saved[0].scalar_type())));
+            require_unpacked(fits(saved[0], saved[1], saved[2], saved[3], d["patch"].toInt(), g) && saved[4].device() == saved[0].device() &&
+                             saved[4].scalar_type() == at::kByte && (!made || (d_logits.sizes() == saved[0].sizes() && d_logits.scalar_type() == saved[0].scalar_type())));
             if (!made) d_logits = at::empty(saved[0].sizes(), saved[0].options());
             const Tensor upstream = grads[0].contiguous();
             Distillation{saved[0], saved[1], saved[2], saved[3], saved[4], d["patch"].toInt(), d["temperature"].toDouble(), d["log_probs"].toBool()}.run(
@@ -204,6 +216,16 @@ struct Distill : torch::autograd::Function<Distill> {
     }
 };
 
+// What the library refuses is left to the Python side too, which raises its error.
+template <class F>
+pybind11::object unless_refused(F call) {
+    try {
+        return call();
+    } catch (const Refused&) {
+        return pybind11::none();
+    }
+}
+
 pybind11::object class_log_probs(const Tensor& logits, const Tensor& target, int64_t k, double temperature) {
     Geometry g;
     if (passed_by(logits) || !plain_logits(logits, g) || target.scalar_type() != at::kLong || !beside(target, logits, 0) || k < 0 || k > 64 || k > g.classes || !(temperature > 0) ||
@@ -213,12 +235,14 @@ pybind11::object class_log_probs(const Tensor& logits, const Tensor& target, int
         const auto none = [](const Tensor& t) { return t.defined() ? pybind11::cast(t) : pybind11::none(); };
         return pybind11::make_tuple(a, b, none(c), none(e));
     };
-    if (at::GradMode::is_enabled() && logits.requires_grad()) {
-        const variable_list out = LogProbs::apply(logits, target, k, temperature);
-        return give(out[0], out[1], k ? out[2] : Tensor(), k ? out[3] : Tensor());
-    }
-    const Scores s = scores(logits, g, target, k, temperature, false);
-    return give(s.log_prob, s.entropy, s.top_log_prob, s.top_class);
+    return unless_refused([&]() -> pybind11::object {
+        if (at::GradMode::is_enabled() && logits.requires_grad()) {
+            const variable_list out = LogProbs::apply(logits, target, k, temperature);
+            return give(out[0], out[1], k ? out[2] : Tensor(), k ? out[3] : Tensor());
+        }
+        const Scores s = scores(logits, g, target, k, temperature, false);
+        return give(s.log_prob, s.entropy, s.top_log_prob, s.top_class);
+    });
 }
 
 pybind11::object distill(const Tensor& logits, const Tensor& top_class, const Tensor& top_value, const std::optional<Tensor>& mask_, int64_t patch,
@@ -228,11 +252,13 @@ pybind11::object distill(const Tensor& logits, const Tensor& top_class, const Te
     if (passed_by(logits) || !fits(logits, top_class, top_value, mask, patch, g) || !(temperature > 0) || temperature > 1e30) return pybind11::none();
     const size_t bytes = mmae_distill_workspace_bytes(dtype_code(logits), g.outer, g.classes, g.inner, (int)top_class.size(1));
     const Tensor workspace = at::empty({(int64_t)bytes}, logits.options().dtype(at::kByte).requires_grad(false));
-    if (at::GradMode::is_enabled() && logits.requires_grad())
-        return pybind11::cast(Distill::apply(logits, top_class, top_value, mask_, workspace, patch, temperature, log_probs));
-    const Tensor loss = at::empty({}, logits.options().dtype(at::kFloat).requires_grad(false));
-    Distillation{logits, top_class, top_value, mask, workspace, patch, temperature, log_probs}.run(nullptr, false, false, loss.data_ptr<float>(), nullptr);
-    return pybind11::cast(loss);
+    return unless_refused([&]() -> pybind11::object {
+        if (at::GradMode::is_enabled() && logits.requires_grad())
+            return pybind11::cast(Distill::apply(logits, top_class, top_value, mask_, workspace, patch, temperature, log_probs));
+        const Tensor loss = at::empty({}, logits.options().dtype(at::kFloat).requires_grad(false));
+        Distillation{logits, top_class, top_value, mask, workspace, patch, temperature, log_probs}.run(nullptr, false, false, loss.data_ptr<float>(), nullptr);
+        return pybind11::cast(loss);
+    });
 }
 
 // The gradient that arrives at this loss will be exactly 1.
@@ -246,6 +272,7 @@ bool mark_unit_upstream(const Tensor& loss) {
 }  // namespace
 
 PYBIND11_MODULE(_nodes, m) {
+    error_type = pybind11::object(pybind11::module_::import("multimae_amd._lib").attr("MmaeError")).release().ptr();
     m.def("class_log_probs", &class_log_probs);
     m.def("distill", &distill);
     m.def("mark_unit_upstream", &mark_unit_upstream);

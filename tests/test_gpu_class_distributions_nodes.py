@@ -112,3 +112,22 @@ def test_forward_mode_and_tracing_are_refused(M, profile, monkeypatch):  # noqa:
             with pytest.raises(MmaeError, match="traced"):
                 make_fx(call)(x)
         assert torch.equal(call(z), want)
+
+
+@pytest.mark.parametrize("profile", [None, []], ids=["C++", "Python"])
+def test_what_the_library_refuses_is_an_error_of_the_package(M, profile, monkeypatch):  # noqa: F811
+    """Calls whose tensors fit, refused behind them: a temperature that is zero in fp32; and a saved tensor that came back smaller."""
+    from multimae_amd import ops
+    from multimae_amd._lib import MmaeError
+    monkeypatch.setattr(ops, "PROFILE", profile)
+    t, v = classes((6,), 300, 2), torch.zeros(6, 1, device="cuda")
+    for z in (scores((6, 300), "f32", 1), scores((6, 300), "f32", 1).requires_grad_(True)):
+        with pytest.raises(MmaeError, match="temperature"):
+            M.class_log_probs(z, t, temperature=1e-50)
+        with pytest.raises(MmaeError, match="temperature"):
+            M.MaskedDistillationLoss(temperature=1e-50)(z, (t.view(6, 1), v))
+    with torch.autograd.graph.saved_tensors_hooks(lambda x: x.detach(), lambda x: x[:1]):
+        values = M.class_log_probs(z, t).entropy.sum(), M.MaskedDistillationLoss()(z, (t.view(6, 1), v))
+    for value in values:
+        with pytest.raises(MmaeError):
+            torch.autograd.grad(value, z, torch.tensor(3.0, device="cuda"))
