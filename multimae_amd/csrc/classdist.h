@@ -135,10 +135,12 @@ __device__ __forceinline__ long load_class(const void* p, int bytes, long i) {
     return bytes == 8 ? (long)((const int64_t*)p)[i] : (long)((const int32_t*)p)[i];
 }
 
-// (m, s, t): maximum, sum of 2^d and sum of d 2^d with d = (z - m) * c.  d is bounded below in t, where 0 * -inf would be NaN.
+// (m, s, t): maximum, sum of 2^d and sum of d 2^d with d = (z - m) * c.  Where d stands beside its exponential it is bounded below,
+// as 0 * -inf would be NaN: at -128, since the exponential instruction gives 0 below -126 (and a bound of -10^4 times a large gradient
+// left fp32).
 struct Stats { float m, s, t; };
 __device__ __forceinline__ float finite_ref(float m) { return m == -INFINITY ? 0.f : m; }
-__device__ __forceinline__ float bounded(float d) { return fmaxf(d, -10000.f); }
+__device__ __forceinline__ float bounded(float d) { return fmaxf(d, -128.f); }
 __device__ __forceinline__ Stats join(const Stats& a, const Stats& b, float c) {
     const float m = fmaxf(a.m, b.m), r = finite_ref(m);
     const float da = (a.m - r) * c, db = (b.m - r) * c;

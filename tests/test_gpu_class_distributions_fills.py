@@ -4,7 +4,8 @@ MaskedDistillationLoss against their definitions in 64 bits, in every form of th
 Tolerances as in test_gpu_class_distributions, with the term's roundings counted one by one: log2(e) / T is off by U / 4 and U, the
 multiply-add, the difference and the product with ln 2 by U each, ln 2 itself by less than U / 4, so 5 U of |log p|; log2 s of a row whose reference
 exponent is off by up to 1/2 adds 2 U.  The definitions below subtract the maximum first, of all classes and of those that a
-teacher does not keep: in 64 bits too, -1e30 would swallow the logarithm of the sum beside it."""
+teacher does not keep: in 64 bits too, -1e30 would swallow the logarithm of the sum beside it.  The exponential instruction gives 0 for
+results below 2^-126: a probability there is off by itself, by less than FLUSHED, and its gradient by that times what stands beside it."""
 import math
 
 import pytest
@@ -16,6 +17,7 @@ from tests.test_gpu_class_distributions import M  # noqa: F401  (the fixture)
 pytestmark = pytest.mark.gpu
 
 FILLS = [-1e5, -1e7, -1.2e7, -1e9, -1e10, -1e15, -1e30, -1e37]
+FLUSHED = 2.0 ** -125
 ids = dict(ids=lambda v: f"{v:g}" if isinstance(v, float) else str(v))
 
 
@@ -53,7 +55,8 @@ def check_scores(M, z, target, k, temperature):
     lph = finite + h.unsqueeze(1)
     want = (gl * (hot - p) - gh * p * lph) / temperature
     size = (gl.abs() * hot + p * (gl.abs() + gh.abs() * (lph.abs() + 1 + math.log(c)))) / temperature
-    close(got, want, half_step(z.dtype, want) + size * (2 * CHAIN + 20 * U * (1 + math.log(c))), "grad")
+    flushed = FLUSHED * (gl.abs() + gh.abs() * (lph.abs() + 1)) / temperature
+    close(got, want, half_step(z.dtype, want) + size * (2 * CHAIN + 20 * U * (1 + math.log(c))) + flushed, "grad")
 
 
 def distil(z, cls, val, temperature, log_probs):
@@ -104,8 +107,9 @@ def check_loss(M, z, cls, val, temperature, log_probs):
     c = z.shape[1]
     rel = 2 * CHAIN + 20 * U * (1 + math.log(c)) + (cls.shape[1] + 16) * U
     close(loss, rows.sum(), sizes.sum() * rel, "loss")
-    close(grad, want, half_step(z.dtype, want) + gsize * (rel + 8 * U * 30), "grad")
-    close(scaled, -3 * want, half_step(z.dtype, 3 * want) + 3 * gsize * (rel + 8 * U * 30), "grad, upstream -3")
+    flushed = 2 * FLUSHED * temperature * c / z.numel()  # (of p (Q + r) and of the rest's share)
+    close(grad, want, half_step(z.dtype, want) + gsize * (rel + 8 * U * 30) + flushed, "grad")
+    close(scaled, -3 * want, half_step(z.dtype, 3 * want) + 3 * gsize * (rel + 8 * U * 30) + 3 * flushed, "grad, upstream -3")
 
 
 def filled(shape, dtype, fill, seed):
@@ -196,3 +200,30 @@ def test_maps_in_registers_beside_finite_fills(M, c, dtype, fill):
         z[8, :, 1] = fill                       # (beside ordinary positions of the same wave)
         z[9, :, 2, 3:] = fill
         check_loss(M, z, cls, val, 1.5, log_probs)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("shape", [(7, 700), (7, 3000), (7, 40007), (7, 70, 3, 5), (7, 150, 3, 5), (7, 1700, 3, 5)], ids=str)
+def test_temperatures_far_from_one(M, shape, dtype):
+    """Low ones leave every row beyond the reference exponents' range, high ones make it uniform."""
+    z = scores(shape, dtype, seed=shape[1])
+    target = classes(shape[:1] + shape[2:], shape[1], seed=4)
+    for temperature in (1e-36, 1e-20, 1e-6, 1e-3, 1e6, 1e30):
+        check_scores(M, z, target, 5, temperature)
+    for temperature in (1e-15, 1e-3, 1e6):
+        for log_probs in (False, True):
+            check_loss(M, z, *teacher_top(shape, 6, 5, log_probs, temperature), temperature, log_probs)
+
+
+@pytest.mark.parametrize("shape", [(7, 700), (7, 40007), (7, 70, 3, 5), (7, 1700, 3, 5)], ids=str)
+def test_large_gradients_of_the_entropy(M, shape):
+    """Classes without any probability have no gradient, however large the one that arrives: 1e36 times a bounded logarithm (128 ln 2)
+    is below 3.4e38."""
+    z = filled(shape, "f32", -1e30, 3)
+    leaf = z.clone().requires_grad_(True)
+    out = M.class_log_probs(leaf, torch.zeros_like(z[:, 0], dtype=torch.long))
+    (got,) = torch.autograd.grad(out.entropy, leaf, torch.full_like(out.entropy, 1e36))
+    (unit,) = torch.autograd.grad(M.class_log_probs(leaf, torch.zeros_like(z[:, 0], dtype=torch.long)).entropy, leaf, torch.ones_like(out.entropy))
+    assert torch.isfinite(got).all() and (got[z == -1e30][unit[z == -1e30] == 0] == 0).all()
+    want = unit.double().cpu() * 1e36
+    close(got, want, want.abs() * 64 * U + 1e36 * (2 * CHAIN + 20 * U * (1 + math.log(shape[1]))) * torch.softmax(z.double().cpu(), 1) * (2 + 2 * math.log(shape[1])), "grad")
