@@ -285,6 +285,7 @@ int mmae_masked_ce(const void* logits, int logits_is_bf16, const int64_t* target
  * has log_prob = -inf (at a valid target), entropy 0 and no gradient.  NaN and +inf logits give NaN, as in torch.
  * mmae_class_log_probs_bwd: d_logits (contiguous, the logits' dtype) for the gradients that arrive at log_prob and entropy
  * (either may be NULL).
+ * temperature: positive, from 4.3e-39 on (distillation: its square a normal fp32 number, divided by the positions too).
  * Up to 2^30 classes and 2^31 - 64 positions; a workspace is 0 bytes for sizes that the call refuses. */
 enum { MMAE_DT_F32 = 0, MMAE_DT_BF16 = 1, MMAE_DT_F16 = 2 };
 size_t mmae_class_log_probs_workspace_bytes(int dtype, int outer, int classes, int inner, int top_k);

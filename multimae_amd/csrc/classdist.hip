@@ -1,6 +1,8 @@
 // Class distributions: entry points and the mask's counts.
 #include "classdist.h"
 
+#include <float.h>
+
 namespace classdist {
 namespace {
 
@@ -47,7 +49,8 @@ int check_logits(const char* name, const void* logits, int dtype, int outer, int
     MMAE_REQUIRE(classes <= MOST_CLASSES, MMAE_ESHAPE, "%s: %d classes", name, classes);
     MMAE_REQUIRE((long)outer * inner <= MOST_POSITIONS, MMAE_ESHAPE, "%s: %d x %d positions are more than 2^31 - 64", name, outer, inner);
     MMAE_REQUIRE(ld >= (long)classes * inner, MMAE_ESHAPE, "%s: samples %ld elements apart hold %d x %d values", name, ld, classes, inner);
-    MMAE_REQUIRE(temperature > 0.f && temperature < INFINITY, MMAE_EINVAL, "%s: temperature %g is not positive and finite", name, temperature);
+    MMAE_REQUIRE(temperature > 0.f && temperature < INFINITY && LOG2E / temperature < INFINITY, MMAE_EINVAL,
+                 "%s: temperature %g is not positive and finite, with a finite reciprocal", name, temperature);
     return MMAE_OK;
 }
 
@@ -113,6 +116,9 @@ extern "C" int mmae_distill(const void* logits, int dtype, int outer, int classe
     const int rc = check_logits("distill", logits, dtype, outer, classes, inner, ld, temperature);
     if (rc != MMAE_OK) return rc;
     MMAE_REQUIRE(top_class && top_value && workspace && (loss || d_logits), MMAE_EINVAL, "distill: null pointer");
+    const double square = (double)temperature * temperature;  // (no position weighs less than one of all)
+    MMAE_REQUIRE(square <= FLT_MAX && square / ((double)outer * inner) >= FLT_MIN, MMAE_EINVAL, "distill: the square of temperature %g, or its share of %d x %d positions, is not held in fp32",
+                 temperature, outer, inner);
     MMAE_REQUIRE(class_bytes == 4 || class_bytes == 8, MMAE_EINVAL, "distill: classes of %d bytes", class_bytes);
     MMAE_REQUIRE(value_dtype >= MMAE_DT_F32 && value_dtype <= MMAE_DT_F16, MMAE_EINVAL, "distill: value dtype code %d", value_dtype);
     MMAE_REQUIRE(k >= 1 && k <= MAX_TOP, MMAE_ESHAPE, "distill: %d kept classes, between 1 and %d are taken", k, MAX_TOP);
@@ -128,7 +134,7 @@ extern "C" int mmae_distill(const void* logits, int dtype, int outer, int classe
     a.tok_w = mask ? width / patch : 1;
     a.tokens = mask ? a.tok_w * (inner / width / patch) : 1;
     a.temperature = temperature;
-    a.weight = (float)((double)temperature * temperature / ((double)outer * inner));
+    a.weight = (float)(square / ((double)outer * inner));
     a.valid = ws; a.count = ws + 4; a.part = loss ? ws + 4 + outer : nullptr;
     a.upstream = upstream; a.skip_unit = skip_unit; a.d_logits = d_logits;
     if (mask && !again) {
