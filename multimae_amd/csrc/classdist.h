@@ -135,18 +135,10 @@ __device__ __forceinline__ long load_class(const void* p, int bytes, long i) {
     return bytes == 8 ? (long)((const int64_t*)p)[i] : (long)((const int32_t*)p)[i];
 }
 
-// (m, s, t): maximum, sum of 2^d and sum of d 2^d with d = (z - m) * c.  Where d stands beside its exponential it is bounded below,
-// as 0 * -inf would be NaN: at -128, since the exponential instruction gives 0 below -126 (and a bound of -10^4 times a large gradient
-// left fp32).
-struct Stats { float m, s, t; };
 __device__ __forceinline__ float finite_ref(float m) { return m == -INFINITY ? 0.f : m; }
+// Where d stands beside 2^d it is bounded below, as 0 * -inf would be NaN: at -128, since the exponential instruction gives 0 below -126
+// (and a bound of -10^4 times a large gradient left fp32).
 __device__ __forceinline__ float bounded(float d) { return fmaxf(d, -128.f); }
-__device__ __forceinline__ Stats join(const Stats& a, const Stats& b, float c) {
-    const float m = fmaxf(a.m, b.m), r = finite_ref(m);
-    const float da = (a.m - r) * c, db = (b.m - r) * c;
-    const float fa = exp2_(da), fb = exp2_(db);
-    return {m, a.s * fa + b.s * fb, fa * (a.t + bounded(da) * a.s) + fb * (b.t + bounded(db) * b.s)};
-}
 
 struct Geometry {
     const void* logits;
@@ -157,21 +149,6 @@ struct Geometry {
     __device__ __forceinline__ float log_p(float z, float m, float l2) const { return (z - m) * inv_t - l2 * LN2; }
     __device__ __forceinline__ long base(long p) const { return inner == 1 ? p * ld : (p / inner) * ld + p % inner; }
 };
-
-__device__ Stats block_stats(Stats v, float c, Stats* red) {
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) {
-        const Stats w = {__shfl_xor(v.m, o, 64), __shfl_xor(v.s, o, 64), __shfl_xor(v.t, o, 64)};
-        v = join(v, w, c);
-    }
-    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, nw = (blockDim.x + 63) >> 6;
-    __syncthreads();
-    if (lane == 0) red[w] = v;
-    __syncthreads();
-    Stats r = red[0];
-    for (int i = 1; i < nw; ++i) r = join(r, red[i], c);
-    return r;
-}
 
 // Sums in the base-2 domain against a reference exponent R: s = sum 2^(z c - R), t = sum (z c - R) 2^(z c - R), m = max z.
 // z c - R is one fused multiply-add without intermediate overflow.  R = m c, held to +-FAR, is a rounded number, and the multiply-add
@@ -298,61 +275,6 @@ __device__ __forceinline__ Kept load_kept(const DistillArgs& a, long p, int lane
     float v;
     read_kept(a, p, lane, cls, v);
     return kept_share(a, cls, v);
-}
-
-// One position, any layout, by a whole workgroup: class after class from memory, differences (z - m) c.  Returns its weighted loss
-// (in the first wave).
-template <class T>
-__device__ float distill_position(const DistillArgs& a, long p, float w, Stats* red, int* s_cls, float* s_q, float* s_tot) {
-    const typename T::E* z = (const typename T::E*)a.g.logits;
-    const long base = a.g.base(p), cs = a.g.inner;
-    const int C = a.g.classes, lane = threadIdx.x & 63;
-    const float c = a.g.c;
-    typename T::E* dz = (typename T::E*)a.d_logits;
-    const long out = a.g.inner == 1 ? p * C : (p / a.g.inner) * C * cs + p % a.g.inner;
-    Kept e = {};
-    __syncthreads();
-    if (threadIdx.x < 64) {
-        e = load_kept(a, p, lane);
-        s_cls[lane] = e.cls;
-        s_q[lane] = e.q;
-        if (lane == 0) { s_tot[0] = e.total; s_tot[1] = e.rest; }
-    }
-    __syncthreads();
-    Stats v = {-INFINITY, 0.f, 0.f}, u = {-INFINITY, 0.f, 0.f};  // all classes; the ones not kept
-    for (int j = threadIdx.x; j < C; j += blockDim.x) {
-        const float x = T::up(z[base + j * cs]);
-        bool kept = !a.log_probs;
-        for (int i = 0; i < a.k && !kept; ++i) kept = s_cls[i] == j;
-        v = join(v, Stats{x, x == -INFINITY ? 0.f : 1.f, 0.f}, c);
-        if (!kept) u = join(u, Stats{x, x == -INFINITY ? 0.f : 1.f, 0.f}, c);
-    }
-    v = block_stats(v, c, red);
-    u = block_stats(u, c, red);
-    const bool empty = v.m == -INFINITY && v.s == 0.f;
-    const float m = finite_ref(v.m), l2 = empty ? 0.f : log2_(v.s);
-    const float um = finite_ref(u.m), ul2 = log2_(u.s);
-    const float rest = u.s != 0.f ? s_tot[1] : 0.f, Q = s_tot[0] + rest;
-    float l = 0.f;
-    if (threadIdx.x < 64) {
-        if (e.q != 0.f) l = e.q * (e.lq - a.g.log_p(T::up(z[base + e.cls * cs]), m, l2));
-        l = wave_sum(l);
-        if (rest != 0.f) l += rest * ((log2_(rest) - (ul2 - l2)) * LN2 - (um - m) * a.g.inv_t);
-        l *= w;
-    }
-    if (!dz) return l;
-    const float gs = empty ? 0.f : w * a.g.inv_t * (a.upstream ? a.upstream[0] : 1.f);
-    for (int j = threadIdx.x; j < C; j += blockDim.x) {
-        const float x = T::up(z[base + j * cs]);
-        float q = 0.f;
-        bool kept = false;
-        for (int i = 0; i < a.k; ++i)
-            if (s_cls[i] == j) { q += s_q[i]; kept = true; }
-        float d = exp2_((x - m) * c - l2) * Q - q;
-        if (!kept && rest != 0.f) d -= rest * exp2_((x - um) * c - ul2);
-        dz[out + j * cs] = T::down(gs * d);
-    }
-    return l;
 }
 
 // ---- maps: a lane per position ------------------------------------------------------------------------------------------

@@ -349,9 +349,6 @@ template <> struct Bits<F32> { typedef uint32_t U; };
 template <class T, bool REST>
 __global__ __launch_bounds__(1024) void distill_map_kernel(DistillArgs a, int tiles) {
     extern __shared__ __align__(16) char smem[];
-    __shared__ Stats red_far[16];
-    __shared__ int far_cls[MAX_TOP];
-    __shared__ float far_q[MAX_TOP], far_tot[2];
     __shared__ uint64_t s_far;
     if (a.upstream && a.skip_unit && a.upstream[0] == 1.f) return;
     typedef typename T::E E;
@@ -423,8 +420,10 @@ __global__ __launch_bounds__(1024) void distill_map_kernel(DistillArgs a, int ti
     }
     s_sums[wave * POS + lane] = v;
     __syncthreads();
+    Sums rest = {};
+    bool far = false;
     if (wave == 0) {
-        Sums rest = s_sums[lane];
+        rest = s_sums[lane];
         for (int i = 1; i < waves; ++i) rest = join(rest, s_sums[i * POS + lane]);
         v = rest;  // the whole position
         if (REST)
@@ -438,27 +437,57 @@ __global__ __launch_bounds__(1024) void distill_map_kernel(DistillArgs a, int ti
         const float l2 = empty ? INFINITY : log2_(v.s);
         const float r = REST && rest.s != 0.f ? left : 0.f, Q = total + r;
         const float gs = empty ? 0.f : w * a.g.inv_t * (a.upstream ? a.upstream[0] : 1.f);
-        const bool far = w != 0.f && (is_far(v.m, c) || (REST && is_far(rest.m, c)));
+        far = w != 0.f && (is_far(v.m, c) || (REST && is_far(rest.m, c)));
         const uint64_t fars = __ballot(far);
+        const float share_log_q = loss;
         for (int i = 0; i < k; ++i) {
             const int cls = s_cls[i * POS + lane];
-            if (cls < 0) continue;
+            if (cls < 0 || far) continue;
             const float q = s_q[i * POS + lane], x = s_z[i * POS + lane];
             if (q != 0.f) loss -= q * row_log_p(a.g, x, v.m, l2);
             s_q[i * POS + lane] = w != 0.f ? gs * (exp2_(__builtin_fmaf(x, c, -v.R) - l2) * Q - q) : 0.f;
         }
         if (r != 0.f) loss += r * (log2_(r) - ((rest.R - v.R) + log2_(rest.s) - l2)) * LN2;
-        loss = w != 0.f && !far ? w * loss : 0.f;
-        loss = wave_sum(loss);
+        const float sum = wave_sum(w != 0.f && !far ? w * loss : 0.f);
         if (lane == 0) {
             s_far = fars;
-            if (a.part) a.part[blockIdx.x] = loss;
+            if (a.part) a.part[blockIdx.x] = sum;
         }
+        loss = share_log_q;
         s_F[lane] = w != 0.f ? gs * (Q * exp2_(rest.R - v.R - l2) - (r != 0.f ? r / rest.s : 0.f)) : 0.f;
-        s_R[lane] = rest.R;
+        s_R[lane] = far ? (rest.m == -INFINITY ? finite_ref(v.m) : rest.m) : rest.R;
     }
     __syncthreads();
     const uint64_t fars = s_far;
+    if (fars) {  // positions beyond FAR: the sums anew, by differences to the maximum of the tile's classes, which R holds there
+        const float um = s_R[lane];
+        float s = 0.f;
+        for (int j = c0; j < c1; ++j) s += exp2_((T::up(tile[j * POS + lane]) - um) * c);
+        s_sums[wave * POS + lane].s = s;
+        __syncthreads();
+        if (wave == 0) {
+            for (int i = 1; i < waves; ++i) s += s_sums[i * POS + lane].s;
+            const float m = finite_ref(v.m), apart = (um - m) * c;
+            float all = s * exp2_(apart);
+            if (REST)
+                for (int i = 0; i < k; ++i)
+                    if (s_cls[i * POS + lane] >= 0) all += exp2_((s_z[i * POS + lane] - m) * c);
+            if (v.m == INFINITY) all = __builtin_nanf("");
+            const float l2 = log2_(all), r = REST && s != 0.f ? left : 0.f, Q = total + r;  // (not empty: a maximum is finite)
+            const float gs = w * a.g.inv_t * (a.upstream ? a.upstream[0] : 1.f);
+            for (int i = 0; i < k; ++i) {
+                if (s_cls[i * POS + lane] < 0 || !far) continue;
+                const float q = s_q[i * POS + lane], x = s_z[i * POS + lane];
+                if (q != 0.f) loss -= q * a.g.log_p(x, m, l2);
+                s_q[i * POS + lane] = gs * (exp2_((x - m) * c - l2) * Q - q);
+            }
+            if (r != 0.f) loss += r * ((log2_(r) - (log2_(s) - l2)) * LN2 - (um - m) * a.g.inv_t);
+            loss = wave_sum(far ? w * loss : 0.f);
+            if (lane == 0 && a.part) a.part[blockIdx.x] += loss;
+            if (far) s_F[lane] = gs * (Q * exp2_(apart - l2) - (r != 0.f ? r / s : 0.f));
+        }
+        __syncthreads();
+    }
     if (a.d_logits) {
         const int px = threadIdx.x % PPR * VEC;  // (the workgroup's size is a multiple of PPR)
         float F[VEC], R[VEC];
@@ -469,8 +498,10 @@ __global__ __launch_bounds__(1024) void distill_map_kernel(DistillArgs a, int ti
             float o[VEC];
 #pragma unroll
             for (int e = 0; e < VEC; ++e) {  // (outside the loss a logit may be anything)
-                const float d = F[e] * exp2_(__builtin_fmaf(T::get(q, e), c, -R[e]));
-                o[e] = F[e] != 0.f ? d : 0.f;
+                const float x = T::get(q, e);
+                float d = __builtin_fmaf(x, c, -R[e]);
+                if (fars && (fars >> (px + e) & 1)) d = (x - R[e]) * c;
+                o[e] = F[e] != 0.f ? F[e] * exp2_(d) : 0.f;
             }
             *(Piece*)(tile + (size_t)id * VEC) = T::pack(o);
         }
@@ -482,12 +513,6 @@ __global__ __launch_bounds__(1024) void distill_map_kernel(DistillArgs a, int ti
         __syncthreads();
         for (int id = threadIdx.x; id < C * PPR; id += blockDim.x)
             store_positions<T>(dz + (long)(id / PPR) * inner, id % PPR * VEC, n, *(const Piece*)(tile + (size_t)id * VEC));
-    }
-    for (uint64_t f = fars; f; f &= f - 1) {
-        const long at = (long)b * inner + i0 + __builtin_ctzll(f);
-        __syncthreads();
-        const float x = distill_position<T>(a, at, position_weight(a, at), red_far, far_cls, far_q, far_tot);
-        if (threadIdx.x == 0 && a.part) a.part[blockIdx.x] += x;
     }
 }
 
@@ -786,50 +811,65 @@ __global__ __launch_bounds__(64, 2) void distill_map_regs_kernel(DistillArgs a, 
             const float one[1] = {s_z[i * POS]};
             add_logits<1, false>(v, one, c);
         }
-    // A wave with a position beyond FAR goes by (z - m) c, class after class from memory, and with a rest by its own maximum.
-    const bool far = __any(is_far(v.m, c) || (REST && is_far(rest.m, c)));
-    const float m = finite_ref(v.m), rest_m = finite_ref(rest.m);
-    if (far) {
-        rest.s = v.s = 0.f;
-        for (int j = 0; j < C; ++j) {
-            const float one = T::up(z[(long)j * inner + px]);
-            v.s += exp2_((one - m) * c);
-            if (!REST) continue;
-            bool out = true;
-            for (int i = 0; i < k; ++i)
-                if (s_cls[i * POS] >= 0 && (s_cls[i * POS] & 0xffff) == j) out = false;
-            if (out) rest.s += exp2_((one - rest_m) * c);
+    // A wave with a position beyond FAR goes by differences to the two maxima, class after class from memory.
+    if (__any(is_far(v.m, c) || (REST && is_far(rest.m, c)))) {
+        const float m = finite_ref(v.m), rest_m = finite_ref(rest.m);
+        auto each = [&](auto take) {  // (class, logit, whether it is kept)
+            for (int j0 = 0; j0 < C; j0 += 8) {
+                float one[8];
+#pragma unroll
+                for (int u = 0; u < 8; ++u) one[u] = T::up(z[(long)(j0 + u < C ? j0 + u : C - 1) * inner + px]);
+                uint32_t word = kept[0];
+#pragma unroll
+                for (int u = 1; u < WORDS; ++u) word = j0 / 32 == u ? kept[u] : word;
+#pragma unroll
+                for (int u = 0; u < 8; ++u)
+                    if (j0 + u < C) take(j0 + u, one[u], word >> ((j0 + u) & 31) & 1);
+            }
+        };
+        float all = 0.f, out = 0.f;
+        each([&](int, float one, uint32_t is_kept) {
+            all += exp2_((one - m) * c);
+            if (REST && !is_kept) out += exp2_((one - rest_m) * c);
+        });
+        if (v.m == INFINITY) all = __builtin_nanf("");
+        const bool empty = v.m == -INFINITY && all == 0.f;
+        const float l2 = empty ? 0.f : log2_(all), out_l2 = log2_(out), r = out != 0.f ? left : 0.f, Q = total + r;
+        const float gs = empty ? 0.f : w * a.g.inv_t * (a.upstream ? a.upstream[0] : 1.f);
+#pragma unroll 1
+        for (int i = 0; i < places; ++i) {
+            const float q = s_d[i * POS], zk = s_z[i * POS];
+            if (q != 0.f) loss -= q * a.g.log_p(zk, m, l2);
+            s_d[i * POS] = w != 0.f ? gs * (exp2_((zk - m) * c - l2) * Q - q) : 0.f;
         }
+        if (r != 0.f) loss += r * ((log2_(r) - (out_l2 - l2)) * LN2 - (rest_m - m) * a.g.inv_t);
+        loss = wave_sum(w != 0.f ? w * loss : 0.f);
+        if (lane == 0 && a.part) a.part[blockIdx.x] = loss;
+        if (!write) return;
+        each([&](int j, float one, uint32_t) {
+            const float d = exp2_((one - m) * c - l2) * Q - (r != 0.f ? r * exp2_((one - rest_m) * c - out_l2) : 0.f);
+            dz[(long)j * inner + px] = T::down(w != 0.f ? gs * d : 0.f);  // (outside the loss a logit may be anything)
+        });
+        for (int i = 0; i < k; ++i)
+            if (s_cls[i * POS] >= 0) dz[(long)(s_cls[i * POS] & 0xffff) * inner + px] = T::down(s_d[(s_cls[i * POS] >> 16) * POS]);
+        return;
     }
     if (v.m == INFINITY) v.s = __builtin_nanf("");
     const bool empty = v.m == -INFINITY && v.s == 0.f;
-    const float own_l2 = empty ? INFINITY : log2_(v.s);  // relative to what the sums are relative to, and to R
-    const float l2 = far && !is_far(v.m, c) ? own_l2 + __builtin_fmaf(m, c, -v.R) : own_l2;
+    const float l2 = empty ? INFINITY : log2_(v.s);
     const float r = REST && rest.s != 0.f ? left : 0.f, Q = total + r;
     const float gs = empty ? 0.f : w * a.g.inv_t * (a.upstream ? a.upstream[0] : 1.f);
 #pragma unroll 1
     for (int i = 0; i < places; ++i) {
         const float q = s_d[i * POS], zk = s_z[i * POS];
         if (q != 0.f) loss -= q * row_log_p(a.g, zk, v.m, l2);
-        const float d = far ? (zk - m) * c : __builtin_fmaf(zk, c, -v.R);
-        s_d[i * POS] = w != 0.f ? gs * (exp2_(d - own_l2) * Q - q) : 0.f;
+        s_d[i * POS] = w != 0.f ? gs * (exp2_(__builtin_fmaf(zk, c, -v.R) - l2) * Q - q) : 0.f;
     }
-    const float rest_l2 = log2_(rest.s);
-    if (r != 0.f) loss += far ? r * ((log2_(r) - (rest_l2 - own_l2)) * LN2 - (rest_m - m) * a.g.inv_t) : r * (log2_(r) - ((rest.R - v.R) + rest_l2 - own_l2)) * LN2;
+    if (r != 0.f) loss += r * (log2_(r) - ((rest.R - v.R) + log2_(rest.s) - l2)) * LN2;
     loss = wave_sum(w != 0.f ? w * loss : 0.f);
     if (lane == 0 && a.part) a.part[blockIdx.x] = loss;
     if (!write) return;
-    if (far) {
-        for (int j = 0; j < C; ++j) {
-            const float one = T::up(z[(long)j * inner + px]);
-            const float d = exp2_((one - m) * c - own_l2) * Q - (r != 0.f ? r * exp2_((one - rest_m) * c - rest_l2) : 0.f);
-            dz[(long)j * inner + px] = T::down(w != 0.f ? gs * d : 0.f);  // (outside the loss a logit may be anything)
-        }
-        for (int i = 0; i < k; ++i)
-            if (s_cls[i * POS] >= 0) dz[(long)(s_cls[i * POS] & 0xffff) * inner + px] = T::down(s_d[(s_cls[i * POS] >> 16) * POS]);
-        return;
-    }
-    const float F = w != 0.f ? gs * (Q * exp2_(rest.R - v.R - own_l2) - (r != 0.f ? r / rest.s : 0.f)) : 0.f;
+    const float F = w != 0.f ? gs * (Q * exp2_(rest.R - v.R - l2) - (r != 0.f ? r / rest.s : 0.f)) : 0.f;
     Global<E>* row = (Global<E>*)dz;
     const float* at = s_d;
 #pragma unroll

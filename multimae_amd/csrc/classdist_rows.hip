@@ -568,6 +568,113 @@ __device__ __forceinline__ RowResult join_row(const DistillArgs& a, long p, floa
     return {gs * (Q * exp2_(rest.R - v.R - l2) - (r != 0.f ? r / rest.s : 0.f)), rest.R, is_far(v.m, c) || (a.log_probs && is_far(rest.m, c))};
 }
 
+template <class T>
+__device__ __forceinline__ Piece load_some(const typename T::E* z, int n) {  // the first n elements
+    if (n == T::VEC) return load_piece<T>(z);
+    Piece q = {};
+#pragma unroll
+    for (int e = 0; e < T::VEC; ++e)
+        if (e < n) T::put(q, e, T::up(z[e]));
+    return q;
+}
+// A row beyond FAR, or whose classes that are not kept are, by a whole workgroup and differences to the two maxima: three passes over
+// memory.  A bit per class modulo 1024 says which classes to look for among the kept ones.  Returns the row's weighted loss (in the first
+// wave).  4096 x 32000 bf16, only the 8 kept classes not switched off: 624 us (140 us within FAR).
+struct FarRoom { uint32_t bits[32]; float red[2][16]; };
+template <class T>
+__device__ __forceinline__ float far_row(const DistillArgs& a, long p, float w, FarRoom& room, int* s_cls, float* s_q, float* s_tot) {
+    const int C = a.g.classes, lane = threadIdx.x & 63, nw = blockDim.x >> 6;
+    const float c = a.g.c;
+    const typename T::E* z = (const typename T::E*)a.g.logits + p * a.g.ld;
+    typename T::E* dz = (typename T::E*)a.d_logits + p * C;
+    Kept e = {};
+    __syncthreads();
+    if (threadIdx.x < 64) {
+        e = load_kept(a, p, lane);
+        s_cls[lane] = e.cls;
+        s_q[lane] = e.q;
+        if (lane == 0) { s_tot[0] = e.total; s_tot[1] = e.rest; }
+        if (lane < 32) room.bits[lane] = 0;
+        if (e.cls >= 0) atomicOr(&room.bits[e.cls >> 5 & 31], 1u << (e.cls & 31));
+    }
+    __syncthreads();
+    auto maybe = [&](int j) __attribute__((always_inline)) { return (room.bits[j >> 5 & 31] >> (j & 31) & 1) != 0; };
+    auto kept = [&](int j) __attribute__((always_inline)) {
+        if (!maybe(j)) return false;
+        for (int i = 0; i < a.k; ++i)
+            if (s_cls[i] == j) return true;
+        return false;
+    };
+    const int first = threadIdx.x * T::VEC, step = blockDim.x * T::VEC;
+    float m = -INFINITY, um = -INFINITY;  // of all classes; of those not kept
+    for (int j = first; j < C; j += step) {
+        const int n = C - j < T::VEC ? C - j : T::VEC;
+        const Piece q = load_some<T>(z + j, n);
+#pragma unroll
+        for (int i = 0; i < T::VEC; ++i) {
+            const float x = i < n ? T::get(q, i) : -INFINITY;
+            m = fmaxf(m, x);
+            if (a.log_probs && !kept(j + i)) um = fmaxf(um, x);
+        }
+    }
+    m = wave_max(m);
+    um = wave_max(um);
+    if (lane == 0) { room.red[0][threadIdx.x >> 6] = m; room.red[1][threadIdx.x >> 6] = um; }
+    __syncthreads();
+    for (int i = 0; i < nw; ++i) { m = fmaxf(m, room.red[0][i]); um = fmaxf(um, room.red[1][i]); }
+    const bool nothing = m == -INFINITY;
+    m = finite_ref(m);
+    um = finite_ref(um);
+    float s = 0.f, us = 0.f;
+    for (int j = first; j < C; j += step) {
+        const int n = C - j < T::VEC ? C - j : T::VEC;
+        const Piece q = load_some<T>(z + j, n);
+#pragma unroll
+        for (int i = 0; i < T::VEC; ++i) {
+            const float x = i < n ? T::get(q, i) : -INFINITY;
+            s += exp2_((x - m) * c);
+            if (a.log_probs && !kept(j + i)) us += exp2_((x - um) * c);
+        }
+    }
+    s = block_sum(s, room.red[0]);
+    us = block_sum(us, room.red[1]);
+    const bool empty = nothing && s == 0.f;
+    const float l2 = empty ? 0.f : log2_(s), ul2 = log2_(us);
+    const float rest = us != 0.f ? s_tot[1] : 0.f, Q = s_tot[0] + rest;
+    float l = 0.f;
+    if (threadIdx.x < 64) {
+        if (e.q != 0.f) l = e.q * (e.lq - a.g.log_p(T::up(z[e.cls]), m, l2));
+        l = wave_sum(l);
+        if (rest != 0.f) l += rest * ((log2_(rest) - (ul2 - l2)) * LN2 - (um - m) * a.g.inv_t);
+        l *= w;
+    }
+    if (!a.d_logits) return l;
+    const float gs = empty ? 0.f : w * a.g.inv_t * (a.upstream ? a.upstream[0] : 1.f);
+    for (int j = first; j < C; j += step) {
+        const int n = C - j < T::VEC ? C - j : T::VEC;
+        const Piece q = load_some<T>(z + j, n);
+        float o[T::VEC];
+#pragma unroll
+        for (int i = 0; i < T::VEC; ++i) {
+            const float x = T::get(q, i);
+            float share = 0.f;
+            bool is_kept = false;
+            if (maybe(j + i))
+                for (int e = 0; e < a.k; ++e)
+                    if (s_cls[e] == j + i) { share += s_q[e]; is_kept = true; }
+            float d = exp2_((x - m) * c - l2) * Q - share;
+            if (!is_kept && rest != 0.f) d -= rest * exp2_((x - um) * c - ul2);
+            o[i] = gs * d;
+        }
+        if (n == T::VEC) store_piece<T>(dz + j, T::pack(o));
+        else
+#pragma unroll
+            for (int i = 0; i < T::VEC; ++i)
+                if (i < n) dz[j + i] = T::down(o[i]);
+    }
+    return l;
+}
+
 template <class T, int NT>
 __device__ __forceinline__ void zero_row(typename T::E* dz, int first, int end) {
     for (int j = first + (int)threadIdx.x * T::VEC; j < end; j += NT * T::VEC) {
@@ -603,11 +710,11 @@ __device__ __forceinline__ float uniform(float v) { return __uint_as_float(__bui
 // A row held in the registers of one workgroup: read once, its gradient written once.  Several workgroups a CU overlap one row's
 // loads with another's stores: 8192 x 32000 fp32 419 us (5.0 TB/s).
 template <class T, int NT, int NV>
-__global__ __launch_bounds__(NT) void distill_rows_kernel(DistillArgs a) {
+__global__ __launch_bounds__(NT, 8) void distill_rows_kernel(DistillArgs a) {
     constexpr int VEC = T::VEC;
     __shared__ __align__(16) uint32_t flags[NT * NV / 4];  // a byte per piece: which of its elements are kept classes
     __shared__ Sums red[NT / 64];
-    __shared__ Stats red_far[NT / 64];
+    __shared__ FarRoom far_room;
     __shared__ int s_cls[MAX_TOP];
     __shared__ float s_d[MAX_TOP], s_row[2];
     __shared__ int s_far;
@@ -661,7 +768,7 @@ __global__ __launch_bounds__(NT) void distill_rows_kernel(DistillArgs a) {
     }
     __syncthreads();
     if (s_far) {
-        const float x = distill_position<T>(a, p, w, red_far, s_cls, s_d, s_row);
+        const float x = far_row<T>(a, p, w, far_room, s_cls, s_d, s_row);
         if (threadIdx.x == 0 && a.part) a.part[p] = x;
         return;
     }
@@ -847,13 +954,13 @@ __global__ __launch_bounds__(NT, long_waves(NT, NV)) void distill_long_rows_kern
 // long rows' pieces).
 template <class T>
 __global__ __launch_bounds__(256) void distill_far_rows_kernel(DistillArgs a, const RowNote* notes) {
-    __shared__ Stats red[4];
+    __shared__ FarRoom room;
     __shared__ int s_cls[MAX_TOP];
     __shared__ float s_q[MAX_TOP], s_tot[2];
     if (a.upstream && a.skip_unit && a.upstream[0] == 1.f) return;
     const long p = blockIdx.x;
     if (!notes[p].far) return;
-    const float x = distill_position<T>(a, p, position_weight(a, p), red, s_cls, s_q, s_tot);
+    const float x = far_row<T>(a, p, position_weight(a, p), room, s_cls, s_q, s_tot);
     if (threadIdx.x == 0 && a.part) a.part[p] = x;
 }
 
@@ -910,9 +1017,9 @@ __global__ __launch_bounds__(NT) void distill_slices_kernel(DistillArgs a, int s
 
 // Second pass: the gradient, a tile per workgroup; the first tile's workgroup writes the row's loss.
 template <class T, int NT, int NV>
-__global__ __launch_bounds__(NT) void distill_tiles_kernel(DistillArgs a, int tiles, int slices, const Sums* parts) {
+__global__ __launch_bounds__(NT, 8) void distill_tiles_kernel(DistillArgs a, int tiles, int slices, const Sums* parts) {
     constexpr int VEC = T::VEC, TILE = NT * NV * VEC;
-    __shared__ Stats red_far[NT / 64];
+    __shared__ FarRoom far_room;
     __shared__ int s_cls[MAX_TOP];
     __shared__ float s_d[MAX_TOP], s_row[2];
     __shared__ int s_far;
@@ -946,7 +1053,7 @@ __global__ __launch_bounds__(NT) void distill_tiles_kernel(DistillArgs a, int ti
     __syncthreads();
     if (s_far) {
         if (tile == 0) {
-            const float x = distill_position<T>(a, p, w, red_far, s_cls, s_d, s_row);
+            const float x = far_row<T>(a, p, w, far_room, s_cls, s_d, s_row);
             if (threadIdx.x == 0 && a.part) a.part[p] = x;
         }
         return;

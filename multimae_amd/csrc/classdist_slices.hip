@@ -170,12 +170,11 @@ __global__ __launch_bounds__(256) void log_probs_map_merge_kernel(LogProbArgs a,
 // position joins them, adds the kept classes and leaves the factors of the gradient; then the gradient, slice by slice.
 constexpr int SLICE_BYTES = 64 * 1024, MOST_WIDTH = SLICE_BYTES / (POS * 2);  // a CU holds two such tiles
 
-struct SliceNotes {  // per position: gradient = F 2^(x c - R) where not kept; the kept classes' gradients beside
-    float *F, *R;
+struct SliceNotes {  // per position: gradient = F 2^(x c - R) where not kept (2^((x - m) c) where m is a number: beyond FAR); the kept classes' beside
+    float *F, *R, *m;
     int* cls;   // [k][positions], -1: none
     float* g;
 };
-__device__ __forceinline__ bool settled(float R) { return R != R; }  // the position's gradient is written
 
 __device__ __forceinline__ bool skip_call(const DistillArgs& a) { return a.upstream && a.skip_unit && a.upstream[0] == 1.f; }
 
@@ -221,9 +220,6 @@ __global__ __launch_bounds__(256) void distill_map_sums_kernel(DistillArgs a, in
 template <class T>
 __global__ __launch_bounds__(64) void distill_map_join_kernel(DistillArgs a, int tiles, int count, const Sums* sums, SliceNotes notes) {
     extern __shared__ int s_cls[];  // [k][POS], then q (later the gradient) and the student's logits alike
-    __shared__ Stats red_far[4];
-    __shared__ int far_cls[MAX_TOP];
-    __shared__ float far_q[MAX_TOP], far_tot[2];
     if (skip_call(a)) return;
     const int inner = a.g.inner, k = a.k, lane = threadIdx.x;
     const int b = blockIdx.x / tiles, i0 = blockIdx.x % tiles * POS, n = inner - i0 < POS ? inner - i0 : POS;
@@ -256,38 +252,57 @@ __global__ __launch_bounds__(64) void distill_map_join_kernel(DistillArgs a, int
                 break;
             }
     }
-    const Sums rest = join_slices(sums + p, count, positions);
+    Sums rest = join_slices(sums + p, count, positions);
     Sums v = rest;
     for (int e = 0; e < k; ++e)
         if (s_cls[e * POS + lane] >= 0) {
             const float x[1] = {s_z[e * POS + lane]};
             add_logits<1, false>(v, x, c);
         }
+    // Beyond FAR, of all classes or of those not kept: the sums anew, by differences to the latter's maximum, class after class from memory.
+    const bool far = w != 0.f && (is_far(v.m, c) || (a.log_probs && is_far(rest.m, c)));
+    const float top = finite_ref(v.m), rest_m = rest.m == -INFINITY ? top : rest.m, apart = (rest_m - top) * c;
+    if (__any(far)) {
+        float s = 0.f;
+        for (int j0 = 0; j0 < a.g.classes; j0 += U) {
+            float x[U];
+#pragma unroll
+            for (int u = 0; u < U; ++u) x[u] = T::up(z[(long)(j0 + u < a.g.classes ? j0 + u : a.g.classes - 1) * inner]);
+            uint32_t out = a.g.classes - j0 < U ? (1u << (a.g.classes - j0)) - 1 : (1u << U) - 1;
+            for (int e = 0; e < k; ++e) {
+                const unsigned at = s_cls[e * POS + lane] - j0;
+                out &= ~(at < U ? 1u << at : 0u);
+            }
+            float s8 = 0.f;
+#pragma unroll
+            for (int u = 0; u < U; ++u) s8 += out >> u & 1 ? exp2_((x[u] - rest_m) * c) : 0.f;
+            s += s8;
+        }
+        float all = s * exp2_(apart);
+        for (int e = 0; e < k; ++e)
+            if (s_cls[e * POS + lane] >= 0) all += exp2_((s_z[e * POS + lane] - top) * c);
+        if (far) { rest.s = s; v.s = all; }
+    }
     if (v.m == INFINITY) v.s = __builtin_nanf("");
     const bool empty = v.m == -INFINITY && v.s == 0.f;
     const float l2 = empty ? INFINITY : log2_(v.s);
     const float r = a.log_probs && rest.s != 0.f ? left : 0.f, Q = total + r;
     const float gs = empty ? 0.f : w * a.g.inv_t * (a.upstream ? a.upstream[0] : 1.f);
-    const bool far = w != 0.f && (is_far(v.m, c) || (a.log_probs && is_far(rest.m, c)));
     for (int e = 0; e < k; ++e) {
-        int cls = s_cls[e * POS + lane];
+        const int cls = s_cls[e * POS + lane];
         const float q = s_q[e * POS + lane], x = s_z[e * POS + lane];
-        if (cls >= 0 && q != 0.f) loss -= q * row_log_p(a.g, x, v.m, l2);
+        if (cls >= 0 && q != 0.f) loss -= q * (far ? a.g.log_p(x, top, l2) : row_log_p(a.g, x, v.m, l2));
         if (a.d_logits && lane < n) {
-            notes.cls[e * positions + p] = w != 0.f && !far ? cls : -1;
-            notes.g[e * positions + p] = gs * (exp2_(__builtin_fmaf(x, c, -v.R) - l2) * Q - q);
+            notes.cls[e * positions + p] = w != 0.f ? cls : -1;
+            notes.g[e * positions + p] = gs * (exp2_((far ? (x - top) * c : __builtin_fmaf(x, c, -v.R)) - l2) * Q - q);
         }
     }
-    if (r != 0.f) loss += r * (log2_(r) - ((rest.R - v.R) + log2_(rest.s) - l2)) * LN2;
-    loss = wave_sum(w != 0.f && !far ? w * loss : 0.f);
+    if (r != 0.f) loss += far ? r * ((log2_(r) - (log2_(rest.s) - l2)) * LN2 - (rest_m - top) * a.g.inv_t) : r * (log2_(r) - ((rest.R - v.R) + log2_(rest.s) - l2)) * LN2;
+    loss = wave_sum(w != 0.f ? w * loss : 0.f);
     if (a.d_logits && lane < n) {
-        notes.F[p] = w != 0.f ? gs * (Q * exp2_(rest.R - v.R - l2) - (r != 0.f ? r / rest.s : 0.f)) : 0.f;
-        notes.R[p] = far ? __builtin_nanf("") : rest.R;
-    }
-    for (uint64_t f = __ballot(far); f; f &= f - 1) {
-        const long at = (long)b * inner + i0 + __builtin_ctzll(f);
-        __syncthreads();
-        loss += distill_position<T>(a, at, position_weight(a, at), red_far, far_cls, far_q, far_tot);
+        notes.F[p] = w != 0.f ? gs * (Q * exp2_((far ? apart : rest.R - v.R) - l2) - (r != 0.f ? r / rest.s : 0.f)) : 0.f;
+        notes.R[p] = rest.R;
+        notes.m[p] = far ? rest_m : __builtin_nanf("");
     }
     if (lane == 0 && a.part) a.part[blockIdx.x] = loss;
 }
@@ -301,8 +316,8 @@ __global__ __launch_bounds__(256) void distill_map_gradient_kernel(DistillArgs a
     const long p = (long)b * inner + i, positions = (long)a.g.outer * inner;
     const float w = position_weight(a, p), c = a.g.c;
     const bool any = __any(w != 0.f);  // (the same in every wave; else the notes are not written)
-    const float F = any ? notes.F[p] : 0.f, R = any ? notes.R[p] : 0.f;
-    const bool mine = lane < n && !settled(R);
+    const float F = any ? notes.F[p] : 0.f, R = any ? notes.R[p] : 0.f, m = any ? notes.m[p] : __builtin_nanf("");
+    const bool mine = lane < n, far = m == m, any_far = __any(far);
     const typename T::E* z = (const typename T::E*)a.g.logits + b * a.g.ld + (long)first * inner + i;
     typename T::E* dz = (typename T::E*)a.d_logits + ((long)b * a.g.classes + first) * inner + i;
     const int c0 = C * wave / 4, c1 = C * (wave + 1) / 4;
@@ -314,7 +329,11 @@ __global__ __launch_bounds__(256) void distill_map_gradient_kernel(DistillArgs a
         }
 #pragma unroll
         for (int u = 0; u < U; ++u)
-            if (mine && j + u < c1) dz[(long)(j + u) * inner] = T::down(any && F != 0.f ? F * exp2_(__builtin_fmaf(x[u], c, -R)) : 0.f);
+            if (mine && j + u < c1) {
+                float d = any ? __builtin_fmaf(x[u], c, -R) : 0.f;
+                if (any_far && far) d = (x[u] - m) * c;
+                dz[(long)(j + u) * inner] = T::down(any && F != 0.f ? F * exp2_(d) : 0.f);
+            }
     }
     if (!any) return;
     __syncthreads();
@@ -327,7 +346,7 @@ __global__ __launch_bounds__(256) void distill_map_gradient_kernel(DistillArgs a
 
 SliceNotes slice_notes(char* at, long positions, int k) {
     float* f = (float*)at;
-    return {f, f + positions, (int*)(f + 2 * positions), f + (2 + k) * positions};
+    return {f, f + positions, f + 2 * positions, (int*)(f + 3 * positions), f + (3 + k) * positions};
 }
 
 }  // namespace
@@ -375,7 +394,7 @@ int log_probs_slices(int dtype, const LogProbArgs& a, MapSlices s, void* workspa
 }
 
 size_t distill_slices_workspace(const MapSlices& s, int outer, int inner, int k) {
-    return s.count == 1 ? 0 : (size_t)outer * inner * (s.count * sizeof(Sums) + (2 + 2 * (size_t)k) * sizeof(float));
+    return s.count == 1 ? 0 : (size_t)outer * inner * (s.count * sizeof(Sums) + (3 + 2 * (size_t)k) * sizeof(float));
 }
 
 int distill_slices(int dtype, const DistillArgs& a, const MapSlices& s, void* workspace, bool again, hipStream_t stream) {
