@@ -272,7 +272,7 @@ __global__ __launch_bounds__(64 * most_waves(K)) void log_probs_map_kernel(LogPr
 // HBM bounds it: 32 x 133 x 96 x 96 bf16 31 us (5.1 TB/s).
 template <class T>
 __global__ __launch_bounds__(256) void log_probs_bwd_map_kernel(LogProbBwdArgs a, int tiles, int splits) {
-    constexpr int VEC = T::VEC, PPR = POS / VEC, ROWS = 256 / PPR, U = 4;
+    constexpr int VEC = T::VEC, PPR = POS / VEC, ROWS = 256 / PPR, U = 4, IGNORED = -2;
     __shared__ float s_ref[POS], s_l2[POS], s_A[POS], s_B[POS], s_gl[POS];
     __shared__ int s_at[POS], s_is_far[POS], s_far;
     const int C = a.g.classes, inner = a.g.inner, tid = threadIdx.x;
@@ -294,7 +294,7 @@ __global__ __launch_bounds__(256) void log_probs_bwd_map_kernel(LogProbBwdArgs a
         s_A[tid] = -(gl + gh * a.entropy[p]);
         s_B[tid] = -gh * LN2;
         s_gl[tid] = gl;
-        s_at[tid] = named ? (int)y : -1;
+        s_at[tid] = named ? (int)y : gh == 0.f ? IGNORED : -1;
         s_is_far[tid] = far;
         const bool any = __any(far);
         if (tid == 0) s_far = any;
@@ -327,7 +327,7 @@ __global__ __launch_bounds__(256) void log_probs_bwd_map_kernel(LogProbBwdArgs a
                 if (any_far && s_is_far[px + e]) d = (x - ref[e]) * c;
                 d -= l2[e];
                 const float g = exp2_(d) * __builtin_fmaf(B[e], bounded(d), A[e]);
-                o[e] = cls == at[e] ? g + gl[e] : g;
+                o[e] = cls == at[e] ? g + gl[e] : at[e] == IGNORED ? 0.f : g;  // (ignored: whatever the logits are)
             }
             store_positions<T>(dz + (long)cls * inner, px, n, T::pack(o));
         }

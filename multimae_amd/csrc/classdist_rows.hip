@@ -468,6 +468,14 @@ __global__ __launch_bounds__(JOIN_NT) void log_probs_join_kernel(LogProbArgs a, 
     finish_row<T, 64>(a, p, z, v, s_keys + slices * k, red, named);
 }
 
+template <class T, int NT>
+__device__ __forceinline__ void zero_row(typename T::E* dz, int first, int end) {
+    for (int j = first + (int)threadIdx.x * T::VEC; j < end; j += NT * T::VEC) {
+        if (j + T::VEC <= end) store_piece<T>(dz + j, Piece{});
+        else for (int e = j; e < end; ++e) dz[e] = T::down(0.f);
+    }
+}
+
 // Rows, backward: a tile per workgroup.  gl 1[j = y] - (gl + gh (log p + H)) p, the second term as p (A + B log2 p).  HBM bounds it: 4095
 // x 64000 bf16 202 us (5.2 TB/s).
 template <class T, int NT, int NV>
@@ -485,6 +493,10 @@ __global__ __launch_bounds__(NT) void log_probs_bwd_rows_kernel(LogProbBwdArgs a
     const float gh = a.d_entropy ? a.d_entropy[p] * a.g.inv_t : 0.f;
     const float A = -(gl + gh * a.entropy[p]), B = -gh * LN2;
     const int at = y >= 0 && y < C ? (int)y : -VEC;
+    if (at < 0 && gh == 0.f) {  // an ignored row: whatever its logits are
+        zero_row<T, NT>(dz, base, C - base < TILE ? C : base + TILE);
+        return;
+    }
     const bool far = is_far(m, c);
     const float R = far ? 0.f : reference_exponent(m, c);
 #pragma unroll
@@ -673,14 +685,6 @@ __device__ __forceinline__ float far_row(const DistillArgs& a, long p, float w, 
                 if (i < n) dz[j + i] = T::down(o[i]);
     }
     return l;
-}
-
-template <class T, int NT>
-__device__ __forceinline__ void zero_row(typename T::E* dz, int first, int end) {
-    for (int j = first + (int)threadIdx.x * T::VEC; j < end; j += NT * T::VEC) {
-        if (j + T::VEC <= end) store_piece<T>(dz + j, Piece{});
-        else for (int e = j; e < end; ++e) dz[e] = T::down(0.f);
-    }
 }
 
 // The pieces stay as they were read: elements unpacked for one phase and kept for the next would hold twice the registers.
