@@ -5,8 +5,8 @@
 // rows [N, C] are inner = 1 and class maps [B, C, H, W] are inner = H * W.  With x = z / T, m = max x, s = sum exp(x - m):
 //   log p_j = x_j - m - log s,   H = -sum p_j log p_j (terms of p = 0 are 0)
 //   d/dz_j (gl log p_y + gh H) = (gl ([j = y] - p_j) - gh p_j (log p_j + H)) / T
-// Everything between the loads and the stores is fp32; exponentials are taken of differences (z - m) * log2(e) / T, formed
-// before scaling, so that logits of the type's lowest value (a mask) stay finite differences where a whole row has them.
+// Everything between the loads and the stores is fp32.  Exponentials are the bare base-2 instruction, which gives 0 for results below
+// 2^-126: probabilities and gradients that fp32 would hold as subnormal numbers are 0.
 #pragma once
 #include "common.h"
 
@@ -147,7 +147,6 @@ struct Geometry {
     float c, inv_t;  // log2(e) / T, 1 / T
     // log p of logit z, formed in natural units: a finite lowest logit times log2(e) would leave the range of fp32
     __device__ __forceinline__ float log_p(float z, float m, float l2) const { return (z - m) * inv_t - l2 * LN2; }
-    __device__ __forceinline__ long base(long p) const { return inner == 1 ? p * ld : (p / inner) * ld + p % inner; }
 };
 
 // Sums in the base-2 domain against a reference exponent R: s = sum 2^(z c - R), t = sum (z c - R) 2^(z c - R), m = max z.

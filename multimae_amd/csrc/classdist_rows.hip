@@ -6,9 +6,10 @@ namespace {
 
 // ---- log probabilities: one pass over a row, or a slice of it -------------------------------------------------------
 // A thread keeps a maximum and the sums s, t against it, rescaled when it grows; H = log2 s - t / s.  HBM bounds it: 4096 x 150016
-// bf16 218 us (5.6 TB/s), with 8 alternatives 234 us; 2047 x 50001 fp32 with 8 82 us (5.0 TB/s).  Short rows with alternatives are
-// bounded by the list's barriers and searches (8192 x 5000 bf16: 20 us without, 59 us with 8); 16-bit rows that begin at odd
-// elements load 16 bytes across lines (4095 x 64007: 116 us, x 64008: 98 us).
+// bf16 214 us (5.7 TB/s), with 8 alternatives 224 - 238 us, where the vector ALU is busy too (87 % of the cycles); 2047 x 50001 fp32 with 8
+// 83 us (4.9 TB/s).  In the first 20 ms of work after an idle card such launches take up to 330 us, until its clocks have settled.
+// Short rows with alternatives are bounded by the list's barriers and searches (8192 x 5000 bf16: 20 us without, 59 us with 8); 16-bit
+// rows that begin at odd elements load 16 bytes across lines (4095 x 64007: 116 us, x 64008: 101 us).
 template <int NT>
 __device__ Sums block_sums(Sums v, Sums* red) {
     v = wave_sums(v);
@@ -425,8 +426,8 @@ __global__ __launch_bounds__(NT) void log_probs_rows_kernel(LogProbArgs a, int s
 }
 
 // Joins the slices of a row: four waves fetch the keys, then one goes on: lane i walks slice i's sorted keys.  Latency: the fetch, and
-// k largest of the lanes' heads (24 x 131072 bf16, 32 slices of 20 alternatives: 19 us with the slices; fetched by one wave, and the
-// largest found by exchanges through the LDS, 24 us).
+// k largest of the lanes' heads (24 x 131072 bf16, 32 slices of 20 alternatives: 7 us after 9 us of the slices; fetched by one wave, and
+// the largest found by exchanges through the LDS, 5 us more).
 constexpr int MAX_SLICES = 64, JOIN_NT = 256;
 template <class T>
 __global__ __launch_bounds__(JOIN_NT) void log_probs_join_kernel(LogProbArgs a, int slices, const char* parts) {
@@ -477,7 +478,7 @@ __device__ __forceinline__ void zero_row(typename T::E* dz, int first, int end) 
 }
 
 // Rows, backward: a tile per workgroup.  gl 1[j = y] - (gl + gh (log p + H)) p, the second term as p (A + B log2 p).  HBM bounds it: 4095
-// x 64000 bf16 202 us (5.2 TB/s).
+// x 64000 bf16 199 us (5.3 TB/s).
 template <class T, int NT, int NV>
 __global__ __launch_bounds__(NT) void log_probs_bwd_rows_kernel(LogProbBwdArgs a, int tiles) {
     constexpr int VEC = T::VEC, TILE = NT * NV * VEC;
@@ -712,7 +713,7 @@ __device__ __forceinline__ Sums tile_sums(Piece (&q)[NV], float c) {  // one thr
 __device__ __forceinline__ float uniform(float v) { return __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(v))); }
 
 // A row held in the registers of one workgroup: read once, its gradient written once.  Several workgroups a CU overlap one row's
-// loads with another's stores: 8192 x 32000 fp32 419 us (5.0 TB/s).
+// loads with another's stores: 8192 x 32000 fp32 414 us (5.1 TB/s).  The bound on the registers (64) keeps eight waves on a SIMD.
 template <class T, int NT, int NV>
 __global__ __launch_bounds__(NT, 8) void distill_rows_kernel(DistillArgs a) {
     constexpr int VEC = T::VEC;
@@ -804,7 +805,7 @@ __global__ __launch_bounds__(NT, 8) void distill_rows_kernel(DistillArgs a) {
 
 // Many rows, and long ones, of which a CU holds one or two: a workgroup takes row after row, and while the pieces of one row's
 // gradient leave, the next row's come into the registers they free, so that reading and writing overlap; the sums in between do
-// not (4096 x 128000 bf16 496 us, 4.2 TB/s; 4095 x 64000 236 us, 4.5 TB/s).  Every piece but the last
+// not (4096 x 128000 bf16 500 us, 4.2 TB/s; 4095 x 64000 232 us, 4.5 TB/s).  Every piece but the last
 // begins at a multiple of NT * VEC elements and the last one ends with the row, so that a piece is a uniform address and the
 // thread's own offset.  The elements that the last piece shares with the one before are -inf in the last one,
 // which writes its zeros first.
@@ -982,7 +983,7 @@ __device__ __forceinline__ void each_kept(int cls, int base, int end, F put) {
 }
 
 // Few or long rows, first pass: the sums outside the kept classes, a slice per workgroup.  Few rows are latency: 16 x 32000 bf16
-// takes 7 us here and 10 us in the second pass; 64 x 128001 25 us together.
+// takes 7 us here and 9 us in the second pass; 64 x 128001 21 us together.
 template <class T, int NT, int NV>
 __global__ __launch_bounds__(NT) void distill_slices_kernel(DistillArgs a, int slices, int slice_tiles, Sums* parts) {
     constexpr int VEC = T::VEC, TILE = NT * NV * VEC;
@@ -1094,8 +1095,8 @@ __global__ __launch_bounds__(NT, 8) void distill_tiles_kernel(DistillArgs a, int
 constexpr int CUS = 256;
 constexpr int SHORT_ROW = 2048;  // up to here a row is one wave's
 // Elements of a tile, a workgroup of 256 threads: in the log probabilities' forward pass, which holds a second tile on its way,
-// 16 a thread (4096 x 150016 bf16, 8 alternatives: 234 us; 8 a thread 259 us, 32 a thread 249 us; 512 threads, which wait for
-// each other at the lists' barriers, 345 us), 32 elsewhere.
+// 16 a thread (8 alternatives, 4096 x 150016 bf16 and 2047 x 50001 fp32: 238 and 88 us; 8 a thread 252 and 92, 32 a thread 240 and 97;
+// 512 threads, which wait for each other at the lists' barriers, 337 and 149; all of them after 200 launches), 32 elsewhere.
 constexpr int LP_NT = 256, LP_EPT = 16, LP_TILE = LP_NT * LP_EPT, ROW_TILE = 8192;
 // Workgroups a row is split into, and the tiles of each: enough for every CU to hold eight, at least a tile each, none empty.
 struct Split { int slices, tiles; };
@@ -1107,9 +1108,10 @@ Split split_row(int rows, int classes, int tile) {
     return {(tiles + per - 1) / per, per};
 }
 // A row of the log probabilities' forward pass is one wave's, which waits for no other, up to SHORT_ROW classes, and where every CU
-// has eight rows up to 8192 (bf16, 4096 x 5000: 13 us, a workgroup of four waves 20; 8192 x 8000: 27 and 34).  The list of
-// alternatives is where one wave is slow: up to 4096 with 16 of them (4096 x 4000, 8 alternatives: 24 and 27 us;
-// 4096 x 6000: 36 and 36; 20 alternatives, 4096 x 4000: 32 and 30).
+// has eight rows up to 8192 (bf16, 4096 x 5000: 12 us, a workgroup of four waves 20; 8192 x 8000: 28 and 37).  The list of
+// alternatives is where one wave is slow: up to 4096 with 16 of them (4096 x 4000, 8 alternatives: 23 and 27 us; 20 alternatives 32 and
+// 29 us).  Beyond 4096 a wave would gain with 8 alternatives (4096 x 6000: 32 and 35 us, 8192 x 5000: 46 and 59 us); what it does with
+// other lists there is not measured.
 bool one_wave(int rows, int classes, int k) { return classes <= (rows < 8 * CUS || k > 16 ? SHORT_ROW : k ? 4096 : 8192); }
 Split log_probs_split(int rows, int classes, int k) {
     return one_wave(rows, classes, k) ? Split{1, (classes + 64 * LP_EPT - 1) / (64 * LP_EPT)} : split_row(rows, classes, LP_TILE);
@@ -1133,16 +1135,20 @@ static void launch_log_probs_rows(const LogProbArgs& a, void* workspace, hipStre
         hipLaunchKernelGGL(log_probs_join_kernel<T>, dim3(rows), dim3(JOIN_NT), sizeof(uint64_t) * (size_t)(d.slices + 1) * a.k, stream, a, d.slices, (const char*)workspace);
 }
 
-// Three ways.  Many rows are walked, each workgroup holding one and the next one on its way.  Fewer rows, if short, are held by
-// one workgroup each; few and long ones are cut into slices and read twice, the second time mostly from the caches.
-// Walked against held: 16-bit rows gain at every length (bf16, 4096 rows of 4000: 37 and 47 us, of 8000: 44 and 64 us, of
-// 32000: 141 and 196 us; 2048 rows of 4000: 26 and 29 us).  fp32 rows fill the same registers with half the classes and gain up
-// to 4096 of them (4096 x 4000: 40 and 48 us; 16384 x 16000: 429 and 405 us).  A row of more than 32768 classes takes half
-// a CU or all of it, and no second workgroup covers its loads: walked from one row per CU on.
+// Three ways.  Many rows are walked, each workgroup holding one and the next one on its way.  Fewer rows, and fp32 ones, if short, are
+// held by one workgroup each; few and long ones are cut into slices and read twice, the second time mostly from the caches.
+// Walked against held, logits and gradients from HBM: 16-bit rows of 2049 - 32768 classes come out even where there are many (bf16,
+// 16384 x 4000: 103 us both; 4096 x 16000: 75 us both; 4096 x 32000: 135 and 137 us), gain at 4096 x 8000 (44 and 47 us) and lose at
+// 16384 x 8000 (137 and 129 us); from 256 to 2047 rows held is ahead below 16000 classes (1024 x 4000: 17 and 24 us, two launches less;
+// 1024 x 32000: 44 and 42 us).  fp32 rows of up to 4096 classes are held (4096 x 4000: 40 and 42 us; 65536 x 4000: 418 and 474 us).  A row
+// of more than 32768 classes takes half a CU or all of it, and no second workgroup covers its loads: walked from one row per CU on
+// (against slices, bf16 1024 x 128000: 152 and 170 us, 256 x 64000: 27 and 28 us; fp32 1024 x 50000: 116 and 122 us, but
+// 256 x 50000: 38 and 32 us).  Held against slices: 256 x 16000 bf16 17 and 21 us, 1024 x 32000 fp32 56 and 68 us.  Rows beyond the
+// registers are sliced however many they are: 4096 x 200000 bf16 941 us, 2048 x 100000 fp32 468 us (3.5 TB/s of the logits and the
+// gradient, which the second reading of the logits is added to).
 bool walked_rows(int rows, int classes, int dtype) {
-    if (classes <= SHORT_ROW) return false;
-    if (dtype == MMAE_DT_F32) return classes <= 65536 && (classes > 32768 ? rows >= CUS : classes <= 4096 && rows >= 8 * CUS);
-    return classes <= 131072 && rows >= (classes > 32768 ? CUS : 8 * CUS);
+    if (dtype == MMAE_DT_F32) return classes > 32768 && classes <= 65536 && rows >= CUS;
+    return classes > SHORT_ROW && classes <= 131072 && rows >= (classes > 32768 ? CUS : 8 * CUS);
 }
 bool held_rows(int rows, int classes) { return classes <= ROW_TILE || (rows >= 256 && classes <= 32768); }
 
@@ -1173,8 +1179,7 @@ static void launch_distill_rows(const DistillArgs& a, int dtype, Sums* parts, bo
             else if (C <= 114688) LONG(512, 28);
             else LONG(512, 32);
         } else {
-            if (C <= 4096) LONG(256, 4);
-            else if (C <= 49152) LONG(512, 24);
+            if (C <= 49152) LONG(512, 24);
             else LONG(512, 32);
         }
     }
