@@ -282,7 +282,8 @@ int mmae_masked_ce(const void* logits, int logits_is_bf16, const int64_t* target
  * mmae_class_log_probs: log_prob = log softmax(x)[target] (0 where target is outside [0, classes), e.g. -100), entropy of
  * softmax(x), and the top_k (<= 64, <= classes) classes by z with their log probabilities: descending, equal values by the
  * lower class, NaN as +inf.  row_max / row_log_sum: what the backward pass needs (both may be NULL).  A position whose logits are all -inf
- * has log_prob = -inf (at a valid target), entropy 0 and no gradient.  NaN and +inf logits give NaN, as in torch.
+ * has log_prob = -inf (at a valid target), entropy 0 and no gradient.  NaN and +inf logits give NaN, as in torch.  Probabilities below
+ * 2^-126 count as 0 in entropy and gradients (log probabilities do not end there).
  * mmae_class_log_probs_bwd: d_logits (contiguous, the logits' dtype) for the gradients that arrive at log_prob and entropy
  * (either may be NULL).
  * temperature: positive, from 4.3e-39 on (distillation: its square a normal fp32 number, divided by the positions too).
@@ -298,7 +299,8 @@ int mmae_class_log_probs_bwd(const void* logits, int dtype, int outer, int class
 /* Distillation from a teacher's k (<= 64) top classes per position: top_class (int32 or int64: class_bytes 4 / 8) and
  * top_value (f32, bf16 or f16: value_dtype), [outer, k, inner].  kind 0: the values are the teacher's logits, q = softmax(value /
  * temperature) over the k; kind 1: its log probabilities at this temperature, q = exp(value), and what they leave, 1 - sum q,
- * stands for all other classes as one outcome.  A class outside [0, classes) is padding; one listed twice counts twice.
+ * stands for all other classes as one outcome (left out where there are none, or all of them are -inf).  A class outside [0, classes) is
+ * padding; one listed twice counts twice.  A position in the loss whose logits are all -inf makes the loss +inf and has no gradient.
  *   loss = temperature^2 * mean of KL(q || p): over the positions in the mask of each sample, then over the samples with any
  * mask i64 [outer, (rows / patch) * (width / patch)] over inner = rows x width positions (nonzero = in the loss), or NULL: the
  * mean over all positions.  loss (f32 scalar) or d_logits (contiguous, the logits' dtype: the loss's gradient times

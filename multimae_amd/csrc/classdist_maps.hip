@@ -60,8 +60,8 @@ __device__ __forceinline__ void load_map_tile(typename T::E* tile, const typenam
 // The 16-bit types leave the low bits of an fp32 number free: there a value carries its class along, so that the sorted list is
 // the answer and the second pass falls away.
 //
-// 256 x 150 x 56 x 56: fp32 115 us (4.2 TB/s), with 8 alternatives 284 us; 167 x 255 x 56 x 56 bf16 73 and 188 us: the lists'
-// arithmetic and, fp32, the second pass.
+// 256 x 150 x 56 x 56: fp32 113 us (4.3 TB/s), with 8 alternatives 283 us; 167 x 255 x 56 x 56 bf16 72 and 186 us: the lists'
+// arithmetic and, fp32, the second pass (the vector ALU is busy in 86 % of the cycles, without a list in 88 %).
 constexpr int QUEUE = 16;
 constexpr int CODE_BITS = 12;                   // of a carried class: the mantissa bits that bf16 (16) and f16 (13) leave
 constexpr uint32_t CODES = (1u << CODE_BITS) - 1, CARRIED_INF = 0x7f800000u - (1u << CODE_BITS);  // above the largest finite value of both
@@ -338,7 +338,7 @@ __global__ __launch_bounds__(256) void log_probs_bwd_map_kernel(LogProbBwdArgs a
 // Wave 0 prepares the kept classes, a lane per position: each class once (an entry listed again adds its q to the entry whose
 // number the tile's element holds last), the student's logits beside them, and -inf in the tile where the sums leave them out.
 // After the sums the tile's logits become the gradient in place, the kept classes get theirs, and the tile is stored.  167 x 255 x
-// 56 x 56 fp32, 8 kept classes: 264 us (4.0 TB/s).
+// 56 x 56 fp32, 8 kept classes: 268 us (4.0 TB/s).
 inline int distill_map_bytes(int element, int classes, int k, int waves) {
     return (classes * POS * element + 15) / 16 * 16 + waves * POS * (int)sizeof(Sums) + 3 * k * POS * 4 + 2 * POS * 4;
 }
@@ -519,7 +519,9 @@ __global__ __launch_bounds__(1024) void distill_map_kernel(DistillArgs a, int ti
 // ---- many positions, up to 136 classes: a wave per tile, the logits in its registers ------------------------------------
 // The tile in the LDS bounds the maps' kernels above by latency: 34 KiB of 133 fp32 classes leave three workgroups on a CU,
 // each in one phase at a time.  Held in registers the same tile takes no LDS and no other wave: 12 waves a CU that wait for
-// nobody: 256 x 133 x 56 x 56 fp32 with 8 alternatives 118 us (4.4 TB/s with the outputs), in the LDS 276 us; bf16 91 and 184 us.
+// nobody: 256 x 133 x 56 x 56 fp32 with 8 alternatives 119 us (4.4 TB/s with the outputs), in the LDS 276 us; bf16 91 and 127 us, where
+// the vector ALU is busy in 74 % of the cycles (32 x 133 x 96 x 96 with 4: 38 us, 52 %; a lane loads two bytes, and 28 bytes a lane of
+// the 16-bit kernels' registers are spilled under the bound of three waves a SIMD).
 // CP: classes held (the first MIN of them exist).
 constexpr int REG_CLASSES = 136, REG_TOP = 16;
 
@@ -704,8 +706,10 @@ __global__ __launch_bounds__(64, 3) void log_probs_map_regs_kernel(LogProbArgs a
 
 // Distillation.  The kept classes of a position are bits of a mask; a kept class has a place in the LDS, the number of kept
 // classes below it, which a walk over the classes counts along.  So its logit gets there and its gradient back without a
-// load or store of its own, each of which would move a line per position.  256 x 133 x 56 x 56, 8 kept classes: fp32 186 us
-// (5.0 TB/s), bf16 157 us, bounded by the arithmetic; in the LDS 366 and 232 us.
+// load or store of its own, each of which would move a line per position.  256 x 133 x 56 x 56, 8 kept classes: fp32 197 us
+// (4.6 TB/s with the kept classes), with the teacher's log probabilities 204 us; in the LDS 242 and 261 us.  bf16 152 and 160 us (LDS 171
+// and 182): neither HBM (2.9 TB/s) nor the vector ALU (39 and 49 % of the cycles) is full; there are as many loads and stores as in
+// fp32, of two bytes a lane, and two waves a SIMD to cover them.
 template <class T, int CP, int MIN, bool REST>
 __global__ __launch_bounds__(64, 2) void distill_map_regs_kernel(DistillArgs a, int tiles) {
     constexpr int WORDS = (CP + 31) / 32;
@@ -933,8 +937,8 @@ int launch_log_probs_map(const LogProbArgs& a, const MapSlices& s, hipStream_t s
     return MMAE_OK;
 }
 // The register kernels take what fits them.  Distillation alone shares a tile of a small map among the waves of a workgroup: its
-// walk over the classes is longer (8 x 133 x 56 x 56 fp32, 392 tiles: 23.1 us in registers, 19.6 us in the LDS; 784 tiles: 26.6
-// and 32.6 us).
+// walk over the classes is longer (8 x 133 x 56 x 56 fp32, 392 tiles: 22.5 us in registers, 20 us in the LDS; 784 tiles: 26.5
+// and 34.9 us).
 constexpr long REG_TILES = 512;
 bool in_registers(int classes, int k) { return classes <= REG_CLASSES && k <= REG_TOP; }
 

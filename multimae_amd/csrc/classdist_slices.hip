@@ -1,10 +1,11 @@
 // Class distributions over maps [B, C, inner] of more classes than a workgroup's LDS holds well: slices of the classes, whose sums
 // (and best classes) are joined per position.  Read once for the log probabilities, twice for distillation with its gradient.
 //
-// A wave's load is one class of 64 neighbouring positions.  131 x 1000 x 32 x 32 fp32 (537 MB): log probabilities 119 us (4.5 TB/s),
-// with 8 alternatives 314 us, where the lists bound them, distillation with its gradient 440 us (three passes, 3.7 TB/s);
-// a workgroup per position, which reads a line for each of its logits, takes 1270, 9121 and 4030 us.  Maps of few positions a
-// sample (2 x 2) leave most lanes idle.
+// A wave's load is one class of 64 neighbouring positions.  The log probabilities' lists of best classes are joined by a lane per
+// position where the slices are few, by a wave per position where they are many.  131 x 1000 x 32 x 32 fp32 (537 MB): log
+// probabilities 118 us (4.6 TB/s), with 8 alternatives 313 us, where the lists bound them (the vector ALU is busy in 91 % of the cycles),
+// distillation with its gradient 438 us (three passes, 3.7 TB/s); a workgroup per position, which reads a line for each of its logits,
+// takes 1270, 9121 and 4030 us.  Maps of few positions a sample (2 x 2) leave most lanes idle.
 #include "classdist.h"
 
 namespace classdist {
@@ -96,7 +97,7 @@ __global__ __launch_bounds__(64) void log_probs_map_join_kernel(LogProbArgs a, i
 
 // The same with a wave per position, a lane per slice: k times the largest of the lanes' heads, whose lane takes its next key.  The
 // last lane holds the best of the slices before, 63 at a time.  Each key costs six exchanges instead of insertions that wait for
-// each other: 16 x 32000 x 16 x 16 bf16, 63 slices, with 8 alternatives 236 us instead of 338, with 64 739 instead of 2351.  4
+// each other: 16 x 32000 x 16 x 16 bf16, 63 slices, with 8 alternatives 202 us (338 by lanes), with 64 719 us (2351).  4
 // slices fill 4 lanes only (131 x 1000 x 32 x 32 fp32 with 8: 742 us instead of 569); from 8 to 16 both take the same.
 template <class T>
 __global__ __launch_bounds__(256) void log_probs_map_merge_kernel(LogProbArgs a, MapSlices sl) {
