@@ -707,8 +707,8 @@ __global__ __launch_bounds__(64, 3) void log_probs_map_regs_kernel(LogProbArgs a
 // Distillation.  The kept classes of a position are bits of a mask; a kept class has a place in the LDS, the number of kept
 // classes below it, which a walk over the classes counts along.  So its logit gets there and its gradient back without a
 // load or store of its own, each of which would move a line per position.  256 x 133 x 56 x 56, 8 kept classes: fp32 197 us
-// (4.6 TB/s with the kept classes), with the teacher's log probabilities 204 us; in the LDS 242 and 261 us.  bf16 152 and 160 us (LDS 171
-// and 182): neither HBM (2.9 TB/s) nor the vector ALU (39 and 49 % of the cycles) is full; there are as many loads and stores as in
+// (4.7 TB/s with the kept classes), with the teacher's log probabilities 204 us; in the LDS 242 and 261 us.  bf16 152 and 160 us (LDS 171
+// and 182): neither HBM (3.0 - 3.2 TB/s) nor the vector ALU (39 and 49 % of the cycles) is full; there are as many loads and stores as in
 // fp32, of two bytes a lane, and two waves a SIMD to cover them.
 template <class T, int CP, int MIN, bool REST>
 __global__ __launch_bounds__(64, 2) void distill_map_regs_kernel(DistillArgs a, int tiles) {
