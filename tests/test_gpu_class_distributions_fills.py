@@ -227,3 +227,39 @@ def test_large_gradients_of_the_entropy(M, shape):
     assert torch.isfinite(got).all() and (got[z == -1e30][unit[z == -1e30] == 0] == 0).all()
     want = unit.double().cpu() * 1e36
     close(got, want, want.abs() * 64 * U + 1e36 * (2 * CHAIN + 20 * U * (1 + math.log(shape[1]))) * torch.softmax(z.double().cpu(), 1) * (2 + 2 * math.log(shape[1])), "grad")
+
+
+@pytest.mark.parametrize("shape", [(3, 300, 8, 12), (40, 20000), (530, 60, 4, 6), (2, 1111, 8, 12)], ids=str)
+def test_fills_in_captured_graphs(M, shape):
+    """Rows beyond the reference exponents in one replay and not in the next: what a call finds out about its rows stays in that call
+    (forms with more than 64 KiB of LDS, in registers and in slices among them)."""
+    z = scores(shape, "f32", 1).requires_grad_(True)
+    target = classes(shape[:1] + shape[2:], shape[1], 3)
+    cls, val = teacher_top(shape, 9, 5, True, 1.0)
+    fn = loss_module(M, 1, 1.0, True)
+
+    def step():
+        loss = fn(z, (cls, val)) * 0.5
+        out = M.class_log_probs(z, target, top_k=20)
+        (grad,) = torch.autograd.grad(loss + out.entropy.mean(), z)
+        return [loss.detach(), out.log_prob.detach(), out.top_class, grad]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        outs = step()
+    for i in range(4):
+        new = scores(shape, "f32", 20 + i)
+        if i % 2 == 0:
+            new[0] = -1e9
+            new[1:] = torch.full_like(new[1:], -1e30).scatter(1, cls[1:], new[1:].gather(1, cls[1:]))
+        with torch.no_grad():
+            z.copy_(new)
+        graph.replay()
+        torch.cuda.synchronize()
+        got = [t.clone() for t in outs]
+        assert all(torch.equal(a, b) for a, b in zip(got, step())), i
+        assert all(torch.isfinite(t).all() for t in got), i
