@@ -104,7 +104,8 @@ class MaskedDistillationLoss(nn.Module):
         """input [B, C, H, W] logits (fp32, bf16 or fp16; also rows [N, C] or sequences [B, C, L]); target = (classes int32 or
         int64 [B, k, H, W], values [B, k, H, W]) with k <= 64; a class outside [0, C) (-1) is padding.  mask
         [B, (H/scale)*(W/scale)] with scale = patch_size // stride (rows: [N], sequences: [B, L]), nonzero = in the loss.
-        A mask that is zero everywhere gives a loss and a gradient of zero."""
+        A mask that is zero everywhere gives a loss and a gradient of zero.  A position in the loss whose logits are all -inf makes
+        the loss +inf and has no gradient."""
         top_class, top_value = target
         if mask is not None:
             if mask.dtype != torch.int64:
